@@ -1,0 +1,1161 @@
+// Losses over rows of logits, forward and backward, and their C ABI
+// (include/cugo_b200.h): the log-probability of a given action and the entropy of its
+// masked categorical (action_logp), the clipped policy loss with an entropy bonus and a
+// KL term (policy_loss), and the preference loss over pairs of sequences
+// (preference_pairs, on action_logp's rows).
+//
+// Mathematics of one row.  With x the logits, all sums run in base 2 and relative to the
+// row's maximum M:
+//   y_j = x_j log2(e) - M log2(e)   (one FMA; its rounding is the only one, so p_j keeps
+//                                    fp32's relative accuracy however large x is)
+//   s = sum 2^y_j,  t = sum 2^y_j y_j,  log2 p_j = y_j - log2 s,  H = ln 2 (log2 s - t/s)
+// A reference row z_j (M', s') adds u = sum 2^y_j (y_j - z_j):
+//   KL(p|q) = ln 2 (u/s - log2 s + log2 s').
+// Every gradient wanted here is, with 1 at the taken action a,
+//   d_j = hot [j = a] + 2^y_j (c_0 + c_1 y_j + c_2 (y_j - z_j)),
+// so a row needs its sums, four coefficients and one more look at its entries.
+//
+// An illegal entry counts as -2^30, and so does every entry below that (-inf, -1e30, a mask
+// of the type's lowest value): its 2^y is 0 beside any other entry and every product
+// stays finite, so no entry needs a branch.  (M log2(e) is off by at most 2^-24 of itself,
+// the same for the whole row: below 2^31 that shifts y by less than 128, which the sums
+// bear.  The bound is a power of two, so that it has no such rounding itself.)  What
+// stands in an illegal place (NaN, infinities) is never used; NaN in a legal place stays
+// NaN.  Sums over rows are taken in 64 bits, per warp or block, and
+// added over the blocks in order: the same result on every run.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/cugo_b200.h"
+
+namespace {
+
+namespace cg = cooperative_groups;
+using i64 = int64_t;
+constexpr unsigned kFull = 0xffffffffu;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kMasked = -1073741824.0f;  // -2^30
+constexpr float kMasked2 = kMasked * kLog2e;  // a maximum of masked entries only
+constexpr int kSms = 148;
+constexpr int kSums = 6;   // policy, entropy, KL, KL to the old policy, clipped, used
+constexpr int kStats = 7;  // the loss, then the means of the six
+
+enum Type : int { kFp32 = 0, kBf16 = 1, kFp16 = 2 };
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+// N values to the gradient's type at element `at`; `wide`: that address is a multiple of
+// the N values' bytes, or of 16.
+template <int N>
+__device__ __forceinline__ void store_grad(void* base, int type, i64 at, const float (&g)[N], bool wide) {
+  if (type == kFp32) {
+    float* d = static_cast<float*>(base) + at;
+    if (wide) {
+#pragma unroll
+      for (int e = 0; e < N; e += 4)
+        *reinterpret_cast<float4*>(d + e) = make_float4(g[e], g[e + 1], g[e + 2], g[e + 3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) d[e] = g[e];
+    }
+    return;
+  }
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    if (type == kBf16) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(g[e], g[e + 1]);
+      w[e / 2] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __half2 h = __floats2half2_rn(g[e], g[e + 1]);
+      w[e / 2] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  uint16_t* d = static_cast<uint16_t*>(base) + at;
+  if (wide) {
+    if constexpr (N == 8) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) d[e] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+  }
+}
+
+__device__ __forceinline__ void store_one(void* base, int type, i64 at, float g) {
+  if (type == kFp32) static_cast<float*>(base)[at] = g;
+  else if (type == kBf16) static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(g);
+  else static_cast<__half*>(base)[at] = __float2half_rn(g);
+}
+
+__host__ __device__ __forceinline__ int type_bytes(int type) { return type == kFp32 ? 4 : 2; }
+
+// What a row's gradient is made of (d_j above; the scale and 1 / s are in it).
+struct Coefs {
+  float hot, c0, c1, c2;
+};
+
+// The sums of a row, or of a part of one (maxima in base-2 units).
+struct Sums {
+  float m, s, t;    // maximum, sum 2^y, sum 2^y y
+  float mr, sr, u;  // the reference's maximum and sum, sum 2^y (y - z)
+};
+
+__device__ __forceinline__ Sums no_sums() { return {kMasked2, 0.0f, 0.0f, kMasked2, 0.0f, 0.0f}; }
+
+// Two parts' sums brought to their common maxima and added.
+template <bool kRef>
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
+  Sums r;
+  r.m = max_nan(a.m, b.m);
+  const float da = a.m - r.m, db = b.m - r.m;
+  const float fa = exp2_fast(da), fb = exp2_fast(db);
+  r.s = a.s * fa + b.s * fb;
+  r.t = fa * (a.t + da * a.s) + fb * (b.t + db * b.s);
+  r.mr = kMasked2;
+  r.sr = r.u = 0.0f;
+  if constexpr (kRef) {
+    r.mr = max_nan(a.mr, b.mr);
+    const float ra = a.mr - r.mr, rb = b.mr - r.mr;
+    r.sr = a.sr * exp2_fast(ra) + b.sr * exp2_fast(rb);
+    r.u = fa * (a.u + (da - ra) * a.s) + fb * (b.u + (db - rb) * b.s);
+  }
+  return r;
+}
+
+template <bool kRef>
+__device__ __forceinline__ Sums join_warp(Sums v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Sums b = no_sums();
+    b.m = __shfl_xor_sync(kFull, v.m, o);
+    b.s = __shfl_xor_sync(kFull, v.s, o);
+    b.t = __shfl_xor_sync(kFull, v.t, o);
+    if constexpr (kRef) {
+      b.mr = __shfl_xor_sync(kFull, v.mr, o);
+      b.sr = __shfl_xor_sync(kFull, v.sr, o);
+      b.u = __shfl_xor_sync(kFull, v.u, o);
+    }
+    // In the order of the lanes: every lane ends with the same bits.
+    v = (threadIdx.x & o) ? join<kRef>(b, v) : join<kRef>(v, b);
+  }
+  return v;
+}
+
+__device__ __forceinline__ float sum_warp(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+
+__device__ __forceinline__ double sum_warp(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+
+__device__ __forceinline__ float max_warp(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+
+struct Rows {
+  const void* logits;
+  i64 ld;
+  const void* ref;    // or null
+  i64 ldr;
+  const bool* legal;  // or null
+  i64 ldm;
+  const i64* actions;
+  const float* weight;  // or null
+  i64 rows;
+  int vocab;
+};
+
+// action_logp's outputs (any may be null).
+struct Score {
+  float* logp;
+  float* entropy;
+  float2* lse;   // {maximum, log2 of the sum}, in base-2 units; {0, +inf}: the row does not count
+  float* zeros;  // [rows] written as 0 (the coefficients that preference_pairs fills in)
+};
+
+struct Policy {
+  const float* logp_old;
+  const float* adv;
+  const float* ref_logp;  // or null
+  float low, high, kl_coef, entropy_coef;
+  float denominator;            // not 0: given; 0: *denominator_dev, the sum of the weights, or the rows
+  const float* denominator_dev;
+  const double* weight_sums;    // partial sums of the weights, or null (sum them here)
+  int n_weight_sums;
+  float grad_scale;
+  const float* grad_scale_dev;  // or null; multiplies grad_scale
+  void* dlogits;                // or null
+  i64 ldd;
+  int dtype, width;             // columns vocab .. width - 1 are written as 0
+  float* logp;                  // or null
+  double* partial;              // [blocks][kSums], or null: no means wanted
+};
+
+// A row's loss terms (times its weight, added to acc) and its gradient's coefficients,
+// from its sums and its action's y.
+template <bool kRef>
+__device__ __forceinline__ Coefs policy_row(const Policy& a, i64 row, const Sums& v, float y_a, float w,
+                                            float scale, double (&acc)[kSums], float& logp) {
+  const float log_s = log2f(v.s), inv_s = 1.0f / v.s, mean_y = v.t * inv_s;
+  logp = kLn2 * (y_a - log_s);
+  const float entropy = kLn2 * (log_s - mean_y);
+  const float log_ratio = logp - a.logp_old[row];
+  const float ratio = expf(log_ratio), adv = a.adv[row];
+  const float bounded = ratio < a.low ? a.low : ratio > a.high ? a.high : ratio;
+  // min(r A, clamp(r) A); where the two are equal the ratio still moves the loss.
+  const bool moves = !(ratio * adv > bounded * adv);
+  const float gain = moves ? ratio * adv : bounded * adv;
+  float g = moves ? -ratio * adv : 0.0f;
+  float kl = 0.0f, mean_d = 0.0f, c2 = 0.0f;
+  if constexpr (kRef) {
+    mean_d = v.u * inv_s;
+    kl = kLn2 * (mean_d - log_s + log2f(v.sr));
+    c2 = a.kl_coef * kLn2;
+  } else if (a.ref_logp) {
+    const float d = a.ref_logp[row] - logp, e = expm1f(d);
+    kl = e - d;
+    g -= a.kl_coef * e;
+  }
+  // lp + H = ln 2 (y - mean y), lp - lq - KL = ln 2 ((y - z) - mean (y - z)).
+  const float c1 = a.entropy_coef * kLn2, k = scale * w, ks = k * inv_s;
+  Coefs c;
+  c.hot = k * g;
+  c.c0 = ks * (-g - c1 * mean_y - c2 * mean_d);
+  c.c1 = ks * c1;
+  c.c2 = ks * c2;
+  const double wd = w;
+  acc[0] -= wd * gain;
+  acc[1] += wd * entropy;
+  acc[2] += wd * kl;
+  acc[3] += wd * (expm1f(log_ratio) - log_ratio);
+  acc[4] += ratio < a.low || ratio > a.high ? wd : 0.0;
+  acc[5] += wd;
+  return c;
+}
+
+// The denominator of the means: given, the sum of the weights, or the rows.  Every block
+// adds the same numbers in the same order.  Uses and synchronises the whole block.
+__device__ double block_denominator(const Policy& a, const float* weight, i64 rows) {
+  if (a.denominator != 0.0f) return a.denominator;
+  if (a.denominator_dev) return *a.denominator_dev;
+  if (!weight) return static_cast<double>(rows);
+  __shared__ double part[32];
+  __shared__ double total;
+  double t = 0.0;
+  if (a.weight_sums)
+    for (int i = threadIdx.x; i < a.n_weight_sums; i += blockDim.x) t += a.weight_sums[i];
+  else
+    for (i64 i = threadIdx.x; i < rows; i += blockDim.x) t += weight[i];
+  t = sum_warp(t);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    t = 0.0;
+    for (unsigned k = 0; k < blockDim.x / 32; ++k) t += part[k];
+    total = t;
+  }
+  __syncthreads();
+  return total;
+}
+
+// The scale of every gradient: a batch without weight has no mean, and no gradient.
+__device__ __forceinline__ float grad_scale_of(const Policy& a, double denominator) {
+  const float g = a.grad_scale * (a.grad_scale_dev ? *a.grad_scale_dev : 1.0f);
+  return denominator == 0.0 ? 0.0f : static_cast<float>(g / denominator);
+}
+
+// The warps' sums of a block, added in order, into partial[block].
+__device__ void store_partial(const Policy& a, const double (&acc)[kSums]) {
+  if (!a.partial) return;
+  __shared__ double part[32][kSums];
+  const int warp = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0)
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) part[warp][k] = acc[k];
+  __syncthreads();
+  if (threadIdx.x < kSums) {
+    double t = 0.0;
+    for (unsigned w = 0; w < blockDim.x / 32; ++w) t += part[w][threadIdx.x];
+    a.partial[(i64)blockIdx.x * kSums + threadIdx.x] = t;
+  }
+}
+
+// ---- short rows: a warp per row, the row in registers -----------------------------------
+//
+// Lane l holds entries l, l + 32, ..., kPer of them: scalar loads, coalesced whatever the
+// row's alignment (a 179-entry row of fp32 starts at any multiple of 4 bytes).
+
+constexpr int kShortWarps = 8;
+
+template <typename T, int kPer, bool kRef, bool kPolicy>
+__global__ void __launch_bounds__(32 * kShortWarps) short_rows_kernel(const Rows r, const Score o, const Policy a) {
+  const int lane = threadIdx.x & 31;
+  float scale = 0.0f;
+  double acc[kSums] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
+  if constexpr (kPolicy) scale = grad_scale_of(a, block_denominator(a, r.weight, r.rows));
+  const i64 stride = (i64)gridDim.x * kShortWarps;
+  for (i64 row = (i64)blockIdx.x * kShortWarps + (threadIdx.x >> 5); row < r.rows; row += stride) {
+    const T* lg = static_cast<const T*>(r.logits) + row * r.ld;
+    const i64 action = r.actions[row];
+    const float w = r.weight ? r.weight[row] : 1.0f;
+    bool used = w != 0.0f && action >= 0 && action < r.vocab;
+    float y[kPer], z[kPer];
+    if (used) {
+      const bool* lm = r.legal ? r.legal + row * r.ldm : nullptr;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const int c = lane + 32 * k;
+        const bool in = c < r.vocab && (!lm || lm[c]);
+        y[k] = in ? max_nan(to_float(lg[c]), kMasked) : kMasked;
+        if constexpr (kRef)
+          z[k] = in ? max_nan(to_float(static_cast<const T*>(r.ref)[row * r.ldr + c]), kMasked) : kMasked;
+      }
+    }
+    Sums v = no_sums();
+    float y_a = 0.0f;
+    if (used) {
+      float top = y[0], top_r = kMasked;
+#pragma unroll
+      for (int k = 1; k < kPer; ++k) top = max_nan(top, y[k]);
+      v.m = max_warp(top) * kLog2e;
+      if constexpr (kRef) {
+        top_r = z[0];
+#pragma unroll
+        for (int k = 1; k < kPer; ++k) top_r = max_nan(top_r, z[k]);
+        v.mr = max_warp(top_r) * kLog2e;
+      }
+      float x_a = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k)
+        if (k == static_cast<int>(action >> 5)) x_a = y[k];
+      x_a = __shfl_sync(kFull, x_a, static_cast<int>(action & 31));
+      used = !(x_a <= kMasked);
+      y_a = fmaf(x_a, kLog2e, -v.m);
+    }
+    if (used) {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        y[k] = fmaf(y[k], kLog2e, -v.m);
+        const float e = exp2_fast(y[k]);
+        v.s += e;
+        v.t = fmaf(e, y[k], v.t);
+        if constexpr (kRef) {
+          z[k] = fmaf(z[k], kLog2e, -v.mr);
+          v.sr += exp2_fast(z[k]);
+          z[k] = y[k] - z[k];
+          v.u = fmaf(e, z[k], v.u);
+        }
+      }
+      v.s = sum_warp(v.s);
+      v.t = sum_warp(v.t);
+      if constexpr (kRef) {
+        v.sr = sum_warp(v.sr);
+        v.u = sum_warp(v.u);
+      }
+    }
+    if constexpr (!kPolicy) {
+      if (lane == 0) {
+        const float log_s = used ? log2f(v.s) : INFINITY;
+        if (o.logp) o.logp[row] = used ? kLn2 * (y_a - log_s) : 0.0f;
+        if (o.entropy) o.entropy[row] = used ? kLn2 * (log_s - v.t / v.s) : 0.0f;
+        if (o.lse) o.lse[row] = make_float2(used ? v.m : 0.0f, log_s);
+        if (o.zeros) o.zeros[row] = 0.0f;
+      }
+    } else {
+      Coefs c{0.0f, 0.0f, 0.0f, 0.0f};
+      float logp = 0.0f;
+      if (used) c = policy_row<kRef>(a, row, v, y_a, w, scale, acc, logp);
+      if (a.logp && lane == 0) a.logp[row] = logp;
+      if (a.dlogits) {
+        const i64 at = row * a.ldd;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          const int j = lane + 32 * k;
+          float g = 0.0f;
+          if (used) {
+            g = fmaf(c.c1, y[k], c.c0);
+            if constexpr (kRef) g = fmaf(c.c2, z[k], g);
+            g *= exp2_fast(y[k]);
+            if (j == static_cast<int>(action)) g += c.hot;
+          }
+          if (j < r.vocab) store_one(a.dlogits, a.dtype, at + j, g);
+        }
+        for (int j = r.vocab + lane; j < a.width; j += 32) store_one(a.dlogits, a.dtype, at + j, 0.0f);
+      }
+    }
+  }
+  if constexpr (kPolicy) store_partial(a, acc);
+}
+
+// ---- long rows: a block, or a cluster of blocks, per row -----------------------------------
+//
+// A row is cut into 16-byte vectors (a head of up to one vector to its first 16-byte
+// boundary, and a tail, entry by entry).  A thread looks at the same vectors twice: once
+// for its sums, with a maximum of its own that rescales them when it grows, once for the
+// gradient.  Between the two the warps' sums are joined through shared memory, and the
+// blocks' of a cluster through distributed shared memory, in the same order everywhere.
+
+constexpr int kLongThreads = 512;
+constexpr int kUnroll = 4;  // vectors of a thread in flight
+
+template <typename T>
+constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+
+// Up to kN flags of `legal`, as bits.
+template <int kN>
+__device__ __forceinline__ unsigned legal_bits(const bool* lm) {
+  unsigned bits = 0;
+  if ((reinterpret_cast<uintptr_t>(lm) & (kN - 1)) == 0) {
+    if constexpr (kN == 8) {
+      const uint2 q = *reinterpret_cast<const uint2*>(lm);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bits |= ((q.x >> (8 * e)) & 1u) << e | ((q.y >> (8 * e)) & 1u) << (e + 4);
+    } else {
+      const uint32_t q = *reinterpret_cast<const uint32_t*>(lm);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bits |= ((q >> (8 * e)) & 1u) << e;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) bits |= static_cast<unsigned>(lm[e]) << e;
+  }
+  return bits;
+}
+
+// The row's part that a block takes, and its vectors.
+template <typename T>
+struct Part {
+  const T* x;         // the row
+  const T* z;         // the reference's row, or null
+  const bool* lm;     // the row's flags, or null
+  int head, vectors;  // entries before the first whole vector; whole vectors
+  int first, last;    // this block's vectors
+  int vocab;
+  bool z_wide;        // the reference's vectors are aligned as the row's are
+
+  __device__ __forceinline__ void load(int v, float (&f)[kVec<T>]) const {
+    const int c = head + v * kVec<T>;
+    unpack(__ldg(reinterpret_cast<const uint4*>(x + c)), f);
+    mask(c, f);
+  }
+  __device__ __forceinline__ void load_ref(int v, float (&f)[kVec<T>]) const {
+    const int c = head + v * kVec<T>;
+    if (z_wide) {
+      unpack(__ldg(reinterpret_cast<const uint4*>(z + c)), f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec<T>; ++e) f[e] = to_float(z[c + e]);
+    }
+    mask(c, f);
+  }
+  __device__ __forceinline__ void mask(int c, float (&f)[kVec<T>]) const {
+#pragma unroll
+    for (int e = 0; e < kVec<T>; ++e) f[e] = max_nan(f[e], kMasked);
+    if (lm) {
+      const unsigned bits = legal_bits<kVec<T>>(lm + c);
+#pragma unroll
+      for (int e = 0; e < kVec<T>; ++e)
+        if (!(bits >> e & 1u)) f[e] = kMasked;
+    }
+  }
+  static __device__ __forceinline__ void unpack(const uint4 raw, float (&f)[kVec<T>]) {
+    const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int e = 0; e < kVec<T>; ++e) f[e] = to_float(t[e]);
+  }
+  // Entry number i of those outside the vectors, or -1: rank 0 takes them all.
+  __device__ __forceinline__ int loose(int i) const {
+    const int tail = head + vectors * kVec<T>;
+    const int c = i < head ? i : tail + i - head;
+    return c < vocab ? c : -1;
+  }
+  __device__ __forceinline__ float one(const T* p, int c) const {
+    return lm && !lm[c] ? kMasked : max_nan(to_float(p[c]), kMasked);
+  }
+};
+
+// Adds kN entries to a thread's running sums.
+template <bool kRef, int kN>
+__device__ __forceinline__ void add(Sums& v, const float (&x)[kN], const float (&z)[kN]) {
+  float top = x[0];
+#pragma unroll
+  for (int e = 1; e < kN; ++e) top = max_nan(top, x[e]);
+  top *= kLog2e;
+  if (!(top <= v.m)) {  // also for NaN
+    const float d = v.m - top, f = exp2_fast(d);
+    v.t = f * (v.t + d * v.s);
+    if constexpr (kRef) v.u = f * (v.u + d * v.s);
+    v.s *= f;
+    v.m = top;
+  }
+  float zz[kN];
+  if constexpr (kRef) {
+    float top_r = z[0];
+#pragma unroll
+    for (int e = 1; e < kN; ++e) top_r = max_nan(top_r, z[e]);
+    top_r *= kLog2e;
+    if (!(top_r <= v.mr)) {
+      const float d = v.mr - top_r;
+      v.u -= d * v.s;
+      v.sr *= exp2_fast(d);
+      v.mr = top_r;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kN; ++e) {
+    const float y = fmaf(x[e], kLog2e, -v.m), p = exp2_fast(y);
+    v.s += p;
+    v.t = fmaf(p, y, v.t);
+    if constexpr (kRef) {
+      zz[e] = fmaf(z[e], kLog2e, -v.mr);
+      v.sr += exp2_fast(zz[e]);
+      v.u = fmaf(p, y - zz[e], v.u);
+    }
+  }
+}
+
+template <typename T, bool kRef, bool kPolicy>
+__global__ void __launch_bounds__(kLongThreads) long_rows_kernel(const Rows r, const Score o, const Policy a) {
+  constexpr int kN = kVec<T>;
+  __shared__ Sums warp_sums[2][kLongThreads / 32];
+  __shared__ Sums block_sums[2];
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int parts = cluster.num_blocks(), rank = cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x / 32;
+  float scale = 0.0f;
+  double acc[kSums] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
+  if constexpr (kPolicy) scale = grad_scale_of(a, block_denominator(a, r.weight, r.rows));
+  int buffer = 0;
+  for (i64 row = blockIdx.x / parts; row < r.rows; row += gridDim.x / parts) {
+    Part<T> p;
+    p.x = static_cast<const T*>(r.logits) + row * r.ld;
+    p.z = kRef ? static_cast<const T*>(r.ref) + row * r.ldr : nullptr;
+    p.lm = r.legal ? r.legal + row * r.ldm : nullptr;
+    p.vocab = r.vocab;
+    p.head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p.x) & 15)) & 15) / static_cast<int>(sizeof(T));
+    if (p.head > r.vocab) p.head = r.vocab;
+    p.vectors = (r.vocab - p.head) / kN;
+    p.z_wide = kRef && (reinterpret_cast<uintptr_t>(p.z + p.head) & 15) == 0;
+    const int each = (p.vectors + parts - 1) / parts;
+    p.first = each * rank < p.vectors ? each * rank : p.vectors;
+    p.last = p.first + each < p.vectors ? p.first + each : p.vectors;
+    const int n_loose = rank == 0 ? r.vocab - p.vectors * kN : 0;
+    const i64 action = r.actions[row];
+    const float w = r.weight ? r.weight[row] : 1.0f;
+    bool used = w != 0.0f && action >= 0 && action < r.vocab;
+    float x_a = kMasked;
+    if (used) x_a = p.one(p.x, static_cast<int>(action));
+    used = used && !(x_a <= kMasked);
+    Sums v = no_sums();
+    if (used) {
+      for (int i = p.first + tid; i < p.last; i += kUnroll * blockDim.x) {
+        float x[kUnroll][kN], z[kUnroll][kN];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k)
+          if (i + k * (int)blockDim.x < p.last) {
+            p.load(i + k * blockDim.x, x[k]);
+            if constexpr (kRef) p.load_ref(i + k * blockDim.x, z[k]);
+          }
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k)
+          if (i + k * (int)blockDim.x < p.last) add<kRef>(v, x[k], z[k]);
+      }
+      if (tid < n_loose) {
+        const int c = p.loose(tid);
+        const float x[1] = {p.one(p.x, c)};
+        const float z[1] = {kRef ? p.one(p.z, c) : 0.0f};
+        add<kRef>(v, x, z);
+      }
+      v = join_warp<kRef>(v);
+      if (lane == 0) warp_sums[buffer][tid >> 5] = v;
+      __syncthreads();
+      v = join_warp<kRef>(lane < warps ? warp_sums[buffer][lane] : no_sums());
+      if (parts > 1) {
+        if (tid == 0) block_sums[buffer] = v;
+        cluster.sync();
+        v = no_sums();
+        for (int q = 0; q < parts; ++q) v = join<kRef>(v, *cluster.map_shared_rank(&block_sums[buffer], q));
+      }
+      buffer ^= 1;
+    }
+    const float y_a = fmaf(x_a, kLog2e, -v.m);
+    if constexpr (!kPolicy) {
+      if (tid == 0 && rank == 0) {
+        const float log_s = used ? log2f(v.s) : INFINITY;
+        if (o.logp) o.logp[row] = used ? kLn2 * (y_a - log_s) : 0.0f;
+        if (o.entropy) o.entropy[row] = used ? kLn2 * (log_s - v.t / v.s) : 0.0f;
+        if (o.lse) o.lse[row] = make_float2(used ? v.m : 0.0f, log_s);
+        if (o.zeros) o.zeros[row] = 0.0f;
+      }
+    } else {
+      Coefs c{0.0f, 0.0f, 0.0f, 0.0f};
+      float logp = 0.0f;
+      // Every thread has the coefficients; one of the row's counts its sums.
+      double mine[kSums] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
+      if (used) c = policy_row<kRef>(a, row, v, y_a, w, scale, mine, logp);
+      if (tid == 0 && rank == 0) {
+        if (a.logp) a.logp[row] = logp;
+#pragma unroll
+        for (int k = 0; k < kSums; ++k) acc[k] += mine[k];
+      }
+      if (a.dlogits) {
+        const i64 at = row * a.ldd;
+        const uintptr_t to = reinterpret_cast<uintptr_t>(a.dlogits) + (at + p.head) * type_bytes(a.dtype);
+        const int bytes = kN * type_bytes(a.dtype);
+        const bool wide = to % (bytes < 16 ? bytes : 16) == 0;
+        const int hot = static_cast<int>(action);
+        for (int i = p.first + tid; i < p.last; i += kUnroll * blockDim.x) {
+          float x[kUnroll][kN], z[kUnroll][kN];
+#pragma unroll
+          for (int k = 0; k < kUnroll; ++k)
+            if (used && i + k * (int)blockDim.x < p.last) {
+              p.load(i + k * blockDim.x, x[k]);
+              if constexpr (kRef) p.load_ref(i + k * blockDim.x, z[k]);
+            }
+#pragma unroll
+          for (int k = 0; k < kUnroll; ++k) {
+            if (i + k * (int)blockDim.x >= p.last) break;
+            const int at_c = p.head + (i + k * blockDim.x) * kN;
+            float g[kN];
+#pragma unroll
+            for (int e = 0; e < kN; ++e) {
+              const float y = fmaf(x[k][e], kLog2e, -v.m);
+              g[e] = fmaf(c.c1, y, c.c0);
+              if constexpr (kRef) g[e] = fmaf(c.c2, y - fmaf(z[k][e], kLog2e, -v.mr), g[e]);
+              g[e] = used ? g[e] * exp2_fast(y) : 0.0f;
+            }
+            if (used && hot >= at_c && hot < at_c + kN)
+#pragma unroll
+              for (int e = 0; e < kN; ++e)
+                if (hot == at_c + e) g[e] += c.hot;
+            store_grad<kN>(a.dlogits, a.dtype, at + at_c, g, wide);
+          }
+        }
+        if (tid < n_loose) {
+          const int j = p.loose(tid);
+          float g = 0.0f;
+          if (used) {
+            const float y = fmaf(p.one(p.x, j), kLog2e, -v.m);
+            g = fmaf(c.c1, y, c.c0);
+            if constexpr (kRef) g = fmaf(c.c2, y - fmaf(p.one(p.z, j), kLog2e, -v.mr), g);
+            g *= exp2_fast(y);
+            if (j == hot) g += c.hot;
+          }
+          store_one(a.dlogits, a.dtype, at + j, g);
+        }
+        if (rank == 0)
+          for (int j = r.vocab + tid; j < a.width; j += blockDim.x) store_one(a.dlogits, a.dtype, at + j, 0.0f);
+      }
+    }
+  }
+  if (parts > 1) cluster.sync();  // no block leaves while another may read its sums
+  if constexpr (kPolicy) store_partial(a, acc);
+}
+
+// ---- the means of policy_loss ---------------------------------------------------------------
+
+constexpr int kWeightBlock = 4096;  // weights a block adds up
+
+__global__ void __launch_bounds__(512) weight_sums_kernel(const float* weight, i64 rows, i64 per_block,
+                                                          double* sums) {
+  __shared__ double part[16];
+  const i64 first = blockIdx.x * per_block;
+  const i64 last = first + per_block < rows ? first + per_block : rows;
+  double t = 0.0;
+  for (i64 i = first + threadIdx.x; i < last; i += blockDim.x) t += weight[i];
+  t = sum_warp(t);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    t = 0.0;
+    for (int k = 0; k < 16; ++k) t += part[k];
+    sums[blockIdx.x] = t;
+  }
+}
+
+__global__ void __launch_bounds__(32 * kSums) policy_means_kernel(const Policy a, const float* weight, i64 rows,
+                                                                  int blocks, float* stats, float* loss) {
+  __shared__ double means[kSums];
+  const double d = block_denominator(a, weight, rows);
+  const int k = threadIdx.x >> 5;
+  double t = 0.0;
+  for (int b = threadIdx.x & 31; b < blocks; b += 32) t += a.partial[(i64)b * kSums + k];
+  t = sum_warp(t);
+  if ((threadIdx.x & 31) == 0) means[k] = d == 0.0 ? 0.0 : t / d;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    stats[0] = static_cast<float>(means[0] - a.entropy_coef * means[1] + a.kl_coef * means[2]);
+    if (loss) *loss = stats[0];
+    for (int q = 0; q < kSums; ++q) stats[q + 1] = static_cast<float>(means[q]);
+    stats[kStats] = static_cast<float>(d);
+  }
+}
+
+// ---- action_logp's backward --------------------------------------------------------------------
+//
+// With a row's maximum and sum kept by the forward nothing is left to reduce: a warp
+// takes kSpan entries of a row (or a whole shorter row) and writes their gradients
+//   d_j = d_logp ([j = a] - p_j) - d_entropy p_j (log p_j + H),  times *scale.
+
+constexpr int kSpan = 2048;
+constexpr int kBackWarps = 8;
+
+struct Back {
+  const float2* lse;
+  const float* entropy;    // or null (no d_entropy)
+  const float* d_logp;     // or null: 0
+  const float* d_entropy;  // or null: 0
+  const float* scale;      // device scalar, or null
+  void* dlogits;
+  i64 ldd;
+  int dtype;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kBackWarps) logp_backward_kernel(const Rows r, const Back b, int spans) {
+  constexpr int kN = kVec<T>;
+  const int lane = threadIdx.x & 31;
+  const i64 unit = (i64)blockIdx.x * kBackWarps + (threadIdx.x >> 5);
+  const i64 row = unit / spans;
+  if (row >= r.rows) return;
+  const int c0 = static_cast<int>(unit - row * spans) * kSpan;
+  const int c1 = c0 + kSpan < r.vocab ? c0 + kSpan : r.vocab;
+  const float2 lse = b.lse[row];
+  const float scale = b.scale ? *b.scale : 1.0f;
+  const float g1 = b.d_logp ? b.d_logp[row] * scale : 0.0f;
+  const float g2 = b.d_entropy ? b.d_entropy[row] * scale : 0.0f;
+  const i64 at = row * b.ldd;
+  // A row that does not count, and one whose gradient is 0, is not read.
+  if (lse.y == INFINITY || (g1 == 0.0f && g2 == 0.0f)) {
+    for (int c = c0 + lane; c < c1; c += 32) store_one(b.dlogits, b.dtype, at + c, 0.0f);
+    return;
+  }
+  const float inv_s = exp2_fast(-lse.y);
+  Coefs k;
+  k.hot = g1;
+  k.c0 = inv_s * (-g1 - g2 * ((b.d_entropy ? b.entropy[row] : 0.0f) - kLn2 * lse.y));
+  k.c1 = inv_s * (-g2 * kLn2);
+  Part<T> p;
+  p.x = static_cast<const T*>(r.logits) + row * r.ld + c0;
+  p.z = nullptr;
+  p.lm = r.legal ? r.legal + row * r.ldm + c0 : nullptr;
+  p.vocab = c1 - c0;
+  p.head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p.x) & 15)) & 15) / static_cast<int>(sizeof(T));
+  if (p.head > p.vocab) p.head = p.vocab;
+  p.vectors = (p.vocab - p.head) / kN;
+  const i64 hot = r.actions[row] - c0;
+  const uintptr_t to = reinterpret_cast<uintptr_t>(b.dlogits) + (at + c0 + p.head) * type_bytes(b.dtype);
+  const int bytes = kN * type_bytes(b.dtype);
+  const bool wide = to % (bytes < 16 ? bytes : 16) == 0;
+  for (int i = lane; i < p.vectors; i += kUnroll * 32) {
+    float x[kUnroll][kN];
+#pragma unroll
+    for (int q = 0; q < kUnroll; ++q)
+      if (i + 32 * q < p.vectors) p.load(i + 32 * q, x[q]);
+#pragma unroll
+    for (int q = 0; q < kUnroll; ++q) {
+      if (i + 32 * q >= p.vectors) break;
+      const int c = p.head + (i + 32 * q) * kN;
+      float g[kN];
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const float y = fmaf(x[q][e], kLog2e, -lse.x);
+        g[e] = fmaf(k.c1, y, k.c0) * exp2_fast(y);
+        if (hot == c + e) g[e] += k.hot;
+      }
+      store_grad<kN>(b.dlogits, b.dtype, at + c0 + c, g, wide);
+    }
+  }
+  for (int i = lane; i < p.vocab - p.vectors * kN; i += 32) {
+    const int c = p.loose(i);
+    const float y = fmaf(p.one(p.x, c), kLog2e, -lse.x);
+    float g = fmaf(k.c1, y, k.c0) * exp2_fast(y);
+    if (hot == c) g += k.hot;
+    store_one(b.dlogits, b.dtype, at + c0 + c, g);
+  }
+}
+
+// ---- the preference loss over pairs --------------------------------------------------------------
+//
+// Sequence j holds rows offsets[j] .. offsets[j + 1] - 1 (bounds outside the rows are
+// brought inside); pair i prefers sequence 2 i to 2 i + 1.  kLanes threads take a pair:
+// the two scores in 64 bits, the margin, then the rows' d loss / d logp.
+
+struct Pairs {
+  const float* logp;
+  const float* ref_logp;
+  const float* weight;  // or null
+  const float2* lse;    // which rows count
+  const i64* offsets;
+  i64 pairs, rows;
+  float beta, smoothing;
+  bool average;
+  float* margin;    // [pairs]
+  float* seq_logp;  // [2 pairs]
+  float* d_logp;    // [rows], or null
+  double* partial;  // [blocks][2]: their sums, of a launch of more
+  float* means[2];  // the loss and the share of margins above 0, written here by a launch of one block
+};
+
+constexpr int kPairThreads = 1024;
+
+template <int kLanes>
+__global__ void __launch_bounds__(kPairThreads) pairs_kernel(const Pairs a) {
+  constexpr int kWarps = kLanes / 32, kGroups = kPairThreads / kLanes;
+  __shared__ double part[kPairThreads / 32][3];
+  __shared__ double block_sums[kPairThreads / 32][2];
+  const int tid = threadIdx.x, lane = tid % kLanes, group = tid / kLanes;
+  double loss = 0.0, above = 0.0;
+  const i64 stride = (i64)gridDim.x * kGroups;
+  // Every group goes round as often as the block's first one, so that the barriers meet.
+  for (i64 base = (i64)blockIdx.x * kGroups; base < a.pairs; base += stride) {
+    const i64 pair = base + group;
+    const bool real = pair < a.pairs;
+    i64 from[2] = {0, 0}, to[2] = {0, 0};
+    double score[2], total[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (real) {
+        from[h] = a.offsets[2 * pair + h];
+        to[h] = a.offsets[2 * pair + h + 1];
+        from[h] = from[h] < 0 ? 0 : from[h];
+        to[h] = to[h] > a.rows ? a.rows : to[h];
+      }
+      double sums[3] = {0.0, 0.0, 0.0};  // w (logp - ref), w logp, w
+      for (i64 t = from[h] + lane; t < to[h]; t += kLanes) {
+        if (a.lse[t].y == INFINITY) continue;
+        const double w = a.weight ? a.weight[t] : 1.0f;
+        sums[0] += w * (static_cast<double>(a.logp[t]) - a.ref_logp[t]);
+        sums[1] += w * a.logp[t];
+        sums[2] += w;
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) sums[k] = sum_warp(sums[k]);
+      if constexpr (kWarps > 1) {
+        __syncthreads();
+        if ((tid & 31) == 0)
+#pragma unroll
+          for (int k = 0; k < 3; ++k) part[tid >> 5][k] = sums[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          sums[k] = 0.0;
+          for (int q = 0; q < kWarps; ++q) sums[k] += part[group * kWarps + q][k];
+        }
+      }
+      const double n = a.average && sums[2] != 0.0 ? 1.0 / sums[2] : 1.0;
+      score[h] = sums[0] * n;
+      total[h] = n;
+      if (real && lane == 0) a.seq_logp[2 * pair + h] = static_cast<float>(sums[1] * n);
+    }
+    if (!real) continue;
+    const double m = a.beta * (score[0] - score[1]);
+    // -log sigmoid(m) and its two slopes, in 64 bits: one pair, one evaluation.
+    const double soft = log1p(exp(-fabs(m)));
+    const double lose = soft + (m < 0.0 ? -m : 0.0), win = soft + (m > 0.0 ? m : 0.0);
+    if (lane == 0) {
+      a.margin[pair] = static_cast<float>(m);
+      loss += (1.0 - a.smoothing) * lose + a.smoothing * win;
+      above += m > 0.0 ? 1.0 : 0.0;
+    }
+    if (a.d_logp) {
+      const double up = 1.0 / (1.0 + exp(-m)), down = 1.0 / (1.0 + exp(m));
+      const double slope = a.beta * (a.smoothing * up - (1.0 - a.smoothing) * down) / a.pairs;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float d = static_cast<float>((h ? -slope : slope) * total[h]);
+        for (i64 t = from[h] + lane; t < to[h]; t += kLanes) a.d_logp[t] = a.weight ? d * a.weight[t] : d;
+      }
+    }
+  }
+  // The groups' sums are in lane 0 of their first warps.
+  if ((tid & 31) == 0) {
+    block_sums[tid >> 5][0] = loss;
+    block_sums[tid >> 5][1] = above;
+  }
+  __syncthreads();
+  if (tid < 2) {
+    double t = 0.0;
+    for (int q = 0; q < kPairThreads / 32; ++q) t += block_sums[q][tid];
+    if (gridDim.x == 1) *a.means[tid] = static_cast<float>(t / a.pairs);
+    else a.partial[(i64)blockIdx.x * 2 + tid] = t;
+  }
+}
+
+__global__ void pair_means_kernel(const double* partial, int blocks, i64 pairs, float* loss, float* above) {
+  const int k = threadIdx.x >> 5;
+  double t = 0.0;
+  for (int b = threadIdx.x & 31; b < blocks; b += 32) t += partial[2 * b + k];
+  t = sum_warp(t);
+  if ((threadIdx.x & 31) == 0) *(k ? above : loss) = static_cast<float>(t / pairs);
+}
+
+// ---- host ------------------------------------------------------------------------------------
+
+inline int launch_status() {
+  return cudaGetLastError() == cudaSuccess ? CUGO_B200_OK : CUGO_B200_ERR_LAUNCH;
+}
+
+inline bool type_ok(int t) { return t == kFp32 || t == kBf16 || t == kFp16; }
+
+inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// A matrix of `rows` rows of `cols` entries: pointer, stride and alignment.
+inline int check_matrix(const void* p, i64 ld, i64 rows, i64 cols, int bytes) {
+  if (rows > 0 && !p) return CUGO_B200_ERR_ARG;
+  if (ld < cols && rows > 1) return CUGO_B200_ERR_ARG;
+  return aligned(p, bytes) ? CUGO_B200_OK : CUGO_B200_ERR_ALIGN;
+}
+
+int check_rows(const Rows& r, int dtype) {
+  if (r.rows < 0 || r.vocab < 1 || !type_ok(dtype)) return CUGO_B200_ERR_ARG;
+  if (r.rows > 0 && !r.actions) return CUGO_B200_ERR_ARG;
+  if (int rc = check_matrix(r.logits, r.ld, r.rows, r.vocab, type_bytes(dtype))) return rc;
+  if (r.ref)
+    if (int rc = check_matrix(r.ref, r.ldr, r.rows, r.vocab, type_bytes(dtype))) return rc;
+  if (r.legal && r.ldm != 0)  // 0: one mask for all rows
+    if (int rc = check_matrix(r.legal, r.ldm, r.rows, r.vocab, 1)) return rc;
+  return CUGO_B200_OK;
+}
+
+constexpr int kShortMost = 1024;  // entries of a short row
+
+// How a launch goes over the rows.
+struct Plan {
+  bool is_short;
+  int threads, blocks, parts;
+};
+
+Plan plan_of(i64 rows, int vocab) {
+  Plan p{};
+  p.is_short = vocab <= kShortMost;
+  p.parts = 1;
+  if (p.is_short) {
+    p.threads = 32 * kShortWarps;
+    const i64 want = (rows + kShortWarps - 1) / kShortWarps;
+    p.blocks = static_cast<int>(want < 8 * kSms ? want : 8 * kSms);
+    return p;
+  }
+  p.threads = vocab <= 4096 ? 128 : vocab <= 16384 ? 256 : kLongThreads;
+  // Few rows: a row over up to 8 blocks, each with at least 4,096 entries.
+  while (p.parts < 8 && rows * p.parts < kSms && vocab / (2 * p.parts) >= 4096) p.parts *= 2;
+  const i64 most = static_cast<i64>(kSms) * (2048 / p.threads) / p.parts;
+  p.blocks = static_cast<int>(rows < most ? rows : most) * p.parts;
+  return p;
+}
+
+template <typename K>
+int launch_long(K kernel, const Plan& p, const Rows& r, const Score& o, const Policy& a, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.blocks);
+  cfg.blockDim = dim3(p.threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, r, o, a) == cudaSuccess ? CUGO_B200_OK : CUGO_B200_ERR_LAUNCH;
+}
+
+template <typename T, bool kRef, bool kPolicy>
+int launch_rows(const Plan& p, const Rows& r, const Score& o, const Policy& a, cudaStream_t stream) {
+  if (!p.is_short) return launch_long(long_rows_kernel<T, kRef, kPolicy>, p, r, o, a, stream);
+  const int per = (r.vocab + 31) / 32;
+#define CUGO_SHORT(n)                                                                            \
+  if (per <= n) {                                                                                \
+    short_rows_kernel<T, n, kRef, kPolicy><<<p.blocks, p.threads, 0, stream>>>(r, o, a);        \
+    return launch_status();                                                                      \
+  }
+  CUGO_SHORT(2)
+  CUGO_SHORT(6)
+  CUGO_SHORT(12)
+  CUGO_SHORT(32)
+#undef CUGO_SHORT
+  return CUGO_B200_ERR_ARG;
+}
+
+template <bool kRef, bool kPolicy>
+int launch_typed(int dtype, const Plan& p, const Rows& r, const Score& o, const Policy& a, cudaStream_t stream) {
+  if (dtype == kFp32) return launch_rows<float, kRef, kPolicy>(p, r, o, a, stream);
+  if (dtype == kBf16) return launch_rows<__nv_bfloat16, kRef, kPolicy>(p, r, o, a, stream);
+  return launch_rows<__half, kRef, kPolicy>(p, r, o, a, stream);
+}
+
+inline i64 weight_blocks(i64 rows) {
+  const i64 b = (rows + kWeightBlock - 1) / kWeightBlock;
+  return b < kSms ? b : kSms;
+}
+
+constexpr int kMostBlocks = 16 * kSms;
+
+}  // namespace
+
+extern "C" {
+
+int cugo_b200_action_logp(const void* logits, int64_t ld, int32_t dtype, const bool* legal, int64_t ldm,
+                          const int64_t* actions, const float* weight, int64_t rows, int64_t vocab,
+                          float* logp, float* entropy, float* lse, float* zeros, cudaStream_t stream) {
+  if (vocab < 1 || vocab > INT32_MAX) return CUGO_B200_ERR_ARG;
+  const Rows r{logits, ld, nullptr, 0, legal, ldm, actions, weight, rows, static_cast<int>(vocab)};
+  if (int rc = check_rows(r, dtype)) return rc;
+  if (rows > 0 && !logp && !entropy && !lse) return CUGO_B200_ERR_ARG;
+  if (!aligned(lse, 8)) return CUGO_B200_ERR_ALIGN;
+  if (rows == 0) return CUGO_B200_OK;
+  const Score o{logp, entropy, reinterpret_cast<float2*>(lse), zeros};
+  return launch_typed<false, false>(dtype, plan_of(rows, r.vocab), r, o, Policy{}, stream);
+}
+
+int cugo_b200_action_logp_backward(const void* logits, int64_t ld, int32_t dtype, const bool* legal,
+                                   int64_t ldm, const int64_t* actions, const float* lse,
+                                   const float* entropy, const float* d_logp, const float* d_entropy,
+                                   const float* scale, int64_t rows, int64_t vocab, void* dlogits,
+                                   int64_t ldd, int32_t grad_dtype, cudaStream_t stream) {
+  if (vocab < 1 || vocab > INT32_MAX) return CUGO_B200_ERR_ARG;
+  const Rows r{logits, ld, nullptr, 0, legal, ldm, actions, nullptr, rows, static_cast<int>(vocab)};
+  if (int rc = check_rows(r, dtype)) return rc;
+  if (!type_ok(grad_dtype) || (rows > 0 && (!lse || (d_entropy && !entropy)))) return CUGO_B200_ERR_ARG;
+  if (int rc = check_matrix(dlogits, ldd, rows, vocab, type_bytes(grad_dtype))) return rc;
+  if (!aligned(lse, 8)) return CUGO_B200_ERR_ALIGN;
+  if (rows == 0) return CUGO_B200_OK;
+  const Back b{reinterpret_cast<const float2*>(lse), entropy, d_logp, d_entropy, scale, dlogits, ldd, grad_dtype};
+  const int spans = static_cast<int>((vocab + kSpan - 1) / kSpan);
+  const i64 blocks = (rows * spans + kBackWarps - 1) / kBackWarps;
+  if (blocks > INT32_MAX) return CUGO_B200_ERR_CAPACITY;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (dtype == kFp32) logp_backward_kernel<float><<<grid, 32 * kBackWarps, 0, stream>>>(r, b, spans);
+  else if (dtype == kBf16) logp_backward_kernel<__nv_bfloat16><<<grid, 32 * kBackWarps, 0, stream>>>(r, b, spans);
+  else logp_backward_kernel<__half><<<grid, 32 * kBackWarps, 0, stream>>>(r, b, spans);
+  return launch_status();
+}
+
+int64_t cugo_b200_policy_loss_scratch_bytes(int64_t rows) {
+  if (rows <= 0) return 0;
+  const int64_t blocks = rows < kMostBlocks ? rows * 8 : kMostBlocks;
+  return (kSms + (blocks < kMostBlocks ? blocks : kMostBlocks) * kSums) * static_cast<int64_t>(sizeof(double));
+}
+
+int cugo_b200_policy_loss(const void* logits, int64_t ld, int32_t dtype, const void* ref_logits, int64_t ldr,
+                          const bool* legal, int64_t ldm, const int64_t* actions, const float* logp_old,
+                          const float* adv, const float* weight, const float* ref_logp, int64_t rows,
+                          int64_t vocab, float clip_low, float clip_high, float kl_coef, float entropy_coef,
+                          float denominator, const float* denominator_dev, float grad_scale,
+                          const float* grad_scale_dev, void* dlogits, int64_t ldd, int32_t grad_dtype,
+                          int64_t width, float* logp, float* stats, float* loss, void* scratch,
+                          int64_t scratch_bytes, cudaStream_t stream) {
+  if (vocab < 1 || vocab > INT32_MAX || width > INT32_MAX) return CUGO_B200_ERR_ARG;
+  const Rows r{logits, ld, ref_logits, ldr, legal, ldm, actions, weight, rows, static_cast<int>(vocab)};
+  if (int rc = check_rows(r, dtype)) return rc;
+  if ((!stats && !dlogits) || (loss && !stats) || (rows > 0 && (!logp_old || !adv)) || (ref_logits && ref_logp))
+    return CUGO_B200_ERR_ARG;
+  if (!(clip_low >= 0.0f) || !(clip_high >= 0.0f)) return CUGO_B200_ERR_ARG;
+  if (dlogits) {
+    if (!type_ok(grad_dtype) || width < vocab) return CUGO_B200_ERR_ARG;
+    if (int rc = check_matrix(dlogits, ldd, rows, width, type_bytes(grad_dtype))) return rc;
+  }
+  if (!aligned(scratch, 8)) return CUGO_B200_ERR_ALIGN;
+  if (rows == 0) {
+    if (stats && cudaMemsetAsync(stats, 0, (kStats + 1) * sizeof(float), stream) != cudaSuccess)
+      return CUGO_B200_ERR_LAUNCH;
+    if (loss && cudaMemsetAsync(loss, 0, sizeof(float), stream) != cudaSuccess) return CUGO_B200_ERR_LAUNCH;
+    return CUGO_B200_OK;
+  }
+  if (!scratch || scratch_bytes < cugo_b200_policy_loss_scratch_bytes(rows)) return CUGO_B200_ERR_CAPACITY;
+  double* sums = static_cast<double*>(scratch);
+  Policy a{};
+  a.logp_old = logp_old;
+  a.adv = adv;
+  a.ref_logp = ref_logp;
+  a.low = 1.0f - clip_low;
+  a.high = 1.0f + clip_high;
+  a.kl_coef = kl_coef;
+  a.entropy_coef = entropy_coef;
+  a.denominator = denominator;
+  a.denominator_dev = denominator_dev;
+  a.grad_scale = grad_scale;
+  a.grad_scale_dev = grad_scale_dev;
+  a.dlogits = dlogits;
+  a.ldd = ldd;
+  a.dtype = grad_dtype;
+  a.width = static_cast<int>(width);
+  a.logp = logp;
+  a.partial = stats ? sums + kSms : nullptr;
+  if (weight && denominator == 0.0f && !denominator_dev && rows > kWeightBlock) {
+    const i64 blocks = weight_blocks(rows);
+    weight_sums_kernel<<<static_cast<unsigned>(blocks), 512, 0, stream>>>(weight, rows, (rows + blocks - 1) / blocks,
+                                                                         sums);
+    if (int rc = launch_status()) return rc;
+    a.weight_sums = sums;
+    a.n_weight_sums = static_cast<int>(blocks);
+  }
+  const Plan p = plan_of(rows, r.vocab);
+  const int rc = ref_logits ? launch_typed<true, true>(dtype, p, r, Score{}, a, stream)
+                            : launch_typed<false, true>(dtype, p, r, Score{}, a, stream);
+  if (rc || !stats) return rc;
+  policy_means_kernel<<<1, 32 * kSums, 0, stream>>>(a, weight, rows, p.blocks, stats, loss);
+  return launch_status();
+}
+
+int64_t cugo_b200_preference_pairs_scratch_bytes(int64_t pairs) {
+  return pairs > 0 ? 2 * kSms * static_cast<int64_t>(sizeof(double)) : 0;
+}
+
+int cugo_b200_preference_pairs(const float* logp, const float* ref_logp, const float* weight, const float* lse,
+                               const int64_t* offsets, int64_t pairs, int64_t rows, float beta, float smoothing,
+                               int32_t average, float* margin, float* seq_logp, float* d_logp, float* loss,
+                               float* accuracy, void* scratch, int64_t scratch_bytes, cudaStream_t stream) {
+  if (pairs < 0 || rows < 0 || !loss || !accuracy || !(smoothing >= 0.0f && smoothing <= 1.0f)) return CUGO_B200_ERR_ARG;
+  if (pairs > 0 && (!offsets || !margin || !seq_logp)) return CUGO_B200_ERR_ARG;
+  if (rows > 0 && (!logp || !ref_logp || !lse)) return CUGO_B200_ERR_ARG;
+  if (!aligned(scratch, 8) || !aligned(lse, 8)) return CUGO_B200_ERR_ALIGN;
+  if (pairs == 0)
+    return cudaMemsetAsync(loss, 0, sizeof(float), stream) == cudaSuccess &&
+                   cudaMemsetAsync(accuracy, 0, sizeof(float), stream) == cudaSuccess
+               ? CUGO_B200_OK
+               : CUGO_B200_ERR_LAUNCH;
+  if (!scratch || scratch_bytes < cugo_b200_preference_pairs_scratch_bytes(pairs)) return CUGO_B200_ERR_CAPACITY;
+  const Pairs a{logp, ref_logp, weight, reinterpret_cast<const float2*>(lse), offsets, pairs, rows, beta, smoothing,
+                average != 0, margin, seq_logp, d_logp, static_cast<double*>(scratch), {loss, accuracy}};
+  // Short sequences: a warp per pair, all in one block while they are few (one launch);
+  // long ones: a block per pair.
+  int blocks;
+  if (rows / pairs <= 256) {
+    const i64 want = (pairs + kPairThreads / 32 - 1) / (kPairThreads / 32);
+    blocks = rows <= 16384 ? 1 : static_cast<int>(want < kSms ? want : kSms);
+    pairs_kernel<32><<<blocks, kPairThreads, 0, stream>>>(a);
+  } else {
+    blocks = static_cast<int>(pairs < kSms ? pairs : kSms);
+    pairs_kernel<kPairThreads><<<blocks, kPairThreads, 0, stream>>>(a);
+  }
+  if (int rc = launch_status()) return rc;
+  if (blocks > 1) pair_means_kernel<<<1, 64, 0, stream>>>(a.partial, blocks, pairs, loss, accuracy);
+  return launch_status();
+}
+
+}  // extern "C"

@@ -1,0 +1,496 @@
+// The AdamW step over many tensors at once, with the gradients' norm clipped, and its C
+// ABI (include/cugo_b200.h).
+//
+//   c = min(1, max_norm / (|g| + 1e-6)), g = c g           (one norm over all tensors)
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+//   p = (1 - lr wd) p - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+//
+// One launch takes up to kMostTensors tensors: their pointers travel as the kernel's
+// parameters (nothing of a call is kept on the device, and a captured graph holds them
+// by value).  A block takes tiles of 2,048 elements, a warp 256 of them, a thread 8; a
+// tile finds its tensor by a search over the tensors' first tiles.
+//
+// States in 8 bits: e4m3 codes with one scale per 256 elements of a tensor, the warp's.
+// The scale is a power of two (an e8m0 byte), the smallest that keeps the block's largest
+// value at or below 448 (e4m3's largest).  Codes are rounded up or down by random bits.
+// Both belong together: m and v move by little per step (v by a thousandth), far less
+// than e4m3's steps of 1/8 to 1/16, and rounding to nearest would leave them where they
+// are; and with a scale that follows the largest value exactly, every code would be
+// re-rounded at every step, where a power of two leaves the grid in place, so that a
+// value that moved by the share f of a step is off its grid by f only, and the noise of
+// the moving average stays at about sqrt(f) steps.  A second moment above 0 never rounds
+// to 0: a step is then too short instead of unbounded.  The step itself uses m and v
+// before rounding.
+//
+// bf16 parameters are rounded by random bits too: lr times the update is mostly below
+// half of bf16's 2^-8, and to nearest nothing would move.
+//
+// The random bits of element number e (counted over the call's tensors in blocks of 256,
+// so that no two elements share one) are a 32-bit mix of e, the step and the seed: one
+// per element, 16 bits for m, 16 for v, and a product of them for p.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/cugo_b200.h"
+
+namespace {
+
+using i64 = int64_t;
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kBlock = 256;              // elements of a scale
+constexpr int kThreads = 256, kPer = 8;  // 8 warps, a scale's block each
+constexpr int kTile = kThreads * kPer;
+constexpr int kSms = 148;
+constexpr int kNormBlocks = 4 * kSms;
+constexpr int kFewTensors = 40, kMostTensors = 448;
+
+struct Tensor {
+  void* p;
+  const void* g;
+  void *m, *v;
+  uint8_t *ms, *vs;  // the scales (8-bit states)
+  i64 n;
+  i64 first_tile;    // of the launch
+  i64 first_block;   // blocks of 256 elements before this tensor in the call
+};
+
+template <int kMost>
+struct Tensors {
+  int count;
+  i64 tiles;
+  Tensor t[kMost];
+};
+
+// What the step's scalars come to, written by prepare_kernel.
+struct Scalars {
+  float clip;       // c
+  float step_size;  // lr / (1 - b1^t)
+  float keep;       // 1 - lr wd
+  float bias2;      // 1 - b2^t
+  uint32_t key;     // of the random bits
+};
+
+struct Options {
+  double lr, beta1, beta2, decay;
+  const float* lr_dev;  // or null
+  float b1, c1, b2, c2, eps, max_norm;
+  uint32_t seed;
+};
+
+// A 32-bit mixer: xor-shifts and odd products (constants found by C. Wellons' search for
+// low bias, 2018).
+__device__ __forceinline__ uint32_t mix(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0x7feb352du;
+  x ^= x >> 15;
+  x *= 0x846ca68bu;
+  return x ^ (x >> 16);
+}
+
+__device__ __forceinline__ double sum_warp(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+
+// The tensor that holds a tile: the last whose first tile is not behind it.
+template <int kMost>
+__device__ __forceinline__ int find(const Tensors<kMost>& a, i64 tile) {
+  int low = 0, high = a.count;
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (a.t[mid].first_tile <= tile) low = mid;
+    else high = mid;
+  }
+  return low;
+}
+
+__device__ __forceinline__ bool vector_ok(const void* p, unsigned bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+}
+
+// 8 consecutive values from element i, zeros from element n on.
+__device__ __forceinline__ void load8(const float* p, i64 i, i64 n, float (&f)[8]) {
+  if (i + 8 <= n && vector_ok(p, 16)) {
+    const float4 a = *reinterpret_cast<const float4*>(p + i), b = *reinterpret_cast<const float4*>(p + i + 4);
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = i + e < n ? p[i + e] : 0.0f;
+  }
+}
+
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, i64 i, i64 n, float (&f)[8]) {
+  if (i + 8 <= n && vector_ok(p, 16)) {
+    const uint4 q = *reinterpret_cast<const uint4*>(p + i);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[2 * e] = __uint_as_float(w[e] << 16);
+      f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = i + e < n ? __bfloat162float(p[i + e]) : 0.0f;
+  }
+}
+
+__device__ __forceinline__ void store8(float* p, i64 i, i64 n, const float (&f)[8]) {
+  if (i + 8 <= n && vector_ok(p, 16)) {
+    *reinterpret_cast<float4*>(p + i) = make_float4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<float4*>(p + i + 4) = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e < n) p[i + e] = f[e];
+  }
+}
+
+// The upper halves of f (rounded there already) as bf16.
+__device__ __forceinline__ void store8(__nv_bfloat16* p, i64 i, i64 n, const float (&f)[8]) {
+  if (i + 8 <= n && vector_ok(p, 16)) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = __byte_perm(__float_as_uint(f[2 * e]), __float_as_uint(f[2 * e + 1]), 0x7632);
+    *reinterpret_cast<uint4*>(p + i) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e < n) reinterpret_cast<uint16_t*>(p)[i + e] = static_cast<uint16_t>(__float_as_uint(f[e]) >> 16);
+  }
+}
+
+__device__ __forceinline__ void load_codes(const uint8_t* p, i64 i, i64 n, float scale, float (&f)[8]) {
+  uint32_t w[2] = {0, 0};
+  if (i + 8 <= n && vector_ok(p, 8)) {
+    const uint2 q = *reinterpret_cast<const uint2*>(p + i);
+    w[0] = q.x, w[1] = q.y;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e < n) w[e / 4] |= static_cast<uint32_t>(p[i + e]) << (8 * (e % 4));
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const __nv_fp8x2_storage_t two = static_cast<__nv_fp8x2_storage_t>(w[e / 2] >> (16 * (e % 2)));
+    const float2 t = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+    f[2 * e] = t.x * scale;
+    f[2 * e + 1] = t.y * scale;
+  }
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* p, i64 i, i64 n, const float (&f)[8]) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    w[e / 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(f[2 * e], f[2 * e + 1]), __NV_SATFINITE,
+                                                                __NV_E4M3))
+                << (16 * (e % 2));
+  if (i + 8 <= n && vector_ok(p, 8)) {
+    *reinterpret_cast<uint2*>(p + i) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e < n) p[i + e] = static_cast<uint8_t>(w[e / 4] >> (8 * (e % 4)));
+  }
+}
+
+// 2^(byte - 127) and its inverse, for the scale bytes 27 .. 247 that this file writes
+// (byte 0, an untouched state, counts as the smallest float that is no denormal).
+__device__ __forceinline__ float scale_of(int byte) { return __uint_as_float((byte > 0 ? byte : 1) << 23); }
+__device__ __forceinline__ float inverse_of(int byte) { return __uint_as_float((254 - byte) << 23); }
+
+// The scale of a block whose largest finite magnitude is `largest`: 448 = 1.75 x 2^8.
+__device__ __forceinline__ int scale_byte(float largest) {
+  const int bits = __float_as_int(largest);
+  const int e = (bits >> 23) - 8 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0);
+  return e < 27 ? 27 : e > 247 ? 247 : e;
+}
+
+// x (at most 448 in magnitude) rounded to e4m3's grid, up where the 16 random bits r say
+// so: below 2^-6 the steps are 2^-9, above they are 1/8 of the power of two.  Infinities
+// and NaN become NaN.
+__device__ __forceinline__ float round_e4m3(float x, uint32_t r) {
+  const float a = fabsf(x);
+  const float low = a < 0.015625f ? 0.015625f : 0.0f;
+  const uint32_t bits = (__float_as_uint(a + low) + (r << 4) + 8u) & 0xfff00000u;
+  const float q = copysignf(__uint_as_float(bits) - low, x);
+  return a <= 448.0f ? q : __uint_as_float(0x7fc00000u);
+}
+
+// The largest of a warp's finite magnitudes (as bits they order as the values do).
+__device__ __forceinline__ float warp_largest(const float (&f)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t b = __float_as_uint(f[e]) & 0x7fffffffu;
+    top = b < 0x7f800000u && b > top ? b : top;
+  }
+  return __uint_as_float(__reduce_max_sync(kFull, top));
+}
+
+__device__ __forceinline__ float sqrt_fast(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+template <typename P, typename G, bool kEight, int kMost>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Tensors<kMost> a, const Options o,
+                                                         const Scalars* scalars) {
+  const Scalars s = *scalars;
+  for (i64 tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+    const Tensor& t = a.t[find(a, tile)];
+    const i64 in = (tile - t.first_tile) * (kTile / kBlock) + (threadIdx.x >> 5);  // the warp's block
+    const i64 i = in * kBlock + (threadIdx.x & 31) * kPer;
+    if (in * kBlock >= t.n) continue;  // the whole warp
+    float p[8], g[8], m[8], v[8];
+    load8(static_cast<const P*>(t.p), i, t.n, p);
+    load8(static_cast<const G*>(t.g), i, t.n, g);
+    if constexpr (kEight) {
+      load_codes(static_cast<const uint8_t*>(t.m), i, t.n, scale_of(t.ms[in]), m);
+      load_codes(static_cast<const uint8_t*>(t.v), i, t.n, scale_of(t.vs[in]), v);
+    } else {
+      load8(static_cast<const float*>(t.m), i, t.n, m);
+      load8(static_cast<const float*>(t.v), i, t.n, v);
+    }
+    const float inv_bias2 = __frcp_rn(s.bias2);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float q = g[e] * s.clip;
+      m[e] = o.b1 * m[e] + o.c1 * q;
+      v[e] = o.b2 * v[e] + o.c2 * (q * q);
+      p[e] = p[e] * s.keep - s.step_size * __fdividef(m[e], sqrt_fast(v[e] * inv_bias2) + o.eps);
+    }
+    uint32_t r[8];
+    if constexpr (kEight || sizeof(P) == 2) {
+      const i64 number = (t.first_block + in) * kBlock + (threadIdx.x & 31) * kPer;
+      const uint32_t key = s.key + static_cast<uint32_t>(number >> 32) * 0x9e3779b9u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = mix(static_cast<uint32_t>(number + e) ^ key);
+    }
+    if constexpr (sizeof(P) == 2) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t b = __float_as_uint(p[e]);
+        // Infinities and NaN stay what they are.
+        p[e] = (b & 0x7f800000u) == 0x7f800000u ? p[e] : __uint_as_float(b + ((r[e] * 0x2c1b3c6du) >> 16));
+      }
+    }
+    store8(static_cast<P*>(t.p), i, t.n, p);
+    if constexpr (kEight) {
+      const int mb = scale_byte(warp_largest(m)), vb = scale_byte(warp_largest(v));
+      const float mi = inverse_of(mb), vi = inverse_of(vb);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        m[e] = round_e4m3(m[e] * mi, r[e] & 0xffffu);
+        const float q = round_e4m3(v[e] * vi, r[e] >> 16);
+        v[e] = v[e] > 0.0f && q == 0.0f ? 0.001953125f : q;  // 2^-9
+      }
+      store_codes(static_cast<uint8_t*>(t.m), i, t.n, m);
+      store_codes(static_cast<uint8_t*>(t.v), i, t.n, v);
+      if ((threadIdx.x & 31) == 0) {
+        t.ms[in] = static_cast<uint8_t>(mb);
+        t.vs[in] = static_cast<uint8_t>(vb);
+      }
+    } else {
+      store8(static_cast<float*>(t.m), i, t.n, m);
+      store8(static_cast<float*>(t.v), i, t.n, v);
+    }
+  }
+}
+
+// Sums of the gradients' squares: 8 in fp32 per thread and tile, from there in 64 bits.
+template <typename G, int kMost>
+__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Tensors<kMost> a, double* partial) {
+  __shared__ double part[kThreads / 32];
+  double sum = 0.0;
+  for (i64 tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+    const Tensor& t = a.t[find(a, tile)];
+    float g[8], q = 0.0f;
+    load8(static_cast<const G*>(t.g), (tile - t.first_tile) * kTile + threadIdx.x * kPer, t.n, g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q = fmaf(g[e], g[e], q);
+    sum += q;
+  }
+  sum = sum_warp(sum);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = 0.0;
+    for (int k = 0; k < kThreads / 32; ++k) sum += part[k];
+    partial[blockIdx.x] = sum;
+  }
+}
+
+// Counts the step and writes its scalars; the partial sums are added in order.
+__global__ void __launch_bounds__(kThreads) prepare_kernel(const Options o, const double* partial, int partials,
+                                                           i64* step, Scalars* scalars, float* norm) {
+  __shared__ double part[kThreads / 32];
+  double sum = 0.0;
+  for (int b = threadIdx.x; b < partials; b += kThreads) sum += partial[b];
+  sum = sum_warp(sum);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  Scalars s;
+  s.clip = 1.0f;
+  if (partials > 0) {
+    sum = 0.0;
+    for (int k = 0; k < kThreads / 32; ++k) sum += part[k];
+    const float n = static_cast<float>(sqrt(sum));
+    const float c = o.max_norm / (n + 1e-6f);
+    s.clip = c > 1.0f ? 1.0f : c;  // NaN stays NaN
+    *norm = n;
+  }
+  const i64 t = *step + 1;
+  *step = t;
+  const double lr = o.lr_dev ? static_cast<double>(*o.lr_dev) : o.lr;
+  s.step_size = static_cast<float>(lr / (1.0 - pow(o.beta1, static_cast<double>(t))));
+  s.keep = static_cast<float>(1.0 - lr * o.decay);
+  s.bias2 = static_cast<float>(1.0 - pow(o.beta2, static_cast<double>(t)));
+  s.key = mix(o.seed + static_cast<uint32_t>(t) * 0x9e3779b9u);
+  *scalars = s;
+}
+
+inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+inline int launch_status() {
+  return cudaGetLastError() == cudaSuccess ? CUGO_B200_OK : CUGO_B200_ERR_LAUNCH;
+}
+
+// The call's tensors, host arrays of `count`.
+struct Lists {
+  void* const* p;
+  const void* const* g;
+  void* const *m, *const *v, *const *ms, *const *vs;
+  const int64_t* n;
+  i64 count;
+};
+
+// Tensors first .. of the lists that fit one launch, empty ones left out; returns the
+// number of the first one that did not.
+template <int kMost>
+i64 fill(const Lists& l, i64 first, i64& blocks_before, Tensors<kMost>& a) {
+  a.count = 0;
+  a.tiles = 0;
+  i64 k = first;
+  for (; k < l.count && a.count < kMost; ++k) {
+    if (l.n[k] == 0) continue;
+    Tensor& t = a.t[a.count++];
+    t = {l.p[k], l.g[k], l.m[k], l.v[k], l.ms ? static_cast<uint8_t*>(l.ms[k]) : nullptr,
+         l.vs ? static_cast<uint8_t*>(l.vs[k]) : nullptr, l.n[k], a.tiles, blocks_before};
+    a.tiles += (l.n[k] + kTile - 1) / kTile;
+    blocks_before += (l.n[k] + kBlock - 1) / kBlock;
+  }
+  return k;
+}
+
+template <typename P, typename G, int kMost>
+int launch_sized(const Lists& l, bool eight, const Options& o, double* partial, int64_t* step, Scalars* scalars,
+                 float* norm, cudaStream_t stream) {
+  Tensors<kMost> a;
+  int partials = 0;
+  if (norm) {
+    i64 before = 0;
+    for (i64 k = 0; k < l.count;) {
+      k = fill<kMost>(l, k, before, a);
+      if (a.tiles == 0) break;
+      const int blocks = static_cast<int>(a.tiles < kNormBlocks ? a.tiles : kNormBlocks);
+      norm_kernel<G, kMost><<<blocks, kThreads, 0, stream>>>(a, partial + partials);
+      partials += blocks;
+    }
+    if (partials == 0) {  // no elements at all: a norm of 0
+      if (cudaMemsetAsync(partial, 0, sizeof(double), stream) != cudaSuccess) return CUGO_B200_ERR_LAUNCH;
+      partials = 1;
+    }
+  }
+  prepare_kernel<<<1, kThreads, 0, stream>>>(o, partial, partials, step, scalars, norm);
+  i64 before = 0;
+  for (i64 k = 0; k < l.count;) {
+    k = fill<kMost>(l, k, before, a);
+    if (a.tiles == 0) break;
+    const i64 most = static_cast<i64>(kSms) * 64;
+    const int blocks = static_cast<int>(a.tiles < most ? a.tiles : most);
+    if (eight) adamw_kernel<P, G, true, kMost><<<blocks, kThreads, 0, stream>>>(a, o, scalars);
+    else adamw_kernel<P, G, false, kMost><<<blocks, kThreads, 0, stream>>>(a, o, scalars);
+  }
+  return launch_status();
+}
+
+template <typename P, typename G>
+int launch(const Lists& l, bool eight, const Options& o, double* partial, int64_t* step, Scalars* scalars,
+           float* norm, cudaStream_t stream) {
+  // The parameters of a launch are copied to the device with it: few tensors, few bytes.
+  return l.count <= kFewTensors ? launch_sized<P, G, kFewTensors>(l, eight, o, partial, step, scalars, norm, stream)
+                                : launch_sized<P, G, kMostTensors>(l, eight, o, partial, step, scalars, norm, stream);
+}
+
+inline i64 launches_of(i64 count) { return count <= kFewTensors ? 1 : (count + kMostTensors - 1) / kMostTensors; }
+
+}  // namespace
+
+extern "C" {
+
+int64_t cugo_b200_adamw_scratch_bytes(int64_t count) {
+  if (count < 0) return 0;
+  return 64 + launches_of(count) * kNormBlocks * static_cast<int64_t>(sizeof(double));
+}
+
+int cugo_b200_adamw(int64_t count, void* const* params, const void* const* grads, void* const* exp_avgs,
+                    void* const* exp_avg_sqs, void* const* exp_avg_scales, void* const* exp_avg_sq_scales,
+                    const int64_t* sizes, int32_t param_dtype, int32_t grad_dtype, int32_t state_bits, double lr,
+                    const float* lr_dev, double beta1, double beta2, double eps, double weight_decay,
+                    double max_norm, uint32_t seed, int64_t* step, float* norm, void* scratch,
+                    int64_t scratch_bytes, cudaStream_t stream) {
+  if (count < 0 || (param_dtype != 0 && param_dtype != 1) || (grad_dtype != 0 && grad_dtype != 1) ||
+      (state_bits != 32 && state_bits != 8) || !step)
+    return CUGO_B200_ERR_ARG;
+  if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) || !(weight_decay >= 0.0) ||
+      (!lr_dev && !(lr >= 0.0)) || (norm && !(max_norm >= 0.0)))
+    return CUGO_B200_ERR_ARG;
+  if (count > 0 && (!params || !grads || !exp_avgs || !exp_avg_sqs || !sizes)) return CUGO_B200_ERR_ARG;
+  const bool eight = state_bits == 8;
+  if (eight && count > 0 && (!exp_avg_scales || !exp_avg_sq_scales)) return CUGO_B200_ERR_ARG;
+  const int p_bytes = param_dtype == 0 ? 4 : 2, g_bytes = grad_dtype == 0 ? 4 : 2;
+  for (int64_t k = 0; k < count; ++k) {
+    if (sizes[k] < 0) return CUGO_B200_ERR_ARG;
+    if (sizes[k] == 0) continue;
+    if (!params[k] || !grads[k] || !exp_avgs[k] || !exp_avg_sqs[k] ||
+        (eight && (!exp_avg_scales[k] || !exp_avg_sq_scales[k])))
+      return CUGO_B200_ERR_ARG;
+    if (!aligned(params[k], p_bytes) || !aligned(grads[k], g_bytes) ||
+        (!eight && (!aligned(exp_avgs[k], 4) || !aligned(exp_avg_sqs[k], 4))))
+      return CUGO_B200_ERR_ALIGN;
+  }
+  if (!aligned(step, 8) || !aligned(scratch, 8)) return CUGO_B200_ERR_ALIGN;
+  if (!scratch || scratch_bytes < cugo_b200_adamw_scratch_bytes(count)) return CUGO_B200_ERR_CAPACITY;
+  Options o{};
+  o.lr = lr;
+  o.lr_dev = lr_dev;
+  o.beta1 = beta1;
+  o.beta2 = beta2;
+  o.decay = weight_decay;
+  o.b1 = static_cast<float>(beta1);
+  o.c1 = static_cast<float>(1.0 - beta1);
+  o.b2 = static_cast<float>(beta2);
+  o.c2 = static_cast<float>(1.0 - beta2);
+  o.eps = static_cast<float>(eps);
+  o.max_norm = static_cast<float>(max_norm);
+  o.seed = seed;
+  const Lists l{params, grads, exp_avgs, exp_avg_sqs, eight ? exp_avg_scales : nullptr,
+                eight ? exp_avg_sq_scales : nullptr, sizes, count};
+  Scalars* scalars = static_cast<Scalars*>(scratch);
+  double* partial = reinterpret_cast<double*>(static_cast<char*>(scratch) + 64);
+  if (param_dtype == 0)
+    return grad_dtype == 0 ? launch<float, float>(l, eight, o, partial, step, scalars, norm, stream)
+                           : launch<float, __nv_bfloat16>(l, eight, o, partial, step, scalars, norm, stream);
+  return grad_dtype == 0 ? launch<__nv_bfloat16, float>(l, eight, o, partial, step, scalars, norm, stream)
+                         : launch<__nv_bfloat16, __nv_bfloat16>(l, eight, o, partial, step, scalars, norm, stream);
+}
+
+}  // extern "C"

@@ -20,6 +20,7 @@ import torch
 from . import build as _build
 
 _VP, _I64, _I32, _U32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_uint32
+_F32, _F64 = ctypes.c_float, ctypes.c_double
 
 # name -> argument types after the leading pointers (all return int status)
 _SIGNATURES: dict[str, list] = {
@@ -84,6 +85,17 @@ _SIGNATURES: dict[str, list] = {
     "cugo_b200_wait_timeout_probe": [_I64, _VP, _VP, _VP],
     "cugo_b200_ppo_loss": [_VP, _I64, _VP, _VP, _VP, _VP, _VP, _I64, _VP, _I64, ctypes.c_float,
                            _VP, ctypes.c_float, _VP, _I64, _VP, _VP, _VP],
+    "cugo_b200_action_logp": [_VP, _I64, _I32, _VP, _I64, _VP, _VP, _I64, _I64, _VP, _VP, _VP,
+                              _VP, _VP],
+    "cugo_b200_action_logp_backward": [_VP, _I64, _I32, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _VP,
+                                       _I64, _I64, _VP, _I64, _I32, _VP],
+    "cugo_b200_policy_loss": [_VP, _I64, _I32, _VP, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _VP,
+                              _I64, _I64, _F32, _F32, _F32, _F32, _F32, _VP, _F32, _VP, _VP, _I64,
+                              _I32, _I64, _VP, _VP, _VP, _VP, _I64, _VP],
+    "cugo_b200_preference_pairs": [_VP, _VP, _VP, _VP, _VP, _I64, _I64, _F32, _F32, _I32, _VP,
+                                   _VP, _VP, _VP, _VP, _VP, _I64, _VP],
+    "cugo_b200_adamw": [_I64, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I32, _I32, _I32, _F64, _VP, _F64,
+                        _F64, _F64, _F64, _F64, _U32, _VP, _VP, _VP, _I64, _VP],
     "cugo_b200_colsum_bf16": [_VP, _I64, _VP, _I64, _I32, _VP, _I64, _I64, _I32, _VP, _VP, _I64,
                               _VP],
     "cugo_b200_scalar_head_backward": [_VP, _VP, _VP, _I64, _I32, _VP, _I64, _I64, _I32, _VP, _VP,
@@ -108,7 +120,12 @@ _CONSTANTS = {
 _EXTRA_CONSTANTS = {"EVENT_IN": "cugo_b200_event_inputs", "START_IN": "cugo_b200_start_inputs"}
 _INT64_FUNCTIONS = {"cugo_b200_colsum_scratch_floats": [_I64, _I32],
                     "cugo_b200_wgrad_scratch_floats": [_I64, _I64, _I64],
-                    "cugo_b200_running_init_scratch": [_I64]}
+                    "cugo_b200_running_init_scratch": [_I64],
+                    "cugo_b200_policy_loss_scratch_bytes": [_I64],
+                    "cugo_b200_preference_pairs_scratch_bytes": [_I64],
+                    "cugo_b200_adamw_scratch_bytes": [_I64]}
+_LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_PARAM_TYPES = {torch.float32: 0, torch.bfloat16: 1}
 _ERRORS = {-1: "invalid argument", -2: "misaligned pointer", -3: "kernel launch failed"}
 
 _LIB: ctypes.CDLL | None = None
@@ -175,6 +192,31 @@ def _check_states(states: torch.Tensor, state_bytes: int) -> None:
         raise RuntimeError("states must have shape [N, STATE_BYTES]")
     if states.size(1) != state_bytes:
         raise RuntimeError("states second dimension must equal STATE_BYTES")
+
+
+def _check_matrix(t: torch.Tensor, op: str, name: str, rows: int, cols: int,
+                  like: torch.Tensor) -> None:
+    """t [rows, >= cols] with unit column stride and rows that do not overlap."""
+    if t.device != like.device:
+        raise RuntimeError(f"{op}: {name} must be on the logits' device")
+    if t.dim() != 2 or t.size(0) != rows or t.size(1) < cols:
+        raise RuntimeError(f"{op}: {name} has the wrong shape")
+    if (t.stride(1) != 1 and t.size(1) > 1) or (rows > 1 and t.stride(0) < t.size(1)):
+        raise RuntimeError(f"{op}: {name} must be row-major (unit column stride)")
+
+
+def _check_vector(t: torch.Tensor, op: str, name: str, n: int, dtype: torch.dtype,
+                  device: torch.device) -> None:
+    if t.dtype != dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise RuntimeError(f"{op}: {name} must be a contiguous {dtype} tensor of {n} entries")
+    if t.device != device:
+        raise RuntimeError(f"{op}: {name} must be on {device}")
+
+
+def _check_scalar(t: torch.Tensor | None, op: str, name: str, dtype: torch.dtype,
+                  device: torch.device) -> None:
+    if t is not None and (t.dtype != dtype or t.numel() != 1 or t.device != device):
+        raise RuntimeError(f"{op}: {name} must be one {dtype} value on {device}")
 
 
 def _same_device(a: torch.Tensor, b: torch.Tensor, an: str, bn: str) -> None:
@@ -546,6 +588,216 @@ class CugoB200Extension:
                 _ptr(adv), _ptr(value), value.stride(0), _ptr(ret), b, float(clip),
                 _ptr(entropy_coef), float(value_coef), _ptr(dlogits), dlogits.stride(0),
                 _ptr(dvalue), _ptr(stats), self._stream(logits.device)), "ppo_loss")
+
+    # -- losses over rows of logits ----------------------------------------------
+    @staticmethod
+    def _check_rows(op: str, logits, actions, legal, weight) -> None:
+        if not logits.is_cuda:
+            raise RuntimeError(f"{op}: logits must be a CUDA tensor")
+        if logits.dtype not in _LOGIT_TYPES:
+            raise RuntimeError(f"{op}: logits must be fp32, bf16 or fp16")
+        if logits.dim() != 2 or logits.size(1) < 1:
+            raise RuntimeError(f"{op}: logits must be [rows, entries >= 1]")
+        rows, vocab = logits.shape
+        _check_matrix(logits, op, "logits", rows, vocab, logits)
+        _check_vector(actions, op, "actions", rows, torch.int64, logits.device)
+        if legal is not None:
+            if legal.dtype != torch.bool or legal.shape != logits.shape:
+                raise RuntimeError(f"{op}: legal must be bool of the logits' shape")
+            if rows < 2 or legal.stride(0) != 0:  # one mask expanded over the rows is fine
+                _check_matrix(legal, op, "legal", rows, vocab, logits)
+            elif legal.device != logits.device or (legal.stride(1) != 1 and vocab > 1):
+                raise RuntimeError(f"{op}: legal must be row-major on the logits' device")
+        if weight is not None:
+            _check_vector(weight, op, "weight", rows, torch.float32, logits.device)
+
+    def action_logp(self, logits: torch.Tensor, actions: torch.Tensor,
+                    legal: torch.Tensor | None = None, weight: torch.Tensor | None = None,
+                    entropy: bool = True, backward: bool = False, zeros: bool = False):
+        """(logp, entropy, lse, zeros) of the rows' actions (see the C declaration), fp32;
+        entropy, lse (`backward`) and zeros only where asked for, else None."""
+        self._check_rows("action_logp", logits, actions, legal, weight)
+        rows, vocab = logits.shape
+        dev = logits.device
+        with torch.cuda.device(dev):
+            logp = torch.empty(rows, dtype=torch.float32, device=dev)
+            ent = torch.empty_like(logp) if entropy else None
+            lse = torch.empty((rows, 2), dtype=torch.float32, device=dev) if backward else None
+            zero = torch.empty_like(logp) if zeros else None
+            _check(self._lib.cugo_b200_action_logp(
+                _ptr(logits), logits.stride(0), _LOGIT_TYPES[logits.dtype], _ptr(legal),
+                0 if legal is None else legal.stride(0), _ptr(actions), _ptr(weight), rows, vocab,
+                _ptr(logp), _ptr(ent), _ptr(lse), _ptr(zero), self._stream(dev)), "action_logp")
+        return logp, ent, lse, zero
+
+    def action_logp_backward(self, logits, actions, legal, lse, entropy, d_logp, d_entropy,
+                             scale: torch.Tensor | None = None,
+                             out: torch.Tensor | None = None) -> torch.Tensor:
+        """d loss / d logits from the gradients of action_logp's outputs (see the C
+        declaration); out: [rows, vocab] of any of the three types, else the logits' type."""
+        op = "action_logp_backward"
+        self._check_rows(op, logits, actions, legal, None)
+        rows, vocab = logits.shape
+        dev = logits.device
+        if lse.shape != (rows, 2) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != dev:
+            raise RuntimeError(f"{op}: lse must be the forward's fp32 [rows, 2]")
+        for t, name in ((entropy, "entropy"), (d_logp, "d_logp"), (d_entropy, "d_entropy")):
+            if t is not None:
+                _check_vector(t, op, name, rows, torch.float32, dev)
+        if d_entropy is not None and entropy is None:
+            raise RuntimeError(f"{op}: d_entropy needs the forward's entropy")
+        _check_scalar(scale, op, "scale", torch.float32, dev)
+        with torch.cuda.device(dev):
+            if out is None:
+                out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+            _check_matrix(out, op, "out", rows, vocab, logits)
+            if out.dtype not in _LOGIT_TYPES:
+                raise RuntimeError(f"{op}: out must be fp32, bf16 or fp16")
+            _check(self._lib.cugo_b200_action_logp_backward(
+                _ptr(logits), logits.stride(0), _LOGIT_TYPES[logits.dtype], _ptr(legal),
+                0 if legal is None else legal.stride(0), _ptr(actions), _ptr(lse), _ptr(entropy),
+                _ptr(d_logp), _ptr(d_entropy), _ptr(scale), rows, vocab, _ptr(out), out.stride(0),
+                _LOGIT_TYPES[out.dtype], self._stream(dev)), op)
+        return out
+
+    def policy_loss(self, logits: torch.Tensor, actions: torch.Tensor, logp_old: torch.Tensor,
+                    adv: torch.Tensor, legal: torch.Tensor | None = None,
+                    weight: torch.Tensor | None = None, ref_logits: torch.Tensor | None = None,
+                    ref_logp: torch.Tensor | None = None, clip_low: float = 0.2,
+                    clip_high: float = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0,
+                    denominator: float = 0.0, denominator_dev: torch.Tensor | None = None,
+                    grad_scale: float = 1.0, grad_scale_dev: torch.Tensor | None = None,
+                    dlogits: torch.Tensor | None = None, stats: bool = True):
+        """The clipped policy loss (see the C declaration): (loss fp32 scalar, stats fp32 [8],
+        logp fp32 [rows]), and d loss / d logits into dlogits [rows, >= vocab] where given;
+        with stats=False the gradient only."""
+        op = "policy_loss"
+        self._check_rows(op, logits, actions, legal, weight)
+        rows, vocab = logits.shape
+        dev = logits.device
+        _check_vector(logp_old, op, "logp_old", rows, torch.float32, dev)
+        _check_vector(adv, op, "adv", rows, torch.float32, dev)
+        if ref_logits is not None:
+            if ref_logits.dtype != logits.dtype or ref_logits.shape != logits.shape:
+                raise RuntimeError(f"{op}: ref_logits must have the logits' type and shape")
+            _check_matrix(ref_logits, op, "ref_logits", rows, vocab, logits)
+        if ref_logp is not None:
+            if ref_logits is not None:
+                raise RuntimeError(f"{op}: give ref_logits or ref_logp, not both")
+            _check_vector(ref_logp, op, "ref_logp", rows, torch.float32, dev)
+        _check_scalar(denominator_dev, op, "denominator", torch.float32, dev)
+        _check_scalar(grad_scale_dev, op, "grad_scale", torch.float32, dev)
+        if dlogits is not None:
+            if dlogits.dtype not in _LOGIT_TYPES:
+                raise RuntimeError(f"{op}: dlogits must be fp32, bf16 or fp16")
+            _check_matrix(dlogits, op, "dlogits", rows, vocab, logits)
+        with torch.cuda.device(dev):
+            lib = self._lib
+            need = lib.cugo_b200_policy_loss_scratch_bytes(rows)
+            scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+            loss = out = logp = None
+            if stats:
+                loss = torch.empty((), dtype=torch.float32, device=dev)
+                out = torch.empty(8, dtype=torch.float32, device=dev)
+                logp = torch.empty(rows, dtype=torch.float32, device=dev)
+            _check(lib.cugo_b200_policy_loss(
+                _ptr(logits), logits.stride(0), _LOGIT_TYPES[logits.dtype], _ptr(ref_logits),
+                0 if ref_logits is None else ref_logits.stride(0), _ptr(legal),
+                0 if legal is None else legal.stride(0), _ptr(actions), _ptr(logp_old), _ptr(adv),
+                _ptr(weight), _ptr(ref_logp), rows, vocab, clip_low, clip_high, kl_coef,
+                entropy_coef, denominator, _ptr(denominator_dev), grad_scale, _ptr(grad_scale_dev),
+                _ptr(dlogits), 0 if dlogits is None else dlogits.stride(0),
+                0 if dlogits is None else _LOGIT_TYPES[dlogits.dtype],
+                vocab if dlogits is None else dlogits.size(1), _ptr(logp), _ptr(out), _ptr(loss),
+                _ptr(scratch), need, self._stream(dev)), op)
+        return loss, out, logp
+
+    def preference_pairs(self, logp: torch.Tensor, ref_logp: torch.Tensor,
+                         weight: torch.Tensor | None, lse: torch.Tensor, offsets: torch.Tensor,
+                         beta: float, smoothing: float = 0.0, average: bool = False,
+                         d_logp: torch.Tensor | None = None):
+        """The preference loss from action_logp's rows (see the C declaration): (loss, margin
+        fp32 [pairs], seq_logp fp32 [2 pairs], accuracy); d_logp fp32 [rows] is written."""
+        op = "preference_loss"
+        rows, dev = logp.numel(), logp.device
+        if offsets.dtype != torch.int64 or offsets.dim() != 1 or offsets.numel() % 2 != 1 \
+                or not offsets.is_contiguous() or offsets.device != dev:
+            raise RuntimeError(f"{op}: offsets must be contiguous int64 [2 pairs + 1] on the logits' device")
+        for t, name in ((logp, "logp"), (ref_logp, "ref_logp"), (weight, "weight"), (d_logp, "d_logp")):
+            if t is not None:
+                _check_vector(t, op, name, rows, torch.float32, dev)
+        if not 0.0 <= smoothing <= 1.0:
+            raise RuntimeError(f"{op}: smoothing must lie in [0, 1]")
+        pairs = offsets.numel() // 2
+        with torch.cuda.device(dev):
+            need = self._lib.cugo_b200_preference_pairs_scratch_bytes(pairs)
+            scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+            margin = torch.empty(pairs, dtype=torch.float32, device=dev)
+            seq = torch.empty(2 * pairs, dtype=torch.float32, device=dev)
+            loss = torch.empty((), dtype=torch.float32, device=dev)
+            accuracy = torch.empty_like(loss)
+            _check(self._lib.cugo_b200_preference_pairs(
+                _ptr(logp), _ptr(ref_logp), _ptr(weight), _ptr(lse), _ptr(offsets), pairs, rows,
+                beta, smoothing, int(average), _ptr(margin), _ptr(seq), _ptr(d_logp), _ptr(loss),
+                _ptr(accuracy), _ptr(scratch), need, self._stream(dev)), op)
+        return loss, margin, seq, accuracy
+
+    # -- the AdamW step -------------------------------------------------------------
+    def adamw(self, params: list, grads: list, exp_avgs: list, exp_avg_sqs: list,
+              step: torch.Tensor, lr, beta1: float, beta2: float, eps: float, weight_decay: float,
+              max_grad_norm: float | None, seed: int, exp_avg_scales: list | None = None,
+              exp_avg_sq_scales: list | None = None) -> torch.Tensor | None:
+        """One AdamW step over the tensors, in place (see the C declaration); returns the
+        gradients' norm (fp32 scalar) where max_grad_norm clips it, else None."""
+        op, n = "adamw", len(params)
+        eight = exp_avg_scales is not None
+        lists = [("params", params), ("grads", grads), ("exp_avgs", exp_avgs),
+                 ("exp_avg_sqs", exp_avg_sqs)]
+        if eight:
+            if exp_avg_sq_scales is None:
+                raise RuntimeError(f"{op}: 8-bit states need both lists of scales")
+            lists += [("exp_avg_scales", exp_avg_scales), ("exp_avg_sq_scales", exp_avg_sq_scales)]
+        if any(len(l) != n for _, l in lists):
+            raise RuntimeError(f"{op}: the lists must have one tensor each per parameter")
+        dev = step.device
+        if not step.is_cuda or step.dtype != torch.int64 or step.numel() != 1:
+            raise RuntimeError(f"{op}: step must be one int64 value on a CUDA device")
+        if n and (params[0].dtype not in _PARAM_TYPES or grads[0].dtype not in _PARAM_TYPES):
+            raise RuntimeError(f"{op}: parameters and gradients must be fp32 or bf16")
+        states = (torch.uint8, torch.float8_e4m3fn) if eight else (torch.float32,)
+        scales = (torch.uint8, torch.float8_e8m0fnu)
+        sizes = [t.numel() for t in params]
+        counts = [(k + 255) // 256 for k in sizes]
+        pointers = []
+        for i, (name, tensors) in enumerate(lists):
+            types = ((params[0].dtype,) if n else (), (grads[0].dtype,) if n else (), states, states,
+                     scales, scales)[i]
+            if [t.numel() for t in tensors] != (sizes if i < 4 else counts):
+                raise RuntimeError(f"{op}: {name} have the wrong sizes")
+            for t in tensors:
+                if t.dtype not in types or t.device != dev or not t.is_contiguous():
+                    raise RuntimeError(f"{op}: {name} must be contiguous, of one type ({types}) and on {dev}")
+            at = [t.data_ptr() for t in tensors]
+            if i != 1 and len(set(at)) != n and len({p for p, k in zip(at, sizes) if k}) != sum(map(bool, sizes)):
+                raise RuntimeError(f"{op}: a tensor is in {name} twice")
+            pointers.append((_VP * n)(*at))
+        lr_dev = None
+        if torch.is_tensor(lr):
+            _check_scalar(lr, op, "lr", torch.float32, dev)
+            lr_dev, lr = lr, 0.0
+        with torch.cuda.device(dev):
+            need = self._lib.cugo_b200_adamw_scratch_bytes(n)
+            scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+            norm = None
+            if max_grad_norm is not None:
+                norm = torch.empty((), dtype=torch.float32, device=dev)
+            _check(self._lib.cugo_b200_adamw(
+                n, *pointers[:4], *(pointers[4:] if eight else (None, None)), (_I64 * n)(*sizes),
+                _PARAM_TYPES[params[0].dtype] if n else 0, _PARAM_TYPES[grads[0].dtype] if n else 0,
+                8 if eight else 32, lr, _ptr(lr_dev), beta1, beta2, eps, weight_decay,
+                0.0 if max_grad_norm is None else max_grad_norm, seed & 0xFFFFFFFF, _ptr(step),
+                _ptr(norm), _ptr(scratch), need, self._stream(dev)), op)
+        return norm
 
     def _colsum_scratch(self, rows: int, n: int, device: torch.device) -> torch.Tensor:
         """The per-block partial sums' buffer, one per device, grown as needed (keep

@@ -375,6 +375,113 @@ CUGO_B200_API int cugo_b200_ppo_loss(const float* logits, int64_t ldl, const boo
                                      int64_t ldd, float* dvalue, float* stats,
                                      cudaStream_t stream);
 
+/* ---- losses over rows of logits ----------------------------------------------------
+ *
+ * Rows of `vocab` logits (any number from 1 to 2^31 - 1; dtype 0 fp32, 1 bf16, 2 fp16),
+ * ld elements apart.  legal (bool, rows ldm bytes apart, 0: one mask for all rows; null:
+ * every entry) masks entries; an entry at or below -2^30 counts as masked too (-inf,
+ * -1e30, the type's lowest value), whatever stands in a masked place is not used, and
+ * logits are taken to lie below 2^30.  A row does not count -- its outputs and
+ * gradients are 0 -- where its action is outside [0, vocab) or masked, or its weight is
+ * 0.  Arithmetic and sums over a row in 32 bits, sums over rows in 64 bits, in a fixed
+ * order (the same result on every run).  No counterpart in the reference, whose
+ * updates compute these with torch (python/cugo_ppo50.py:558-623). */
+
+/* log p of the rows' actions and the entropy of their distributions, fp32 [rows] each
+ * (either may be null).  lse (fp32 [rows, 2], 8-byte aligned, may be null) keeps each
+ * row's maximum and sum for the backward; zeros (fp32 [rows], may be null) is set to 0
+ * in passing.  weight (fp32 [rows], may be null): rows of weight 0 do not count. */
+CUGO_B200_API int cugo_b200_action_logp(const void* logits, int64_t ld, int32_t dtype,
+                                        const bool* legal, int64_t ldm, const int64_t* actions,
+                                        const float* weight, int64_t rows, int64_t vocab,
+                                        float* logp, float* entropy, float* lse, float* zeros,
+                                        cudaStream_t stream);
+
+/* Backward of cugo_b200_action_logp: d loss / d logits (grad_dtype, rows ldd apart) from
+ * d_logp and d_entropy (fp32 [rows], either may be null: 0), both times *scale (device
+ * fp32, may be null: 1); lse and entropy as the forward wrote them.  A row whose two
+ * gradients are 0 is not read. */
+CUGO_B200_API int cugo_b200_action_logp_backward(
+    const void* logits, int64_t ld, int32_t dtype, const bool* legal, int64_t ldm,
+    const int64_t* actions, const float* lse, const float* entropy, const float* d_logp,
+    const float* d_entropy, const float* scale, int64_t rows, int64_t vocab, void* dlogits,
+    int64_t ldd, int32_t grad_dtype, cudaStream_t stream);
+
+/* The clipped policy loss with an entropy bonus and a KL term, and its gradient, in one
+ * pass over the logits:
+ *   r = exp(log p(action) - logp_old)
+ *   loss = sum_i w_i (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A)
+ *                     - entropy_coef H + kl_coef K) / D
+ * K is KL(p | q) over the legal entries with q from ref_logits (same dtype, rows ldr
+ * apart), or with ref_logp (fp32 [rows], the reference's log p of the action) the
+ * estimate exp(d) - 1 - d, d = ref_logp - log p; at most one of the two.  weight fp32
+ * [rows] or null (1).  D = denominator where that is not 0, else *denominator_dev (device
+ * fp32) if given, else the sum of the weights, or the rows; D = 0 gives a loss and
+ * gradients of 0.
+ * dlogits (grad_dtype, rows ldd apart, may be null) gets d loss / d logits times
+ * grad_scale and *grad_scale_dev (device fp32, may be null); columns vocab .. width - 1
+ * are set to 0.  logp fp32 [rows] (may be null).  stats fp32 [8] (may be null where
+ * dlogits is not): the loss, the weighted means of policy loss, H, K, the KL estimate
+ * (r - 1) - log r, the share of clipped ratios and the share of rows that count, and D;
+ * loss (fp32, may be null): the loss once more.  scratch: at least
+ * cugo_b200_policy_loss_scratch_bytes(rows) bytes of the call's own, 8-byte aligned. */
+CUGO_B200_API int cugo_b200_policy_loss(
+    const void* logits, int64_t ld, int32_t dtype, const void* ref_logits, int64_t ldr,
+    const bool* legal, int64_t ldm, const int64_t* actions, const float* logp_old,
+    const float* adv, const float* weight, const float* ref_logp, int64_t rows, int64_t vocab,
+    float clip_low, float clip_high, float kl_coef, float entropy_coef, float denominator,
+    const float* denominator_dev, float grad_scale, const float* grad_scale_dev, void* dlogits,
+    int64_t ldd, int32_t grad_dtype, int64_t width, float* logp, float* stats, float* loss,
+    void* scratch, int64_t scratch_bytes, cudaStream_t stream);
+
+CUGO_B200_API int64_t cugo_b200_policy_loss_scratch_bytes(int64_t rows);
+
+/* The preference loss over pairs of sequences, from action_logp's rows: sequence j holds
+ * rows offsets[j] .. offsets[j + 1] - 1 (offsets int64 [2 pairs + 1], not decreasing; what
+ * lies outside the rows is left out) and pair i prefers sequence 2 i to 2 i + 1.
+ *   score_j = sum of w (logp - ref_logp) over its rows that count, / sum of w if `average`
+ *   m_i = beta (score_2i - score_2i+1)
+ *   loss = mean of -(1 - smoothing) log sigmoid(m_i) - smoothing log sigmoid(-m_i)
+ * margin fp32 [pairs] gets m; seq_logp fp32 [2 pairs] each sequence's log p (summed, or
+ * averaged, as the score); d_logp (fp32 [rows], may be null) d loss / d logp of the
+ * sequences' rows; loss and accuracy (fp32) the loss and the share of positive margins.  lse as
+ * cugo_b200_action_logp wrote it.  scratch: the call's own, 8-byte aligned. */
+CUGO_B200_API int cugo_b200_preference_pairs(
+    const float* logp, const float* ref_logp, const float* weight, const float* lse,
+    const int64_t* offsets, int64_t pairs, int64_t rows, float beta, float smoothing,
+    int32_t average, float* margin, float* seq_logp, float* d_logp, float* loss, float* accuracy,
+    void* scratch, int64_t scratch_bytes, cudaStream_t stream);
+
+CUGO_B200_API int64_t cugo_b200_preference_pairs_scratch_bytes(int64_t pairs);
+
+/* ---- the AdamW step ---------------------------------------------------------------
+ *
+ * One step over `count` tensors, given as host arrays of device pointers and sizes
+ * (elements; contiguous tensors, none twice):
+ *   g = g min(1, max_norm / (|g| + 1e-6))   where norm is given (the norm of all tensors)
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p = (1 - lr weight_decay) p - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+ * params: param_dtype (0 fp32, 1 bf16, rounded up or down by random bits), grads:
+ * grad_dtype (0 fp32, 1 bf16).  state_bits 32: exp_avgs, exp_avg_sqs fp32; 8: e4m3 codes
+ * with one e8m0 scale byte per 256 elements of a tensor (exp_avg_scales,
+ * exp_avg_sq_scales: ceil(size / 256) bytes each), rounded up or down by random bits; all
+ * zero is a fresh state.  lr_dev (device fp32, may be null) replaces lr.  t = ++*step
+ * (device int64).  norm (device fp32, may be null) gets the gradients' norm before
+ * clipping.  The random bits depend on seed, t and an element's number, counted over the
+ * tensors in order, each padded to 256.  scratch: at least
+ * cugo_b200_adamw_scratch_bytes(count) bytes of the call's own, 8-byte aligned.
+ * Replaces clip_grad_norm_ and the optimizer step of python/cugo_ppo50.py:610-623. */
+CUGO_B200_API int cugo_b200_adamw(int64_t count, void* const* params, const void* const* grads,
+                                  void* const* exp_avgs, void* const* exp_avg_sqs,
+                                  void* const* exp_avg_scales, void* const* exp_avg_sq_scales,
+                                  const int64_t* sizes, int32_t param_dtype, int32_t grad_dtype,
+                                  int32_t state_bits, double lr, const float* lr_dev, double beta1,
+                                  double beta2, double eps, double weight_decay, double max_norm,
+                                  uint32_t seed, int64_t* step, float* norm, void* scratch,
+                                  int64_t scratch_bytes, cudaStream_t stream);
+
+CUGO_B200_API int64_t cugo_b200_adamw_scratch_bytes(int64_t count);
+
 /* Column sums (fp32 [n], 8 <= n <= 2048, n a multiple of 8) of bf16 x [rows, n]
  * (row stride ldx); with z (bf16, ldz), of dz = x * act'(z) (act 0 none, 1 ReLU,
  * 2 SiLU), which is also written to dz (bf16, ldd).  The bias gradients of the

@@ -29,6 +29,7 @@
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "../../include/cugo_b200.h"
 
@@ -58,12 +59,66 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Two floats in one register pair, an instruction for both.
+struct Two {
+  uint64_t v;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(Two t, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(t.v));
+}
+__device__ __forceinline__ Two add(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float both(Two t) {
+  float a, b;
+  split(t, a, b);
+  return a + b;
+}
+
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
 // N values to the gradient's type at element `at`; `wide`: that address is a multiple of
 // the N values' bytes, or of 16.
+__device__ __forceinline__ uint32_t pack_grad(int type, float a, float b) {  // of 16-bit types
+  if (type == kBf16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 template <int N>
 __device__ __forceinline__ void store_grad(void* base, int type, i64 at, const float (&g)[N], bool wide) {
   if (type == kFp32) {
@@ -71,7 +126,7 @@ __device__ __forceinline__ void store_grad(void* base, int type, i64 at, const f
     if (wide) {
 #pragma unroll
       for (int e = 0; e < N; e += 4)
-        *reinterpret_cast<float4*>(d + e) = make_float4(g[e], g[e + 1], g[e + 2], g[e + 3]);
+        __stcs(reinterpret_cast<float4*>(d + e), make_float4(g[e], g[e + 1], g[e + 2], g[e + 3]));
     } else {
 #pragma unroll
       for (int e = 0; e < N; ++e) d[e] = g[e];
@@ -80,19 +135,11 @@ __device__ __forceinline__ void store_grad(void* base, int type, i64 at, const f
   }
   uint32_t w[N / 2];
 #pragma unroll
-  for (int e = 0; e < N; e += 2) {
-    if (type == kBf16) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(g[e], g[e + 1]);
-      w[e / 2] = *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-      const __half2 h = __floats2half2_rn(g[e], g[e + 1]);
-      w[e / 2] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-  }
+  for (int e = 0; e < N; e += 2) w[e / 2] = pack_grad(type, g[e], g[e + 1]);
   uint16_t* d = static_cast<uint16_t*>(base) + at;
   if (wide) {
-    if constexpr (N == 8) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-    else *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
+    if constexpr (N == 8) __stcs(reinterpret_cast<uint4*>(d), make_uint4(w[0], w[1], w[2], w[3]));
+    else __stcs(reinterpret_cast<uint2*>(d), make_uint2(w[0], w[1]));
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e) d[e] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
@@ -159,21 +206,24 @@ __device__ __forceinline__ Sums join_warp(Sums v) {
   return v;
 }
 
-__device__ __forceinline__ float sum_warp(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-  return v;
-}
-
 __device__ __forceinline__ double sum_warp(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
   return v;
 }
 
-__device__ __forceinline__ float max_warp(float v) {
+// Over the kLanes lanes that share a row (all lanes of the warp take part).
+template <int kLanes>
+__device__ __forceinline__ float sum_lanes(float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(kFull, v, o));
+  for (int o = kLanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+
+template <int kLanes>
+__device__ __forceinline__ float max_lanes(float v) {
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(kFull, v, o));
   return v;
 }
 
@@ -216,16 +266,60 @@ struct Policy {
   double* partial;              // [blocks][kSums], or null: no means wanted
 };
 
-// A row's loss terms (times its weight, added to acc) and its gradient's coefficients,
-// from its sums and its action's y.
+// What policy_loss reads of a row beside its logits.
+struct RowInputs {
+  i64 action;
+  float weight, logp_old, adv, ref_logp;
+};
+
+template <bool kPolicy>
+__device__ __forceinline__ RowInputs row_inputs(const Rows& r, const Policy& a, i64 row) {
+  RowInputs in;
+  in.action = r.actions[row];
+  in.weight = r.weight ? r.weight[row] : 1.0f;
+  in.logp_old = in.adv = in.ref_logp = 0.0f;
+  if constexpr (kPolicy) {
+    in.logp_old = a.logp_old[row];
+    in.adv = a.adv[row];
+    if (a.ref_logp) in.ref_logp = a.ref_logp[row];
+  }
+  return in;
+}
+
+// log p of an entry.  kLog2e is log2(e) (1 - 1.335e-8): the sums are those of the logits
+// times that, and d log p / d (a factor of the logits) = x_a - mean x, so to first order
+// the factor comes out by one more FMA.
+__device__ __forceinline__ float log_prob(float y_a, float log_s, float mean_y) {
+  return kLn2 * fmaf(1.335e-8f, y_a - mean_y, y_a - log_s);
+}
+
+// A row's outputs in action_logp.
+__device__ __forceinline__ void store_score(const Score& o, i64 row, bool used, const Sums& v, float y_a) {
+  const float log_s = used ? log2f(v.s) : INFINITY, mean_y = v.t / v.s;
+  if (o.logp) o.logp[row] = used ? log_prob(y_a, log_s, mean_y) : 0.0f;
+  if (o.entropy) o.entropy[row] = used ? kLn2 * (log_s - mean_y) : 0.0f;
+  if (o.lse) o.lse[row] = make_float2(used ? v.m : 0.0f, log_s);
+  if (o.zeros) o.zeros[row] = 0.0f;
+}
+
+// What a row adds to the means, before its weight.
+struct Terms {
+  float v[kSums];
+  __device__ __forceinline__ void add_to(double* acc, float w) const {
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) acc[k] += static_cast<double>(w) * v[k];
+  }
+};
+
+// A row's loss terms and its gradient's coefficients, from its sums and its action's y.
 template <bool kRef>
-__device__ __forceinline__ Coefs policy_row(const Policy& a, i64 row, const Sums& v, float y_a, float w,
-                                            float scale, double (&acc)[kSums], float& logp) {
+__device__ __forceinline__ Coefs policy_row(const Policy& a, const RowInputs& in, const Sums& v, float y_a,
+                                            float scale, Terms& terms, float& logp) {
   const float log_s = log2f(v.s), inv_s = 1.0f / v.s, mean_y = v.t * inv_s;
-  logp = kLn2 * (y_a - log_s);
-  const float entropy = kLn2 * (log_s - mean_y);
-  const float log_ratio = logp - a.logp_old[row];
-  const float ratio = expf(log_ratio), adv = a.adv[row];
+  logp = log_prob(y_a, log_s, mean_y);
+  const float entropy = kLn2 * (log_s - mean_y), w = in.weight;
+  const float log_ratio = logp - in.logp_old;
+  const float ratio = expf(log_ratio), adv = in.adv;
   const float bounded = ratio < a.low ? a.low : ratio > a.high ? a.high : ratio;
   // min(r A, clamp(r) A); where the two are equal the ratio still moves the loss.
   const bool moves = !(ratio * adv > bounded * adv);
@@ -237,7 +331,7 @@ __device__ __forceinline__ Coefs policy_row(const Policy& a, i64 row, const Sums
     kl = kLn2 * (mean_d - log_s + log2f(v.sr));
     c2 = a.kl_coef * kLn2;
   } else if (a.ref_logp) {
-    const float d = a.ref_logp[row] - logp, e = expm1f(d);
+    const float d = in.ref_logp - logp, e = expm1f(d);
     kl = e - d;
     g -= a.kl_coef * e;
   }
@@ -248,13 +342,7 @@ __device__ __forceinline__ Coefs policy_row(const Policy& a, i64 row, const Sums
   c.c0 = ks * (-g - c1 * mean_y - c2 * mean_d);
   c.c1 = ks * c1;
   c.c2 = ks * c2;
-  const double wd = w;
-  acc[0] -= wd * gain;
-  acc[1] += wd * entropy;
-  acc[2] += wd * kl;
-  acc[3] += wd * (expm1f(log_ratio) - log_ratio);
-  acc[4] += ratio < a.low || ratio > a.high ? wd : 0.0;
-  acc[5] += wd;
+  terms = {{-gain, entropy, kl, expm1f(log_ratio) - log_ratio, ratio < a.low || ratio > a.high ? 1.0f : 0.0f, 1.0f}};
   return c;
 }
 
@@ -305,111 +393,235 @@ __device__ void store_partial(const Policy& a, const double (&acc)[kSums]) {
   }
 }
 
-// ---- short rows: a warp per row, the row in registers -----------------------------------
+// ---- short rows: 8, 16 or 32 lanes per row, the row in registers ------------------------
 //
-// Lane l holds entries l, l + 32, ..., kPer of them: scalar loads, coalesced whatever the
-// row's alignment (a 179-entry row of fp32 starts at any multiple of 4 bytes).
+// Lane l of a row's kLanes holds entries l, l + kLanes, ..., kPer of them.  A warp takes
+// 32 / kLanes consecutive rows: few entries per lane would leave the row's reductions and
+// its one logarithm to most of the time.  Rows that lie one after another (a stride of
+// little more than the entries) are copied as one run of 16-byte vectors into the warp's
+// own shared memory, the next rows' while these are computed, so the loads are wide and in
+// flight however the rows are aligned (a row of 179 fp32 starts at any multiple of 4
+// bytes); the gradient leaves the same way.
 
 constexpr int kShortWarps = 8;
 
-template <typename T, int kPer, bool kRef, bool kPolicy>
-__global__ void __launch_bounds__(32 * kShortWarps) short_rows_kernel(const Rows r, const Score o, const Policy a) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void copy16(void* to, const void* from, int bytes) {
+  const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+}
+
+// Where a run of rows stands in shared memory: the 16-byte granules that hold it, from
+// its first byte's granule on (an allocation starts at a granule, so that lies inside);
+// what lies behind its last byte is not read.
+__device__ __forceinline__ void copy_run(char* to, const void* from, int bytes, int lane) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(from);
+  const int skip = static_cast<int>(at & 15), total = skip + bytes;
+  const char* base = reinterpret_cast<const char*>(at - skip);
+  for (int k = 16 * lane; k < total; k += 512) copy16(to + k, base + k, total - k < 16 ? total - k : 16);
+}
+
+// The run's row number `back` there, or in global memory where it was not copied.
+template <typename V>
+__device__ __forceinline__ const V* staged_row(const char* stage, bool staged, const V* first, i64 back, i64 ld) {
+  const V* base = staged ? reinterpret_cast<const V*>(stage + (reinterpret_cast<uintptr_t>(first) & 15)) : first;
+  return base + back * ld;
+}
+
+// The warp's shared memory, in bytes (multiples of 16).
+struct Layout {
+  int logits, ref, legal, grad;  // of one stage; the gradient has one
+  __host__ __device__ int stage() const { return logits + ref + legal; }
+  __host__ __device__ int warp() const { return 2 * stage() + grad; }
+};
+
+template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy>
+__global__ void __launch_bounds__(32 * kShortWarps, 2) short_rows_kernel(const Rows r, const Score o, const Policy a,
+                                                                        const Layout lay) {
+  constexpr int kRows = 32 / kLanes;
+  extern __shared__ __align__(16) char shared[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % kLanes, sub = lane / kLanes;
+  char* const own = shared + warp * lay.warp();
+  char* const out = own + 2 * lay.stage();
   float scale = 0.0f;
   double acc[kSums] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
   if constexpr (kPolicy) scale = grad_scale_of(a, block_denominator(a, r.weight, r.rows));
-  const i64 stride = (i64)gridDim.x * kShortWarps;
-  for (i64 row = (i64)blockIdx.x * kShortWarps + (threadIdx.x >> 5); row < r.rows; row += stride) {
-    const T* lg = static_cast<const T*>(r.logits) + row * r.ld;
-    const i64 action = r.actions[row];
-    const float w = r.weight ? r.weight[row] : 1.0f;
-    bool used = w != 0.0f && action >= 0 && action < r.vocab;
-    float y[kPer], z[kPer];
-    if (used) {
-      const bool* lm = r.legal ? r.legal + row * r.ldm : nullptr;
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        const int c = lane + 32 * k;
-        const bool in = c < r.vocab && (!lm || lm[c]);
-        y[k] = in ? max_nan(to_float(lg[c]), kMasked) : kMasked;
-        if constexpr (kRef)
-          z[k] = in ? max_nan(to_float(static_cast<const T*>(r.ref)[row * r.ldr + c]), kMasked) : kMasked;
-      }
+  const i64 stride = (i64)gridDim.x * kShortWarps * kRows;
+  i64 first = ((i64)blockIdx.x * kShortWarps + warp) * kRows;
+  const int grad_bytes = type_bytes(a.dtype);
+
+  const auto fetch = [&](i64 row, int at) {
+    const int n = static_cast<int>(r.rows - row < kRows ? r.rows - row : kRows);
+    char* to = own + at * lay.stage();
+    const int size = static_cast<int>(sizeof(T));
+    if (lay.logits)
+      copy_run(to, static_cast<const T*>(r.logits) + row * r.ld,
+                             static_cast<int>(((n - 1) * r.ld + r.vocab) * size), lane);
+    if (kRef && lay.ref)
+      copy_run(to + lay.logits, static_cast<const T*>(r.ref) + row * r.ldr,
+                             static_cast<int>(((n - 1) * r.ldr + r.vocab) * size), lane);
+    if (lay.legal)
+      copy_run(to + lay.logits + lay.ref, r.legal + row * r.ldm,
+                             static_cast<int>((n - 1) * r.ldm + r.vocab), lane);
+  };
+
+  RowInputs next;
+  if (first < r.rows) {
+    fetch(first, 0);
+    next = row_inputs<kPolicy>(r, a, first + sub < r.rows ? first + sub : r.rows - 1);
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  int at = 0;
+  for (; first < r.rows; first += stride, at ^= 1) {
+    const RowInputs in = next;
+    if (first + stride < r.rows) {
+      fetch(first + stride, at ^ 1);
+      next = row_inputs<kPolicy>(r, a, first + stride + sub < r.rows ? first + stride + sub : r.rows - 1);
     }
-    Sums v = no_sums();
-    float y_a = 0.0f;
-    if (used) {
-      float top = y[0], top_r = kMasked;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    const bool real = first + sub < r.rows;
+    const i64 row = real ? first + sub : r.rows - 1;
+    const int back = static_cast<int>(row - first);  // the row's place in the run
+    const char* const stage = own + at * lay.stage();
+    const T* const x = staged_row(stage, lay.logits, static_cast<const T*>(r.logits) + first * r.ld, back, r.ld);
+    const T* z_row = nullptr;
+    if constexpr (kRef)
+      z_row = staged_row(stage + lay.logits, lay.ref, static_cast<const T*>(r.ref) + first * r.ldr, back, r.ldr);
+    const bool* lm = nullptr;
+    if (r.legal) lm = staged_row(stage + lay.logits + lay.ref, lay.legal, r.legal + first * r.ldm, back, r.ldm);
+    bool used = real && in.weight != 0.0f && in.action >= 0 && in.action < r.vocab;
+    const int action = used ? static_cast<int>(in.action) : 0;
+    float x_a = max_nan(to_float(x[action]), kMasked);
+    if (lm && !lm[action]) x_a = kMasked;
+    used = used && !(x_a <= kMasked);
+
+    float y[kPer], z[kPer], e[kPer];
+    // The last entries of a lane may lie past the row; the others do not.
 #pragma unroll
-      for (int k = 1; k < kPer; ++k) top = max_nan(top, y[k]);
-      v.m = max_warp(top) * kLog2e;
-      if constexpr (kRef) {
-        top_r = z[0];
-#pragma unroll
-        for (int k = 1; k < kPer; ++k) top_r = max_nan(top_r, z[k]);
-        v.mr = max_warp(top_r) * kLog2e;
-      }
-      float x_a = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kPer; ++k)
-        if (k == static_cast<int>(action >> 5)) x_a = y[k];
-      x_a = __shfl_sync(kFull, x_a, static_cast<int>(action & 31));
-      used = !(x_a <= kMasked);
-      y_a = fmaf(x_a, kLog2e, -v.m);
-    }
-    if (used) {
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        y[k] = fmaf(y[k], kLog2e, -v.m);
-        const float e = exp2_fast(y[k]);
-        v.s += e;
-        v.t = fmaf(e, y[k], v.t);
+    for (int k = 0; k < kPer; ++k) {
+      const int c = l + kLanes * k;
+      y[k] = kMasked;
+      if (k * kLanes < r.vocab) {  // the same for all lanes
+        const int at_c = c < r.vocab ? c : r.vocab - 1;
+        const float f = max_nan(to_float(x[at_c]), kMasked);
+        bool in_row = c < r.vocab;
+        if (lm) in_row = in_row && lm[at_c];
+        y[k] = in_row ? f : kMasked;
         if constexpr (kRef) {
-          z[k] = fmaf(z[k], kLog2e, -v.mr);
-          v.sr += exp2_fast(z[k]);
-          z[k] = y[k] - z[k];
-          v.u = fmaf(e, z[k], v.u);
+          const float g = max_nan(to_float(z_row[at_c]), kMasked);
+          z[k] = in_row ? g : kMasked;
         }
-      }
-      v.s = sum_warp(v.s);
-      v.t = sum_warp(v.t);
-      if constexpr (kRef) {
-        v.sr = sum_warp(v.sr);
-        v.u = sum_warp(v.u);
+      } else if constexpr (kRef) {
+        z[k] = kMasked;
       }
     }
-    if constexpr (!kPolicy) {
-      if (lane == 0) {
-        const float log_s = used ? log2f(v.s) : INFINITY;
-        if (o.logp) o.logp[row] = used ? kLn2 * (y_a - log_s) : 0.0f;
-        if (o.entropy) o.entropy[row] = used ? kLn2 * (log_s - v.t / v.s) : 0.0f;
-        if (o.lse) o.lse[row] = make_float2(used ? v.m : 0.0f, log_s);
-        if (o.zeros) o.zeros[row] = 0.0f;
+    float top = kMasked, top_r = kMasked;
+#pragma unroll
+    for (int k = 0; k < kPer; k += 2) {
+      top = max_nan(top, y[k], y[k + 1]);
+      if constexpr (kRef) top_r = max_nan(top_r, z[k], z[k + 1]);
+    }
+    Sums v;
+    v.m = max_lanes<kLanes>(top) * kLog2e;
+    v.mr = kRef ? max_lanes<kLanes>(top_r) * kLog2e : 0.0f;
+    const Two unit = two(kLog2e, kLog2e), from = two(-v.m, -v.m), from_r = two(-v.mr, -v.mr);
+    Two s2 = two(0.0f, 0.0f), t2 = s2, sr2 = s2, u2 = s2;
+#pragma unroll
+    for (int k = 0; k < kPer; k += 2) {
+      const Two yy = fma(two(y[k], y[k + 1]), unit, from);
+      split(yy, y[k], y[k + 1]);
+      e[k] = exp2_fast(y[k]);
+      e[k + 1] = exp2_fast(y[k + 1]);
+      const Two ee = two(e[k], e[k + 1]);
+      s2 = add(s2, ee);
+      t2 = fma(ee, yy, t2);
+      if constexpr (kRef) {
+        const Two zz = fma(two(z[k], z[k + 1]), unit, from_r);
+        split(zz, z[k], z[k + 1]);
+        sr2 = add(sr2, two(exp2_fast(z[k]), exp2_fast(z[k + 1])));
+        const Two d = fma(zz, two(-1.0f, -1.0f), yy);
+        split(d, z[k], z[k + 1]);
+        u2 = fma(ee, d, u2);
       }
+    }
+    v.s = sum_lanes<kLanes>(both(s2));
+    v.t = sum_lanes<kLanes>(both(t2));
+    v.sr = v.u = 0.0f;
+    if constexpr (kRef) {
+      v.sr = sum_lanes<kLanes>(both(sr2));
+      v.u = sum_lanes<kLanes>(both(u2));
+    }
+    const float y_a = fmaf(x_a, kLog2e, -v.m);
+    if constexpr (!kPolicy) {
+      if (l == 0 && real) store_score(o, row, used, v, y_a);
     } else {
       Coefs c{0.0f, 0.0f, 0.0f, 0.0f};
       float logp = 0.0f;
-      if (used) c = policy_row<kRef>(a, row, v, y_a, w, scale, acc, logp);
-      if (a.logp && lane == 0) a.logp[row] = logp;
+      if (used) {
+        Terms terms;
+        c = policy_row<kRef>(a, in, v, y_a, scale, terms, logp);
+        if (l == 0) terms.add_to(acc, in.weight);
+      }
+      if (a.logp && l == 0 && real) a.logp[row] = logp;
       if (a.dlogits) {
-        const i64 at = row * a.ldd;
+        const Two c0 = two(c.c0, c.c0), c1 = two(c.c1, c.c1), c2 = two(c.c2, c.c2);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-          const int j = lane + 32 * k;
-          float g = 0.0f;
-          if (used) {
-            g = fmaf(c.c1, y[k], c.c0);
-            if constexpr (kRef) g = fmaf(c.c2, z[k], g);
-            g *= exp2_fast(y[k]);
-            if (j == static_cast<int>(action)) g += c.hot;
-          }
-          if (j < r.vocab) store_one(a.dlogits, a.dtype, at + j, g);
+        for (int k = 0; k < kPer; k += 2) {
+          Two g = fma(c1, two(y[k], y[k + 1]), c0);
+          if constexpr (kRef) g = fma(c2, two(z[k], z[k + 1]), g);
+          g = mul(g, two(e[k], e[k + 1]));
+          split(g, y[k], y[k + 1]);
         }
-        for (int j = r.vocab + lane; j < a.width; j += 32) store_one(a.dlogits, a.dtype, at + j, 0.0f);
+        // The action's entry once more, with the hot term, by the lane that holds it.
+        float hot = 0.0f;
+        const bool mine = l == action % kLanes;
+        if (used && mine) {
+          hot = fmaf(c.c1, y_a, c.c0);
+          if constexpr (kRef) {
+            const float z_a = fmaf(max_nan(to_float(z_row[action]), kMasked), kLog2e, -v.mr);
+            hot = fmaf(c.c2, y_a - z_a, hot);
+          }
+          hot = fmaf(hot, exp2_fast(y_a), c.hot);
+        }
+        const uintptr_t to = reinterpret_cast<uintptr_t>(a.dlogits) + first * a.ldd * grad_bytes;
+        const int lead = lay.grad ? static_cast<int>(to & 15) : 0;
+        void* const base = lay.grad ? static_cast<void*>(out + lead) : a.dlogits;
+        const i64 d_row = lay.grad ? static_cast<i64>(sub) * a.ldd : row * a.ldd;
+        if (real) {
+#pragma unroll
+          for (int k = 0; k < kPer; ++k) {
+            const int j = l + kLanes * k;
+            // A row that does not count may hold anything: its zeros are written as such.
+            if (j < r.vocab) store_one(base, a.dtype, d_row + j, used ? y[k] : 0.0f);
+          }
+          for (int j = r.vocab + l; j < a.width; j += kLanes) store_one(base, a.dtype, d_row + j, 0.0f);
+          if (used && mine) store_one(base, a.dtype, d_row + action, hot);
+        }
+        if (lay.grad) {
+          __syncwarp();
+          const int n = static_cast<int>(r.rows - first < kRows ? r.rows - first : kRows);
+          const int end = lead + static_cast<int>(((n - 1) * a.ldd + a.width) * grad_bytes);
+          char* const global = reinterpret_cast<char*>(to - lead);
+          for (int k = 16 * lane; k < end; k += 512) {
+            if (k >= lead && k + 16 <= end) {
+              __stcs(reinterpret_cast<uint4*>(global + k), *reinterpret_cast<const uint4*>(out + k));
+            } else {  // the run's ends: its own bytes only
+              for (int b = k < lead ? lead : k; b < k + 16 && b < end; b += 2)
+                *reinterpret_cast<uint16_t*>(global + b) = *reinterpret_cast<const uint16_t*>(out + b);
+            }
+          }
+        }
       }
     }
+    __syncwarp();  // the stage and the gradient's place are free again
   }
-  if constexpr (kPolicy) store_partial(a, acc);
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if constexpr (kPolicy) {
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) acc[k] = sum_warp(acc[k]);
+    store_partial(a, acc);
+  }
 }
 
 // ---- long rows: a block, or a cluster of blocks, per row -----------------------------------
@@ -425,6 +637,27 @@ constexpr int kUnroll = 4;  // vectors of a thread in flight
 
 template <typename T>
 constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4 raw, float (&f)[kVec<T>]) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = __uint_as_float(raw.x), f[1] = __uint_as_float(raw.y);
+    f[2] = __uint_as_float(raw.z), f[3] = __uint_as_float(raw.w);
+  } else {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        f[2 * e] = __uint_as_float(w[e] << 16);
+        f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+      } else {
+        const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+        f[2 * e] = t.x;
+        f[2 * e + 1] = t.y;
+      }
+    }
+  }
+}
 
 // Up to kN flags of `legal`, as bits.
 template <int kN>
@@ -458,35 +691,44 @@ struct Part {
   int vocab;
   bool z_wide;        // the reference's vectors are aligned as the row's are
 
-  __device__ __forceinline__ void load(int v, float (&f)[kVec<T>]) const {
-    const int c = head + v * kVec<T>;
-    unpack(__ldg(reinterpret_cast<const uint4*>(x + c)), f);
-    mask(c, f);
+  // Vector v's 16 bytes.  The last look at an entry says that it is the last.
+  template <bool kLast>
+  __device__ __forceinline__ uint4 load(int v) const {
+    const uint4* at = reinterpret_cast<const uint4*>(x + head + v * kVec<T>);
+    return kLast ? __ldcs(at) : __ldg(at);
   }
-  __device__ __forceinline__ void load_ref(int v, float (&f)[kVec<T>]) const {
-    const int c = head + v * kVec<T>;
-    if (z_wide) {
-      unpack(__ldg(reinterpret_cast<const uint4*>(z + c)), f);
-    } else {
+  __device__ __forceinline__ uint4 load_ref(int v) const {
+    const T* at = z + head + v * kVec<T>;
+    if (z_wide) return __ldg(reinterpret_cast<const uint4*>(at));
+    union {
+      uint4 raw;
+      uint16_t half[8];
+      uint32_t word[4];
+    } u;
 #pragma unroll
-      for (int e = 0; e < kVec<T>; ++e) f[e] = to_float(z[c + e]);
+    for (int e = 0; e < kVec<T>; ++e) {
+      if constexpr (sizeof(T) == 4) u.word[e] = reinterpret_cast<const uint32_t*>(at)[e];
+      else u.half[e] = reinterpret_cast<const uint16_t*>(at)[e];
     }
-    mask(c, f);
+    return u.raw;
   }
-  __device__ __forceinline__ void mask(int c, float (&f)[kVec<T>]) const {
+  // The vector's entries, masked.  Entries at or below the bound are rare: one look at
+  // the smallest tells.
+  __device__ __forceinline__ void entries(int v, const uint4 raw, float (&f)[kVec<T>]) const {
+    unpack<T>(raw, f);
+    float low = min3(f[0], f[1], f[2]);
+    if constexpr (kVec<T> == 8) low = min3(min3(low, f[3], f[4]), min3(f[5], f[6], f[7]), f[7]);
+    else low = fminf(low, f[3]);
+    if (!(low > kMasked)) {
 #pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) f[e] = max_nan(f[e], kMasked);
+      for (int e = 0; e < kVec<T>; ++e) f[e] = max_nan(f[e], kMasked);
+    }
     if (lm) {
-      const unsigned bits = legal_bits<kVec<T>>(lm + c);
+      const unsigned bits = legal_bits<kVec<T>>(lm + head + v * kVec<T>);
 #pragma unroll
       for (int e = 0; e < kVec<T>; ++e)
         if (!(bits >> e & 1u)) f[e] = kMasked;
     }
-  }
-  static __device__ __forceinline__ void unpack(const uint4 raw, float (&f)[kVec<T>]) {
-    const T* t = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) f[e] = to_float(t[e]);
   }
   // Entry number i of those outside the vectors, or -1: rank 0 takes them all.
   __device__ __forceinline__ int loose(int i) const {
@@ -499,59 +741,100 @@ struct Part {
   }
 };
 
-// Adds kN entries to a thread's running sums.
+// A thread's running sums, the odd and the even entries' side by side.
+struct Running {
+  float m, mr;
+  Two s, t, sr, u;
+};
+
 template <bool kRef, int kN>
-__device__ __forceinline__ void add(Sums& v, const float (&x)[kN], const float (&z)[kN]) {
-  float top = x[0];
-#pragma unroll
-  for (int e = 1; e < kN; ++e) top = max_nan(top, x[e]);
-  top *= kLog2e;
+__device__ __forceinline__ float largest(const float (&x)[kN]) {
+  float top = max_nan(x[0], x[1], x[2]);
+  if constexpr (kN == 8) return max_nan(max_nan(top, x[3], x[4]), max_nan(x[5], x[6], x[7]));
+  else return max_nan(top, x[3]);
+}
+
+// Adds kN entries, with a new maximum where they bring one.
+template <bool kRef, int kN>
+__device__ __forceinline__ void accumulate(Running& v, const float (&x)[kN], const float (&z)[kN]) {
+  const float top = largest<kRef>(x) * kLog2e;
   if (!(top <= v.m)) {  // also for NaN
     const float d = v.m - top, f = exp2_fast(d);
-    v.t = f * (v.t + d * v.s);
-    if constexpr (kRef) v.u = f * (v.u + d * v.s);
-    v.s *= f;
+    const Two dd = two(d, d), ff = two(f, f);
+    v.t = mul(ff, fma(dd, v.s, v.t));
+    if constexpr (kRef) v.u = mul(ff, fma(dd, v.s, v.u));
+    v.s = mul(v.s, ff);
     v.m = top;
   }
-  float zz[kN];
   if constexpr (kRef) {
-    float top_r = z[0];
-#pragma unroll
-    for (int e = 1; e < kN; ++e) top_r = max_nan(top_r, z[e]);
-    top_r *= kLog2e;
+    const float top_r = largest<kRef>(z) * kLog2e;
     if (!(top_r <= v.mr)) {
-      const float d = v.mr - top_r;
-      v.u -= d * v.s;
-      v.sr *= exp2_fast(d);
+      const float d = v.mr - top_r, f = exp2_fast(d);
+      v.u = fma(two(-d, -d), v.s, v.u);
+      v.sr = mul(v.sr, two(f, f));
       v.mr = top_r;
     }
   }
+  const Two unit = two(kLog2e, kLog2e), from = two(-v.m, -v.m), from_r = two(-v.mr, -v.mr);
 #pragma unroll
-  for (int e = 0; e < kN; ++e) {
-    const float y = fmaf(x[e], kLog2e, -v.m), p = exp2_fast(y);
-    v.s += p;
-    v.t = fmaf(p, y, v.t);
+  for (int e = 0; e < kN; e += 2) {
+    const Two y = fma(two(x[e], x[e + 1]), unit, from);
+    float y0, y1;
+    split(y, y0, y1);
+    const Two p = two(exp2_fast(y0), exp2_fast(y1));
+    v.s = add(v.s, p);
+    v.t = fma(p, y, v.t);
     if constexpr (kRef) {
-      zz[e] = fmaf(z[e], kLog2e, -v.mr);
-      v.sr += exp2_fast(zz[e]);
-      v.u = fmaf(p, y - zz[e], v.u);
+      const Two q = fma(two(z[e], z[e + 1]), unit, from_r);
+      float q0, q1;
+      split(q, q0, q1);
+      v.sr = add(v.sr, two(exp2_fast(q0), exp2_fast(q1)));
+      v.u = fma(p, fma(q, two(-1.0f, -1.0f), y), v.u);
     }
   }
 }
 
+// d_j of a vector's entries; `hot`: the action's place among them, or none of theirs.
+template <bool kRef, int kN>
+__device__ __forceinline__ void gradient(const Coefs& c, float m, float mr, const float (&x)[kN],
+                                         const float (&z)[kN], int hot, float (&g)[kN]) {
+  const Two unit = two(kLog2e, kLog2e), from = two(-m, -m), from_r = two(-mr, -mr);
+  const Two c0 = two(c.c0, c.c0), c1 = two(c.c1, c.c1), c2 = two(c.c2, c.c2);
+#pragma unroll
+  for (int e = 0; e < kN; e += 2) {
+    const Two y = fma(two(x[e], x[e + 1]), unit, from);
+    Two d = fma(c1, y, c0);
+    if constexpr (kRef) {
+      const Two q = fma(two(z[e], z[e + 1]), unit, from_r);
+      d = fma(c2, fma(q, two(-1.0f, -1.0f), y), d);
+    }
+    float y0, y1;
+    split(y, y0, y1);
+    split(mul(d, two(exp2_fast(y0), exp2_fast(y1))), g[e], g[e + 1]);
+  }
+  if (hot >= 0 && hot < kN)
+#pragma unroll
+    for (int e = 0; e < kN; ++e)
+      if (hot == e) g[e] += c.hot;
+}
+
 template <typename T, bool kRef, bool kPolicy>
-__global__ void __launch_bounds__(kLongThreads) long_rows_kernel(const Rows r, const Score o, const Policy a) {
+__global__ void __launch_bounds__(kLongThreads, 2) long_rows_kernel(const Rows r, const Score o, const Policy a) {
   constexpr int kN = kVec<T>;
   __shared__ Sums warp_sums[2][kLongThreads / 32];
   __shared__ Sums block_sums[2];
   const cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), rank = cluster.block_rank();
-  const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x / 32, step = blockDim.x;
+  __shared__ double block_acc[kSums];  // thread 0's
   float scale = 0.0f;
-  double acc[kSums] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
+  if (tid == 0)
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) block_acc[k] = 0.0;
   if constexpr (kPolicy) scale = grad_scale_of(a, block_denominator(a, r.weight, r.rows));
   int buffer = 0;
   for (i64 row = blockIdx.x / parts; row < r.rows; row += gridDim.x / parts) {
+    const RowInputs in = row_inputs<kPolicy>(r, a, row);
     Part<T> p;
     p.x = static_cast<const T*>(r.logits) + row * r.ld;
     p.z = kRef ? static_cast<const T*>(r.ref) + row * r.ldr : nullptr;
@@ -565,31 +848,48 @@ __global__ void __launch_bounds__(kLongThreads) long_rows_kernel(const Rows r, c
     p.first = each * rank < p.vectors ? each * rank : p.vectors;
     p.last = p.first + each < p.vectors ? p.first + each : p.vectors;
     const int n_loose = rank == 0 ? r.vocab - p.vectors * kN : 0;
-    const i64 action = r.actions[row];
-    const float w = r.weight ? r.weight[row] : 1.0f;
-    bool used = w != 0.0f && action >= 0 && action < r.vocab;
-    float x_a = kMasked;
-    if (used) x_a = p.one(p.x, static_cast<int>(action));
-    used = used && !(x_a <= kMasked);
+    bool used = in.weight != 0.0f && in.action >= 0 && in.action < r.vocab;  // the same in the whole cluster
+    const int action = used ? static_cast<int>(in.action) : 0;
+    const float x_a = p.one(p.x, action);
     Sums v = no_sums();
     if (used) {
-      for (int i = p.first + tid; i < p.last; i += kUnroll * blockDim.x) {
-        float x[kUnroll][kN], z[kUnroll][kN];
+      Running run;
+      run.m = run.mr = kMasked2;
+      run.s = run.t = run.sr = run.u = two(0.0f, 0.0f);
+      for (int i = p.first + tid; i < p.last; i += kUnroll * step) {
+        uint4 x[kUnroll], z[kUnroll];
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k)
-          if (i + k * (int)blockDim.x < p.last) {
-            p.load(i + k * blockDim.x, x[k]);
-            if constexpr (kRef) p.load_ref(i + k * blockDim.x, z[k]);
+          if (i + k * step < p.last) {
+            x[k] = p.template load<!kPolicy>(i + k * step);
+            if constexpr (kRef) z[k] = p.load_ref(i + k * step);
           }
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k)
-          if (i + k * (int)blockDim.x < p.last) add<kRef>(v, x[k], z[k]);
+          if (i + k * step < p.last) {
+            float f[kN], q[kN];
+            p.entries(i + k * step, x[k], f);
+            if constexpr (kRef) p.entries(i + k * step, z[k], q);
+            accumulate<kRef>(run, f, q);
+          }
       }
       if (tid < n_loose) {
+        // One entry, and three that add nothing beside it.
         const int c = p.loose(tid);
-        const float x[1] = {p.one(p.x, c)};
-        const float z[1] = {kRef ? p.one(p.z, c) : 0.0f};
-        add<kRef>(v, x, z);
+        const float f[4] = {p.one(p.x, c), kMasked, kMasked, kMasked};
+        float q[4] = {kMasked, kMasked, kMasked, kMasked};
+        if constexpr (kRef) q[0] = p.one(p.z, c);
+        // Where nothing else was seen the three would weigh as much as a masked entry:
+        // a row of nothing else does not count, and beside any other they are 0.
+        accumulate<kRef>(run, f, q);
+      }
+      v.m = run.m;
+      v.s = both(run.s);
+      v.t = both(run.t);
+      if constexpr (kRef) {
+        v.mr = run.mr;
+        v.sr = both(run.sr);
+        v.u = both(run.u);
       }
       v = join_warp<kRef>(v);
       if (lane == 0) warp_sums[buffer][tid >> 5] = v;
@@ -603,56 +903,46 @@ __global__ void __launch_bounds__(kLongThreads) long_rows_kernel(const Rows r, c
       }
       buffer ^= 1;
     }
+    used = used && !(x_a <= kMasked);
     const float y_a = fmaf(x_a, kLog2e, -v.m);
     if constexpr (!kPolicy) {
-      if (tid == 0 && rank == 0) {
-        const float log_s = used ? log2f(v.s) : INFINITY;
-        if (o.logp) o.logp[row] = used ? kLn2 * (y_a - log_s) : 0.0f;
-        if (o.entropy) o.entropy[row] = used ? kLn2 * (log_s - v.t / v.s) : 0.0f;
-        if (o.lse) o.lse[row] = make_float2(used ? v.m : 0.0f, log_s);
-        if (o.zeros) o.zeros[row] = 0.0f;
-      }
+      if (tid == 0 && rank == 0) store_score(o, row, used, v, y_a);
     } else {
       Coefs c{0.0f, 0.0f, 0.0f, 0.0f};
       float logp = 0.0f;
-      // Every thread has the coefficients; one of the row's counts its sums.
-      double mine[kSums] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
-      if (used) c = policy_row<kRef>(a, row, v, y_a, w, scale, mine, logp);
+      // Every thread has the coefficients; one of the row's counts its terms.
+      Terms terms;
+      if (used) c = policy_row<kRef>(a, in, v, y_a, scale, terms, logp);
       if (tid == 0 && rank == 0) {
         if (a.logp) a.logp[row] = logp;
-#pragma unroll
-        for (int k = 0; k < kSums; ++k) acc[k] += mine[k];
+        if (used) terms.add_to(block_acc, in.weight);
       }
       if (a.dlogits) {
         const i64 at = row * a.ldd;
         const uintptr_t to = reinterpret_cast<uintptr_t>(a.dlogits) + (at + p.head) * type_bytes(a.dtype);
         const int bytes = kN * type_bytes(a.dtype);
         const bool wide = to % (bytes < 16 ? bytes : 16) == 0;
-        const int hot = static_cast<int>(action);
-        for (int i = p.first + tid; i < p.last; i += kUnroll * blockDim.x) {
-          float x[kUnroll][kN], z[kUnroll][kN];
+        for (int i = p.first + tid; i < p.last; i += kUnroll * step) {
+          uint4 x[kUnroll], z[kUnroll];
 #pragma unroll
           for (int k = 0; k < kUnroll; ++k)
-            if (used && i + k * (int)blockDim.x < p.last) {
-              p.load(i + k * blockDim.x, x[k]);
-              if constexpr (kRef) p.load_ref(i + k * blockDim.x, z[k]);
+            if (used && i + k * step < p.last) {
+              x[k] = p.template load<true>(i + k * step);
+              if constexpr (kRef) z[k] = p.load_ref(i + k * step);
             }
 #pragma unroll
           for (int k = 0; k < kUnroll; ++k) {
-            if (i + k * (int)blockDim.x >= p.last) break;
-            const int at_c = p.head + (i + k * blockDim.x) * kN;
-            float g[kN];
+            if (i + k * step >= p.last) break;
+            const int at_c = p.head + (i + k * step) * kN;
+            float f[kN], q[kN], g[kN];
+            if (used) {
+              p.entries(i + k * step, x[k], f);
+              if constexpr (kRef) p.entries(i + k * step, z[k], q);
+              gradient<kRef>(c, v.m, v.mr, f, q, action - at_c, g);
+            } else {
 #pragma unroll
-            for (int e = 0; e < kN; ++e) {
-              const float y = fmaf(x[k][e], kLog2e, -v.m);
-              g[e] = fmaf(c.c1, y, c.c0);
-              if constexpr (kRef) g[e] = fmaf(c.c2, y - fmaf(z[k][e], kLog2e, -v.mr), g[e]);
-              g[e] = used ? g[e] * exp2_fast(y) : 0.0f;
+              for (int e = 0; e < kN; ++e) g[e] = 0.0f;
             }
-            if (used && hot >= at_c && hot < at_c + kN)
-#pragma unroll
-              for (int e = 0; e < kN; ++e)
-                if (hot == at_c + e) g[e] += c.hot;
             store_grad<kN>(a.dlogits, a.dtype, at + at_c, g, wide);
           }
         }
@@ -664,17 +954,20 @@ __global__ void __launch_bounds__(kLongThreads) long_rows_kernel(const Rows r, c
             g = fmaf(c.c1, y, c.c0);
             if constexpr (kRef) g = fmaf(c.c2, y - fmaf(p.one(p.z, j), kLog2e, -v.mr), g);
             g *= exp2_fast(y);
-            if (j == hot) g += c.hot;
+            if (j == action) g += c.hot;
           }
           store_one(a.dlogits, a.dtype, at + j, g);
         }
         if (rank == 0)
-          for (int j = r.vocab + tid; j < a.width; j += blockDim.x) store_one(a.dlogits, a.dtype, at + j, 0.0f);
+          for (int j = r.vocab + tid; j < a.width; j += step) store_one(a.dlogits, a.dtype, at + j, 0.0f);
       }
     }
   }
   if (parts > 1) cluster.sync();  // no block leaves while another may read its sums
-  if constexpr (kPolicy) store_partial(a, acc);
+  if constexpr (kPolicy)
+    if (tid == 0 && a.partial)
+#pragma unroll
+      for (int k = 0; k < kSums; ++k) a.partial[(i64)blockIdx.x * kSums + k] = block_acc[k];
 }
 
 // ---- the means of policy_loss ---------------------------------------------------------------
@@ -768,26 +1061,22 @@ __global__ void __launch_bounds__(32 * kBackWarps) logp_backward_kernel(const Ro
   p.head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p.x) & 15)) & 15) / static_cast<int>(sizeof(T));
   if (p.head > p.vocab) p.head = p.vocab;
   p.vectors = (p.vocab - p.head) / kN;
-  const i64 hot = r.actions[row] - c0;
+  const int hot = static_cast<int>(r.actions[row]) - c0;  // in the row: it counts
   const uintptr_t to = reinterpret_cast<uintptr_t>(b.dlogits) + (at + c0 + p.head) * type_bytes(b.dtype);
   const int bytes = kN * type_bytes(b.dtype);
   const bool wide = to % (bytes < 16 ? bytes : 16) == 0;
   for (int i = lane; i < p.vectors; i += kUnroll * 32) {
-    float x[kUnroll][kN];
+    uint4 x[kUnroll];
 #pragma unroll
     for (int q = 0; q < kUnroll; ++q)
-      if (i + 32 * q < p.vectors) p.load(i + 32 * q, x[q]);
+      if (i + 32 * q < p.vectors) x[q] = p.template load<true>(i + 32 * q);
 #pragma unroll
     for (int q = 0; q < kUnroll; ++q) {
       if (i + 32 * q >= p.vectors) break;
       const int c = p.head + (i + 32 * q) * kN;
-      float g[kN];
-#pragma unroll
-      for (int e = 0; e < kN; ++e) {
-        const float y = fmaf(x[q][e], kLog2e, -lse.x);
-        g[e] = fmaf(k.c1, y, k.c0) * exp2_fast(y);
-        if (hot == c + e) g[e] += k.hot;
-      }
+      float f[kN], g[kN];
+      p.entries(i + 32 * q, x[q], f);
+      gradient<false>(k, lse.x, 0.0f, f, f, hot - c, g);
       store_grad<kN>(b.dlogits, b.dtype, at + c0 + c, g, wide);
     }
   }
@@ -943,30 +1232,33 @@ int check_rows(const Rows& r, int dtype) {
   return CUGO_B200_OK;
 }
 
-constexpr int kShortMost = 1024;  // entries of a short row
+constexpr int kShortShared = 111 << 10;  // bytes of shared memory of a block of short rows: two per SM
 
 // How a launch goes over the rows.
 struct Plan {
-  bool is_short;
   int threads, blocks, parts;
 };
 
-Plan plan_of(i64 rows, int vocab) {
+// A block per row, or a cluster: few rows are spread over up to 8 blocks, each with at
+// least 4,096 entries.
+Plan long_plan(i64 rows, int vocab) {
   Plan p{};
-  p.is_short = vocab <= kShortMost;
   p.parts = 1;
-  if (p.is_short) {
-    p.threads = 32 * kShortWarps;
-    const i64 want = (rows + kShortWarps - 1) / kShortWarps;
-    p.blocks = static_cast<int>(want < 8 * kSms ? want : 8 * kSms);
-    return p;
-  }
-  p.threads = vocab <= 4096 ? 128 : vocab <= 16384 ? 256 : kLongThreads;
-  // Few rows: a row over up to 8 blocks, each with at least 4,096 entries.
+  p.threads = vocab <= 4096 ? 128 : vocab <= 65536 ? 256 : kLongThreads;
   while (p.parts < 8 && rows * p.parts < kSms && vocab / (2 * p.parts) >= 4096) p.parts *= 2;
-  const i64 most = static_cast<i64>(kSms) * (2048 / p.threads) / p.parts;
+  const i64 most = static_cast<i64>(kSms) * (1024 / p.threads) / p.parts;
   p.blocks = static_cast<int>(rows < most ? rows : most) * p.parts;
   return p;
+}
+
+inline int round16(i64 n) { return static_cast<int>((n + 15) / 16 * 16); }
+
+// Bytes of a run of n rows in shared memory (with a granule for its alignment), or 0
+// where the rows do not lie one after another (up to 64 bytes between them are copied
+// along).
+inline int run_bytes(i64 n, i64 ld, i64 vocab, int size) {
+  if (n > 1 && (ld < vocab || (ld - vocab) * size > 64)) return 0;
+  return round16(((n - 1) * ld + vocab) * size + 15);
 }
 
 template <typename K>
@@ -984,28 +1276,53 @@ int launch_long(K kernel, const Plan& p, const Rows& r, const Score& o, const Po
   return cudaLaunchKernelEx(&cfg, kernel, r, o, a) == cudaSuccess ? CUGO_B200_OK : CUGO_B200_ERR_LAUNCH;
 }
 
-template <typename T, bool kRef, bool kPolicy>
-int launch_rows(const Plan& p, const Rows& r, const Score& o, const Policy& a, cudaStream_t stream) {
-  if (!p.is_short) return launch_long(long_rows_kernel<T, kRef, kPolicy>, p, r, o, a, stream);
-  const int per = (r.vocab + 31) / 32;
-#define CUGO_SHORT(n)                                                                            \
-  if (per <= n) {                                                                                \
-    short_rows_kernel<T, n, kRef, kPolicy><<<p.blocks, p.threads, 0, stream>>>(r, o, a);        \
-    return launch_status();                                                                      \
+template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy>
+int launch_short(const Rows& r, const Score& o, const Policy& a, cudaStream_t stream, int& blocks) {
+  constexpr int kRows = 32 / kLanes;
+  const auto kernel = short_rows_kernel<T, kLanes, kPer, kRef, kPolicy>;
+  Layout lay{};
+  lay.logits = run_bytes(kRows, r.ld, r.vocab, sizeof(T));
+  if (kRef) lay.ref = run_bytes(kRows, r.ldr, r.vocab, sizeof(T));
+  if (r.legal) lay.legal = run_bytes(kRows, r.ldm, r.vocab, 1);
+  // Between the rows of a wider gradient stands what is not this call's to write.
+  if (a.dlogits && (a.ldd == a.width || kRows == 1)) lay.grad = run_bytes(kRows, a.ldd, a.width, type_bytes(a.dtype));
+  while (lay.warp() * kShortWarps > kShortShared) {  // the largest goes without
+    int& most = lay.grad >= lay.logits && lay.grad >= lay.ref ? lay.grad : lay.logits >= lay.ref ? lay.logits : lay.ref;
+    most = 0;
   }
-  CUGO_SHORT(2)
-  CUGO_SHORT(6)
-  CUGO_SHORT(12)
-  CUGO_SHORT(32)
-#undef CUGO_SHORT
-  return CUGO_B200_ERR_ARG;
+  const int shared = lay.warp() * kShortWarps;
+  if (shared > (44 << 10) &&  // with the static part, past what needs no opt-in
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShortShared) != cudaSuccess)
+    return CUGO_B200_ERR_LAUNCH;
+  const i64 want = (r.rows + kShortWarps * kRows - 1) / (kShortWarps * kRows);
+  int per_sm = shared > 0 ? (220 << 10) / (shared + 1024) : 4;
+  per_sm = per_sm > 4 ? 4 : per_sm;
+  blocks = static_cast<int>(want < per_sm * kSms ? want : per_sm * kSms);
+  kernel<<<blocks, 32 * kShortWarps, shared, stream>>>(r, o, a, lay);
+  return launch_status();
 }
 
+template <typename T, bool kRef, bool kPolicy>
+int launch_rows(const Rows& r, const Score& o, const Policy& a, cudaStream_t stream, int& blocks) {
+#define CUGO_SHORT(lanes, per) \
+  if (r.vocab <= (lanes) * (per)) return launch_short<T, lanes, per, kRef, kPolicy>(r, o, a, stream, blocks)
+  CUGO_SHORT(8, 4);
+  CUGO_SHORT(8, 8);
+  CUGO_SHORT(8, 24);
+  CUGO_SHORT(16, 24);
+  CUGO_SHORT(32, 32);
+#undef CUGO_SHORT
+  const Plan p = long_plan(r.rows, r.vocab);
+  blocks = p.blocks;
+  return launch_long(long_rows_kernel<T, kRef, kPolicy>, p, r, o, a, stream);
+}
+
+// blocks: how many ran, each with a partial sum.
 template <bool kRef, bool kPolicy>
-int launch_typed(int dtype, const Plan& p, const Rows& r, const Score& o, const Policy& a, cudaStream_t stream) {
-  if (dtype == kFp32) return launch_rows<float, kRef, kPolicy>(p, r, o, a, stream);
-  if (dtype == kBf16) return launch_rows<__nv_bfloat16, kRef, kPolicy>(p, r, o, a, stream);
-  return launch_rows<__half, kRef, kPolicy>(p, r, o, a, stream);
+int launch_typed(int dtype, const Rows& r, const Score& o, const Policy& a, cudaStream_t stream, int& blocks) {
+  if (dtype == kFp32) return launch_rows<float, kRef, kPolicy>(r, o, a, stream, blocks);
+  if (dtype == kBf16) return launch_rows<__nv_bfloat16, kRef, kPolicy>(r, o, a, stream, blocks);
+  return launch_rows<__half, kRef, kPolicy>(r, o, a, stream, blocks);
 }
 
 inline i64 weight_blocks(i64 rows) {
@@ -1013,7 +1330,7 @@ inline i64 weight_blocks(i64 rows) {
   return b < kSms ? b : kSms;
 }
 
-constexpr int kMostBlocks = 16 * kSms;
+constexpr int kMostBlocks = 8 * kSms;  // of any launch over rows
 
 }  // namespace
 
@@ -1029,7 +1346,8 @@ int cugo_b200_action_logp(const void* logits, int64_t ld, int32_t dtype, const b
   if (!aligned(lse, 8)) return CUGO_B200_ERR_ALIGN;
   if (rows == 0) return CUGO_B200_OK;
   const Score o{logp, entropy, reinterpret_cast<float2*>(lse), zeros};
-  return launch_typed<false, false>(dtype, plan_of(rows, r.vocab), r, o, Policy{}, stream);
+  int blocks;
+  return launch_typed<false, false>(dtype, r, o, Policy{}, stream, blocks);
 }
 
 int cugo_b200_action_logp_backward(const void* logits, int64_t ld, int32_t dtype, const bool* legal,
@@ -1114,11 +1432,11 @@ int cugo_b200_policy_loss(const void* logits, int64_t ld, int32_t dtype, const v
     a.weight_sums = sums;
     a.n_weight_sums = static_cast<int>(blocks);
   }
-  const Plan p = plan_of(rows, r.vocab);
-  const int rc = ref_logits ? launch_typed<true, true>(dtype, p, r, Score{}, a, stream)
-                            : launch_typed<false, true>(dtype, p, r, Score{}, a, stream);
+  int blocks = 0;
+  const int rc = ref_logits ? launch_typed<true, true>(dtype, r, Score{}, a, stream, blocks)
+                            : launch_typed<false, true>(dtype, r, Score{}, a, stream, blocks);
   if (rc || !stats) return rc;
-  policy_means_kernel<<<1, 32 * kSums, 0, stream>>>(a, weight, rows, p.blocks, stats, loss);
+  policy_means_kernel<<<1, 32 * kSums, 0, stream>>>(a, weight, rows, blocks, stats, loss);
   return launch_status();
 }
 

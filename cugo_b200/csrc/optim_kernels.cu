@@ -70,7 +70,7 @@ struct Scalars {
   float clip;       // c
   float step_size;  // lr / (1 - b1^t)
   float keep;       // 1 - lr wd
-  float bias2;      // 1 - b2^t
+  float inv_bias2;  // 1 / (1 - b2^t)
   uint32_t key;     // of the random bits
 };
 
@@ -83,13 +83,13 @@ struct Options {
 
 // A 32-bit mixer: xor-shifts and odd products (constants found by C. Wellons' search for
 // low bias, 2018).
-__device__ __forceinline__ uint32_t mix(uint32_t x) {
-  x ^= x >> 16;
+__device__ __forceinline__ uint32_t mix_rest(uint32_t x) {  // after the first shift
   x *= 0x7feb352du;
   x ^= x >> 15;
   x *= 0x846ca68bu;
   return x ^ (x >> 16);
 }
+__device__ __forceinline__ uint32_t mix(uint32_t x) { return mix_rest(x ^ (x >> 16)); }
 
 __device__ __forceinline__ double sum_warp(double v) {
 #pragma unroll
@@ -164,7 +164,8 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, i64 i, i64 n, const flo
   }
 }
 
-__device__ __forceinline__ void load_codes(const uint8_t* p, i64 i, i64 n, float scale, float (&f)[8]) {
+// 8 codes as floats, not scaled.
+__device__ __forceinline__ void load_codes(const uint8_t* p, i64 i, i64 n, float (&f)[8]) {
   uint32_t w[2] = {0, 0};
   if (i + 8 <= n && vector_ok(p, 8)) {
     const uint2 q = *reinterpret_cast<const uint2*>(p + i);
@@ -178,18 +179,19 @@ __device__ __forceinline__ void load_codes(const uint8_t* p, i64 i, i64 n, float
   for (int e = 0; e < 4; ++e) {
     const __nv_fp8x2_storage_t two = static_cast<__nv_fp8x2_storage_t>(w[e / 2] >> (16 * (e % 2)));
     const float2 t = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
-    f[2 * e] = t.x * scale;
-    f[2 * e + 1] = t.y * scale;
+    f[2 * e] = t.x;
+    f[2 * e + 1] = t.y;
   }
 }
 
 __device__ __forceinline__ void store_codes(uint8_t* p, i64 i, i64 n, const float (&f)[8]) {
-  uint32_t w[2] = {0, 0};
+  uint32_t w[2];
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    w[e / 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(f[2 * e], f[2 * e + 1]), __NV_SATFINITE,
-                                                                __NV_E4M3))
-                << (16 * (e % 2));
+  for (int e = 0; e < 2; ++e) {
+    const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * e], f[4 * e + 1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * e + 2], f[4 * e + 3]), __NV_SATFINITE, __NV_E4M3);
+    w[e] = __byte_perm(a, b, 0x5410);
+  }
   if (i + 8 <= n && vector_ok(p, 8)) {
     *reinterpret_cast<uint2*>(p + i) = make_uint2(w[0], w[1]);
   } else {
@@ -211,19 +213,26 @@ __device__ __forceinline__ int scale_byte(float largest) {
   return e < 27 ? 27 : e > 247 ? 247 : e;
 }
 
-// x (at most 448 in magnitude) rounded to e4m3's grid, up where the 16 random bits r say
-// so: below 2^-6 the steps are 2^-9, above they are 1/8 of the power of two.  Infinities
-// and NaN become NaN.
-__device__ __forceinline__ float round_e4m3(float x, uint32_t r) {
-  const float a = fabsf(x);
-  const float low = a < 0.015625f ? 0.015625f : 0.0f;
-  const uint32_t bits = (__float_as_uint(a + low) + (r << 4) + 8u) & 0xfff00000u;
-  const float q = copysignf(__uint_as_float(bits) - low, x);
-  return a <= 448.0f ? q : __uint_as_float(0x7fc00000u);
+// The magnitude a (at most 448) rounded to e4m3's grid, up where the 16 random bits in
+// r16 (at bit 4) say so: below 2^-6 the steps are 2^-9, which 2^-6 more gives the bits
+// the same place; above they are 1/8 of the power of two.
+__device__ __forceinline__ float round_e4m3(float a, uint32_t r16) {
+  float small;  // 1 below 2^-6, else 0
+  asm("set.lt.f32.f32 %0, %1, %2;" : "=f"(small) : "f"(a), "f"(0.015625f));
+  const uint32_t bits = (__float_as_uint(fmaf(small, 0.015625f, a)) + r16 + 8u) & 0xfff00000u;
+  return fmaf(small, -0.015625f, __uint_as_float(bits));
 }
 
-// The largest of a warp's finite magnitudes (as bits they order as the values do).
+// A warp's largest (of non-negative floats, which order as their bits do).
 __device__ __forceinline__ float warp_largest(const float (&f)[8]) {
+  float top = fabsf(f[0]);
+#pragma unroll
+  for (int e = 1; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+  return __uint_as_float(__reduce_max_sync(kFull, __float_as_uint(top)));
+}
+
+// The same over the finite magnitudes only.
+__device__ __noinline__ float warp_largest_finite(const float (&f)[8]) {
   uint32_t top = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -239,61 +248,132 @@ __device__ __forceinline__ float sqrt_fast(float x) {
   return r;
 }
 
+// Two floats in one instruction each.
+struct Two {
+  uint64_t v;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(Two t, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(t.v));
+}
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 template <typename P, typename G, bool kEight, int kMost>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Tensors<kMost> a, const Options o,
                                                          const Scalars* scalars) {
+  constexpr bool kRandom = kEight || sizeof(P) == 2;
   const Scalars s = *scalars;
+  const int lane = threadIdx.x & 31;
   for (i64 tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const Tensor& t = a.t[find(a, tile)];
     const i64 in = (tile - t.first_tile) * (kTile / kBlock) + (threadIdx.x >> 5);  // the warp's block
-    const i64 i = in * kBlock + (threadIdx.x & 31) * kPer;
+    const i64 i = in * kBlock + lane * kPer;
     if (in * kBlock >= t.n) continue;  // the whole warp
     float p[8], g[8], m[8], v[8];
     load8(static_cast<const P*>(t.p), i, t.n, p);
     load8(static_cast<const G*>(t.g), i, t.n, g);
-    if constexpr (kEight) {
-      load_codes(static_cast<const uint8_t*>(t.m), i, t.n, scale_of(t.ms[in]), m);
-      load_codes(static_cast<const uint8_t*>(t.v), i, t.n, scale_of(t.vs[in]), v);
+    float b1 = o.b1, b2 = o.b2;
+    if constexpr (kEight) {  // the scale is a power of two: exact in the factor
+      load_codes(static_cast<const uint8_t*>(t.m), i, t.n, m);
+      load_codes(static_cast<const uint8_t*>(t.v), i, t.n, v);
+      b1 *= scale_of(t.ms[in]);
+      b2 *= scale_of(t.vs[in]);
     } else {
       load8(static_cast<const float*>(t.m), i, t.n, m);
       load8(static_cast<const float*>(t.v), i, t.n, v);
     }
-    const float inv_bias2 = __frcp_rn(s.bias2);
+    const Two clip = two(s.clip, s.clip), c1 = two(o.c1, o.c1), c2 = two(o.c2, o.c2), d1 = two(b1, b1),
+              d2 = two(b2, b2), keep = two(s.keep, s.keep), inv = two(s.inv_bias2, s.inv_bias2);
+    float finite = 0.0f;  // NaN where a parameter is not finite after the step
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float q = g[e] * s.clip;
-      m[e] = o.b1 * m[e] + o.c1 * q;
-      v[e] = o.b2 * v[e] + o.c2 * (q * q);
-      p[e] = p[e] * s.keep - s.step_size * __fdividef(m[e], sqrt_fast(v[e] * inv_bias2) + o.eps);
+    for (int e = 0; e < 8; e += 2) {
+      const Two q = mul(two(g[e], g[e + 1]), clip);
+      const Two mm = fma2(two(m[e], m[e + 1]), d1, mul(q, c1));
+      const Two vv = fma2(two(v[e], v[e + 1]), d2, mul(mul(q, q), c2));
+      const Two kept = mul(two(p[e], p[e + 1]), keep), root = mul(vv, inv);
+      float r[2];
+      split(mm, m[e], m[e + 1]);
+      split(vv, v[e], v[e + 1]);
+      split(kept, p[e], p[e + 1]);
+      split(root, r[0], r[1]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float u = __fdividef(m[e + h], sqrt_fast(r[h]) + o.eps);
+        p[e + h] = fmaf(-s.step_size, u, p[e + h]);
+        if constexpr (kRandom) finite = fmaf(p[e + h], 0.0f, finite);
+      }
     }
     uint32_t r[8];
-    if constexpr (kEight || sizeof(P) == 2) {
-      const i64 number = (t.first_block + in) * kBlock + (threadIdx.x & 31) * kPer;
-      const uint32_t key = s.key + static_cast<uint32_t>(number >> 32) * 0x9e3779b9u;
+    bool rare = false;  // of the warp
+    if constexpr (kRandom) {
+      // i is a multiple of 8, so element e's number differs in the last three bits only:
+      // the mix's first shift is the same for all eight.
+      const i64 number = t.first_block * kBlock + i;
+      uint32_t x = static_cast<uint32_t>(number) ^ (s.key + static_cast<uint32_t>(number >> 32) * 0x9e3779b9u);
+      x ^= x >> 16;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] = mix(static_cast<uint32_t>(number + e) ^ key);
+      for (int e = 0; e < 8; ++e) r[e] = mix_rest(x ^ e);
+      rare = __any_sync(kFull, !(finite == 0.0f));
     }
     if constexpr (sizeof(P) == 2) {
+      if (!rare) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t b = __float_as_uint(p[e]);
-        // Infinities and NaN stay what they are.
-        p[e] = (b & 0x7f800000u) == 0x7f800000u ? p[e] : __uint_as_float(b + ((r[e] * 0x2c1b3c6du) >> 16));
+        for (int e = 0; e < 8; ++e) p[e] = __uint_as_float(__float_as_uint(p[e]) + ((r[e] * 0x2c1b3c6du) >> 16));
+      } else {  // infinities and NaN stay what they are
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t b = __float_as_uint(p[e]);
+          p[e] = (b & 0x7f800000u) == 0x7f800000u ? p[e] : __uint_as_float(b + ((r[e] * 0x2c1b3c6du) >> 16));
+        }
       }
     }
     store8(static_cast<P*>(t.p), i, t.n, p);
     if constexpr (kEight) {
-      const int mb = scale_byte(warp_largest(m)), vb = scale_byte(warp_largest(v));
+      float top_m = warp_largest(m), top_v = warp_largest(v);
+      // A second moment can overflow while its step, and so its parameter, stays finite.
+      rare = rare || !(top_v < INFINITY);
+      if (rare) {
+        top_m = warp_largest_finite(m);
+        top_v = warp_largest_finite(v);
+      }
+      const int mb = scale_byte(top_m), vb = scale_byte(top_v);
       const float mi = inverse_of(mb), vi = inverse_of(vb);
+      const Two mi2 = two(mi, mi), vi2 = two(vi, vi);
+      float cm[8], cv[8];
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        split(mul(two(m[e], m[e + 1]), mi2), cm[e], cm[e + 1]);
+        split(mul(two(v[e], v[e + 1]), vi2), cv[e], cv[e + 1]);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        m[e] = round_e4m3(m[e] * mi, r[e] & 0xffffu);
-        const float q = round_e4m3(v[e] * vi, r[e] >> 16);
-        v[e] = v[e] > 0.0f && q == 0.0f ? 0.001953125f : q;  // 2^-9
+        cm[e] = copysignf(round_e4m3(fabsf(cm[e]), (r[e] << 4) & 0xffff0u), cm[e]);
+        const float q = round_e4m3(cv[e], (r[e] >> 12) & 0xffff0u);
+        cv[e] = v[e] > 0.0f ? fmaxf(q, 0.001953125f) : q;  // 2^-9
       }
-      store_codes(static_cast<uint8_t*>(t.m), i, t.n, m);
-      store_codes(static_cast<uint8_t*>(t.v), i, t.n, v);
-      if ((threadIdx.x & 31) == 0) {
+      if (rare) {  // infinities and NaN become NaN
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (!(fabsf(m[e]) < INFINITY)) cm[e] = __uint_as_float(0x7fc00000u);
+          if (!(v[e] < INFINITY)) cv[e] = __uint_as_float(0x7fc00000u);
+        }
+      }
+      store_codes(static_cast<uint8_t*>(t.m), i, t.n, cm);
+      store_codes(static_cast<uint8_t*>(t.v), i, t.n, cv);
+      if (lane == 0) {
         t.ms[in] = static_cast<uint8_t>(mb);
         t.vs[in] = static_cast<uint8_t>(vb);
       }
@@ -352,7 +432,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const Options o, cons
   const double lr = o.lr_dev ? static_cast<double>(*o.lr_dev) : o.lr;
   s.step_size = static_cast<float>(lr / (1.0 - pow(o.beta1, static_cast<double>(t))));
   s.keep = static_cast<float>(1.0 - lr * o.decay);
-  s.bias2 = static_cast<float>(1.0 - pow(o.beta2, static_cast<double>(t)));
+  s.inv_bias2 = static_cast<float>(1.0 / (1.0 - pow(o.beta2, static_cast<double>(t))));
   s.key = mix(o.seed + static_cast<uint32_t>(t) * 0x9e3779b9u);
   *scalars = s;
 }

@@ -108,48 +108,54 @@ __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
-// N values to the gradient's type at element `at`; `wide`: that address is a multiple of
-// the N values' bytes, or of 16.
-__device__ __forceinline__ uint32_t pack_grad(int type, float a, float b) {  // of 16-bit types
-  if (type == kBf16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
+template <int kType>
+using Stored = std::conditional_t<kType == kFp32, float, std::conditional_t<kType == kBf16, __nv_bfloat16, __half>>;
+
+template <int kType>
+__device__ __forceinline__ void store_one(void* base, i64 at, float g) {
+  if constexpr (kType == kFp32) static_cast<float*>(base)[at] = g;
+  else if constexpr (kType == kBf16) static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(g);
+  else static_cast<__half*>(base)[at] = __float2half_rn(g);
 }
 
-template <int N>
-__device__ __forceinline__ void store_grad(void* base, int type, i64 at, const float (&g)[N], bool wide) {
-  if (type == kFp32) {
-    float* d = static_cast<float*>(base) + at;
-    if (wide) {
+// N values at element `at`, not read again soon; `wide`: that address is a multiple of the
+// N values' bytes, or of 16.
+template <int kType, int N>
+__device__ __forceinline__ void store_grad(void* base, i64 at, const float (&g)[N], bool wide) {
+  if (!wide) {
 #pragma unroll
-      for (int e = 0; e < N; e += 4)
-        __stcs(reinterpret_cast<float4*>(d + e), make_float4(g[e], g[e + 1], g[e + 2], g[e + 3]));
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) d[e] = g[e];
-    }
+    for (int e = 0; e < N; ++e) store_one<kType>(base, at + e, g[e]);
     return;
   }
-  uint32_t w[N / 2];
+  if constexpr (kType == kFp32) {
+    float* d = static_cast<float*>(base) + at;
 #pragma unroll
-  for (int e = 0; e < N; e += 2) w[e / 2] = pack_grad(type, g[e], g[e + 1]);
-  uint16_t* d = static_cast<uint16_t*>(base) + at;
-  if (wide) {
+    for (int e = 0; e < N; e += 4)
+      __stcs(reinterpret_cast<float4*>(d + e), make_float4(g[e], g[e + 1], g[e + 2], g[e + 3]));
+  } else {
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      if constexpr (kType == kBf16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(g[e], g[e + 1]);
+        w[e / 2] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(g[e], g[e + 1]);
+        w[e / 2] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    uint16_t* d = static_cast<uint16_t*>(base) + at;
     if constexpr (N == 8) __stcs(reinterpret_cast<uint4*>(d), make_uint4(w[0], w[1], w[2], w[3]));
     else __stcs(reinterpret_cast<uint2*>(d), make_uint2(w[0], w[1]));
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) d[e] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
   }
 }
 
-__device__ __forceinline__ void store_one(void* base, int type, i64 at, float g) {
-  if (type == kFp32) static_cast<float*>(base)[at] = g;
-  else if (type == kBf16) static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(g);
-  else static_cast<__half*>(base)[at] = __float2half_rn(g);
+// f with the type as a constant: one branch around a loop instead of one inside.
+template <typename F>
+__device__ __forceinline__ void with_type(int type, F f) {
+  if (type == kFp32) f(std::integral_constant<int, kFp32>{});
+  else if (type == kBf16) f(std::integral_constant<int, kBf16>{});
+  else f(std::integral_constant<int, kFp16>{});
 }
 
 __host__ __device__ __forceinline__ int type_bytes(int type) { return type == kFp32 ? 4 : 2; }
@@ -187,23 +193,35 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
   return r;
 }
 
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+__device__ __forceinline__ float sum_warp(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;  // the same bits in every lane: each addition has the same two operands in both
+}
+
+// A warp's 32 parts joined: every part is brought to the warp's maximum once.
 template <bool kRef>
 __device__ __forceinline__ Sums join_warp(Sums v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums b = no_sums();
-    b.m = __shfl_xor_sync(kFull, v.m, o);
-    b.s = __shfl_xor_sync(kFull, v.s, o);
-    b.t = __shfl_xor_sync(kFull, v.t, o);
-    if constexpr (kRef) {
-      b.mr = __shfl_xor_sync(kFull, v.mr, o);
-      b.sr = __shfl_xor_sync(kFull, v.sr, o);
-      b.u = __shfl_xor_sync(kFull, v.u, o);
-    }
-    // In the order of the lanes: every lane ends with the same bits.
-    v = (threadIdx.x & o) ? join<kRef>(b, v) : join<kRef>(v, b);
+  Sums r;
+  r.m = warp_max_nan(v.m);
+  const float d = v.m - r.m, f = exp2_fast(d);
+  r.t = sum_warp(f * (v.t + d * v.s));
+  r.s = sum_warp(f * v.s);
+  r.mr = kMasked2;
+  r.sr = r.u = 0.0f;
+  if constexpr (kRef) {
+    r.mr = warp_max_nan(v.mr);
+    const float dr = v.mr - r.mr;
+    r.sr = sum_warp(v.sr * exp2_fast(dr));
+    r.u = sum_warp(f * (v.u + (d - dr) * v.s));
   }
-  return v;
+  return r;
 }
 
 __device__ __forceinline__ double sum_warp(double v) {
@@ -401,7 +419,7 @@ __device__ void store_partial(const Policy& a, const double (&acc)[kSums]) {
 // little more than the entries) are copied as one run of 16-byte vectors into the warp's
 // own shared memory, the next rows' while these are computed, so the loads are wide and in
 // flight however the rows are aligned (a row of 179 fp32 starts at any multiple of 4
-// bytes); the gradient leaves the same way.
+// bytes); the gradient leaves the same way.  Other rows (kStaged false) are read in place.
 
 constexpr int kShortWarps = 8;
 
@@ -410,9 +428,9 @@ __device__ __forceinline__ void copy16(void* to, const void* from, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
 }
 
-// Where a run of rows stands in shared memory: the 16-byte granules that hold it, from
-// its first byte's granule on (an allocation starts at a granule, so that lies inside);
-// what lies behind its last byte is not read.
+// Copies a run of rows: the 16-byte granules that hold it, from its first byte's granule
+// on (an allocation starts at a granule, so that lies inside); what lies behind its last
+// byte is not read.  The run's first byte stands at to + (its address mod 16).
 __device__ __forceinline__ void copy_run(char* to, const void* from, int bytes, int lane) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(from);
   const int skip = static_cast<int>(at & 15), total = skip + bytes;
@@ -420,48 +438,43 @@ __device__ __forceinline__ void copy_run(char* to, const void* from, int bytes, 
   for (int k = 16 * lane; k < total; k += 512) copy16(to + k, base + k, total - k < 16 ? total - k : 16);
 }
 
-// The run's row number `back` there, or in global memory where it was not copied.
-template <typename V>
-__device__ __forceinline__ const V* staged_row(const char* stage, bool staged, const V* first, i64 back, i64 ld) {
-  const V* base = staged ? reinterpret_cast<const V*>(stage + (reinterpret_cast<uintptr_t>(first) & 15)) : first;
-  return base + back * ld;
-}
-
-// The warp's shared memory, in bytes (multiples of 16).
+// The warp's shared memory, in bytes (multiples of 16): two stages, one gradient.
 struct Layout {
-  int logits, ref, legal, grad;  // of one stage; the gradient has one
+  int logits, ref, legal, grad;
   __host__ __device__ int stage() const { return logits + ref + legal; }
   __host__ __device__ int warp() const { return 2 * stage() + grad; }
 };
 
-template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy>
-__global__ void __launch_bounds__(32 * kShortWarps, 2) short_rows_kernel(const Rows r, const Score o, const Policy a,
-                                                                        const Layout lay) {
+template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy, bool kStaged>
+__global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 2 : 3)
+    short_rows_kernel(const Rows r, const Score o, const Policy a, const Layout lay) {
   constexpr int kRows = 32 / kLanes;
   extern __shared__ __align__(16) char shared[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % kLanes, sub = lane / kLanes;
-  char* const own = shared + warp * lay.warp();
-  char* const out = own + 2 * lay.stage();
+  const int own = warp * lay.warp(), out = own + 2 * lay.stage();  // offsets in `shared`
+  const int vocab = r.vocab;
   float scale = 0.0f;
   double acc[kSums] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
   if constexpr (kPolicy) scale = grad_scale_of(a, block_denominator(a, r.weight, r.rows));
   const i64 stride = (i64)gridDim.x * kShortWarps * kRows;
   i64 first = ((i64)blockIdx.x * kShortWarps + warp) * kRows;
-  const int grad_bytes = type_bytes(a.dtype);
 
+  const auto address = [](const auto* base, i64 row, i64 ld) { return base + row * ld; };
+  const auto skip = [](const void* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15); };
+  const T* const logits = static_cast<const T*>(r.logits);
+  const T* const refs = static_cast<const T*>(r.ref);
   const auto fetch = [&](i64 row, int at) {
-    const int n = static_cast<int>(r.rows - row < kRows ? r.rows - row : kRows);
-    char* to = own + at * lay.stage();
-    const int size = static_cast<int>(sizeof(T));
-    if (lay.logits)
-      copy_run(to, static_cast<const T*>(r.logits) + row * r.ld,
-                             static_cast<int>(((n - 1) * r.ld + r.vocab) * size), lane);
-    if (kRef && lay.ref)
-      copy_run(to + lay.logits, static_cast<const T*>(r.ref) + row * r.ldr,
-                             static_cast<int>(((n - 1) * r.ldr + r.vocab) * size), lane);
-    if (lay.legal)
-      copy_run(to + lay.logits + lay.ref, r.legal + row * r.ldm,
-                             static_cast<int>((n - 1) * r.ldm + r.vocab), lane);
+    if constexpr (kStaged) {
+      const int n = static_cast<int>(r.rows - row < kRows ? r.rows - row : kRows) - 1;
+      char* to = shared + own + at * lay.stage();
+      const int size = static_cast<int>(sizeof(T));
+      copy_run(to, address(logits, row, r.ld), (n * static_cast<int>(r.ld) + vocab) * size, lane);
+      if constexpr (kRef)
+        copy_run(to + lay.logits, address(refs, row, r.ldr), (n * static_cast<int>(r.ldr) + vocab) * size, lane);
+      if (r.legal)
+        copy_run(to + lay.logits + lay.ref, address(r.legal, row, r.ldm), n * static_cast<int>(r.ldm) + vocab, lane);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
   };
 
   RowInputs next;
@@ -469,51 +482,61 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) short_rows_kernel(const R
     fetch(first, 0);
     next = row_inputs<kPolicy>(r, a, first + sub < r.rows ? first + sub : r.rows - 1);
   }
-  asm volatile("cp.async.commit_group;" ::: "memory");
   int at = 0;
   for (; first < r.rows; first += stride, at ^= 1) {
     const RowInputs in = next;
     if (first + stride < r.rows) {
       fetch(first + stride, at ^ 1);
       next = row_inputs<kPolicy>(r, a, first + stride + sub < r.rows ? first + stride + sub : r.rows - 1);
+      if constexpr (kStaged) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else if constexpr (kStaged) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncwarp();
     const bool real = first + sub < r.rows;
     const i64 row = real ? first + sub : r.rows - 1;
     const int back = static_cast<int>(row - first);  // the row's place in the run
-    const char* const stage = own + at * lay.stage();
-    const T* const x = staged_row(stage, lay.logits, static_cast<const T*>(r.logits) + first * r.ld, back, r.ld);
-    const T* z_row = nullptr;
-    if constexpr (kRef)
-      z_row = staged_row(stage + lay.logits, lay.ref, static_cast<const T*>(r.ref) + first * r.ldr, back, r.ldr);
+    const int stage = own + at * lay.stage();
+    const T *x, *z_row = nullptr;
     const bool* lm = nullptr;
-    if (r.legal) lm = staged_row(stage + lay.logits + lay.ref, lay.legal, r.legal + first * r.ldm, back, r.ldm);
-    bool used = real && in.weight != 0.0f && in.action >= 0 && in.action < r.vocab;
+    if constexpr (kStaged) {
+      x = reinterpret_cast<const T*>(shared + stage + skip(address(logits, first, r.ld))) +
+          back * static_cast<int>(r.ld);
+      if constexpr (kRef)
+        z_row = reinterpret_cast<const T*>(shared + stage + lay.logits + skip(address(refs, first, r.ldr))) +
+                back * static_cast<int>(r.ldr);
+      lm = reinterpret_cast<const bool*>(shared + stage + lay.logits + lay.ref +
+                                         skip(address(r.legal, first, r.ldm))) +
+           back * static_cast<int>(r.ldm);
+    } else {
+      x = address(logits, row, r.ld);
+      if constexpr (kRef) z_row = address(refs, row, r.ldr);
+      lm = address(r.legal, row, r.ldm);
+    }
+    bool used = real && in.weight != 0.0f && in.action >= 0 && in.action < vocab;
     const int action = used ? static_cast<int>(in.action) : 0;
     float x_a = max_nan(to_float(x[action]), kMasked);
-    if (lm && !lm[action]) x_a = kMasked;
+    if (r.legal && !lm[action]) x_a = kMasked;
     used = used && !(x_a <= kMasked);
 
     float y[kPer], z[kPer], e[kPer];
-    // The last entries of a lane may lie past the row; the others do not.
+    // Entry l + kLanes k lies in the row where behind < -kLanes k.  A staged row may be
+    // read past its end (the stage is that long); what stands there is not used.
+    const int behind = l - vocab;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      const int c = l + kLanes * k;
-      y[k] = kMasked;
-      if (k * kLanes < r.vocab) {  // the same for all lanes
-        const int at_c = c < r.vocab ? c : r.vocab - 1;
-        const float f = max_nan(to_float(x[at_c]), kMasked);
-        bool in_row = c < r.vocab;
-        if (lm) in_row = in_row && lm[at_c];
-        y[k] = in_row ? f : kMasked;
-        if constexpr (kRef) {
-          const float g = max_nan(to_float(z_row[at_c]), kMasked);
-          z[k] = in_row ? g : kMasked;
-        }
-      } else if constexpr (kRef) {
-        z[k] = kMasked;
+      const bool in_row = behind < -kLanes * k;
+      const int c = kStaged || in_row ? l + kLanes * k : vocab - 1;
+      y[k] = in_row ? max_nan(to_float(x[c]), kMasked) : kMasked;
+      if constexpr (kRef) z[k] = in_row ? max_nan(to_float(z_row[c]), kMasked) : kMasked;
+    }
+    if (r.legal) {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const int c = kStaged || behind < -kLanes * k ? l + kLanes * k : vocab - 1;
+        const bool open = lm[c];
+        y[k] = open ? y[k] : kMasked;
+        if constexpr (kRef) z[k] = open ? z[k] : kMasked;
       }
     }
     float top = kMasked, top_r = kMasked;
@@ -573,10 +596,13 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) short_rows_kernel(const R
           g = mul(g, two(e[k], e[k + 1]));
           split(g, y[k], y[k + 1]);
         }
+        if (!used)  // the row may hold anything: its zeros are written as such
+#pragma unroll
+          for (int k = 0; k < kPer; ++k) y[k] = 0.0f;
         // The action's entry once more, with the hot term, by the lane that holds it.
         float hot = 0.0f;
-        const bool mine = l == action % kLanes;
-        if (used && mine) {
+        const bool mine = used && l == action % kLanes;
+        if (mine) {
           hot = fmaf(c.c1, y_a, c.c0);
           if constexpr (kRef) {
             const float z_a = fmaf(max_nan(to_float(z_row[action]), kMasked), kLog2e, -v.mr);
@@ -584,39 +610,39 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) short_rows_kernel(const R
           }
           hot = fmaf(hot, exp2_fast(y_a), c.hot);
         }
-        const uintptr_t to = reinterpret_cast<uintptr_t>(a.dlogits) + first * a.ldd * grad_bytes;
-        const int lead = lay.grad ? static_cast<int>(to & 15) : 0;
-        void* const base = lay.grad ? static_cast<void*>(out + lead) : a.dlogits;
-        const i64 d_row = lay.grad ? static_cast<i64>(sub) * a.ldd : row * a.ldd;
-        if (real) {
+        with_type(a.dtype, [&](auto type) {
+          constexpr int kType = decltype(type)::value, kBytes = sizeof(Stored<kType>);
+          const auto write = [&](void* base) {  // the lane's entries of a row
 #pragma unroll
-          for (int k = 0; k < kPer; ++k) {
-            const int j = l + kLanes * k;
-            // A row that does not count may hold anything: its zeros are written as such.
-            if (j < r.vocab) store_one(base, a.dtype, d_row + j, used ? y[k] : 0.0f);
-          }
-          for (int j = r.vocab + l; j < a.width; j += kLanes) store_one(base, a.dtype, d_row + j, 0.0f);
-          if (used && mine) store_one(base, a.dtype, d_row + action, hot);
-        }
-        if (lay.grad) {
-          __syncwarp();
-          const int n = static_cast<int>(r.rows - first < kRows ? r.rows - first : kRows);
-          const int end = lead + static_cast<int>(((n - 1) * a.ldd + a.width) * grad_bytes);
-          char* const global = reinterpret_cast<char*>(to - lead);
-          for (int k = 16 * lane; k < end; k += 512) {
-            if (k >= lead && k + 16 <= end) {
-              __stcs(reinterpret_cast<uint4*>(global + k), *reinterpret_cast<const uint4*>(out + k));
-            } else {  // the run's ends: its own bytes only
-              for (int b = k < lead ? lead : k; b < k + 16 && b < end; b += 2)
-                *reinterpret_cast<uint16_t*>(global + b) = *reinterpret_cast<const uint16_t*>(out + b);
+            for (int k = 0; k < kPer; ++k)
+              if (behind < -kLanes * k) store_one<kType>(base, l + kLanes * k, y[k]);
+            for (int j = vocab + l; j < a.width; j += kLanes) store_one<kType>(base, j, 0.0f);
+            if (mine) store_one<kType>(base, action, hot);
+          };
+          if (lay.grad) {
+            const uintptr_t to = reinterpret_cast<uintptr_t>(a.dlogits) + first * a.ldd * kBytes;
+            const int lead = static_cast<int>(to & 15);
+            if (real) write(shared + out + lead + sub * static_cast<int>(a.ldd) * kBytes);
+            __syncwarp();
+            const int n = static_cast<int>(r.rows - first < kRows ? r.rows - first : kRows);
+            const int end = lead + ((n - 1) * static_cast<int>(a.ldd) + a.width) * kBytes;
+            char* const global = reinterpret_cast<char*>(to - lead);
+            for (int k = 16 * lane; k < end; k += 512) {
+              if (k >= lead && k + 16 <= end) {
+                __stcs(reinterpret_cast<uint4*>(global + k), *reinterpret_cast<const uint4*>(shared + out + k));
+              } else {  // the run's ends: its own bytes only
+                for (int b = k < lead ? lead : k; b < k + 16 && b < end; b += 2)
+                  *reinterpret_cast<uint16_t*>(global + b) = *reinterpret_cast<const uint16_t*>(shared + out + b);
+              }
             }
+          } else if (real) {
+            write(static_cast<char*>(a.dlogits) + row * a.ldd * kBytes);
           }
-        }
+        });
       }
     }
     __syncwarp();  // the stage and the gradient's place are free again
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
   if constexpr (kPolicy) {
 #pragma unroll
     for (int k = 0; k < kSums; ++k) acc[k] = sum_warp(acc[k]);
@@ -627,13 +653,22 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) short_rows_kernel(const R
 // ---- long rows: a block, or a cluster of blocks, per row -----------------------------------
 //
 // A row is cut into 16-byte vectors (a head of up to one vector to its first 16-byte
-// boundary, and a tail, entry by entry).  A thread looks at the same vectors twice: once
-// for its sums, with a maximum of its own that rescales them when it grows, once for the
-// gradient.  Between the two the warps' sums are joined through shared memory, and the
-// blocks' of a cluster through distributed shared memory, in the same order everywhere.
+// boundary, and a tail, entry by entry), and over the blocks of a cluster where it is
+// longer than a block's shared memory, or where there are few rows.  A thread looks at
+// its vectors twice: once for its sums, with a maximum of its own that rescales them when
+// it grows, once for the gradient.  Between the two the warps' sums are joined through
+// shared memory, and the blocks' of a cluster through distributed shared memory.
+//
+// A thread's vectors stand in its own slots of shared memory, from which it takes them both
+// times, so that the logits cross the memory bus once; a slot that has been looked at for
+// the last time is filled with the next row's vector at once, so the copies run on under
+// the second look, its stores and the next row's reductions.  The copies are waited for
+// in four chunks of the slots.  Vectors that no slot holds (rows longer than eight blocks'
+// slots) are read from memory both times.
 
 constexpr int kLongThreads = 512;
-constexpr int kUnroll = 4;  // vectors of a thread in flight
+constexpr int kGroup = 2;   // vectors of a thread looked at together
+constexpr int kChunks = 4;  // of a row's slots, waited for one after another
 
 template <typename T>
 constexpr int kVec = 16 / static_cast<int>(sizeof(T));
@@ -656,6 +691,45 @@ __device__ __forceinline__ void unpack(const uint4 raw, float (&f)[kVec<T>]) {
         f[2 * e + 1] = t.y;
       }
     }
+  }
+}
+
+// -inf in every entry.
+template <typename T>
+__device__ __forceinline__ uint4 nothing() {
+  const uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __nv_bfloat16> ? 0xff80ff80u : 0xfc00fc00u;
+  return make_uint4(w, w, w, w);
+}
+
+// The largest entry of a group of vectors (NaN stays) and the smallest (NaN does not), in
+// the entries' own type: two at once where it has 16 bits.
+template <typename T, int kCount>
+__device__ __forceinline__ void extremes(const uint4 (&x)[kCount], float& top, float& low) {
+  if constexpr (sizeof(T) == 4) {
+    top = __uint_as_float(x[0].x);
+    low = top;
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) {
+      const float a = __uint_as_float(x[k].x), b = __uint_as_float(x[k].y), c = __uint_as_float(x[k].z),
+                  d = __uint_as_float(x[k].w);
+      top = max_nan(max_nan(top, a, b), c, d);
+      low = min3(min3(low, a, b), c, d);
+    }
+  } else {
+    using Pair = std::conditional_t<std::is_same_v<T, __nv_bfloat16>, __nv_bfloat162, __half2>;
+    const auto pair = [](uint32_t w) { return *reinterpret_cast<const Pair*>(&w); };
+    Pair hi = pair(x[0].x), lo = hi;
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) {
+      const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        hi = __hmax2_nan(hi, pair(w[e]));
+        lo = __hmin2(lo, pair(w[e]));
+      }
+    }
+    top = max_nan(to_float(hi.x), to_float(hi.y));
+    low = fminf(to_float(lo.x), to_float(lo.y));
   }
 }
 
@@ -687,9 +761,25 @@ struct Part {
   const T* z;         // the reference's row, or null
   const bool* lm;     // the row's flags, or null
   int head, vectors;  // entries before the first whole vector; whole vectors
-  int first, last;    // this block's vectors
+  int first, last;    // the vectors to look at
   int vocab;
   bool z_wide;        // the reference's vectors are aligned as the row's are
+
+  // `entries` entries of a row from entry c0 on; of their vectors, the share of block
+  // `rank` of `parts`.
+  __device__ __forceinline__ Part(const Rows& r, i64 row, int c0, int entries, int parts, int rank) {
+    x = static_cast<const T*>(r.logits) + row * r.ld + c0;
+    z = r.ref ? static_cast<const T*>(r.ref) + row * r.ldr + c0 : nullptr;
+    lm = r.legal ? r.legal + row * r.ldm + c0 : nullptr;
+    vocab = entries;
+    head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T));
+    if (head > entries) head = entries;
+    vectors = (entries - head) / kVec<T>;
+    z_wide = (reinterpret_cast<uintptr_t>(z + head) & 15) == 0;
+    const int each = (vectors + parts - 1) / parts;
+    first = each * rank < vectors ? each * rank : vectors;
+    last = first + each < vectors ? first + each : vectors;
+  }
 
   // Vector v's 16 bytes.  The last look at an entry says that it is the last.
   template <bool kLast>
@@ -700,29 +790,21 @@ struct Part {
   __device__ __forceinline__ uint4 load_ref(int v) const {
     const T* at = z + head + v * kVec<T>;
     if (z_wide) return __ldg(reinterpret_cast<const uint4*>(at));
-    union {
-      uint4 raw;
-      uint16_t half[8];
-      uint32_t word[4];
-    } u;
+    uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) {
-      if constexpr (sizeof(T) == 4) u.word[e] = reinterpret_cast<const uint32_t*>(at)[e];
-      else u.half[e] = reinterpret_cast<const uint16_t*>(at)[e];
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (sizeof(T) == 4) w[e] = reinterpret_cast<const uint32_t*>(at)[e];
+      else w[e] = reinterpret_cast<const uint16_t*>(at)[2 * e] |
+                  static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(at)[2 * e + 1]) << 16;
     }
-    return u.raw;
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  // The vector's entries, masked.  Entries at or below the bound are rare: one look at
-  // the smallest tells.
-  __device__ __forceinline__ void entries(int v, const uint4 raw, float (&f)[kVec<T>]) const {
+  // The vector's entries; `careful`: some may be at or below the bound, or there is a mask.
+  __device__ __forceinline__ void entries(int v, const uint4 raw, bool careful, float (&f)[kVec<T>]) const {
     unpack<T>(raw, f);
-    float low = min3(f[0], f[1], f[2]);
-    if constexpr (kVec<T> == 8) low = min3(min3(low, f[3], f[4]), min3(f[5], f[6], f[7]), f[7]);
-    else low = fminf(low, f[3]);
-    if (!(low > kMasked)) {
+    if (!careful) return;
 #pragma unroll
-      for (int e = 0; e < kVec<T>; ++e) f[e] = max_nan(f[e], kMasked);
-    }
+    for (int e = 0; e < kVec<T>; ++e) f[e] = max_nan(f[e], kMasked);
     if (lm) {
       const unsigned bits = legal_bits<kVec<T>>(lm + head + v * kVec<T>);
 #pragma unroll
@@ -747,18 +829,10 @@ struct Running {
   Two s, t, sr, u;
 };
 
-template <bool kRef, int kN>
-__device__ __forceinline__ float largest(const float (&x)[kN]) {
-  float top = max_nan(x[0], x[1], x[2]);
-  if constexpr (kN == 8) return max_nan(max_nan(top, x[3], x[4]), max_nan(x[5], x[6], x[7]));
-  else return max_nan(top, x[3]);
-}
-
-// Adds kN entries, with a new maximum where they bring one.
-template <bool kRef, int kN>
-__device__ __forceinline__ void accumulate(Running& v, const float (&x)[kN], const float (&z)[kN]) {
-  const float top = largest<kRef>(x) * kLog2e;
-  if (!(top <= v.m)) {  // also for NaN
+// New maxima (base-2 units) where they are larger, also for NaN.
+template <bool kRef>
+__device__ __forceinline__ void raise(Running& v, float top, float top_r) {
+  if (!(top <= v.m)) {
     const float d = v.m - top, f = exp2_fast(d);
     const Two dd = two(d, d), ff = two(f, f);
     v.t = mul(ff, fma(dd, v.s, v.t));
@@ -767,7 +841,6 @@ __device__ __forceinline__ void accumulate(Running& v, const float (&x)[kN], con
     v.m = top;
   }
   if constexpr (kRef) {
-    const float top_r = largest<kRef>(z) * kLog2e;
     if (!(top_r <= v.mr)) {
       const float d = v.mr - top_r, f = exp2_fast(d);
       v.u = fma(two(-d, -d), v.s, v.u);
@@ -775,6 +848,11 @@ __device__ __forceinline__ void accumulate(Running& v, const float (&x)[kN], con
       v.mr = top_r;
     }
   }
+}
+
+// Adds kN entries, none above the maxima.
+template <bool kRef, int kN>
+__device__ __forceinline__ void accumulate(Running& v, const float (&x)[kN], const float (&z)[kN]) {
   const Two unit = two(kLog2e, kLog2e), from = two(-v.m, -v.m), from_r = two(-v.mr, -v.mr);
 #pragma unroll
   for (int e = 0; e < kN; e += 2) {
@@ -791,6 +869,39 @@ __device__ __forceinline__ void accumulate(Running& v, const float (&x)[kN], con
       v.sr = add(v.sr, two(exp2_fast(q0), exp2_fast(q1)));
       v.u = fma(p, fma(q, two(-1.0f, -1.0f), y), v.u);
     }
+  }
+}
+
+template <int kN>
+__device__ __forceinline__ float largest(const float (&x)[kN]) {
+  const float top = max_nan(max_nan(x[0], x[1], x[2]), x[3]);
+  if constexpr (kN == 8) return max_nan(max_nan(top, x[4], x[5]), x[6], x[7]);
+  else return top;
+}
+
+// A group of vectors, number first + k step the k-th: one look at their largest entry for
+// all.  With a mask the largest is only known entry by entry, so vector by vector.
+template <typename T, bool kRef>
+__device__ __forceinline__ void accumulate_group(Running& v, const Part<T>& p, int first, int step,
+                                                 const uint4 (&x)[kGroup], const uint4 (&z)[kGroup], int last) {
+  constexpr int kN = kVec<T>;
+  bool careful = p.lm != nullptr, careful_r = careful;
+  if (!careful) {
+    float top, low, top_r = kMasked, low_r = 0.0f;
+    extremes<T>(x, top, low);
+    if constexpr (kRef) extremes<T>(z, top_r, low_r);
+    careful = !(low > kMasked);
+    careful_r = !(low_r > kMasked);
+    raise<kRef>(v, max_nan(top, kMasked) * kLog2e, max_nan(top_r, kMasked) * kLog2e);
+  }
+#pragma unroll
+  for (int k = 0; k < kGroup; ++k) {
+    if (first + k * step >= last) break;
+    float f[kN], q[kN];
+    p.entries(first + k * step, x[k], careful, f);
+    if constexpr (kRef) p.entries(first + k * step, z[k], careful_r, q);
+    if (p.lm) raise<kRef>(v, largest(f) * kLog2e, kRef ? largest(q) * kLog2e : kMasked2);
+    accumulate<kRef>(v, f, q);
   }
 }
 
@@ -812,77 +923,173 @@ __device__ __forceinline__ void gradient(const Coefs& c, float m, float mr, cons
     split(y, y0, y1);
     split(mul(d, two(exp2_fast(y0), exp2_fast(y1))), g[e], g[e + 1]);
   }
-  if (hot >= 0 && hot < kN)
+  if (static_cast<unsigned>(hot) < kN)
 #pragma unroll
     for (int e = 0; e < kN; ++e)
       if (hot == e) g[e] += c.hot;
 }
 
-template <typename T, bool kRef, bool kPolicy>
-__global__ void __launch_bounds__(kLongThreads, 2) long_rows_kernel(const Rows r, const Score o, const Policy a) {
+// Writes the gradient of a group of vectors, number first + k step the k-th; all zeros
+// where the row does not count.
+template <typename T, bool kRef, int kType>
+__device__ __forceinline__ void write_group(const Part<T>& p, const Coefs& c, float m, float mr, bool used, int action,
+                                            void* row, bool wide, int first, int step, const uint4 (&x)[kGroup],
+                                            const uint4 (&z)[kGroup]) {
   constexpr int kN = kVec<T>;
-  __shared__ Sums warp_sums[2][kLongThreads / 32];
+  bool careful = p.lm != nullptr, careful_r = careful;
+  if (used && !careful) {
+    float top, low, low_r = 0.0f;
+    extremes<T>(x, top, low);
+    if constexpr (kRef) extremes<T>(z, top, low_r);
+    careful = !(low > kMasked);
+    careful_r = !(low_r > kMasked);
+  }
+#pragma unroll
+  for (int k = 0; k < kGroup; ++k) {
+    if (first + k * step >= p.last) break;
+    const int at = p.head + (first + k * step) * kN;
+    float f[kN], q[kN], g[kN];
+    if (used) {
+      p.entries(first + k * step, x[k], careful, f);
+      if constexpr (kRef) p.entries(first + k * step, z[k], careful_r, q);
+      gradient<kRef>(c, m, mr, f, q, action - at, g);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) g[e] = 0.0f;
+    }
+    store_grad<kType>(row, at, g, wide);
+  }
+}
+
+// Whether a row's vectors are aligned in the gradient.
+template <typename T, int kType>
+__device__ __forceinline__ bool grad_wide(const void* row, int head) {
+  constexpr int kBytes = kVec<T> * static_cast<int>(sizeof(Stored<kType>));
+  const uintptr_t to = reinterpret_cast<uintptr_t>(row) + head * sizeof(Stored<kType>);
+  return to % (kBytes < 16 ? kBytes : 16) == 0;
+}
+
+// What one thread works out of a row for all.
+struct RowResult {
+  Coefs c;
+  float m, mr;
+  bool used;
+};
+
+template <int kLeft>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+
+// slots: vectors of a thread that shared memory holds, a multiple of kGroup.
+template <typename T, bool kRef, bool kPolicy>
+__global__ void __launch_bounds__(kLongThreads, 2)
+    long_rows_kernel(const Rows r, const Score o, const Policy a, const int slots) {
+  extern __shared__ __align__(16) uint4 slot[];  // [slots][threads], then the reference's
+  __shared__ Sums warp_sums[kLongThreads / 32];
   __shared__ Sums block_sums[2];
+  __shared__ RowInputs row_in;   // thread 32's, for thread 0
+  __shared__ float row_x;        // the action's entry
+  __shared__ RowResult result;   // thread 0's, for all
+  __shared__ double block_acc[kSums];
   const cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), rank = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x / 32, step = blockDim.x;
-  __shared__ double block_acc[kSums];  // thread 0's
+  const int chunk = (slots + kChunks * kGroup - 1) / (kChunks * kGroup) * kGroup;
+  const auto chunk_end = [&](int c) { return (c + 1) * chunk < slots ? (c + 1) * chunk : slots; };
+  uint4* const mine = slot + tid;
+  uint4* const mine_r = mine + slots * step;
   float scale = 0.0f;
   if (tid == 0)
 #pragma unroll
     for (int k = 0; k < kSums; ++k) block_acc[k] = 0.0;
   if constexpr (kPolicy) scale = grad_scale_of(a, block_denominator(a, r.weight, r.rows));
+  const i64 rows_step = gridDim.x / parts;
+
+  // Whether a row may count (the action's own entry is still to be seen); the same in the
+  // whole cluster.
+  const auto maybe_used = [&](i64 row) {
+    if (row >= r.rows) return false;
+    const i64 action = r.actions[row];
+    return action >= 0 && action < r.vocab && !(r.weight && r.weight[row] == 0.0f);
+  };
+  // Starts the copies of a chunk of a row's slots; always a group of its own.
+  const auto fetch = [&](bool wanted, i64 row, int c) {
+    if (wanted) {
+      const Part<T> p(r, row, 0, r.vocab, parts, rank);
+      const int size = static_cast<int>(sizeof(T));
+      for (int k = c * chunk; k < chunk_end(c); ++k) {
+        const int i = p.first + tid + k * step;
+        if (i >= p.last) break;
+        copy16(mine + k * step, p.x + p.head + i * (16 / size), 16);
+        if constexpr (kRef) copy16(mine_r + k * step, p.z + p.head + i * (16 / size), 16);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
   int buffer = 0;
-  for (i64 row = blockIdx.x / parts; row < r.rows; row += gridDim.x / parts) {
-    const RowInputs in = row_inputs<kPolicy>(r, a, row);
-    Part<T> p;
-    p.x = static_cast<const T*>(r.logits) + row * r.ld;
-    p.z = kRef ? static_cast<const T*>(r.ref) + row * r.ldr : nullptr;
-    p.lm = r.legal ? r.legal + row * r.ldm : nullptr;
-    p.vocab = r.vocab;
-    p.head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p.x) & 15)) & 15) / static_cast<int>(sizeof(T));
-    if (p.head > r.vocab) p.head = r.vocab;
-    p.vectors = (r.vocab - p.head) / kN;
-    p.z_wide = kRef && (reinterpret_cast<uintptr_t>(p.z + p.head) & 15) == 0;
-    const int each = (p.vectors + parts - 1) / parts;
-    p.first = each * rank < p.vectors ? each * rank : p.vectors;
-    p.last = p.first + each < p.vectors ? p.first + each : p.vectors;
-    const int n_loose = rank == 0 ? r.vocab - p.vectors * kN : 0;
-    bool used = in.weight != 0.0f && in.action >= 0 && in.action < r.vocab;  // the same in the whole cluster
-    const int action = used ? static_cast<int>(in.action) : 0;
-    const float x_a = p.one(p.x, action);
-    Sums v = no_sums();
-    if (used) {
-      Running run;
-      run.m = run.mr = kMasked2;
-      run.s = run.t = run.sr = run.u = two(0.0f, 0.0f);
-      for (int i = p.first + tid; i < p.last; i += kUnroll * step) {
-        uint4 x[kUnroll], z[kUnroll];
+  i64 row = blockIdx.x / parts;
+  bool maybe = maybe_used(row);
+  const bool write = kPolicy && a.dlogits;  // a second look
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k)
-          if (i + k * step < p.last) {
-            x[k] = p.template load<!kPolicy>(i + k * step);
-            if constexpr (kRef) z[k] = p.load_ref(i + k * step);
-          }
+  for (int c = 0; c < kChunks; ++c) fetch(maybe, row, c);
+  for (; row < r.rows; row += rows_step) {
+    const bool next = maybe_used(row + rows_step);
+    const i64 action = r.actions[row];
+    const Part<T> p(r, row, 0, r.vocab, parts, rank);
+    const int i0 = p.first + tid, resident = p.first + slots * step;
+    const int n_loose = rank == 0 ? r.vocab - p.vectors * kVec<T> : 0;
+    if (maybe && tid == 32) {
+      row_in = row_inputs<kPolicy>(r, a, row);
+      row_x = p.one(p.x, static_cast<int>(action));
+    }
+    Running run;
+    run.m = run.mr = kMasked2;
+    run.s = run.t = run.sr = run.u = two(0.0f, 0.0f);
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k)
-          if (i + k * step < p.last) {
-            float f[kN], q[kN];
-            p.entries(i + k * step, x[k], f);
-            if constexpr (kRef) p.entries(i + k * step, z[k], q);
-            accumulate<kRef>(run, f, q);
+    for (int c = 0; c < kChunks; ++c) {
+      if (!write || c == 0) wait_copies<kChunks - 1>();
+      else if (c == 1) wait_copies<kChunks - 2>();
+      else if (c == 2) wait_copies<kChunks - 3>();
+      else wait_copies<0>();
+      if (maybe)
+#pragma unroll 1
+        for (int k = c * chunk; k < chunk_end(c) && i0 + k * step < p.last; k += kGroup) {
+          uint4 x[kGroup], z[kGroup];
+#pragma unroll
+          for (int h = 0; h < kGroup; ++h) {
+            const bool there = i0 + (k + h) * step < p.last;
+            x[h] = there ? mine[(k + h) * step] : nothing<T>();
+            if constexpr (kRef) z[h] = there ? mine_r[(k + h) * step] : nothing<T>();
           }
+          accumulate_group<T, kRef>(run, p, i0 + k * step, step, x, z, p.last);
+        }
+      if (!write) fetch(next, row + rows_step, c);
+    }
+    if (maybe) {
+#pragma unroll 1
+      for (int i = resident + tid; i < p.last; i += kGroup * step) {
+        uint4 x[kGroup], z[kGroup];
+#pragma unroll
+        for (int h = 0; h < kGroup; ++h) {
+          const bool there = i + h * step < p.last;
+          x[h] = there ? p.template load<!kPolicy>(i + h * step) : nothing<T>();
+          if constexpr (kRef) z[h] = there ? p.load_ref(i + h * step) : nothing<T>();
+        }
+        accumulate_group<T, kRef>(run, p, i, step, x, z, p.last);
       }
       if (tid < n_loose) {
-        // One entry, and three that add nothing beside it.
+        // One entry, and one that adds nothing beside it: were there nothing else, it would
+        // weigh as much as a masked entry, and a row of such does not count.
         const int c = p.loose(tid);
-        const float f[4] = {p.one(p.x, c), kMasked, kMasked, kMasked};
-        float q[4] = {kMasked, kMasked, kMasked, kMasked};
+        const float f[2] = {p.one(p.x, c), kMasked};
+        float q[2] = {kMasked, kMasked};
         if constexpr (kRef) q[0] = p.one(p.z, c);
-        // Where nothing else was seen the three would weigh as much as a masked entry:
-        // a row of nothing else does not count, and beside any other they are 0.
+        raise<kRef>(run, f[0] * kLog2e, q[0] * kLog2e);
         accumulate<kRef>(run, f, q);
       }
+      Sums v = no_sums();
       v.m = run.m;
       v.s = both(run.s);
       v.t = both(run.t);
@@ -892,76 +1099,93 @@ __global__ void __launch_bounds__(kLongThreads, 2) long_rows_kernel(const Rows r
         v.u = both(run.u);
       }
       v = join_warp<kRef>(v);
-      if (lane == 0) warp_sums[buffer][tid >> 5] = v;
+      if (lane == 0) warp_sums[tid >> 5] = v;
       __syncthreads();
-      v = join_warp<kRef>(lane < warps ? warp_sums[buffer][lane] : no_sums());
+      if (tid < 32) v = join_warp<kRef>(lane < warps ? warp_sums[lane] : no_sums());
       if (parts > 1) {
         if (tid == 0) block_sums[buffer] = v;
         cluster.sync();
-        v = no_sums();
-        for (int q = 0; q < parts; ++q) v = join<kRef>(v, *cluster.map_shared_rank(&block_sums[buffer], q));
+        // Every block adds the blocks' sums in the same order.
+        if (tid < 32) v = join_warp<kRef>(lane < parts ? *cluster.map_shared_rank(&block_sums[buffer], lane) : no_sums());
+        buffer ^= 1;
       }
-      buffer ^= 1;
-    }
-    used = used && !(x_a <= kMasked);
-    const float y_a = fmaf(x_a, kLog2e, -v.m);
-    if constexpr (!kPolicy) {
-      if (tid == 0 && rank == 0) store_score(o, row, used, v, y_a);
-    } else {
-      Coefs c{0.0f, 0.0f, 0.0f, 0.0f};
-      float logp = 0.0f;
-      // Every thread has the coefficients; one of the row's counts its terms.
-      Terms terms;
-      if (used) c = policy_row<kRef>(a, in, v, y_a, scale, terms, logp);
-      if (tid == 0 && rank == 0) {
-        if (a.logp) a.logp[row] = logp;
-        if (used) terms.add_to(block_acc, in.weight);
-      }
-      if (a.dlogits) {
-        const i64 at = row * a.ldd;
-        const uintptr_t to = reinterpret_cast<uintptr_t>(a.dlogits) + (at + p.head) * type_bytes(a.dtype);
-        const int bytes = kN * type_bytes(a.dtype);
-        const bool wide = to % (bytes < 16 ? bytes : 16) == 0;
-        for (int i = p.first + tid; i < p.last; i += kUnroll * step) {
-          uint4 x[kUnroll], z[kUnroll];
-#pragma unroll
-          for (int k = 0; k < kUnroll; ++k)
-            if (used && i + k * step < p.last) {
-              x[k] = p.template load<true>(i + k * step);
-              if constexpr (kRef) z[k] = p.load_ref(i + k * step);
-            }
-#pragma unroll
-          for (int k = 0; k < kUnroll; ++k) {
-            if (i + k * step >= p.last) break;
-            const int at_c = p.head + (i + k * step) * kN;
-            float f[kN], q[kN], g[kN];
-            if (used) {
-              p.entries(i + k * step, x[k], f);
-              if constexpr (kRef) p.entries(i + k * step, z[k], q);
-              gradient<kRef>(c, v.m, v.mr, f, q, action - at_c, g);
-            } else {
-#pragma unroll
-              for (int e = 0; e < kN; ++e) g[e] = 0.0f;
-            }
-            store_grad<kN>(a.dlogits, a.dtype, at + at_c, g, wide);
-          }
-        }
-        if (tid < n_loose) {
-          const int j = p.loose(tid);
-          float g = 0.0f;
+      if (tid == 0) {
+        const RowInputs in = row_in;
+        const bool used = !(row_x <= kMasked);
+        const float y_a = fmaf(row_x, kLog2e, -v.m);
+        if constexpr (!kPolicy) {
+          if (rank == 0) store_score(o, row, used, v, y_a);
+        } else {
+          float logp = 0.0f;
           if (used) {
-            const float y = fmaf(p.one(p.x, j), kLog2e, -v.m);
-            g = fmaf(c.c1, y, c.c0);
-            if constexpr (kRef) g = fmaf(c.c2, y - fmaf(p.one(p.z, j), kLog2e, -v.mr), g);
-            g *= exp2_fast(y);
-            if (j == action) g += c.hot;
+            Terms terms;
+            result.c = policy_row<kRef>(a, in, v, y_a, scale, terms, logp);
+            if (rank == 0) terms.add_to(block_acc, in.weight);
           }
-          store_one(a.dlogits, a.dtype, at + j, g);
+          if (a.logp && rank == 0) a.logp[row] = logp;
+          result.m = v.m;
+          result.mr = v.mr;
+          result.used = used;
         }
-        if (rank == 0)
-          for (int j = r.vocab + tid; j < a.width; j += step) store_one(a.dlogits, a.dtype, at + j, 0.0f);
+      }
+    } else if (tid == 0 && rank == 0) {
+      if constexpr (!kPolicy) store_score(o, row, false, no_sums(), 0.0f);
+      else if (a.logp) a.logp[row] = 0.0f;
+    }
+    __syncthreads();  // the result is there; row_in and warp_sums are free again
+    if constexpr (kPolicy) {
+      if (write) {
+        const Coefs c = result.c;  // of a row that counts; not used for another
+        const float m = result.m, mr = result.mr;
+        const bool used = maybe && result.used;
+        const int hot = used ? static_cast<int>(action) : -1;
+        with_type(a.dtype, [&](auto type) {
+          constexpr int kType = decltype(type)::value;
+          void* const to = static_cast<Stored<kType>*>(a.dlogits) + row * a.ldd;
+          const bool wide = grad_wide<T, kType>(to, p.head);
+          for (int q = 0; q < kChunks; ++q) {
+#pragma unroll 1
+            for (int k = q * chunk; k < chunk_end(q) && i0 + k * step < p.last; k += kGroup) {
+              uint4 x[kGroup], z[kGroup];
+#pragma unroll
+              for (int h = 0; h < kGroup; ++h) {
+                const bool there = i0 + (k + h) * step < p.last;
+                x[h] = there ? mine[(k + h) * step] : nothing<T>();
+                if constexpr (kRef) z[h] = there ? mine_r[(k + h) * step] : nothing<T>();
+              }
+              write_group<T, kRef, kType>(p, c, m, mr, used, hot, to, wide, i0 + k * step, step, x, z);
+            }
+            fetch(next, row + rows_step, q);
+          }
+#pragma unroll 1
+          for (int i = resident + tid; i < p.last; i += kGroup * step) {
+            uint4 x[kGroup], z[kGroup];
+#pragma unroll
+            for (int h = 0; h < kGroup; ++h) {
+              const bool there = used && i + h * step < p.last;
+              x[h] = there ? p.template load<true>(i + h * step) : nothing<T>();
+              if constexpr (kRef) z[h] = there ? p.load_ref(i + h * step) : nothing<T>();
+            }
+            write_group<T, kRef, kType>(p, c, m, mr, used, hot, to, wide, i, step, x, z);
+          }
+          if (tid < n_loose) {
+            const int j = p.loose(tid);
+            float g = 0.0f;
+            if (used) {
+              const float y = fmaf(p.one(p.x, j), kLog2e, -m);
+              g = fmaf(c.c1, y, c.c0);
+              if constexpr (kRef) g = fmaf(c.c2, y - fmaf(p.one(p.z, j), kLog2e, -mr), g);
+              g *= exp2_fast(y);
+              if (j == hot) g += c.hot;
+            }
+            store_one<kType>(to, j, g);
+          }
+          if (rank == 0)
+            for (int j = r.vocab + tid; j < a.width; j += step) store_one<kType>(to, j, 0.0f);
+        });
       }
     }
+    maybe = next;
   }
   if (parts > 1) cluster.sync();  // no block leaves while another may read its sums
   if constexpr (kPolicy)
@@ -1015,7 +1239,7 @@ __global__ void __launch_bounds__(32 * kSums) policy_means_kernel(const Policy a
 // takes kSpan entries of a row (or a whole shorter row) and writes their gradients
 //   d_j = d_logp ([j = a] - p_j) - d_entropy p_j (log p_j + H),  times *scale.
 
-constexpr int kSpan = 2048;
+constexpr int kSpan = 4096;
 constexpr int kBackWarps = 8;
 
 struct Back {
@@ -1030,63 +1254,50 @@ struct Back {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(32 * kBackWarps) logp_backward_kernel(const Rows r, const Back b, int spans) {
-  constexpr int kN = kVec<T>;
+__global__ void __launch_bounds__(32 * kBackWarps, 4) logp_backward_kernel(const Rows r, const Back b, int spans) {
   const int lane = threadIdx.x & 31;
   const i64 unit = (i64)blockIdx.x * kBackWarps + (threadIdx.x >> 5);
   const i64 row = unit / spans;
   if (row >= r.rows) return;
   const int c0 = static_cast<int>(unit - row * spans) * kSpan;
-  const int c1 = c0 + kSpan < r.vocab ? c0 + kSpan : r.vocab;
   const float2 lse = b.lse[row];
   const float scale = b.scale ? *b.scale : 1.0f;
   const float g1 = b.d_logp ? b.d_logp[row] * scale : 0.0f;
   const float g2 = b.d_entropy ? b.d_entropy[row] * scale : 0.0f;
-  const i64 at = row * b.ldd;
   // A row that does not count, and one whose gradient is 0, is not read.
-  if (lse.y == INFINITY || (g1 == 0.0f && g2 == 0.0f)) {
-    for (int c = c0 + lane; c < c1; c += 32) store_one(b.dlogits, b.dtype, at + c, 0.0f);
-    return;
-  }
+  const bool used = lse.y != INFINITY && !(g1 == 0.0f && g2 == 0.0f);
   const float inv_s = exp2_fast(-lse.y);
   Coefs k;
   k.hot = g1;
   k.c0 = inv_s * (-g1 - g2 * ((b.d_entropy ? b.entropy[row] : 0.0f) - kLn2 * lse.y));
   k.c1 = inv_s * (-g2 * kLn2);
-  Part<T> p;
-  p.x = static_cast<const T*>(r.logits) + row * r.ld + c0;
-  p.z = nullptr;
-  p.lm = r.legal ? r.legal + row * r.ldm + c0 : nullptr;
-  p.vocab = c1 - c0;
-  p.head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p.x) & 15)) & 15) / static_cast<int>(sizeof(T));
-  if (p.head > p.vocab) p.head = p.vocab;
-  p.vectors = (p.vocab - p.head) / kN;
-  const int hot = static_cast<int>(r.actions[row]) - c0;  // in the row: it counts
-  const uintptr_t to = reinterpret_cast<uintptr_t>(b.dlogits) + (at + c0 + p.head) * type_bytes(b.dtype);
-  const int bytes = kN * type_bytes(b.dtype);
-  const bool wide = to % (bytes < 16 ? bytes : 16) == 0;
-  for (int i = lane; i < p.vectors; i += kUnroll * 32) {
-    uint4 x[kUnroll];
+  k.c2 = 0.0f;
+  const Part<T> p(r, row, c0, r.vocab - c0 < kSpan ? r.vocab - c0 : kSpan, 1, 0);
+  const int hot = used ? static_cast<int>(r.actions[row]) - c0 : -1;
+  with_type(b.dtype, [&](auto type) {
+    constexpr int kType = decltype(type)::value;
+    void* const to = static_cast<Stored<kType>*>(b.dlogits) + row * b.ldd + c0;
+    const bool wide = grad_wide<T, kType>(to, p.head);
+    for (int i = lane; i < p.vectors; i += 2 * kGroup * 32) {  // two groups' loads in flight
+      uint4 x[2][kGroup];
 #pragma unroll
-    for (int q = 0; q < kUnroll; ++q)
-      if (i + 32 * q < p.vectors) x[q] = p.template load<true>(i + 32 * q);
+      for (int h = 0; h < 2 * kGroup; ++h)
+        x[h / kGroup][h % kGroup] = used && i + h * 32 < p.vectors ? p.template load<true>(i + h * 32) : nothing<T>();
 #pragma unroll
-    for (int q = 0; q < kUnroll; ++q) {
-      if (i + 32 * q >= p.vectors) break;
-      const int c = p.head + (i + 32 * q) * kN;
-      float f[kN], g[kN];
-      p.entries(i + 32 * q, x[q], f);
-      gradient<false>(k, lse.x, 0.0f, f, f, hot - c, g);
-      store_grad<kN>(b.dlogits, b.dtype, at + c0 + c, g, wide);
+      for (int h = 0; h < 2; ++h)
+        write_group<T, false, kType>(p, k, lse.x, 0.0f, used, hot, to, wide, i + h * kGroup * 32, 32, x[h], x[h]);
     }
-  }
-  for (int i = lane; i < p.vocab - p.vectors * kN; i += 32) {
-    const int c = p.loose(i);
-    const float y = fmaf(p.one(p.x, c), kLog2e, -lse.x);
-    float g = fmaf(k.c1, y, k.c0) * exp2_fast(y);
-    if (hot == c) g += k.hot;
-    store_one(b.dlogits, b.dtype, at + c0 + c, g);
-  }
+    for (int i = lane; i < p.vocab - p.vectors * kVec<T>; i += 32) {
+      const int c = p.loose(i);
+      float g = 0.0f;
+      if (used) {
+        const float y = fmaf(p.one(p.x, c), kLog2e, -lse.x);
+        g = fmaf(k.c1, y, k.c0) * exp2_fast(y);
+        if (hot == c) g += k.hot;
+      }
+      store_one<kType>(to, c, g);
+    }
+  });
 }
 
 // ---- the preference loss over pairs --------------------------------------------------------------
@@ -1232,38 +1443,64 @@ int check_rows(const Rows& r, int dtype) {
   return CUGO_B200_OK;
 }
 
-constexpr int kShortShared = 111 << 10;  // bytes of shared memory of a block of short rows: two per SM
+constexpr int kShortShared = 222 << 10;  // bytes of shared memory that a block of short rows may have
 
-// How a launch goes over the rows.
+// How a launch goes over long rows.
 struct Plan {
-  int threads, blocks, parts;
+  int threads, blocks, parts, slots, shared;
 };
 
-// A block per row, or a cluster: few rows are spread over up to 8 blocks, each with at
-// least 4,096 entries.
-Plan long_plan(i64 rows, int vocab) {
+// A block per row, of as many threads as leave each about ten vectors; a cluster of blocks
+// where the row is longer than the slots of one (two blocks of 512 threads share an SM),
+// and where rows are few: up to 8, each with at least 4,096 entries.
+Plan long_plan(i64 rows, int vocab, int size, bool ref, bool stage) {
+  constexpr int kBudget = 224 << 10, kStatic = 3 << 10;  // an SM's shared memory, a block's other part
   Plan p{};
+  const int copies = ref ? 2 : 1;
+  const i64 vectors = static_cast<i64>(vocab) * size / 16;
+  const auto most_slots = [&](int threads) { return (kBudget * threads / 1024 - kStatic) / (threads * 16 * copies); };
   p.parts = 1;
-  p.threads = vocab <= 4096 ? 128 : vocab <= 65536 ? 256 : kLongThreads;
+  while (p.parts < 8 && vectors > static_cast<i64>(p.parts) * kLongThreads * most_slots(kLongThreads)) p.parts *= 2;
   while (p.parts < 8 && rows * p.parts < kSms && vocab / (2 * p.parts) >= 4096) p.parts *= 2;
-  const i64 most = static_cast<i64>(kSms) * (1024 / p.threads) / p.parts;
+  const i64 each = (vectors + p.parts - 1) / p.parts;
+  p.threads = 128;
+  while (p.threads < kLongThreads && each > static_cast<i64>(p.threads) * most_slots(p.threads)) p.threads *= 2;
+  if (stage) {
+    const i64 want = (each + p.threads - 1) / p.threads;
+    const i64 room = most_slots(p.threads);
+    p.slots = static_cast<int>(((want < room ? want : room) + kGroup - 1) / kGroup * kGroup);
+    if (p.slots > room) p.slots -= kGroup;
+  }
+  p.shared = p.slots * p.threads * 16 * copies;
+  const int per_sm = 1024 / p.threads;
+  const i64 most = static_cast<i64>(kSms) * per_sm / p.parts;
   p.blocks = static_cast<int>(rows < most ? rows : most) * p.parts;
   return p;
 }
 
 inline int round16(i64 n) { return static_cast<int>((n + 15) / 16 * 16); }
 
-// Bytes of a run of n rows in shared memory (with a granule for its alignment), or 0
-// where the rows do not lie one after another (up to 64 bytes between them are copied
-// along).
-inline int run_bytes(i64 n, i64 ld, i64 vocab, int size) {
-  if (n > 1 && (ld < vocab || (ld - vocab) * size > 64)) return 0;
-  return round16(((n - 1) * ld + vocab) * size + 15);
-}
+// Whether rows lie one after another: up to 64 bytes between them are copied along.
+inline bool is_run(i64 ld, i64 vocab, int size) { return ld >= vocab && (ld - vocab) * size <= 64; }
 
-template <typename K>
-int launch_long(K kernel, const Plan& p, const Rows& r, const Score& o, const Policy& a, cudaStream_t stream) {
+// Bytes of a run of n rows in shared memory, its last row `width` entries long, with a
+// granule for its alignment.
+inline int run_bytes(i64 n, i64 ld, i64 width, int size) { return round16(((n - 1) * ld + width) * size + 15); }
+
+template <typename T, bool kRef, bool kPolicy>
+int launch_long(const Rows& r, const Score& o, const Policy& a, cudaStream_t stream, int& blocks) {
+  const auto kernel = long_rows_kernel<T, kRef, kPolicy>;
+  // The reference's vectors are copied beside the logits' where both are aligned alike.
+  constexpr int kSize = sizeof(T);
+  const bool stage = !kRef || ((reinterpret_cast<uintptr_t>(r.ref) - reinterpret_cast<uintptr_t>(r.logits)) % 16 == 0 &&
+                               (r.rows <= 1 || (r.ldr - r.ld) * kSize % 16 == 0));
+  const Plan p = long_plan(r.rows, r.vocab, kSize, kRef, stage);
+  blocks = p.blocks;
+  if (p.shared > (40 << 10) &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.shared) != cudaSuccess)
+    return CUGO_B200_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = p.shared;
   cfg.gridDim = dim3(p.blocks);
   cfg.blockDim = dim3(p.threads);
   cfg.stream = stream;
@@ -1273,48 +1510,62 @@ int launch_long(K kernel, const Plan& p, const Rows& r, const Score& o, const Po
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, r, o, a) == cudaSuccess ? CUGO_B200_OK : CUGO_B200_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, kernel, r, o, a, p.slots) == cudaSuccess ? CUGO_B200_OK : CUGO_B200_ERR_LAUNCH;
 }
 
-template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy>
-int launch_short(const Rows& r, const Score& o, const Policy& a, cudaStream_t stream, int& blocks) {
-  constexpr int kRows = 32 / kLanes;
-  const auto kernel = short_rows_kernel<T, kLanes, kPer, kRef, kPolicy>;
-  Layout lay{};
-  lay.logits = run_bytes(kRows, r.ld, r.vocab, sizeof(T));
-  if (kRef) lay.ref = run_bytes(kRows, r.ldr, r.vocab, sizeof(T));
-  if (r.legal) lay.legal = run_bytes(kRows, r.ldm, r.vocab, 1);
-  // Between the rows of a wider gradient stands what is not this call's to write.
-  if (a.dlogits && (a.ldd == a.width || kRows == 1)) lay.grad = run_bytes(kRows, a.ldd, a.width, type_bytes(a.dtype));
-  while (lay.warp() * kShortWarps > kShortShared) {  // the largest goes without
-    int& most = lay.grad >= lay.logits && lay.grad >= lay.ref ? lay.grad : lay.logits >= lay.ref ? lay.logits : lay.ref;
-    most = 0;
-  }
+template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy, bool kStaged>
+int launch_short(const Rows& r, const Score& o, const Policy& a, const Layout& lay, cudaStream_t stream, int& blocks) {
+  const auto kernel = short_rows_kernel<T, kLanes, kPer, kRef, kPolicy, kStaged>;
   const int shared = lay.warp() * kShortWarps;
   if (shared > (44 << 10) &&  // with the static part, past what needs no opt-in
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShortShared) != cudaSuccess)
     return CUGO_B200_ERR_LAUNCH;
-  const i64 want = (r.rows + kShortWarps * kRows - 1) / (kShortWarps * kRows);
-  int per_sm = shared > 0 ? (220 << 10) / (shared + 1024) : 4;
-  per_sm = per_sm > 4 ? 4 : per_sm;
+  constexpr int kRows = kShortWarps * 32 / kLanes;
+  const i64 want = (r.rows + kRows - 1) / kRows;
+  int per_sm = (226 << 10) / (shared + (3 << 10));
+  if (per_sm > (kPolicy ? 2 : 3)) per_sm = kPolicy ? 2 : 3;
   blocks = static_cast<int>(want < per_sm * kSms ? want : per_sm * kSms);
   kernel<<<blocks, 32 * kShortWarps, shared, stream>>>(r, o, a, lay);
   return launch_status();
 }
 
+// The staged form where everything of a row lies in runs and two stages fit.
+template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy>
+bool stage_layout(const Rows& r, const Policy& a, Layout& lay) {
+  constexpr int kRows = 32 / kLanes, kLong = kLanes * kPer;  // entries that a row is read to
+  const int size = sizeof(T);
+  lay = {};
+  if (kRows > 1 && (!is_run(r.ld, r.vocab, size) || (kRef && !is_run(r.ldr, r.vocab, size)) ||
+                    (r.legal && !is_run(r.ldm, r.vocab, 1))))
+    return false;
+  lay.logits = run_bytes(kRows, kRows > 1 ? r.ld : 0, kLong, size);
+  if (kRef) lay.ref = run_bytes(kRows, kRows > 1 ? r.ldr : 0, kLong, size);
+  if (r.legal) lay.legal = run_bytes(kRows, kRows > 1 ? r.ldm : 0, kLong, 1);
+  if (lay.warp() * kShortWarps > kShortShared) return false;
+  // Between the rows of a wider gradient stands what is not this call's to write.
+  if (a.dlogits && (kRows == 1 || a.ldd == a.width)) {
+    const i64 grad = run_bytes(kRows, kRows > 1 ? a.ldd : 0, a.width, type_bytes(a.dtype));
+    if ((lay.warp() + grad) * kShortWarps <= kShortShared) lay.grad = static_cast<int>(grad);
+  }
+  return true;
+}
+
 template <typename T, bool kRef, bool kPolicy>
 int launch_rows(const Rows& r, const Score& o, const Policy& a, cudaStream_t stream, int& blocks) {
-#define CUGO_SHORT(lanes, per) \
-  if (r.vocab <= (lanes) * (per)) return launch_short<T, lanes, per, kRef, kPolicy>(r, o, a, stream, blocks)
-  CUGO_SHORT(8, 4);
-  CUGO_SHORT(8, 8);
-  CUGO_SHORT(8, 24);
-  CUGO_SHORT(16, 24);
-  CUGO_SHORT(32, 32);
+  Layout lay;
+#define CUGO_SHORT(lanes, per)                                                  \
+  if (r.vocab <= (lanes) * (per)) {                                             \
+    if (stage_layout<T, lanes, per, kRef, kPolicy>(r, a, lay))                  \
+      return launch_short<T, lanes, per, kRef, kPolicy, true>(r, o, a, lay, stream, blocks); \
+    return launch_short<T, 32, 32, kRef, kPolicy, false>(r, o, a, Layout{}, stream, blocks); \
+  }
+  CUGO_SHORT(8, 4)
+  CUGO_SHORT(8, 8)
+  CUGO_SHORT(8, 24)
+  CUGO_SHORT(16, 24)
+  CUGO_SHORT(32, 32)
 #undef CUGO_SHORT
-  const Plan p = long_plan(r.rows, r.vocab);
-  blocks = p.blocks;
-  return launch_long(long_rows_kernel<T, kRef, kPolicy>, p, r, o, a, stream);
+  return launch_long<T, kRef, kPolicy>(r, o, a, stream, blocks);
 }
 
 // blocks: how many ran, each with a partial sum.

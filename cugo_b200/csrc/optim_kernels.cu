@@ -46,7 +46,7 @@ constexpr int kThreads = 256, kPer = 8;  // 8 warps, a scale's block each
 constexpr int kTile = kThreads * kPer;
 constexpr int kSms = 148;
 constexpr int kNormBlocks = 4 * kSms;
-constexpr int kFewTensors = 40, kMostTensors = 448;
+constexpr int kFewTensors = 40, kMostTensors = 400;
 
 struct Tensor {
   void* p;
@@ -54,6 +54,7 @@ struct Tensor {
   void *m, *v;
   uint8_t *ms, *vs;  // the scales (8-bit states)
   i64 n;
+  i64 wide;          // every pointer is a multiple of 16 bytes
   i64 first_tile;    // of the launch
   i64 first_block;   // blocks of 256 elements before this tensor in the call
 };
@@ -68,9 +69,10 @@ struct Tensors {
 // What the step's scalars come to, written by prepare_kernel.
 struct Scalars {
   float clip;       // c
+  float c1;         // c (1 - b1)
   float step_size;  // lr / (1 - b1^t)
   float keep;       // 1 - lr wd
-  float inv_bias2;  // 1 / (1 - b2^t)
+  float root;       // 1 / sqrt(1 - b2^t)
   uint32_t key;     // of the random bits
 };
 
@@ -83,13 +85,15 @@ struct Options {
 
 // A 32-bit mixer: xor-shifts and odd products (constants found by C. Wellons' search for
 // low bias, 2018).
-__device__ __forceinline__ uint32_t mix_rest(uint32_t x) {  // after the first shift
+__device__ __forceinline__ uint32_t mix_middle(uint32_t x) {  // between its first and last shift
   x *= 0x7feb352du;
   x ^= x >> 15;
-  x *= 0x846ca68bu;
+  return x * 0x846ca68bu;
+}
+__device__ __forceinline__ uint32_t mix(uint32_t x) {
+  x = mix_middle(x ^ (x >> 16));
   return x ^ (x >> 16);
 }
-__device__ __forceinline__ uint32_t mix(uint32_t x) { return mix_rest(x ^ (x >> 16)); }
 
 __device__ __forceinline__ double sum_warp(double v) {
 #pragma unroll
@@ -109,13 +113,11 @@ __device__ __forceinline__ int find(const Tensors<kMost>& a, i64 tile) {
   return low;
 }
 
-__device__ __forceinline__ bool vector_ok(const void* p, unsigned bytes) {
-  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
-}
-
-// 8 consecutive values from element i, zeros from element n on.
+// 8 consecutive values from element i, whole and aligned where kWide is set, else those
+// before element n, and zeros.
+template <bool kWide>
 __device__ __forceinline__ void load8(const float* p, i64 i, i64 n, float (&f)[8]) {
-  if (i + 8 <= n && vector_ok(p, 16)) {
+  if constexpr (kWide) {
     const float4 a = *reinterpret_cast<const float4*>(p + i), b = *reinterpret_cast<const float4*>(p + i + 4);
     f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
   } else {
@@ -124,8 +126,9 @@ __device__ __forceinline__ void load8(const float* p, i64 i, i64 n, float (&f)[8
   }
 }
 
+template <bool kWide>
 __device__ __forceinline__ void load8(const __nv_bfloat16* p, i64 i, i64 n, float (&f)[8]) {
-  if (i + 8 <= n && vector_ok(p, 16)) {
+  if constexpr (kWide) {
     const uint4 q = *reinterpret_cast<const uint4*>(p + i);
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -139,8 +142,9 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, i64 i, i64 n, floa
   }
 }
 
+template <bool kWide>
 __device__ __forceinline__ void store8(float* p, i64 i, i64 n, const float (&f)[8]) {
-  if (i + 8 <= n && vector_ok(p, 16)) {
+  if constexpr (kWide) {
     *reinterpret_cast<float4*>(p + i) = make_float4(f[0], f[1], f[2], f[3]);
     *reinterpret_cast<float4*>(p + i + 4) = make_float4(f[4], f[5], f[6], f[7]);
   } else {
@@ -151,8 +155,9 @@ __device__ __forceinline__ void store8(float* p, i64 i, i64 n, const float (&f)[
 }
 
 // The upper halves of f (rounded there already) as bf16.
+template <bool kWide>
 __device__ __forceinline__ void store8(__nv_bfloat16* p, i64 i, i64 n, const float (&f)[8]) {
-  if (i + 8 <= n && vector_ok(p, 16)) {
+  if constexpr (kWide) {
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = __byte_perm(__float_as_uint(f[2 * e]), __float_as_uint(f[2 * e + 1]), 0x7632);
@@ -165,9 +170,10 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, i64 i, i64 n, const flo
 }
 
 // 8 codes as floats, not scaled.
+template <bool kWide>
 __device__ __forceinline__ void load_codes(const uint8_t* p, i64 i, i64 n, float (&f)[8]) {
   uint32_t w[2] = {0, 0};
-  if (i + 8 <= n && vector_ok(p, 8)) {
+  if constexpr (kWide) {
     const uint2 q = *reinterpret_cast<const uint2*>(p + i);
     w[0] = q.x, w[1] = q.y;
   } else {
@@ -184,6 +190,7 @@ __device__ __forceinline__ void load_codes(const uint8_t* p, i64 i, i64 n, float
   }
 }
 
+template <bool kWide>
 __device__ __forceinline__ void store_codes(uint8_t* p, i64 i, i64 n, const float (&f)[8]) {
   uint32_t w[2];
 #pragma unroll
@@ -192,7 +199,7 @@ __device__ __forceinline__ void store_codes(uint8_t* p, i64 i, i64 n, const floa
     const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * e + 2], f[4 * e + 3]), __NV_SATFINITE, __NV_E4M3);
     w[e] = __byte_perm(a, b, 0x5410);
   }
-  if (i + 8 <= n && vector_ok(p, 8)) {
+  if constexpr (kWide) {
     *reinterpret_cast<uint2*>(p + i) = make_uint2(w[0], w[1]);
   } else {
 #pragma unroll
@@ -213,25 +220,33 @@ __device__ __forceinline__ int scale_byte(float largest) {
   return e < 27 ? 27 : e > 247 ? 247 : e;
 }
 
-// The magnitude a (at most 448) rounded to e4m3's grid, up where the 16 random bits in
-// r16 (at bit 4) say so: below 2^-6 the steps are 2^-9, which 2^-6 more gives the bits
+// The magnitude a (at most 448) rounded to e4m3's grid, up where the random number r says
+// so: 16 bits, as a share of a step, from bit 4 on (what stands below them counts for
+// less than 2^-16 of a step).  Below 2^-6 the steps are 2^-9, which 2^-6 more brings to
 // the same place; above they are 1/8 of the power of two.
-__device__ __forceinline__ float round_e4m3(float a, uint32_t r16) {
+__device__ __forceinline__ float round_e4m3(float a, uint32_t r) {
   float small;  // 1 below 2^-6, else 0
   asm("set.lt.f32.f32 %0, %1, %2;" : "=f"(small) : "f"(a), "f"(0.015625f));
-  const uint32_t bits = (__float_as_uint(fmaf(small, 0.015625f, a)) + r16 + 8u) & 0xfff00000u;
+  const uint32_t bits = (__float_as_uint(fmaf(small, 0.015625f, a)) + r) & 0xfff00000u;
   return fmaf(small, -0.015625f, __uint_as_float(bits));
 }
 
-// A warp's largest (of non-negative floats, which order as their bits do).
-__device__ __forceinline__ float warp_largest(const float (&f)[8]) {
-  float top = fabsf(f[0]);
-#pragma unroll
-  for (int e = 1; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
-  return __uint_as_float(__reduce_max_sync(kFull, __float_as_uint(top)));
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
-// The same over the finite magnitudes only.
+// A warp's largest magnitude; infinite or NaN where one is.
+__device__ __forceinline__ float warp_largest(const float (&f)[8]) {
+  float top = 0.0f, r;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) top = max_nan(top, fabsf(f[e]), fabsf(f[e + 1]));
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(top));
+  return r;
+}
+
+// The same over the finite magnitudes only (as bits they order as the values do).
 __device__ __noinline__ float warp_largest_finite(const float (&f)[8]) {
   uint32_t top = 0;
 #pragma unroll
@@ -271,116 +286,119 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
   return r;
 }
 
+// A warp's block `in` of tensor t, this thread's 8 elements from i on.
+template <typename P, typename G, bool kEight, bool kWide>
+__device__ __forceinline__ void step8(const Tensor& t, const Options& o, const Scalars& s, i64 in, i64 i) {
+  constexpr bool kRandom = kEight || sizeof(P) == 2;
+  float p[8], g[8], m[8], v[8];
+  load8<kWide>(static_cast<const P*>(t.p), i, t.n, p);
+  load8<kWide>(static_cast<const G*>(t.g), i, t.n, g);
+  float b1 = o.b1, b2 = o.b2;
+  if constexpr (kEight) {  // the scale is a power of two: exact in the factor
+    load_codes<kWide>(static_cast<const uint8_t*>(t.m), i, t.n, m);
+    load_codes<kWide>(static_cast<const uint8_t*>(t.v), i, t.n, v);
+    b1 *= scale_of(t.ms[in]);
+    b2 *= scale_of(t.vs[in]);
+  } else {
+    load8<kWide>(static_cast<const float*>(t.m), i, t.n, m);
+    load8<kWide>(static_cast<const float*>(t.v), i, t.n, v);
+  }
+  const Two c1 = two(s.c1, s.c1), clip = two(s.clip, s.clip), c2 = two(o.c2, o.c2), d1 = two(b1, b1), d2 = two(b2, b2),
+            keep = two(s.keep, s.keep);
+  float finite = 0.0f;  // NaN where a parameter is not finite after the step
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const Two gg = two(g[e], g[e + 1]), q = mul(gg, clip);
+    split(fma2(two(m[e], m[e + 1]), d1, mul(gg, c1)), m[e], m[e + 1]);
+    split(fma2(two(v[e], v[e + 1]), d2, mul(mul(q, q), c2)), v[e], v[e + 1]);
+    split(mul(two(p[e], p[e + 1]), keep), p[e], p[e + 1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float u = __fdividef(m[e + h], fmaf(sqrt_fast(v[e + h]), s.root, o.eps));
+      p[e + h] = fmaf(-s.step_size, u, p[e + h]);
+      if constexpr (sizeof(P) == 2) finite = fmaf(p[e + h], 0.0f, finite);
+    }
+  }
+  uint32_t x[8];  // the mix before its last shift, x ^= x >> 16
+  if constexpr (kRandom) {
+    // i is a multiple of 8, so element e's number differs in the last three bits only: the
+    // mix's first shift is the same for all eight.
+    const i64 number = t.first_block * kBlock + i;
+    uint32_t n = static_cast<uint32_t>(number) ^ (s.key + static_cast<uint32_t>(number >> 32) * 0x9e3779b9u);
+    n ^= n >> 16;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = mix_middle(n ^ e);
+  }
+  if constexpr (sizeof(P) == 2) {
+    float kept[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      kept[e] = p[e];
+      p[e] = __uint_as_float(__float_as_uint(p[e]) + (((x[e] ^ (x[e] >> 16)) * 0x2c1b3c6du) >> 16));
+    }
+    if (!(finite == 0.0f))  // infinities and NaN stay what they are
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = fabsf(kept[e]) < INFINITY ? p[e] : kept[e];
+  }
+  store8<kWide>(static_cast<P*>(t.p), i, t.n, p);
+  if constexpr (kEight) {
+    float top_m = warp_largest(m), top_v = warp_largest(v);
+    const bool rare = !(top_m < INFINITY && top_v < INFINITY);
+    if (rare) {
+      top_m = warp_largest_finite(m);
+      top_v = warp_largest_finite(v);
+    }
+    const int mb = scale_byte(top_m), vb = scale_byte(top_v);
+    const float mi = inverse_of(mb), vi = inverse_of(vb);
+    const Two mi2 = two(mi, mi), vi2 = two(vi, vi);
+    float cm[8], cv[8], low = 448.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      split(mul(two(m[e], m[e + 1]), mi2), cm[e], cm[e + 1]);
+      split(mul(two(v[e], v[e + 1]), vi2), cv[e], cv[e + 1]);
+      low = fminf(fminf(low, cv[e]), cv[e + 1]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t high = x[e] >> 16;
+      const float q = round_e4m3(fabsf(cm[e]), ((x[e] ^ high) & 0xffffu) * 16u + 8u);
+      cm[e] = __uint_as_float(__float_as_uint(q) | (__float_as_uint(cm[e]) & 0x80000000u));
+      cv[e] = round_e4m3(cv[e], x[e] >> 12);
+    }
+    if (low < 0.001953125f) {  // 2^-9: a second moment above 0 does not become 0
+#pragma unroll
+      for (int e = 0; e < 8; ++e) cv[e] = v[e] > 0.0f ? fmaxf(cv[e], 0.001953125f) : cv[e];
+    }
+    if (rare) {  // infinities and NaN become NaN
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (!(fabsf(m[e]) < INFINITY)) cm[e] = __uint_as_float(0x7fc00000u);
+        if (!(v[e] < INFINITY)) cv[e] = __uint_as_float(0x7fc00000u);
+      }
+    }
+    store_codes<kWide>(static_cast<uint8_t*>(t.m), i, t.n, cm);
+    store_codes<kWide>(static_cast<uint8_t*>(t.v), i, t.n, cv);
+    if ((threadIdx.x & 31) == 0) {
+      t.ms[in] = static_cast<uint8_t>(mb);
+      t.vs[in] = static_cast<uint8_t>(vb);
+    }
+  } else {
+    store8<kWide>(static_cast<float*>(t.m), i, t.n, m);
+    store8<kWide>(static_cast<float*>(t.v), i, t.n, v);
+  }
+}
+
 template <typename P, typename G, bool kEight, int kMost>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Tensors<kMost> a, const Options o,
                                                          const Scalars* scalars) {
-  constexpr bool kRandom = kEight || sizeof(P) == 2;
   const Scalars s = *scalars;
-  const int lane = threadIdx.x & 31;
   for (i64 tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const Tensor& t = a.t[find(a, tile)];
     const i64 in = (tile - t.first_tile) * (kTile / kBlock) + (threadIdx.x >> 5);  // the warp's block
-    const i64 i = in * kBlock + lane * kPer;
+    const i64 i = in * kBlock + (threadIdx.x & 31) * kPer;
     if (in * kBlock >= t.n) continue;  // the whole warp
-    float p[8], g[8], m[8], v[8];
-    load8(static_cast<const P*>(t.p), i, t.n, p);
-    load8(static_cast<const G*>(t.g), i, t.n, g);
-    float b1 = o.b1, b2 = o.b2;
-    if constexpr (kEight) {  // the scale is a power of two: exact in the factor
-      load_codes(static_cast<const uint8_t*>(t.m), i, t.n, m);
-      load_codes(static_cast<const uint8_t*>(t.v), i, t.n, v);
-      b1 *= scale_of(t.ms[in]);
-      b2 *= scale_of(t.vs[in]);
-    } else {
-      load8(static_cast<const float*>(t.m), i, t.n, m);
-      load8(static_cast<const float*>(t.v), i, t.n, v);
-    }
-    const Two clip = two(s.clip, s.clip), c1 = two(o.c1, o.c1), c2 = two(o.c2, o.c2), d1 = two(b1, b1),
-              d2 = two(b2, b2), keep = two(s.keep, s.keep), inv = two(s.inv_bias2, s.inv_bias2);
-    float finite = 0.0f;  // NaN where a parameter is not finite after the step
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const Two q = mul(two(g[e], g[e + 1]), clip);
-      const Two mm = fma2(two(m[e], m[e + 1]), d1, mul(q, c1));
-      const Two vv = fma2(two(v[e], v[e + 1]), d2, mul(mul(q, q), c2));
-      const Two kept = mul(two(p[e], p[e + 1]), keep), root = mul(vv, inv);
-      float r[2];
-      split(mm, m[e], m[e + 1]);
-      split(vv, v[e], v[e + 1]);
-      split(kept, p[e], p[e + 1]);
-      split(root, r[0], r[1]);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float u = __fdividef(m[e + h], sqrt_fast(r[h]) + o.eps);
-        p[e + h] = fmaf(-s.step_size, u, p[e + h]);
-        if constexpr (kRandom) finite = fmaf(p[e + h], 0.0f, finite);
-      }
-    }
-    uint32_t r[8];
-    bool rare = false;  // of the warp
-    if constexpr (kRandom) {
-      // i is a multiple of 8, so element e's number differs in the last three bits only:
-      // the mix's first shift is the same for all eight.
-      const i64 number = t.first_block * kBlock + i;
-      uint32_t x = static_cast<uint32_t>(number) ^ (s.key + static_cast<uint32_t>(number >> 32) * 0x9e3779b9u);
-      x ^= x >> 16;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] = mix_rest(x ^ e);
-      rare = __any_sync(kFull, !(finite == 0.0f));
-    }
-    if constexpr (sizeof(P) == 2) {
-      if (!rare) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = __uint_as_float(__float_as_uint(p[e]) + ((r[e] * 0x2c1b3c6du) >> 16));
-      } else {  // infinities and NaN stay what they are
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t b = __float_as_uint(p[e]);
-          p[e] = (b & 0x7f800000u) == 0x7f800000u ? p[e] : __uint_as_float(b + ((r[e] * 0x2c1b3c6du) >> 16));
-        }
-      }
-    }
-    store8(static_cast<P*>(t.p), i, t.n, p);
-    if constexpr (kEight) {
-      float top_m = warp_largest(m), top_v = warp_largest(v);
-      // A second moment can overflow while its step, and so its parameter, stays finite.
-      rare = rare || !(top_v < INFINITY);
-      if (rare) {
-        top_m = warp_largest_finite(m);
-        top_v = warp_largest_finite(v);
-      }
-      const int mb = scale_byte(top_m), vb = scale_byte(top_v);
-      const float mi = inverse_of(mb), vi = inverse_of(vb);
-      const Two mi2 = two(mi, mi), vi2 = two(vi, vi);
-      float cm[8], cv[8];
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        split(mul(two(m[e], m[e + 1]), mi2), cm[e], cm[e + 1]);
-        split(mul(two(v[e], v[e + 1]), vi2), cv[e], cv[e + 1]);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        cm[e] = copysignf(round_e4m3(fabsf(cm[e]), (r[e] << 4) & 0xffff0u), cm[e]);
-        const float q = round_e4m3(cv[e], (r[e] >> 12) & 0xffff0u);
-        cv[e] = v[e] > 0.0f ? fmaxf(q, 0.001953125f) : q;  // 2^-9
-      }
-      if (rare) {  // infinities and NaN become NaN
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (!(fabsf(m[e]) < INFINITY)) cm[e] = __uint_as_float(0x7fc00000u);
-          if (!(v[e] < INFINITY)) cv[e] = __uint_as_float(0x7fc00000u);
-        }
-      }
-      store_codes(static_cast<uint8_t*>(t.m), i, t.n, cm);
-      store_codes(static_cast<uint8_t*>(t.v), i, t.n, cv);
-      if (lane == 0) {
-        t.ms[in] = static_cast<uint8_t>(mb);
-        t.vs[in] = static_cast<uint8_t>(vb);
-      }
-    } else {
-      store8(static_cast<float*>(t.m), i, t.n, m);
-      store8(static_cast<float*>(t.v), i, t.n, v);
-    }
+    if (t.wide && (in + 1) * kBlock <= t.n) step8<P, G, kEight, true>(t, o, s, in, i);
+    else step8<P, G, kEight, false>(t, o, s, in, i);
   }
 }
 
@@ -392,7 +410,9 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ 
   for (i64 tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const Tensor& t = a.t[find(a, tile)];
     float g[8], q = 0.0f;
-    load8(static_cast<const G*>(t.g), (tile - t.first_tile) * kTile + threadIdx.x * kPer, t.n, g);
+    const i64 i = (tile - t.first_tile) * kTile + threadIdx.x * kPer;
+    if (t.wide && i + kPer <= t.n) load8<true>(static_cast<const G*>(t.g), i, t.n, g);
+    else load8<false>(static_cast<const G*>(t.g), i, t.n, g);
 #pragma unroll
     for (int e = 0; e < 8; ++e) q = fmaf(g[e], g[e], q);
     sum += q;
@@ -432,7 +452,8 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const Options o, cons
   const double lr = o.lr_dev ? static_cast<double>(*o.lr_dev) : o.lr;
   s.step_size = static_cast<float>(lr / (1.0 - pow(o.beta1, static_cast<double>(t))));
   s.keep = static_cast<float>(1.0 - lr * o.decay);
-  s.inv_bias2 = static_cast<float>(1.0 / (1.0 - pow(o.beta2, static_cast<double>(t))));
+  s.root = static_cast<float>(1.0 / sqrt(1.0 - pow(o.beta2, static_cast<double>(t))));
+  s.c1 = s.clip * o.c1;
   s.key = mix(o.seed + static_cast<uint32_t>(t) * 0x9e3779b9u);
   *scalars = s;
 }
@@ -462,8 +483,9 @@ i64 fill(const Lists& l, i64 first, i64& blocks_before, Tensors<kMost>& a) {
   for (; k < l.count && a.count < kMost; ++k) {
     if (l.n[k] == 0) continue;
     Tensor& t = a.t[a.count++];
+    const bool wide = aligned(l.p[k], 16) && aligned(l.g[k], 16) && aligned(l.m[k], 16) && aligned(l.v[k], 16);
     t = {l.p[k], l.g[k], l.m[k], l.v[k], l.ms ? static_cast<uint8_t*>(l.ms[k]) : nullptr,
-         l.vs ? static_cast<uint8_t*>(l.vs[k]) : nullptr, l.n[k], a.tiles, blocks_before};
+         l.vs ? static_cast<uint8_t*>(l.vs[k]) : nullptr, l.n[k], wide, a.tiles, blocks_before};
     a.tiles += (l.n[k] + kTile - 1) / kTile;
     blocks_before += (l.n[k] + kBlock - 1) / kBlock;
   }

@@ -89,11 +89,14 @@ class _PolicyLoss(torch.autograd.Function):
         ctx.coefs, ctx.denominator = coefs, stats[7:]
         stats = stats[:7]
         ctx.mark_non_differentiable(stats, logp)
+        ctx.set_materialize_grads(False)
         return loss, stats, logp
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss, *_):
+        if d_loss is None:
+            return (None,) * 9
         logits = ctx.saved_tensors[0]
         d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         # The denominator that the forward found; the logits are read once more.
@@ -172,11 +175,14 @@ class _PreferenceLoss(torch.autograd.Function):
         out, lse, d_logp = _preference(logits, actions, offsets, ref_logp, legal, weight, options, True)
         ctx.save_for_backward(logits, actions, legal, lse, d_logp)
         ctx.mark_non_differentiable(*out[1:])
+        ctx.set_materialize_grads(False)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss, *_):
+        if d_loss is None:
+            return (None,) * 7
         logits, actions, legal, lse, d_logp = ctx.saved_tensors
         d = load_extension().action_logp_backward(logits, actions, legal, lse, None, d_logp, None,
                                                   scale=d_loss)

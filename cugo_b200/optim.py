@@ -1,6 +1,6 @@
 """The AdamW step over many tensors at once, with the clipping of the gradients' norm in
 it, on the kernels of optim_kernels.cu: two launches for all tensors of a group (three
-with clipping, up to 448 tensors each), and states in 32 bits or in 8.
+with clipping, up to 400 tensors each), and states in 32 bits or in 8.
 
 `AdamW` is a torch optimizer to use in place of clip_grad_norm_ and torch.optim.AdamW;
 `adamw_step` is its one step on tensors that the caller keeps.

@@ -219,7 +219,11 @@ def test_masks_by_value(vocab):
     want = action_logp(x, actions, mask)
     for value in (-1e30, -float("inf"), torch.finfo(torch.float32).min):
         got = action_logp(x.masked_fill(~mask, value), actions)
-        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        # Long rows bring in a new maximum at other places where a mask is read, so each of
+        # the two is off by its own rounding: twice the bound of one.
+        c = 2 * chain(vocab) * U
+        near(got[0], want[0].double(), c * (1 + want[0].double().abs()), "logp")
+        near(got[1], want[1].double(), c * (1 + 2 * want[1].double() + math.log(vocab)), "entropy")
     flat = torch.full((3, vocab), -1e9, device=DEV)
     logp, entropy = action_logp(flat, torch.zeros(3, dtype=torch.int64, device=DEV))
     assert float((logp + math.log(vocab)).abs().max()) < 2e-5 and float((entropy - math.log(vocab)).abs().max()) < 2e-5
@@ -257,7 +261,7 @@ def test_no_rows_and_no_weight(vocab):
     z = torch.zeros(5, device=DEV)
     out = policy_loss(x, actions, z, z + 1, weight=z, entropy_coef=0.1)
     d, = torch.autograd.grad(out.loss, x)
-    assert float(out.loss) == 0.0 and not bool(d.any())
+    assert float(out.loss.detach()) == 0.0 and not bool(d.any())
 
 
 def test_denominator_of_a_larger_batch():
@@ -345,7 +349,11 @@ def test_strides_streams_graphs_and_the_same_bits():
     big = torch.zeros((1000, 200), device=DEV)
     big[::2, 3:182] = x
     sub, d3 = policy_loss_grad(big[::2, 3:182], actions, old, adv, **k)
-    assert torch.equal(d, d3) and torch.equal(out.stats, sub.stats)
+    # (Rows apart are added up in another order than rows one after another.)
+    want, stats, logp, p, _ = policy64(x, actions, old, adv, **k)
+    worst, size = policy_tols(179, x, actions, k, adv, p, stats, 500)
+    near(d3, want, grad_tol(179, p, actions, size, torch.float32, want), "rows apart")
+    near(sub.stats, stats, worst * (1 + stats.abs()), "rows apart")
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):

@@ -313,7 +313,7 @@ __device__ __forceinline__ float log_prob(float y_a, float log_s, float mean_y) 
 
 // A row's outputs in action_logp.
 __device__ __forceinline__ void store_score(const Score& o, i64 row, bool used, const Sums& v, float y_a) {
-  const float log_s = used ? log2f(v.s) : INFINITY, mean_y = v.t / v.s;
+  const float log_s = used ? log2f(v.s) : INFINITY, mean_y = __fdividef(v.t, v.s);
   if (o.logp) o.logp[row] = used ? log_prob(y_a, log_s, mean_y) : 0.0f;
   if (o.entropy) o.entropy[row] = used ? kLn2 * (log_s - mean_y) : 0.0f;
   if (o.lse) o.lse[row] = make_float2(used ? v.m : 0.0f, log_s);
@@ -421,9 +421,9 @@ __device__ void store_partial(const Policy& a, const double (&acc)[kSums]) {
 // flight however the rows are aligned (a row of 179 fp32 starts at any multiple of 4
 // bytes); the gradient leaves the same way.  Other rows (kStaged false) are read in place.
 
-constexpr int kShortWarps = 8;
+constexpr int kShortWarps = 4;
 
-__device__ __forceinline__ void copy16(void* to, const void* from, int bytes) {
+__device__ __forceinline__ void copy16(void* to, const void* from, int bytes = 16) {
   const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to));
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
 }
@@ -433,9 +433,15 @@ __device__ __forceinline__ void copy16(void* to, const void* from, int bytes) {
 // byte is not read.  The run's first byte stands at to + (its address mod 16).
 __device__ __forceinline__ void copy_run(char* to, const void* from, int bytes, int lane) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(from);
-  const int skip = static_cast<int>(at & 15), total = skip + bytes;
-  const char* base = reinterpret_cast<const char*>(at - skip);
-  for (int k = 16 * lane; k < total; k += 512) copy16(to + k, base + k, total - k < 16 ? total - k : 16);
+  const int skip = static_cast<int>(at & 15), total = skip + bytes, whole = total >> 4;
+  const char* base = reinterpret_cast<const char*>(at - skip) + 16 * lane;
+  to += 16 * lane;
+  int k = lane;
+  for (; k + 96 < whole; k += 128, to += 2048, base += 2048)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) copy16(to + 512 * q, base + 512 * q);
+  for (; k < whole; k += 32, to += 512, base += 512) copy16(to, base);
+  if (k == whole && (total & 15)) copy16(to, base, total & 15);
 }
 
 // The warp's shared memory, in bytes (multiples of 16): two stages, one gradient.
@@ -446,7 +452,7 @@ struct Layout {
 };
 
 template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy, bool kStaged>
-__global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 2 : 3)
+__global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
     short_rows_kernel(const Rows r, const Score o, const Policy a, const Layout lay) {
   constexpr int kRows = 32 / kLanes;
   extern __shared__ __align__(16) char shared[];
@@ -667,8 +673,8 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 2 : 3)
 // slots) are read from memory both times.
 
 constexpr int kLongThreads = 512;
-constexpr int kGroup = 2;   // vectors of a thread looked at together
-constexpr int kChunks = 4;  // of a row's slots, waited for one after another
+constexpr int kGroup = 4;   // vectors of a thread looked at together
+constexpr int kChunks = 2;  // of a row's slots, waited for one after another
 
 template <typename T>
 constexpr int kVec = 16 / static_cast<int>(sizeof(T));
@@ -694,42 +700,31 @@ __device__ __forceinline__ void unpack(const uint4 raw, float (&f)[kVec<T>]) {
   }
 }
 
-// -inf in every entry.
-template <typename T>
-__device__ __forceinline__ uint4 nothing() {
-  const uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __nv_bfloat16> ? 0xff80ff80u : 0xfc00fc00u;
-  return make_uint4(w, w, w, w);
-}
-
-// The largest entry of a group of vectors (NaN stays) and the smallest (NaN does not), in
-// the entries' own type: two at once where it has 16 bits.
-template <typename T, int kCount>
-__device__ __forceinline__ void extremes(const uint4 (&x)[kCount], float& top, float& low) {
+// The largest (kMost; NaN stays) or smallest entry of vectors, in the entries' own type:
+// two at once where it has 16 bits.
+template <typename T, bool kMost, int kCount>
+__device__ __forceinline__ float extreme(const uint4 (&x)[kCount]) {
   if constexpr (sizeof(T) == 4) {
-    top = __uint_as_float(x[0].x);
-    low = top;
+    float r = __uint_as_float(x[0].x);
 #pragma unroll
     for (int k = 0; k < kCount; ++k) {
       const float a = __uint_as_float(x[k].x), b = __uint_as_float(x[k].y), c = __uint_as_float(x[k].z),
                   d = __uint_as_float(x[k].w);
-      top = max_nan(max_nan(top, a, b), c, d);
-      low = min3(min3(low, a, b), c, d);
+      if constexpr (kMost) r = max_nan(max_nan(r, a, b), c, d);
+      else r = min3(min3(r, a, b), c, d);
     }
+    return r;
   } else {
     using Pair = std::conditional_t<std::is_same_v<T, __nv_bfloat16>, __nv_bfloat162, __half2>;
     const auto pair = [](uint32_t w) { return *reinterpret_cast<const Pair*>(&w); };
-    Pair hi = pair(x[0].x), lo = hi;
+    Pair r = pair(x[0].x);
 #pragma unroll
     for (int k = 0; k < kCount; ++k) {
       const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        hi = __hmax2_nan(hi, pair(w[e]));
-        lo = __hmin2(lo, pair(w[e]));
-      }
+      for (int e = 0; e < 4; ++e) r = kMost ? __hmax2_nan(r, pair(w[e])) : __hmin2(r, pair(w[e]));
     }
-    top = max_nan(to_float(hi.x), to_float(hi.y));
-    low = fminf(to_float(lo.x), to_float(lo.y));
+    return kMost ? max_nan(to_float(r.x), to_float(r.y)) : fminf(to_float(r.x), to_float(r.y));
   }
 }
 
@@ -781,13 +776,11 @@ struct Part {
     last = first + each < vectors ? first + each : vectors;
   }
 
-  // Vector v's 16 bytes.  The last look at an entry says that it is the last.
-  template <bool kLast>
-  __device__ __forceinline__ uint4 load(int v) const {
-    const uint4* at = reinterpret_cast<const uint4*>(x + head + v * kVec<T>);
-    return kLast ? __ldcs(at) : __ldg(at);
+  __device__ __forceinline__ const uint4* vector(int v) const {
+    return reinterpret_cast<const uint4*>(x + head) + v;
   }
-  __device__ __forceinline__ uint4 load_ref(int v) const {
+  // The reference's entries beside vector v.
+  __device__ __forceinline__ uint4 ref_vector(int v) const {
     const T* at = z + head + v * kVec<T>;
     if (z_wide) return __ldg(reinterpret_cast<const uint4*>(at));
     uint32_t w[4];
@@ -799,10 +792,9 @@ struct Part {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  // The vector's entries; `careful`: some may be at or below the bound, or there is a mask.
-  __device__ __forceinline__ void entries(int v, const uint4 raw, bool careful, float (&f)[kVec<T>]) const {
+  // A vector's entries with all masks applied.
+  __device__ __forceinline__ void masked(int v, const uint4 raw, float (&f)[kVec<T>]) const {
     unpack<T>(raw, f);
-    if (!careful) return;
 #pragma unroll
     for (int e = 0; e < kVec<T>; ++e) f[e] = max_nan(f[e], kMasked);
     if (lm) {
@@ -872,6 +864,21 @@ __device__ __forceinline__ void accumulate(Running& v, const float (&x)[kN], con
   }
 }
 
+// Adds whole vectors as they are: one look at their largest entry for all.  An entry of
+// -inf makes the sums NaN (0 times -inf); the row is then taken again with care.
+template <typename T, bool kRef, int kCount>
+__device__ __forceinline__ void add_vectors(Running& v, const uint4 (&x)[kCount], const uint4 (&z)[kCount]) {
+  constexpr int kN = kVec<T>;
+  raise<kRef>(v, extreme<T, true>(x) * kLog2e, kRef ? extreme<T, true>(z) * kLog2e : kMasked2);
+#pragma unroll
+  for (int k = 0; k < kCount; ++k) {
+    float f[kN], q[kN];
+    unpack<T>(x[k], f);
+    if constexpr (kRef) unpack<T>(z[k], q);
+    accumulate<kRef>(v, f, q);
+  }
+}
+
 template <int kN>
 __device__ __forceinline__ float largest(const float (&x)[kN]) {
   const float top = max_nan(max_nan(x[0], x[1], x[2]), x[3]);
@@ -879,28 +886,15 @@ __device__ __forceinline__ float largest(const float (&x)[kN]) {
   else return top;
 }
 
-// A group of vectors, number first + k step the k-th: one look at their largest entry for
-// all.  With a mask the largest is only known entry by entry, so vector by vector.
+// A part's sums by `step` threads of which this is number tid, from memory, with masks.
 template <typename T, bool kRef>
-__device__ __forceinline__ void accumulate_group(Running& v, const Part<T>& p, int first, int step,
-                                                 const uint4 (&x)[kGroup], const uint4 (&z)[kGroup], int last) {
+__device__ __noinline__ void add_masked(Running& v, const Part<T>& p, int tid, int step) {
   constexpr int kN = kVec<T>;
-  bool careful = p.lm != nullptr, careful_r = careful;
-  if (!careful) {
-    float top, low, top_r = kMasked, low_r = 0.0f;
-    extremes<T>(x, top, low);
-    if constexpr (kRef) extremes<T>(z, top_r, low_r);
-    careful = !(low > kMasked);
-    careful_r = !(low_r > kMasked);
-    raise<kRef>(v, max_nan(top, kMasked) * kLog2e, max_nan(top_r, kMasked) * kLog2e);
-  }
-#pragma unroll
-  for (int k = 0; k < kGroup; ++k) {
-    if (first + k * step >= last) break;
+  for (int i = p.first + tid; i < p.last; i += step) {
     float f[kN], q[kN];
-    p.entries(first + k * step, x[k], careful, f);
-    if constexpr (kRef) p.entries(first + k * step, z[k], careful_r, q);
-    if (p.lm) raise<kRef>(v, largest(f) * kLog2e, kRef ? largest(q) * kLog2e : kMasked2);
+    p.masked(i, __ldg(p.vector(i)), f);
+    if constexpr (kRef) p.masked(i, p.ref_vector(i), q);
+    raise<kRef>(v, largest(f) * kLog2e, kRef ? largest(q) * kLog2e : kMasked2);
     accumulate<kRef>(v, f, q);
   }
 }
@@ -929,35 +923,39 @@ __device__ __forceinline__ void gradient(const Coefs& c, float m, float mr, cons
       if (hot == e) g[e] += c.hot;
 }
 
-// Writes the gradient of a group of vectors, number first + k step the k-th; all zeros
-// where the row does not count.
+// A part's gradient by `step` threads of which this is number tid, from memory, with masks.
 template <typename T, bool kRef, int kType>
-__device__ __forceinline__ void write_group(const Part<T>& p, const Coefs& c, float m, float mr, bool used, int action,
-                                            void* row, bool wide, int first, int step, const uint4 (&x)[kGroup],
-                                            const uint4 (&z)[kGroup]) {
+__device__ __noinline__ void write_masked(const Part<T>& p, const Coefs& c, float m, float mr, int action, void* row,
+                                          bool wide, int tid, int step) {
   constexpr int kN = kVec<T>;
-  bool careful = p.lm != nullptr, careful_r = careful;
-  if (used && !careful) {
-    float top, low, low_r = 0.0f;
-    extremes<T>(x, top, low);
-    if constexpr (kRef) extremes<T>(z, top, low_r);
-    careful = !(low > kMasked);
-    careful_r = !(low_r > kMasked);
-  }
-#pragma unroll
-  for (int k = 0; k < kGroup; ++k) {
-    if (first + k * step >= p.last) break;
-    const int at = p.head + (first + k * step) * kN;
+  for (int i = p.first + tid; i < p.last; i += step) {
     float f[kN], q[kN], g[kN];
-    if (used) {
-      p.entries(first + k * step, x[k], careful, f);
-      if constexpr (kRef) p.entries(first + k * step, z[k], careful_r, q);
-      gradient<kRef>(c, m, mr, f, q, action - at, g);
-    } else {
+    p.masked(i, __ldg(p.vector(i)), f);
+    if constexpr (kRef) p.masked(i, p.ref_vector(i), q);
+    gradient<kRef>(c, m, mr, f, q, action - p.head - i * kN, g);
+    store_grad<kType>(row, p.head + i * kN, g, wide);
+  }
+}
+
+template <typename T, int kType>
+__device__ __forceinline__ void write_zeros(const Part<T>& p, void* row, bool wide, int tid, int step) {
+  float g[kVec<T>] = {};
+  for (int i = p.first + tid; i < p.last; i += step) store_grad<kType>(row, p.head + i * kVec<T>, g, wide);
+}
+
+// The gradient of whole vectors as they are, `apart` entries from one to the next in `row`;
+// `hot`: the action's place in the first.
+template <typename T, bool kRef, int kType, int kCount>
+__device__ __forceinline__ void write_vectors(const Coefs& c, float m, float mr, int hot, Stored<kType>* row, int apart,
+                                              bool wide, const uint4 (&x)[kCount], const uint4 (&z)[kCount]) {
+  constexpr int kN = kVec<T>;
 #pragma unroll
-      for (int e = 0; e < kN; ++e) g[e] = 0.0f;
-    }
-    store_grad<kType>(row, at, g, wide);
+  for (int k = 0; k < kCount; ++k) {
+    float f[kN], q[kN], g[kN];
+    unpack<T>(x[k], f);
+    if constexpr (kRef) unpack<T>(z[k], q);
+    gradient<kRef>(c, m, mr, f, q, hot - k * apart, g);
+    store_grad<kType>(row, k * apart, g, wide);
   }
 }
 
@@ -973,7 +971,7 @@ __device__ __forceinline__ bool grad_wide(const void* row, int head) {
 struct RowResult {
   Coefs c;
   float m, mr;
-  bool used;
+  bool used, again;
 };
 
 template <int kLeft>
@@ -981,10 +979,11 @@ __device__ __forceinline__ void wait_copies() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
-// slots: vectors of a thread that shared memory holds, a multiple of kGroup.
+// slots: vectors of a thread that shared memory holds.
 template <typename T, bool kRef, bool kPolicy>
 __global__ void __launch_bounds__(kLongThreads, 2)
     long_rows_kernel(const Rows r, const Score o, const Policy a, const int slots) {
+  constexpr int kN = kVec<T>;
   extern __shared__ __align__(16) uint4 slot[];  // [slots][threads], then the reference's
   __shared__ Sums warp_sums[kLongThreads / 32];
   __shared__ Sums block_sums[2];
@@ -996,7 +995,6 @@ __global__ void __launch_bounds__(kLongThreads, 2)
   const int parts = cluster.num_blocks(), rank = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x / 32, step = blockDim.x;
   const int chunk = (slots + kChunks * kGroup - 1) / (kChunks * kGroup) * kGroup;
-  const auto chunk_end = [&](int c) { return (c + 1) * chunk < slots ? (c + 1) * chunk : slots; };
   uint4* const mine = slot + tid;
   uint4* const mine_r = mine + slots * step;
   float scale = 0.0f;
@@ -1013,16 +1011,26 @@ __global__ void __launch_bounds__(kLongThreads, 2)
     const i64 action = r.actions[row];
     return action >= 0 && action < r.vocab && !(r.weight && r.weight[row] == 0.0f);
   };
+  // Of a part's vectors, how many are this thread's and in slots.
+  const auto slotted = [&](const Part<T>& p) {
+    const int n = (p.last - p.first - tid + step - 1) / step;
+    return p.last - p.first <= tid ? 0 : n < slots ? n : slots;
+  };
   // Starts the copies of a chunk of a row's slots; always a group of its own.
   const auto fetch = [&](bool wanted, i64 row, int c) {
     if (wanted) {
       const Part<T> p(r, row, 0, r.vocab, parts, rank);
-      const int size = static_cast<int>(sizeof(T));
-      for (int k = c * chunk; k < chunk_end(c); ++k) {
-        const int i = p.first + tid + k * step;
-        if (i >= p.last) break;
-        copy16(mine + k * step, p.x + p.head + i * (16 / size), 16);
-        if constexpr (kRef) copy16(mine_r + k * step, p.z + p.head + i * (16 / size), 16);
+      const int n = slotted(p), end = (c + 1) * chunk < n ? (c + 1) * chunk : n;
+      const uint4* from = p.vector(p.first + tid + c * chunk * step);
+      const uint4* from_r = kRef ? reinterpret_cast<const uint4*>(p.z + p.head) + p.first + tid + c * chunk * step : nullptr;
+      uint4 *to = mine + c * chunk * step, *to_r = mine_r + c * chunk * step;
+      for (int k = c * chunk; k < end; ++k, from += step, to += step) {
+        copy16(to, from);
+        if constexpr (kRef) {
+          copy16(to_r, from_r);
+          from_r += step;
+          to_r += step;
+        }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -1038,46 +1046,73 @@ __global__ void __launch_bounds__(kLongThreads, 2)
     const bool next = maybe_used(row + rows_step);
     const i64 action = r.actions[row];
     const Part<T> p(r, row, 0, r.vocab, parts, rank);
-    const int i0 = p.first + tid, resident = p.first + slots * step;
-    const int n_loose = rank == 0 ? r.vocab - p.vectors * kVec<T> : 0;
+    const int i0 = p.first + tid, n_slotted = slotted(p);
+    const int n_loose = rank == 0 ? r.vocab - p.vectors * kN : 0;
     if (maybe && tid == 32) {
       row_in = row_inputs<kPolicy>(r, a, row);
       row_x = p.one(p.x, static_cast<int>(action));
     }
+    bool careful = p.lm != nullptr;
     Running run;
     run.m = run.mr = kMasked2;
     run.s = run.t = run.sr = run.u = two(0.0f, 0.0f);
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      if (!write || c == 0) wait_copies<kChunks - 1>();
-      else if (c == 1) wait_copies<kChunks - 2>();
-      else if (c == 2) wait_copies<kChunks - 3>();
-      else wait_copies<0>();
-      if (maybe)
+      if (write && c > 0) wait_copies<0>();
+      else wait_copies<kChunks - 1>();
+      static_assert(kChunks == 2, "the waits are for two");
+      if (maybe && !careful) {
+        const int end = (c + 1) * chunk < n_slotted ? (c + 1) * chunk : n_slotted;
+        const uint4 *at = mine + c * chunk * step, *at_r = mine_r + c * chunk * step;
+        int k = c * chunk;
 #pragma unroll 1
-        for (int k = c * chunk; k < chunk_end(c) && i0 + k * step < p.last; k += kGroup) {
+        for (; k + kGroup <= end; k += kGroup, at += kGroup * step, at_r += kGroup * step) {
           uint4 x[kGroup], z[kGroup];
 #pragma unroll
           for (int h = 0; h < kGroup; ++h) {
-            const bool there = i0 + (k + h) * step < p.last;
-            x[h] = there ? mine[(k + h) * step] : nothing<T>();
-            if constexpr (kRef) z[h] = there ? mine_r[(k + h) * step] : nothing<T>();
+            x[h] = at[h * step];
+            if constexpr (kRef) z[h] = at_r[h * step];
           }
-          accumulate_group<T, kRef>(run, p, i0 + k * step, step, x, z, p.last);
+          add_vectors<T, kRef>(run, x, z);
         }
+#pragma unroll 1
+        for (; k < end; ++k, at += step, at_r += step) {
+          const uint4 x[1] = {*at};
+          uint4 z[1];
+          if constexpr (kRef) z[0] = *at_r;
+          add_vectors<T, kRef>(run, x, z);
+        }
+      }
       if (!write) fetch(next, row + rows_step, c);
     }
-    if (maybe) {
+    if (maybe && !careful) {
 #pragma unroll 1
-      for (int i = resident + tid; i < p.last; i += kGroup * step) {
-        uint4 x[kGroup], z[kGroup];
-#pragma unroll
-        for (int h = 0; h < kGroup; ++h) {
-          const bool there = i + h * step < p.last;
-          x[h] = there ? p.template load<!kPolicy>(i + h * step) : nothing<T>();
-          if constexpr (kRef) z[h] = there ? p.load_ref(i + h * step) : nothing<T>();
+      for (int i = i0 + slots * step; i < p.last; i += 2 * step) {  // what no slot holds
+        uint4 x[2], z[2];
+        const bool both_there = i + step < p.last;
+        x[0] = __ldg(p.vector(i));
+        x[1] = both_there ? __ldg(p.vector(i + step)) : x[0];
+        if constexpr (kRef) {
+          z[0] = p.ref_vector(i);
+          z[1] = both_there ? p.ref_vector(i + step) : z[0];
         }
-        accumulate_group<T, kRef>(run, p, i, step, x, z, p.last);
+        if (both_there) {
+          add_vectors<T, kRef>(run, x, z);
+        } else {
+          const uint4 x1[1] = {x[0]}, z1[1] = {z[0]};
+          add_vectors<T, kRef>(run, x1, z1);
+        }
+      }
+    }
+    while (maybe) {
+      if (careful) {
+        run.m = run.mr = kMasked2;
+        run.s = run.t = run.sr = run.u = two(0.0f, 0.0f);
+        // Copies for the call: what its arguments point to would leave the registers.
+        Running masked = run;
+        const Part<T> part = p;
+        add_masked<T, kRef>(masked, part, tid, step);
+        run = masked;
       }
       if (tid < n_loose) {
         // One entry, and one that adds nothing beside it: were there nothing else, it would
@@ -1110,64 +1145,93 @@ __global__ void __launch_bounds__(kLongThreads, 2)
         buffer ^= 1;
       }
       if (tid == 0) {
+        // Not a number: for an entry that is one, or for one of -inf.
+        const float sum = v.s + v.t + (kRef ? v.sr + v.u : 0.0f);
+        result.again = !careful && !(fabsf(sum) < INFINITY);
         const RowInputs in = row_in;
         const bool used = !(row_x <= kMasked);
         const float y_a = fmaf(row_x, kLog2e, -v.m);
-        if constexpr (!kPolicy) {
-          if (rank == 0) store_score(o, row, used, v, y_a);
-        } else {
-          float logp = 0.0f;
-          if (used) {
-            Terms terms;
-            result.c = policy_row<kRef>(a, in, v, y_a, scale, terms, logp);
-            if (rank == 0) terms.add_to(block_acc, in.weight);
+        if (!result.again) {
+          if constexpr (!kPolicy) {
+            if (rank == 0) store_score(o, row, used, v, y_a);
+          } else {
+            float logp = 0.0f;
+            if (used) {
+              Terms terms;
+              result.c = policy_row<kRef>(a, in, v, y_a, scale, terms, logp);
+              if (rank == 0) terms.add_to(block_acc, in.weight);
+            }
+            if (a.logp && rank == 0) a.logp[row] = logp;
+            result.m = v.m;
+            result.mr = v.mr;
+            result.used = used;
           }
-          if (a.logp && rank == 0) a.logp[row] = logp;
-          result.m = v.m;
-          result.mr = v.mr;
-          result.used = used;
         }
       }
-    } else if (tid == 0 && rank == 0) {
+      __syncthreads();  // the result is there; row_in and warp_sums are free again
+      if (careful || !result.again) break;
+      careful = true;
+    }
+    if (!maybe && tid == 0 && rank == 0) {
       if constexpr (!kPolicy) store_score(o, row, false, no_sums(), 0.0f);
       else if (a.logp) a.logp[row] = 0.0f;
     }
-    __syncthreads();  // the result is there; row_in and warp_sums are free again
     if constexpr (kPolicy) {
       if (write) {
         const Coefs c = result.c;  // of a row that counts; not used for another
         const float m = result.m, mr = result.mr;
         const bool used = maybe && result.used;
-        const int hot = used ? static_cast<int>(action) : -1;
+        const int hot = static_cast<int>(action);
         with_type(a.dtype, [&](auto type) {
           constexpr int kType = decltype(type)::value;
-          void* const to = static_cast<Stored<kType>*>(a.dlogits) + row * a.ldd;
+          using S = Stored<kType>;
+          S* const to = static_cast<S*>(a.dlogits) + row * a.ldd;
           const bool wide = grad_wide<T, kType>(to, p.head);
+          if (!used) {
+            write_zeros<T, kType>(p, to, wide, tid, step);
+          } else if (careful) {
+            const Coefs coefs = c;
+            const Part<T> part = p;
+            write_masked<T, kRef, kType>(part, coefs, m, mr, hot, to, wide, tid, step);
+          }
+          const bool plain = used && !careful;
           for (int q = 0; q < kChunks; ++q) {
+            if (plain) {
+              const int end = (q + 1) * chunk < n_slotted ? (q + 1) * chunk : n_slotted;
+              const uint4 *at = mine + q * chunk * step, *at_r = mine_r + q * chunk * step;
+              int k = q * chunk;
+              int place = p.head + (i0 + k * step) * kN;
 #pragma unroll 1
-            for (int k = q * chunk; k < chunk_end(q) && i0 + k * step < p.last; k += kGroup) {
-              uint4 x[kGroup], z[kGroup];
+              for (; k + kGroup <= end; k += kGroup, at += kGroup * step, at_r += kGroup * step) {
+                uint4 x[kGroup], z[kGroup];
 #pragma unroll
-              for (int h = 0; h < kGroup; ++h) {
-                const bool there = i0 + (k + h) * step < p.last;
-                x[h] = there ? mine[(k + h) * step] : nothing<T>();
-                if constexpr (kRef) z[h] = there ? mine_r[(k + h) * step] : nothing<T>();
+                for (int h = 0; h < kGroup; ++h) {
+                  x[h] = at[h * step];
+                  if constexpr (kRef) z[h] = at_r[h * step];
+                }
+                write_vectors<T, kRef, kType>(c, m, mr, hot - place, to + place, step * kN, wide, x, z);
+                place += kGroup * step * kN;
               }
-              write_group<T, kRef, kType>(p, c, m, mr, used, hot, to, wide, i0 + k * step, step, x, z);
+#pragma unroll 1
+              for (; k < end; ++k, at += step, at_r += step) {
+                const uint4 x[1] = {*at};
+                uint4 z[1];
+                if constexpr (kRef) z[0] = *at_r;
+                write_vectors<T, kRef, kType>(c, m, mr, hot - place, to + place, 0, wide, x, z);
+                place += step * kN;
+              }
             }
             fetch(next, row + rows_step, q);
           }
+          if (plain)
 #pragma unroll 1
-          for (int i = resident + tid; i < p.last; i += kGroup * step) {
-            uint4 x[kGroup], z[kGroup];
-#pragma unroll
-            for (int h = 0; h < kGroup; ++h) {
-              const bool there = used && i + h * step < p.last;
-              x[h] = there ? p.template load<true>(i + h * step) : nothing<T>();
-              if constexpr (kRef) z[h] = there ? p.load_ref(i + h * step) : nothing<T>();
+            for (int i = i0 + slots * step; i < p.last; i += step) {
+              const uint4 x[1] = {__ldcs(p.vector(i))};
+              uint4 z[1];
+              if constexpr (kRef) z[0] = p.ref_vector(i);
+              const int place = p.head + i * kN;
+              write_vectors<T, kRef, kType>(c, m, mr, hot - place, to + place, 0, wide, x, z);
             }
-            write_group<T, kRef, kType>(p, c, m, mr, used, hot, to, wide, i, step, x, z);
-          }
           if (tid < n_loose) {
             const int j = p.loose(tid);
             float g = 0.0f;
@@ -1276,16 +1340,28 @@ __global__ void __launch_bounds__(32 * kBackWarps, 4) logp_backward_kernel(const
   const int hot = used ? static_cast<int>(r.actions[row]) - c0 : -1;
   with_type(b.dtype, [&](auto type) {
     constexpr int kType = decltype(type)::value;
-    void* const to = static_cast<Stored<kType>*>(b.dlogits) + row * b.ldd + c0;
+    Stored<kType>* const to = static_cast<Stored<kType>*>(b.dlogits) + row * b.ldd + c0;
     const bool wide = grad_wide<T, kType>(to, p.head);
-    for (int i = lane; i < p.vectors; i += 2 * kGroup * 32) {  // two groups' loads in flight
-      uint4 x[2][kGroup];
+    if (!used) {
+      write_zeros<T, kType>(p, to, wide, lane, 32);
+    } else {
+      bool careful = p.lm != nullptr;
+      int i = lane;
+      for (; !careful && i + (kGroup - 1) * 32 < p.last; i += kGroup * 32) {
+        uint4 x[kGroup];
 #pragma unroll
-      for (int h = 0; h < 2 * kGroup; ++h)
-        x[h / kGroup][h % kGroup] = used && i + h * 32 < p.vectors ? p.template load<true>(i + h * 32) : nothing<T>();
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        write_group<T, false, kType>(p, k, lse.x, 0.0f, used, hot, to, wide, i + h * kGroup * 32, 32, x[h], x[h]);
+        for (int h = 0; h < kGroup; ++h) x[h] = __ldcs(p.vector(i + 32 * h));
+        careful = !(extreme<T, false>(x) > kMasked);
+        const int place = p.head + i * kVec<T>;
+        if (!careful) write_vectors<T, false, kType>(k, lse.x, 0.0f, hot - place, to + place, 32 * kVec<T>, wide, x, x);
+        else break;
+      }
+      for (; i < p.last; i += 32) {  // what is left of a group, or may be masked
+        float f[kVec<T>], g[kVec<T>];
+        p.masked(i, __ldcs(p.vector(i)), f);
+        gradient<false>(k, lse.x, 0.0f, f, f, hot - p.head - i * kVec<T>, g);
+        store_grad<kType>(to, p.head + i * kVec<T>, g, wide);
+      }
     }
     for (int i = lane; i < p.vocab - p.vectors * kVec<T>; i += 32) {
       const int c = p.loose(i);
@@ -1374,18 +1450,19 @@ __global__ void __launch_bounds__(kPairThreads) pairs_kernel(const Pairs a) {
       if (real && lane == 0) a.seq_logp[2 * pair + h] = static_cast<float>(sums[1] * n);
     }
     if (!real) continue;
-    const double m = a.beta * (score[0] - score[1]);
-    // -log sigmoid(m) and its two slopes, in 64 bits: one pair, one evaluation.
-    const double soft = log1p(exp(-fabs(m)));
-    const double lose = soft + (m < 0.0 ? -m : 0.0), win = soft + (m > 0.0 ? m : 0.0);
+    const float m = static_cast<float>(a.beta * (score[0] - score[1]));
+    // -log sigmoid(m), -log sigmoid(-m) and the two sigmoids from one exponential.
+    const float e = expf(-fabsf(m)), soft = log1pf(e);
+    const float lose = soft + fmaxf(-m, 0.0f), win = soft + fmaxf(m, 0.0f);
     if (lane == 0) {
-      a.margin[pair] = static_cast<float>(m);
-      loss += (1.0 - a.smoothing) * lose + a.smoothing * win;
-      above += m > 0.0 ? 1.0 : 0.0;
+      a.margin[pair] = m;
+      loss += (1.0f - a.smoothing) * lose + a.smoothing * win;
+      above += m > 0.0f ? 1.0 : 0.0;
     }
     if (a.d_logp) {
-      const double up = 1.0 / (1.0 + exp(-m)), down = 1.0 / (1.0 + exp(m));
-      const double slope = a.beta * (a.smoothing * up - (1.0 - a.smoothing) * down) / a.pairs;
+      const float large = 1.0f / (1.0f + e), small = e * large;
+      const float up = m > 0.0f ? large : small, down = m > 0.0f ? small : large;
+      const float slope = a.beta * (a.smoothing * up - (1.0f - a.smoothing) * down) / static_cast<float>(a.pairs);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float d = static_cast<float>((h ? -slope : slope) * total[h]);
@@ -1492,8 +1569,8 @@ int launch_long(const Rows& r, const Score& o, const Policy& a, cudaStream_t str
   const auto kernel = long_rows_kernel<T, kRef, kPolicy>;
   // The reference's vectors are copied beside the logits' where both are aligned alike.
   constexpr int kSize = sizeof(T);
-  const bool stage = !kRef || ((reinterpret_cast<uintptr_t>(r.ref) - reinterpret_cast<uintptr_t>(r.logits)) % 16 == 0 &&
-                               (r.rows <= 1 || (r.ldr - r.ld) * kSize % 16 == 0));
+  const bool stage = !r.legal && (!kRef || ((reinterpret_cast<uintptr_t>(r.ref) - reinterpret_cast<uintptr_t>(r.logits)) % 16 == 0 &&
+                               (r.rows <= 1 || (r.ldr - r.ld) * kSize % 16 == 0)));
   const Plan p = long_plan(r.rows, r.vocab, kSize, kRef, stage);
   blocks = p.blocks;
   if (p.shared > (40 << 10) &&
@@ -1523,7 +1600,7 @@ int launch_short(const Rows& r, const Score& o, const Policy& a, const Layout& l
   constexpr int kRows = kShortWarps * 32 / kLanes;
   const i64 want = (r.rows + kRows - 1) / kRows;
   int per_sm = (226 << 10) / (shared + (3 << 10));
-  if (per_sm > (kPolicy ? 2 : 3)) per_sm = kPolicy ? 2 : 3;
+  if (per_sm > (kPolicy ? 4 : 6)) per_sm = kPolicy ? 4 : 6;  // by registers
   blocks = static_cast<int>(want < per_sm * kSms ? want : per_sm * kSms);
   kernel<<<blocks, 32 * kShortWarps, shared, stream>>>(r, o, a, lay);
   return launch_status();
@@ -1711,12 +1788,11 @@ int cugo_b200_preference_pairs(const float* logp, const float* ref_logp, const f
   if (!scratch || scratch_bytes < cugo_b200_preference_pairs_scratch_bytes(pairs)) return CUGO_B200_ERR_CAPACITY;
   const Pairs a{logp, ref_logp, weight, reinterpret_cast<const float2*>(lse), offsets, pairs, rows, beta, smoothing,
                 average != 0, margin, seq_logp, d_logp, static_cast<double*>(scratch), {loss, accuracy}};
-  // Short sequences: a warp per pair, all in one block while they are few (one launch);
-  // long ones: a block per pair.
+  // Short sequences: a warp per pair; long ones: a block per pair.
   int blocks;
   if (rows / pairs <= 256) {
     const i64 want = (pairs + kPairThreads / 32 - 1) / (kPairThreads / 32);
-    blocks = rows <= 16384 ? 1 : static_cast<int>(want < kSms ? want : kSms);
+    blocks = static_cast<int>(want < kSms ? want : kSms);
     pairs_kernel<32><<<blocks, kPairThreads, 0, stream>>>(a);
   } else {
     blocks = static_cast<int>(pairs < kSms ? pairs : kSms);

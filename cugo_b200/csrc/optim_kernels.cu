@@ -7,8 +7,8 @@
 //
 // One launch takes up to kMostTensors tensors: their pointers travel as the kernel's
 // parameters (nothing of a call is kept on the device, and a captured graph holds them
-// by value).  A block takes tiles of 2,048 elements, a warp 256 of them, a thread 8; a
-// tile finds its tensor by a search over the tensors' first tiles.
+// by value).  A warp takes 256 elements at a time, a thread 8 of them; a tile of 8 or 32
+// such blocks finds its tensor by a search over the tensors' first tiles.
 //
 // States in 8 bits: e4m3 codes with one scale per 256 elements of a tensor, the warp's.
 // The scale is a power of two (an e8m0 byte), the smallest that keeps the block's largest
@@ -42,10 +42,10 @@ namespace {
 using i64 = int64_t;
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kBlock = 256;              // elements of a scale
-constexpr int kThreads = 256, kPer = 8;  // 8 warps, a scale's block each
-constexpr int kTile = kThreads * kPer;
+constexpr int kThreads = 256, kPer = 8;  // 8 warps, a scale's block at a time each
+constexpr int kWarps = kThreads / 32;
 constexpr int kSms = 148;
-constexpr int kNormBlocks = 4 * kSms;
+constexpr int kNormBlocks = 8 * kSms;
 constexpr int kFewTensors = 40, kMostTensors = 400;
 
 struct Tensor {
@@ -54,15 +54,15 @@ struct Tensor {
   void *m, *v;
   uint8_t *ms, *vs;  // the scales (8-bit states)
   i64 n;
-  i64 wide;          // every pointer is a multiple of 16 bytes
-  i64 first_tile;    // of the launch
+  int wide;          // every pointer is a multiple of 16 bytes
+  int first_tile;    // of the launch
   i64 first_block;   // blocks of 256 elements before this tensor in the call
 };
 
+// A tile is kWarps x per_warp blocks of 256 elements, per_warp consecutive ones a warp.
 template <int kMost>
 struct Tensors {
-  int count;
-  i64 tiles;
+  int count, tiles, per_warp;
   Tensor t[kMost];
 };
 
@@ -103,7 +103,7 @@ __device__ __forceinline__ double sum_warp(double v) {
 
 // The tensor that holds a tile: the last whose first tile is not behind it.
 template <int kMost>
-__device__ __forceinline__ int find(const Tensors<kMost>& a, i64 tile) {
+__device__ __forceinline__ int find(const Tensors<kMost>& a, int tile) {
   int low = 0, high = a.count;
   while (high - low > 1) {
     const int mid = (low + high) >> 1;
@@ -170,6 +170,17 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, i64 i, i64 n, const flo
 }
 
 // 8 codes as floats, not scaled.
+__device__ __forceinline__ void decode(uint32_t a, uint32_t b, float (&f)[8]) {
+  const uint32_t w[2] = {a, b};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const __nv_fp8x2_storage_t two = static_cast<__nv_fp8x2_storage_t>(w[e / 2] >> (16 * (e % 2)));
+    const float2 t = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+    f[2 * e] = t.x;
+    f[2 * e + 1] = t.y;
+  }
+}
+
 template <bool kWide>
 __device__ __forceinline__ void load_codes(const uint8_t* p, i64 i, i64 n, float (&f)[8]) {
   uint32_t w[2] = {0, 0};
@@ -181,13 +192,7 @@ __device__ __forceinline__ void load_codes(const uint8_t* p, i64 i, i64 n, float
     for (int e = 0; e < 8; ++e)
       if (i + e < n) w[e / 4] |= static_cast<uint32_t>(p[i + e]) << (8 * (e % 4));
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const __nv_fp8x2_storage_t two = static_cast<__nv_fp8x2_storage_t>(w[e / 2] >> (16 * (e % 2)));
-    const float2 t = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
-    f[2 * e] = t.x;
-    f[2 * e + 1] = t.y;
-  }
+  decode(w[0], w[1], f);
 }
 
 template <bool kWide>
@@ -247,7 +252,7 @@ __device__ __forceinline__ float warp_largest(const float (&f)[8]) {
 }
 
 // The same over the finite magnitudes only (as bits they order as the values do).
-__device__ __noinline__ float warp_largest_finite(const float (&f)[8]) {
+__device__ __forceinline__ float warp_largest_finite(const float (&f)[8]) {
   uint32_t top = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -286,22 +291,16 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
   return r;
 }
 
-// A warp's block `in` of tensor t, this thread's 8 elements from i on.
-template <typename P, typename G, bool kEight, bool kWide>
-__device__ __forceinline__ void step8(const Tensor& t, const Options& o, const Scalars& s, i64 in, i64 i) {
+// The step of a warp's block `in` of tensor t, this thread's 8 elements from i on: their
+// values, with the states' codes not scaled yet (scales ms, vs).
+template <typename P, bool kEight, bool kWide>
+__device__ __forceinline__ void step8(const Tensor& t, const Options& o, const Scalars& s, i64 in, i64 i, int ms,
+                                      int vs, float (&p)[8], const float (&g)[8], float (&m)[8], float (&v)[8]) {
   constexpr bool kRandom = kEight || sizeof(P) == 2;
-  float p[8], g[8], m[8], v[8];
-  load8<kWide>(static_cast<const P*>(t.p), i, t.n, p);
-  load8<kWide>(static_cast<const G*>(t.g), i, t.n, g);
   float b1 = o.b1, b2 = o.b2;
   if constexpr (kEight) {  // the scale is a power of two: exact in the factor
-    load_codes<kWide>(static_cast<const uint8_t*>(t.m), i, t.n, m);
-    load_codes<kWide>(static_cast<const uint8_t*>(t.v), i, t.n, v);
-    b1 *= scale_of(t.ms[in]);
-    b2 *= scale_of(t.vs[in]);
-  } else {
-    load8<kWide>(static_cast<const float*>(t.m), i, t.n, m);
-    load8<kWide>(static_cast<const float*>(t.v), i, t.n, v);
+    b1 *= scale_of(ms);
+    b2 *= scale_of(vs);
   }
   const Two c1 = two(s.c1, s.c1), clip = two(s.clip, s.clip), c2 = two(o.c2, o.c2), d1 = two(b1, b1), d2 = two(b2, b2),
             keep = two(s.keep, s.keep);
@@ -330,15 +329,12 @@ __device__ __forceinline__ void step8(const Tensor& t, const Options& o, const S
     for (int e = 0; e < 8; ++e) x[e] = mix_middle(n ^ e);
   }
   if constexpr (sizeof(P) == 2) {
-    float kept[8];
+    const bool all = finite == 0.0f;  // infinities and NaN stay what they are
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      kept[e] = p[e];
-      p[e] = __uint_as_float(__float_as_uint(p[e]) + (((x[e] ^ (x[e] >> 16)) * 0x2c1b3c6du) >> 16));
+      const uint32_t r = ((x[e] ^ (x[e] >> 16)) * 0x2c1b3c6du) >> 16;
+      if (all || fabsf(p[e]) < INFINITY) p[e] = __uint_as_float(__float_as_uint(p[e]) + r);
     }
-    if (!(finite == 0.0f))  // infinities and NaN stay what they are
-#pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] = fabsf(kept[e]) < INFINITY ? p[e] : kept[e];
   }
   store8<kWide>(static_cast<P*>(t.p), i, t.n, p);
   if constexpr (kEight) {
@@ -361,7 +357,7 @@ __device__ __forceinline__ void step8(const Tensor& t, const Options& o, const S
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t high = x[e] >> 16;
-      const float q = round_e4m3(fabsf(cm[e]), ((x[e] ^ high) & 0xffffu) * 16u + 8u);
+      const float q = round_e4m3(fabsf(cm[e]), ((x[e] ^ high) & 0xffffu) * 16u);
       cm[e] = __uint_as_float(__float_as_uint(q) | (__float_as_uint(cm[e]) & 0x80000000u));
       cv[e] = round_e4m3(cv[e], x[e] >> 12);
     }
@@ -388,34 +384,145 @@ __device__ __forceinline__ void step8(const Tensor& t, const Options& o, const S
   }
 }
 
-template <typename P, typename G, bool kEight, int kMost>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Tensors<kMost> a, const Options o,
+// States in 32 bits: 8 elements of everything straight into registers.
+template <typename P, typename G, int kMost>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Tensors<kMost> a, const __grid_constant__ Options o,
                                                          const Scalars* scalars) {
   const Scalars s = *scalars;
-  for (i64 tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+  for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const Tensor& t = a.t[find(a, tile)];
-    const i64 in = (tile - t.first_tile) * (kTile / kBlock) + (threadIdx.x >> 5);  // the warp's block
-    const i64 i = in * kBlock + (threadIdx.x & 31) * kPer;
-    if (in * kBlock >= t.n) continue;  // the whole warp
-    if (t.wide && (in + 1) * kBlock <= t.n) step8<P, G, kEight, true>(t, o, s, in, i);
-    else step8<P, G, kEight, false>(t, o, s, in, i);
+    const i64 first = (static_cast<i64>(tile - t.first_tile) * kWarps + (threadIdx.x >> 5)) * a.per_warp;
+    for (int u = 0; u < a.per_warp; ++u) {
+      const i64 in = first + u, i = in * kBlock + (threadIdx.x & 31) * kPer;
+      if (in * kBlock >= t.n) break;  // the whole warp
+      float p[8], g[8], m[8], v[8];
+      if (t.wide && (in + 1) * kBlock <= t.n) {
+        load8<true>(static_cast<const P*>(t.p), i, t.n, p);
+        load8<true>(static_cast<const G*>(t.g), i, t.n, g);
+        load8<true>(static_cast<const float*>(t.m), i, t.n, m);
+        load8<true>(static_cast<const float*>(t.v), i, t.n, v);
+        step8<P, false, true>(t, o, s, in, i, 0, 0, p, g, m, v);
+      } else {
+        load8<false>(static_cast<const P*>(t.p), i, t.n, p);
+        load8<false>(static_cast<const G*>(t.g), i, t.n, g);
+        load8<false>(static_cast<const float*>(t.m), i, t.n, m);
+        load8<false>(static_cast<const float*>(t.v), i, t.n, v);
+        step8<P, false, false>(t, o, s, in, i, 0, 0, p, g, m, v);
+      }
+    }
   }
 }
 
-// Sums of the gradients' squares: 8 in fp32 per thread and tile, from there in 64 bits.
+// A block that is not whole, or of a tensor that is not aligned; a call of its own, so that
+// its registers are no one else's.
+template <typename P, typename G>
+__device__ __noinline__ void step8_direct(const Tensor& t, const Options& o, const Scalars* scalars, i64 in, i64 i,
+                                          int ms, int vs) {
+  const Scalars s = *scalars;
+  float p[8], g[8], m[8], v[8];
+  load8<false>(static_cast<const P*>(t.p), i, t.n, p);
+  load8<false>(static_cast<const G*>(t.g), i, t.n, g);
+  load_codes<false>(static_cast<const uint8_t*>(t.m), i, t.n, m);
+  load_codes<false>(static_cast<const uint8_t*>(t.v), i, t.n, v);
+  step8<P, true, false>(t, o, s, in, i, ms, vs, p, g, m, v);
+}
+
+// States in 8 bits: 60 instructions an element leave few registers for loads in flight, so
+// a warp's blocks are copied to shared memory ahead of the arithmetic, kDepth of them.
+template <typename P, typename G>
+struct Stage {
+  static constexpr int kP = kBlock * sizeof(P), kG = kBlock * sizeof(G), kBytes = kP + kG + 2 * kBlock;
+  static constexpr int kDepth = kBytes <= 1536 ? 3 : 2;
+};
+
+__device__ __forceinline__ void copy16(char* to, const void* from) {
+  const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from) : "memory");
+}
+
+template <typename P, typename G, int kMost>
+__global__ void __launch_bounds__(kThreads, 3) adamw8_kernel(const __grid_constant__ Tensors<kMost> a, const __grid_constant__ Options o,
+                                                             const Scalars* scalars) {
+  using S = Stage<P, G>;
+  __shared__ __align__(16) char shared[kWarps][S::kDepth][S::kBytes];
+  const Scalars s = *scalars;
+  const int lane = threadIdx.x & 31;
+  char(*const own)[S::kBytes] = shared[threadIdx.x >> 5];
+  for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+    const Tensor& t = a.t[find(a, tile)];
+    const i64 first = (static_cast<i64>(tile - t.first_tile) * kWarps + (threadIdx.x >> 5)) * a.per_warp;
+    const i64 blocks = (t.n + kBlock - 1) / kBlock;
+    const int count = blocks <= first ? 0 : blocks - first < a.per_warp ? static_cast<int>(blocks - first) : a.per_warp;
+    // Blocks that are whole and aligned, from the first on.
+    const i64 whole = t.wide ? t.n / kBlock - first : 0;
+    const int staged = whole <= 0 ? 0 : whole < count ? static_cast<int>(whole) : count;
+    int ms = 0, vs = 0;  // lane u: block u's scales
+    if (lane < count) {
+      ms = t.ms[first + lane];
+      vs = t.vs[first + lane];
+    }
+    const char* const p0 = static_cast<const char*>(t.p) + first * S::kP + 16 * lane;
+    const char* const g0 = static_cast<const char*>(t.g) + first * S::kG + 16 * lane;
+    // The lower half of the warp copies m's codes, the upper v's.
+    const char* const c0 = static_cast<const char*>(lane < 16 ? t.m : t.v) + first * kBlock + 16 * (lane & 15);
+    const auto fetch = [&](int u, char* to) {
+      if (u < staged) {
+#pragma unroll
+        for (int k = 0; k < S::kP; k += 512) copy16(to + k + 16 * lane, p0 + u * S::kP + k);
+#pragma unroll
+        for (int k = 0; k < S::kG; k += 512) copy16(to + S::kP + k + 16 * lane, g0 + u * S::kG + k);
+        copy16(to + S::kP + S::kG + 16 * lane, c0 + u * kBlock);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int u = 0; u < S::kDepth; ++u) fetch(u, own[u]);
+    int slot = 0;
+    for (int u = 0; u < count; ++u) {
+      const i64 in = first + u, i = in * kBlock + lane * kPer;
+      const int bm = __shfl_sync(kFull, ms, u), bv = __shfl_sync(kFull, vs, u);
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::kDepth - 1) : "memory");
+      __syncwarp();
+      if (u < staged) {
+        float p[8], g[8], m[8], v[8];
+        const char* const at = own[slot];
+        load8<true>(reinterpret_cast<const P*>(at), lane * kPer, kBlock, p);
+        load8<true>(reinterpret_cast<const G*>(at + S::kP), lane * kPer, kBlock, g);
+        const uint2 cm = *reinterpret_cast<const uint2*>(at + S::kP + S::kG + 8 * lane);
+        const uint2 cv = *reinterpret_cast<const uint2*>(at + S::kP + S::kG + kBlock + 8 * lane);
+        decode(cm.x, cm.y, m);
+        decode(cv.x, cv.y, v);
+        __syncwarp();  // the slot is read
+        fetch(u + S::kDepth, own[slot]);
+        step8<P, true, true>(t, o, s, in, i, bm, bv, p, g, m, v);
+      } else {
+        fetch(u + S::kDepth, own[slot]);
+        step8_direct<P, G>(t, o, scalars, in, i, bm, bv);
+      }
+      slot = slot + 1 == S::kDepth ? 0 : slot + 1;
+    }
+  }
+}
+
+// Sums of the gradients' squares: 8 in fp32 per thread and block, from there in 64 bits.
 template <typename G, int kMost>
 __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Tensors<kMost> a, double* partial) {
   __shared__ double part[kThreads / 32];
   double sum = 0.0;
-  for (i64 tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+  for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const Tensor& t = a.t[find(a, tile)];
-    float g[8], q = 0.0f;
-    const i64 i = (tile - t.first_tile) * kTile + threadIdx.x * kPer;
-    if (t.wide && i + kPer <= t.n) load8<true>(static_cast<const G*>(t.g), i, t.n, g);
-    else load8<false>(static_cast<const G*>(t.g), i, t.n, g);
+    const i64 first = (static_cast<i64>(tile - t.first_tile) * kWarps + (threadIdx.x >> 5)) * a.per_warp;
+    const G* const at = static_cast<const G*>(t.g);
+#pragma unroll 2
+    for (int u = 0; u < a.per_warp; ++u) {
+      const i64 i = (first + u) * kBlock + (threadIdx.x & 31) * kPer;
+      float g[8], q = 0.0f;
+      if (t.wide && i + kPer <= t.n) load8<true>(at, i, t.n, g);
+      else load8<false>(at, i, t.n, g);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q = fmaf(g[e], g[e], q);
-    sum += q;
+      for (int e = 0; e < 8; ++e) q = fmaf(g[e], g[e], q);
+      sum += q;
+    }
   }
   sum = sum_warp(sum);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
@@ -474,35 +581,44 @@ struct Lists {
 };
 
 // Tensors first .. of the lists that fit one launch, empty ones left out; returns the
-// number of the first one that did not.
+// number of the first one that did not, or -1 where they have too many tiles.
 template <int kMost>
-i64 fill(const Lists& l, i64 first, i64& blocks_before, Tensors<kMost>& a) {
+i64 fill(const Lists& l, i64 first, int per_warp, i64& blocks_before, Tensors<kMost>& a) {
   a.count = 0;
-  a.tiles = 0;
-  i64 k = first;
+  a.per_warp = per_warp;
+  i64 tiles = 0, k = first;
   for (; k < l.count && a.count < kMost; ++k) {
     if (l.n[k] == 0) continue;
+    const i64 blocks = (l.n[k] - 1) / kBlock + 1, more = (blocks - 1) / (kWarps * per_warp) + 1;
+    if (tiles + more > INT32_MAX) return -1;
     Tensor& t = a.t[a.count++];
     const bool wide = aligned(l.p[k], 16) && aligned(l.g[k], 16) && aligned(l.m[k], 16) && aligned(l.v[k], 16);
     t = {l.p[k], l.g[k], l.m[k], l.v[k], l.ms ? static_cast<uint8_t*>(l.ms[k]) : nullptr,
-         l.vs ? static_cast<uint8_t*>(l.vs[k]) : nullptr, l.n[k], wide, a.tiles, blocks_before};
-    a.tiles += (l.n[k] + kTile - 1) / kTile;
-    blocks_before += (l.n[k] + kBlock - 1) / kBlock;
+         l.vs ? static_cast<uint8_t*>(l.vs[k]) : nullptr, l.n[k], wide, static_cast<int>(tiles), blocks_before};
+    tiles += more;
+    blocks_before += blocks;
   }
+  a.tiles = static_cast<int>(tiles);
   return k;
 }
 
 template <typename P, typename G, int kMost>
 int launch_sized(const Lists& l, bool eight, const Options& o, double* partial, int64_t* step, Scalars* scalars,
                  float* norm, cudaStream_t stream) {
+  // Four blocks a warp share the search for their tensor and keep copies in flight; where
+  // that leaves an SM less than two rounds of tiles, one, for balance.
+  i64 total = 0;
+  for (i64 k = 0; k < l.count; ++k) total += l.n[k] / kBlock;
+  const int per_warp = total >= static_cast<i64>(kSms) * 4 * kWarps * 4 * 2 ? 4 : 1;
   Tensors<kMost> a;
   int partials = 0;
   if (norm) {
     i64 before = 0;
     for (i64 k = 0; k < l.count;) {
-      k = fill<kMost>(l, k, before, a);
+      k = fill<kMost>(l, k, per_warp, before, a);
+      if (k < 0) return CUGO_B200_ERR_CAPACITY;
       if (a.tiles == 0) break;
-      const int blocks = static_cast<int>(a.tiles < kNormBlocks ? a.tiles : kNormBlocks);
+      const int blocks = a.tiles < kNormBlocks ? a.tiles : kNormBlocks;
       norm_kernel<G, kMost><<<blocks, kThreads, 0, stream>>>(a, partial + partials);
       partials += blocks;
     }
@@ -514,12 +630,12 @@ int launch_sized(const Lists& l, bool eight, const Options& o, double* partial, 
   prepare_kernel<<<1, kThreads, 0, stream>>>(o, partial, partials, step, scalars, norm);
   i64 before = 0;
   for (i64 k = 0; k < l.count;) {
-    k = fill<kMost>(l, k, before, a);
+    k = fill<kMost>(l, k, per_warp, before, a);
+    if (k < 0) return CUGO_B200_ERR_CAPACITY;
     if (a.tiles == 0) break;
-    const i64 most = static_cast<i64>(kSms) * 64;
-    const int blocks = static_cast<int>(a.tiles < most ? a.tiles : most);
-    if (eight) adamw_kernel<P, G, true, kMost><<<blocks, kThreads, 0, stream>>>(a, o, scalars);
-    else adamw_kernel<P, G, false, kMost><<<blocks, kThreads, 0, stream>>>(a, o, scalars);
+    const int blocks = a.tiles < kSms * 64 ? a.tiles : kSms * 64;
+    if (eight) adamw8_kernel<P, G, kMost><<<blocks, kThreads, 0, stream>>>(a, o, scalars);
+    else adamw_kernel<P, G, kMost><<<blocks, kThreads, 0, stream>>>(a, o, scalars);
   }
   return launch_status();
 }
@@ -532,6 +648,7 @@ int launch(const Lists& l, bool eight, const Options& o, double* partial, int64_
                                 : launch_sized<P, G, kMostTensors>(l, eight, o, partial, step, scalars, norm, stream);
 }
 
+// Launches that `count` tensors may take.
 inline i64 launches_of(i64 count) { return count <= kFewTensors ? 1 : (count + kMostTensors - 1) / kMostTensors; }
 
 }  // namespace

@@ -430,18 +430,21 @@ __device__ __forceinline__ void copy16(void* to, const void* from, int bytes = 1
 
 // Copies a run of rows: the 16-byte granules that hold it, from its first byte's granule
 // on (an allocation starts at a granule, so that lies inside); what lies behind its last
-// byte is not read.  The run's first byte stands at to + (its address mod 16).
-__device__ __forceinline__ void copy_run(char* to, const void* from, int bytes, int lane) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(from);
-  const int skip = static_cast<int>(at & 15), total = skip + bytes, whole = total >> 4;
-  const char* base = reinterpret_cast<const char*>(at - skip) + 16 * lane;
+// byte is not read.  The run's first byte stands at to + (its address mod 16).  kMost: the
+// run's largest number of bytes.
+template <int kMost>
+__device__ __forceinline__ void copy_run(char* to, const char* from, int bytes, int lane) {
+  const int skip = static_cast<int>(reinterpret_cast<uintptr_t>(from)) & 15, total = skip + bytes;
+  const int behind = 16 * lane - (total & ~15);  // of whole granules
+  from += 16 * lane - skip;
   to += 16 * lane;
-  int k = lane;
-  for (; k + 96 < whole; k += 128, to += 2048, base += 2048)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) copy16(to + 512 * q, base + 512 * q);
-  for (; k < whole; k += 32, to += 512, base += 512) copy16(to, base);
-  if (k == whole && (total & 15)) copy16(to, base, total & 15);
+  for (int k = 0; k < kMost + 15; k += 512)
+    if (behind < -k) copy16(to + k, from + k);
+  if (total & 15) {  // the last granule, in part: after the whole ones, at the same stride
+    const int k = total >> 4 << 4;
+    if ((k >> 4 & 31) == lane) copy16(to + k - 16 * lane, from + k - 16 * lane, total & 15);
+  }
 }
 
 // The warp's shared memory, in bytes (multiples of 16): two stages, one gradient.
@@ -465,34 +468,40 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
   const i64 stride = (i64)gridDim.x * kShortWarps * kRows;
   i64 first = ((i64)blockIdx.x * kShortWarps + warp) * kRows;
 
-  const auto address = [](const auto* base, i64 row, i64 ld) { return base + row * ld; };
-  const auto skip = [](const void* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15); };
-  const T* const logits = static_cast<const T*>(r.logits);
-  const T* const refs = static_cast<const T*>(r.ref);
-  const auto fetch = [&](i64 row, int at) {
+  // Where the rows of this warp's turn begin, and how far its next turn is; of staged rows
+  // the turn after, whose copies are started, too.
+  const T* x_first = static_cast<const T*>(r.logits) + first * r.ld;
+  const T* z_first = kRef ? static_cast<const T*>(r.ref) + first * r.ldr : nullptr;
+  const bool* m_first = r.legal + first * r.ldm;
+  const i64 x_step = stride * r.ld, z_step = kRef ? stride * r.ldr : 0, m_step = stride * r.ldm;
+  const int ld = static_cast<int>(r.ld), ldr = static_cast<int>(r.ldr), ldm = static_cast<int>(r.ldm);
+  const auto skip = [](const void* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p)) & 15; };
+  const auto fetch = [&](i64 row, const T* x, const T* z, const bool* m, int at) {
     if constexpr (kStaged) {
-      const int n = static_cast<int>(r.rows - row < kRows ? r.rows - row : kRows) - 1;
+      constexpr int kGap = kRows > 1 ? 64 : 0, kSize = sizeof(T);
+      const int n = r.rows - row < kRows ? static_cast<int>(r.rows - row) - 1 : kRows - 1;
       char* to = shared + own + at * lay.stage();
-      const int size = static_cast<int>(sizeof(T));
-      copy_run(to, address(logits, row, r.ld), (n * static_cast<int>(r.ld) + vocab) * size, lane);
+      constexpr int kMost = kRows * (kLanes * kPer * kSize + kGap);
+      copy_run<kMost>(to, reinterpret_cast<const char*>(x), (n * ld + vocab) * kSize, lane);
       if constexpr (kRef)
-        copy_run(to + lay.logits, address(refs, row, r.ldr), (n * static_cast<int>(r.ldr) + vocab) * size, lane);
+        copy_run<kMost>(to + lay.logits, reinterpret_cast<const char*>(z), (n * ldr + vocab) * kSize, lane);
       if (r.legal)
-        copy_run(to + lay.logits + lay.ref, address(r.legal, row, r.ldm), n * static_cast<int>(r.ldm) + vocab, lane);
+        copy_run<kRows * (kLanes * kPer + kGap)>(to + lay.logits + lay.ref, reinterpret_cast<const char*>(m),
+                                                 n * ldm + vocab, lane);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
   };
 
   RowInputs next;
   if (first < r.rows) {
-    fetch(first, 0);
+    fetch(first, x_first, z_first, m_first, 0);
     next = row_inputs<kPolicy>(r, a, first + sub < r.rows ? first + sub : r.rows - 1);
   }
   int at = 0;
-  for (; first < r.rows; first += stride, at ^= 1) {
+  for (; first < r.rows; first += stride, at ^= 1, x_first += x_step, z_first += z_step, m_first += m_step) {
     const RowInputs in = next;
     if (first + stride < r.rows) {
-      fetch(first + stride, at ^ 1);
+      fetch(first + stride, x_first + x_step, z_first + z_step, m_first + m_step, at ^ 1);
       next = row_inputs<kPolicy>(r, a, first + stride + sub < r.rows ? first + stride + sub : r.rows - 1);
       if constexpr (kStaged) asm volatile("cp.async.wait_group 1;" ::: "memory");
     } else if constexpr (kStaged) {
@@ -500,24 +509,19 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
     }
     __syncwarp();
     const bool real = first + sub < r.rows;
-    const i64 row = real ? first + sub : r.rows - 1;
-    const int back = static_cast<int>(row - first);  // the row's place in the run
+    const int back = real ? sub : static_cast<int>(r.rows - 1 - first);  // the row's place in the run
+    const i64 row = first + back;
     const int stage = own + at * lay.stage();
     const T *x, *z_row = nullptr;
-    const bool* lm = nullptr;
+    const bool* lm;
     if constexpr (kStaged) {
-      x = reinterpret_cast<const T*>(shared + stage + skip(address(logits, first, r.ld))) +
-          back * static_cast<int>(r.ld);
-      if constexpr (kRef)
-        z_row = reinterpret_cast<const T*>(shared + stage + lay.logits + skip(address(refs, first, r.ldr))) +
-                back * static_cast<int>(r.ldr);
-      lm = reinterpret_cast<const bool*>(shared + stage + lay.logits + lay.ref +
-                                         skip(address(r.legal, first, r.ldm))) +
-           back * static_cast<int>(r.ldm);
+      x = reinterpret_cast<const T*>(shared + stage + skip(x_first)) + back * ld;
+      if constexpr (kRef) z_row = reinterpret_cast<const T*>(shared + stage + lay.logits + skip(z_first)) + back * ldr;
+      lm = reinterpret_cast<const bool*>(shared + stage + lay.logits + lay.ref + skip(m_first)) + back * ldm;
     } else {
-      x = address(logits, row, r.ld);
-      if constexpr (kRef) z_row = address(refs, row, r.ldr);
-      lm = address(r.legal, row, r.ldm);
+      x = x_first + back * r.ld;
+      if constexpr (kRef) z_row = z_first + back * r.ldr;
+      lm = m_first + back * r.ldm;
     }
     bool used = real && in.weight != 0.0f && in.action >= 0 && in.action < vocab;
     const int action = used ? static_cast<int>(in.action) : 0;
@@ -899,10 +903,10 @@ __device__ __noinline__ void add_masked(Running& v, const Part<T>& p, int tid, i
   }
 }
 
-// d_j of a vector's entries; `hot`: the action's place among them, or none of theirs.
+// d_j of a vector's entries, without the action's own term.
 template <bool kRef, int kN>
 __device__ __forceinline__ void gradient(const Coefs& c, float m, float mr, const float (&x)[kN],
-                                         const float (&z)[kN], int hot, float (&g)[kN]) {
+                                         const float (&z)[kN], float (&g)[kN]) {
   const Two unit = two(kLog2e, kLog2e), from = two(-m, -m), from_r = two(-mr, -mr);
   const Two c0 = two(c.c0, c.c0), c1 = two(c.c1, c.c1), c2 = two(c.c2, c.c2);
 #pragma unroll
@@ -917,22 +921,37 @@ __device__ __forceinline__ void gradient(const Coefs& c, float m, float mr, cons
     split(y, y0, y1);
     split(mul(d, two(exp2_fast(y0), exp2_fast(y1))), g[e], g[e + 1]);
   }
-  if (static_cast<unsigned>(hot) < kN)
-#pragma unroll
-    for (int e = 0; e < kN; ++e)
-      if (hot == e) g[e] += c.hot;
+}
+
+// Entry j's, with the action's term where it is the action.
+template <typename T, bool kRef>
+__device__ __forceinline__ float gradient_of(const Part<T>& p, const Coefs& c, float m, float mr, int j, bool hot) {
+  const float y = fmaf(p.one(p.x, j), kLog2e, -m);
+  float g = fmaf(c.c1, y, c.c0);
+  if constexpr (kRef) g = fmaf(c.c2, y - fmaf(p.one(p.z, j), kLog2e, -mr), g);
+  return fmaf(g, exp2_fast(y), hot ? c.hot : 0.0f);
+}
+
+// The action's entry once more, by the thread that wrote its vector: so no entry has to be
+// compared with it.
+template <typename T, bool kRef, int kType>
+__device__ __forceinline__ void write_hot(const Part<T>& p, const Coefs& c, float m, float mr, int action, void* row,
+                                          int tid, int step) {
+  const int v = (action - p.head) / kVec<T>;
+  if (action >= p.head && v >= p.first && v < p.last && (v - p.first) % step == tid)
+    store_one<kType>(row, action, gradient_of<T, kRef>(p, c, m, mr, action, true));
 }
 
 // A part's gradient by `step` threads of which this is number tid, from memory, with masks.
 template <typename T, bool kRef, int kType>
-__device__ __noinline__ void write_masked(const Part<T>& p, const Coefs& c, float m, float mr, int action, void* row,
-                                          bool wide, int tid, int step) {
+__device__ __noinline__ void write_masked(const Part<T>& p, const Coefs& c, float m, float mr, void* row, bool wide,
+                                          int tid, int step) {
   constexpr int kN = kVec<T>;
   for (int i = p.first + tid; i < p.last; i += step) {
     float f[kN], q[kN], g[kN];
     p.masked(i, __ldg(p.vector(i)), f);
     if constexpr (kRef) p.masked(i, p.ref_vector(i), q);
-    gradient<kRef>(c, m, mr, f, q, action - p.head - i * kN, g);
+    gradient<kRef>(c, m, mr, f, q, g);
     store_grad<kType>(row, p.head + i * kN, g, wide);
   }
 }
@@ -943,19 +962,18 @@ __device__ __forceinline__ void write_zeros(const Part<T>& p, void* row, bool wi
   for (int i = p.first + tid; i < p.last; i += step) store_grad<kType>(row, p.head + i * kVec<T>, g, wide);
 }
 
-// The gradient of whole vectors as they are, `apart` entries from one to the next in `row`;
-// `hot`: the action's place in the first.
+// The gradient of whole vectors as they are, `apart` entries from one to the next.
 template <typename T, bool kRef, int kType, int kCount>
-__device__ __forceinline__ void write_vectors(const Coefs& c, float m, float mr, int hot, Stored<kType>* row, int apart,
-                                              bool wide, const uint4 (&x)[kCount], const uint4 (&z)[kCount]) {
+__device__ __forceinline__ void write_vectors(const Coefs& c, float m, float mr, Stored<kType>* to, int apart, bool wide,
+                                              const uint4 (&x)[kCount], const uint4 (&z)[kCount]) {
   constexpr int kN = kVec<T>;
 #pragma unroll
   for (int k = 0; k < kCount; ++k) {
     float f[kN], q[kN], g[kN];
     unpack<T>(x[k], f);
     if constexpr (kRef) unpack<T>(z[k], q);
-    gradient<kRef>(c, m, mr, f, q, hot - k * apart, g);
-    store_grad<kType>(row, k * apart, g, wide);
+    gradient<kRef>(c, m, mr, f, q, g);
+    store_grad<kType>(to, k * apart, g, wide);
   }
 }
 
@@ -1007,7 +1025,6 @@ __global__ void __launch_bounds__(kLongThreads, 2)
   // Whether a row may count (the action's own entry is still to be seen); the same in the
   // whole cluster.
   const auto maybe_used = [&](i64 row) {
-    if (row >= r.rows) return false;
     const i64 action = r.actions[row];
     return action >= 0 && action < r.vocab && !(r.weight && r.weight[row] == 0.0f);
   };
@@ -1036,19 +1053,43 @@ __global__ void __launch_bounds__(kLongThreads, 2)
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
+  // The next row from `row` on that may count; those before it get their zeros here, so
+  // that copies are always under way for the row that comes next.
+  const auto skip = [&](i64 row) {
+    for (; row < r.rows && !maybe_used(row); row += rows_step) {
+      if (tid == 0 && rank == 0) {
+        if constexpr (!kPolicy) store_score(o, row, false, no_sums(), 0.0f);
+        else if (a.logp) a.logp[row] = 0.0f;
+      }
+      if constexpr (kPolicy)
+        if (a.dlogits)
+          with_type(a.dtype, [&](auto type) {
+            constexpr int kType = decltype(type)::value;
+            const Part<T> p(r, row, 0, r.vocab, parts, rank);
+            Stored<kType>* const to = static_cast<Stored<kType>*>(a.dlogits) + row * a.ldd;
+            write_zeros<T, kType>(p, to, grad_wide<T, kType>(to, p.head), tid, step);
+            if (rank == 0) {
+              if (tid < r.vocab - p.vectors * kN) store_one<kType>(to, p.loose(tid), 0.0f);
+              for (int j = r.vocab + tid; j < a.width; j += step) store_one<kType>(to, j, 0.0f);
+            }
+          });
+    }
+    return row;
+  };
+
   int buffer = 0;
-  i64 row = blockIdx.x / parts;
-  bool maybe = maybe_used(row);
+  i64 row = skip(blockIdx.x / parts), next_row;
   const bool write = kPolicy && a.dlogits;  // a second look
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) fetch(maybe, row, c);
-  for (; row < r.rows; row += rows_step) {
-    const bool next = maybe_used(row + rows_step);
+  for (int c = 0; c < kChunks; ++c) fetch(row < r.rows, row, c);
+  for (; row < r.rows; row = next_row) {
+    next_row = skip(row + rows_step);
+    const bool next = next_row < r.rows;
     const i64 action = r.actions[row];
     const Part<T> p(r, row, 0, r.vocab, parts, rank);
     const int i0 = p.first + tid, n_slotted = slotted(p);
     const int n_loose = rank == 0 ? r.vocab - p.vectors * kN : 0;
-    if (maybe && tid == 32) {
+    if (tid == 32) {
       row_in = row_inputs<kPolicy>(r, a, row);
       row_x = p.one(p.x, static_cast<int>(action));
     }
@@ -1061,7 +1102,7 @@ __global__ void __launch_bounds__(kLongThreads, 2)
       if (write && c > 0) wait_copies<0>();
       else wait_copies<kChunks - 1>();
       static_assert(kChunks == 2, "the waits are for two");
-      if (maybe && !careful) {
+      if (!careful) {
         const int end = (c + 1) * chunk < n_slotted ? (c + 1) * chunk : n_slotted;
         const uint4 *at = mine + c * chunk * step, *at_r = mine_r + c * chunk * step;
         int k = c * chunk;
@@ -1083,9 +1124,9 @@ __global__ void __launch_bounds__(kLongThreads, 2)
           add_vectors<T, kRef>(run, x, z);
         }
       }
-      if (!write) fetch(next, row + rows_step, c);
+      if (!write) fetch(next, next_row, c);
     }
-    if (maybe && !careful) {
+    if (!careful) {
 #pragma unroll 1
       for (int i = i0 + slots * step; i < p.last; i += 2 * step) {  // what no slot holds
         uint4 x[2], z[2];
@@ -1104,7 +1145,7 @@ __global__ void __launch_bounds__(kLongThreads, 2)
         }
       }
     }
-    while (maybe) {
+    for (;;) {
       if (careful) {
         run.m = run.mr = kMasked2;
         run.s = run.t = run.sr = run.u = two(0.0f, 0.0f);
@@ -1172,15 +1213,11 @@ __global__ void __launch_bounds__(kLongThreads, 2)
       if (careful || !result.again) break;
       careful = true;
     }
-    if (!maybe && tid == 0 && rank == 0) {
-      if constexpr (!kPolicy) store_score(o, row, false, no_sums(), 0.0f);
-      else if (a.logp) a.logp[row] = 0.0f;
-    }
     if constexpr (kPolicy) {
       if (write) {
         const Coefs c = result.c;  // of a row that counts; not used for another
         const float m = result.m, mr = result.mr;
-        const bool used = maybe && result.used;
+        const bool used = result.used;
         const int hot = static_cast<int>(action);
         with_type(a.dtype, [&](auto type) {
           constexpr int kType = decltype(type)::value;
@@ -1192,7 +1229,7 @@ __global__ void __launch_bounds__(kLongThreads, 2)
           } else if (careful) {
             const Coefs coefs = c;
             const Part<T> part = p;
-            write_masked<T, kRef, kType>(part, coefs, m, mr, hot, to, wide, tid, step);
+            write_masked<T, kRef, kType>(part, coefs, m, mr, to, wide, tid, step);
           }
           const bool plain = used && !careful;
           for (int q = 0; q < kChunks; ++q) {
@@ -1200,7 +1237,7 @@ __global__ void __launch_bounds__(kLongThreads, 2)
               const int end = (q + 1) * chunk < n_slotted ? (q + 1) * chunk : n_slotted;
               const uint4 *at = mine + q * chunk * step, *at_r = mine_r + q * chunk * step;
               int k = q * chunk;
-              int place = p.head + (i0 + k * step) * kN;
+              S* place = to + p.head + (i0 + k * step) * kN;
 #pragma unroll 1
               for (; k + kGroup <= end; k += kGroup, at += kGroup * step, at_r += kGroup * step) {
                 uint4 x[kGroup], z[kGroup];
@@ -1209,7 +1246,7 @@ __global__ void __launch_bounds__(kLongThreads, 2)
                   x[h] = at[h * step];
                   if constexpr (kRef) z[h] = at_r[h * step];
                 }
-                write_vectors<T, kRef, kType>(c, m, mr, hot - place, to + place, step * kN, wide, x, z);
+                write_vectors<T, kRef, kType>(c, m, mr, place, step * kN, wide, x, z);
                 place += kGroup * step * kN;
               }
 #pragma unroll 1
@@ -1217,11 +1254,11 @@ __global__ void __launch_bounds__(kLongThreads, 2)
                 const uint4 x[1] = {*at};
                 uint4 z[1];
                 if constexpr (kRef) z[0] = *at_r;
-                write_vectors<T, kRef, kType>(c, m, mr, hot - place, to + place, 0, wide, x, z);
+                write_vectors<T, kRef, kType>(c, m, mr, place, 0, wide, x, z);
                 place += step * kN;
               }
             }
-            fetch(next, row + rows_step, q);
+            fetch(next, next_row, q);
           }
           if (plain)
 #pragma unroll 1
@@ -1229,27 +1266,18 @@ __global__ void __launch_bounds__(kLongThreads, 2)
               const uint4 x[1] = {__ldcs(p.vector(i))};
               uint4 z[1];
               if constexpr (kRef) z[0] = p.ref_vector(i);
-              const int place = p.head + i * kN;
-              write_vectors<T, kRef, kType>(c, m, mr, hot - place, to + place, 0, wide, x, z);
+              write_vectors<T, kRef, kType>(c, m, mr, to + p.head + i * kN, 0, wide, x, z);
             }
+          if (used) write_hot<T, kRef, kType>(p, c, m, mr, hot, to, tid, step);
           if (tid < n_loose) {
             const int j = p.loose(tid);
-            float g = 0.0f;
-            if (used) {
-              const float y = fmaf(p.one(p.x, j), kLog2e, -m);
-              g = fmaf(c.c1, y, c.c0);
-              if constexpr (kRef) g = fmaf(c.c2, y - fmaf(p.one(p.z, j), kLog2e, -mr), g);
-              g *= exp2_fast(y);
-              if (j == hot) g += c.hot;
-            }
-            store_one<kType>(to, j, g);
+            store_one<kType>(to, j, used ? gradient_of<T, kRef>(p, c, m, mr, j, j == hot) : 0.0f);
           }
           if (rank == 0)
             for (int j = r.vocab + tid; j < a.width; j += step) store_one<kType>(to, j, 0.0f);
         });
       }
     }
-    maybe = next;
   }
   if (parts > 1) cluster.sync();  // no block leaves while another may read its sums
   if constexpr (kPolicy)
@@ -1352,26 +1380,20 @@ __global__ void __launch_bounds__(32 * kBackWarps, 4) logp_backward_kernel(const
 #pragma unroll
         for (int h = 0; h < kGroup; ++h) x[h] = __ldcs(p.vector(i + 32 * h));
         careful = !(extreme<T, false>(x) > kMasked);
-        const int place = p.head + i * kVec<T>;
-        if (!careful) write_vectors<T, false, kType>(k, lse.x, 0.0f, hot - place, to + place, 32 * kVec<T>, wide, x, x);
-        else break;
+        if (careful) break;
+        write_vectors<T, false, kType>(k, lse.x, 0.0f, to + p.head + i * kVec<T>, 32 * kVec<T>, wide, x, x);
       }
       for (; i < p.last; i += 32) {  // what is left of a group, or may be masked
         float f[kVec<T>], g[kVec<T>];
         p.masked(i, __ldcs(p.vector(i)), f);
-        gradient<false>(k, lse.x, 0.0f, f, f, hot - p.head - i * kVec<T>, g);
+        gradient<false>(k, lse.x, 0.0f, f, f, g);
         store_grad<kType>(to, p.head + i * kVec<T>, g, wide);
       }
+      write_hot<T, false, kType>(p, k, lse.x, 0.0f, hot, to, lane, 32);
     }
     for (int i = lane; i < p.vocab - p.vectors * kVec<T>; i += 32) {
       const int c = p.loose(i);
-      float g = 0.0f;
-      if (used) {
-        const float y = fmaf(p.one(p.x, c), kLog2e, -lse.x);
-        g = fmaf(k.c1, y, k.c0) * exp2_fast(y);
-        if (hot == c) g += k.hot;
-      }
-      store_one<kType>(to, c, g);
+      store_one<kType>(to, c, used ? gradient_of<T, false>(p, k, lse.x, 0.0f, c, c == hot) : 0.0f);
     }
   });
 }

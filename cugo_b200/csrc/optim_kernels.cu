@@ -81,6 +81,7 @@ struct Options {
   const float* lr_dev;  // or null
   float b1, c1, b2, c2, eps, max_norm;
   uint32_t seed;
+  uint32_t one, sixteen;  // 1 and 16, not known when compiled: see mad
 };
 
 // A 32-bit mixer: xor-shifts and odd products (constants found by C. Wellons' search for
@@ -90,6 +91,8 @@ __device__ __forceinline__ uint32_t mix_middle(uint32_t x) {  // between its fir
   x ^= x >> 15;
   return x * 0x846ca68bu;
 }
+// A parameter's 16 bits, from the mix before its last shift.
+__device__ __forceinline__ uint32_t random_p(uint32_t x) { return ((x ^ (x >> 16)) * 0x2c1b3c6du) >> 16; }
 __device__ __forceinline__ uint32_t mix(uint32_t x) {
   x = mix_middle(x ^ (x >> 16));
   return x ^ (x >> 16);
@@ -225,14 +228,22 @@ __device__ __forceinline__ int scale_byte(float largest) {
   return e < 27 ? 27 : e > 247 ? 247 : e;
 }
 
+// a b + c on the multipliers: of the 8-bit step's instructions most are logic and shifts,
+// which bound it, so its additions and comparisons go to the pipe that has room.
+__device__ __forceinline__ uint32_t mad(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("mad.lo.u32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
 // The magnitude a (at most 448) rounded to e4m3's grid, up where the random number r says
-// so: 16 bits, as a share of a step, from bit 4 on (what stands below them counts for
-// less than 2^-16 of a step).  Below 2^-6 the steps are 2^-9, which 2^-6 more brings to
-// the same place; above they are 1/8 of the power of two.
-__device__ __forceinline__ float round_e4m3(float a, uint32_t r) {
-  float small;  // 1 below 2^-6, else 0
-  asm("set.lt.f32.f32 %0, %1, %2;" : "=f"(small) : "f"(a), "f"(0.015625f));
-  const uint32_t bits = (__float_as_uint(fmaf(small, 0.015625f, a)) + r) & 0xfff00000u;
+// so: 16 bits, as a share of a step, r times `unit` having them from bit 4 on (what stands
+// below counts for less than 2^-16 of a step).  Below 2^-6 the steps are 2^-9, which 2^-6
+// more brings to the same place; above they are 1/8 of the power of two.
+__device__ __forceinline__ float round_e4m3(float a, uint32_t r, uint32_t unit) {
+  // 1 below 2^-6, else 0: a clamped line that is steeper than any float is near 2^-6.
+  const float small = __saturatef(fmaf(a, -0x1p100f, 0x1p94f));
+  const uint32_t bits = mad(r, unit, __float_as_uint(fmaf(small, 0.015625f, a))) & 0xfff00000u;
   return fmaf(small, -0.015625f, __uint_as_float(bits));
 }
 
@@ -242,11 +253,21 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
   return r;
 }
 
-// A warp's largest magnitude; infinite or NaN where one is.
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// A warp's largest magnitude; infinite or NaN where one is.  kSigned: some may be negative.
+template <bool kSigned>
 __device__ __forceinline__ float warp_largest(const float (&f)[8]) {
   float top = 0.0f, r;
 #pragma unroll
-  for (int e = 0; e < 8; e += 2) top = max_nan(top, fabsf(f[e]), fabsf(f[e + 1]));
+  for (int e = 0; e < 8; e += 2) {
+    if constexpr (kSigned) top = max_nan(top, fabsf(f[e]), fabsf(f[e + 1]));
+    else top = max_nan(top, f[e], f[e + 1]);
+  }
   asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(top));
   return r;
 }
@@ -329,16 +350,18 @@ __device__ __forceinline__ void step8(const Tensor& t, const Options& o, const S
     for (int e = 0; e < 8; ++e) x[e] = mix_middle(n ^ e);
   }
   if constexpr (sizeof(P) == 2) {
-    const bool all = finite == 0.0f;  // infinities and NaN stay what they are
+    if (__any_sync(kFull, !(finite == 0.0f))) {  // infinities and NaN stay what they are
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t r = ((x[e] ^ (x[e] >> 16)) * 0x2c1b3c6du) >> 16;
-      if (all || fabsf(p[e]) < INFINITY) p[e] = __uint_as_float(__float_as_uint(p[e]) + r);
+      for (int e = 0; e < 8; ++e)
+        if (fabsf(p[e]) < INFINITY) p[e] = __uint_as_float(__float_as_uint(p[e]) + random_p(x[e]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = __uint_as_float(mad(random_p(x[e]), o.one, __float_as_uint(p[e])));
     }
   }
   store8<kWide>(static_cast<P*>(t.p), i, t.n, p);
   if constexpr (kEight) {
-    float top_m = warp_largest(m), top_v = warp_largest(v);
+    float top_m = warp_largest<true>(m), top_v = warp_largest<false>(v);
     const bool rare = !(top_m < INFINITY && top_v < INFINITY);
     if (rare) {
       top_m = warp_largest_finite(m);
@@ -352,14 +375,14 @@ __device__ __forceinline__ void step8(const Tensor& t, const Options& o, const S
     for (int e = 0; e < 8; e += 2) {
       split(mul(two(m[e], m[e + 1]), mi2), cm[e], cm[e + 1]);
       split(mul(two(v[e], v[e + 1]), vi2), cv[e], cv[e + 1]);
-      low = fminf(fminf(low, cv[e]), cv[e + 1]);
+      low = min3(low, cv[e], cv[e + 1]);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t high = x[e] >> 16;
-      const float q = round_e4m3(fabsf(cm[e]), ((x[e] ^ high) & 0xffffu) * 16u);
+      const float q = round_e4m3(fabsf(cm[e]), (x[e] ^ high) & 0xffffu, o.sixteen);
       cm[e] = __uint_as_float(__float_as_uint(q) | (__float_as_uint(cm[e]) & 0x80000000u));
-      cv[e] = round_e4m3(cv[e], x[e] >> 12);
+      cv[e] = round_e4m3(cv[e], x[e] >> 12, o.one);
     }
     if (low < 0.001953125f) {  // 2^-9: a second moment above 0 does not become 0
 #pragma unroll
@@ -701,6 +724,8 @@ int cugo_b200_adamw(int64_t count, void* const* params, const void* const* grads
   o.eps = static_cast<float>(eps);
   o.max_norm = static_cast<float>(max_norm);
   o.seed = seed;
+  o.one = 1;
+  o.sixteen = 16;
   const Lists l{params, grads, exp_avgs, exp_avg_sqs, eight ? exp_avg_scales : nullptr,
                 eight ? exp_avg_sq_scales : nullptr, sizes, count};
   Scalars* scalars = static_cast<Scalars*>(scratch);

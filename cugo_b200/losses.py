@@ -27,6 +27,17 @@ from torch.autograd.function import once_differentiable
 
 from .ext import load_extension
 
+_EXT = None
+
+
+def _ext():
+    """The extension, looked up once: these calls are short enough for the look to count."""
+    global _EXT
+    if _EXT is None:
+        _EXT = load_extension()
+    return _EXT
+
+
 STATS = ("loss", "policy", "entropy", "kl", "kl_old", "clip_fraction", "used")
 
 
@@ -53,7 +64,7 @@ class PreferenceLoss(NamedTuple):
 class _ActionLogp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, legal):
-        logp, entropy, lse, _ = load_extension().action_logp(logits, actions, legal, backward=True)
+        logp, entropy, lse, _ = _ext().action_logp(logits, actions, legal, backward=True)
         ctx.save_for_backward(logits, actions, legal, lse, entropy)
         ctx.set_materialize_grads(False)
         return logp, entropy
@@ -66,7 +77,7 @@ class _ActionLogp(torch.autograd.Function):
         logits, actions, legal, lse, entropy = ctx.saved_tensors
         d_logp = d_logp if d_logp is None else d_logp.contiguous()
         d_entropy = d_entropy if d_entropy is None else d_entropy.contiguous()
-        return load_extension().action_logp_backward(logits, actions, legal, lse, entropy, d_logp,
+        return _ext().action_logp_backward(logits, actions, legal, lse, entropy, d_logp,
                                                      d_entropy), None, None
 
 
@@ -76,14 +87,14 @@ def action_logp(logits: torch.Tensor, actions: torch.Tensor,
     differentiable in the logits."""
     if torch.is_grad_enabled() and logits.requires_grad:
         return _ActionLogp.apply(logits, actions, legal)
-    logp, entropy, _, _ = load_extension().action_logp(logits, actions, legal)
+    logp, entropy, _, _ = _ext().action_logp(logits, actions, legal)
     return logp, entropy
 
 
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, logp_old, adv, legal, weight, ref_logits, ref_logp, coefs):
-        loss, stats, logp = load_extension().policy_loss(
+        loss, stats, logp, _ = _ext().policy_loss(
             logits, actions, logp_old, adv, legal, weight, ref_logits, ref_logp, *coefs)
         ctx.save_for_backward(logits, actions, logp_old, adv, legal, weight, ref_logits, ref_logp)
         ctx.coefs, ctx.denominator = coefs, stats[7:]
@@ -98,10 +109,9 @@ class _PolicyLoss(torch.autograd.Function):
         if d_loss is None:
             return (None,) * 9
         logits = ctx.saved_tensors[0]
-        d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        # The denominator that the forward found; the logits are read once more.
-        load_extension().policy_loss(*ctx.saved_tensors, *ctx.coefs[:4], 0.0, ctx.denominator,
-                                     grad_scale_dev=d_loss, dlogits=d, stats=False)
+        # With the denominator that the forward found; the logits are read once more.
+        d = _ext().policy_loss(*ctx.saved_tensors, *ctx.coefs[:4], 0.0, ctx.denominator,
+                               grad_scale_dev=d_loss, grad_dtype=logits.dtype, stats=False)[3]
         return (d,) + (None,) * 8
 
 
@@ -137,12 +147,11 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, logp_old: torch.Ten
     if torch.is_grad_enabled() and logits.requires_grad:
         return PolicyLoss(*_PolicyLoss.apply(logits, actions, logp_old, adv, legal, weight, ref_logits,
                                              ref_logp, coefs))
-    loss, stats, logp = load_extension().policy_loss(logits, actions, logp_old, adv, legal, weight,
-                                                     ref_logits, ref_logp, *coefs)
+    loss, stats, logp, _ = _ext().policy_loss(logits, actions, logp_old, adv, legal, weight, ref_logits,
+                                              ref_logp, *coefs)
     return PolicyLoss(loss, stats[:7], logp)
 
 
-@torch.no_grad()
 def policy_loss_grad(logits: torch.Tensor, actions: torch.Tensor, logp_old: torch.Tensor,
                      adv: torch.Tensor, *, legal: torch.Tensor | None = None,
                      weight: torch.Tensor | None = None, ref_logits: torch.Tensor | None = None,
@@ -158,14 +167,13 @@ def policy_loss_grad(logits: torch.Tensor, actions: torch.Tensor, logp_old: torc
     (the logits' type)."""
     coefs = _coefs(clip_low, clip_high, kl_coef, entropy_coef, denominator)
     if dlogits is None:
-        dlogits = torch.empty(logits.shape, dtype=grad_dtype or logits.dtype, device=logits.device)
+        grad_dtype = grad_dtype or logits.dtype
     elif grad_dtype is not None and grad_dtype != dlogits.dtype:
         raise RuntimeError("policy_loss: dlogits is not of grad_dtype")
-    on_device = torch.is_tensor(grad_scale)
-    loss, stats, logp = load_extension().policy_loss(
-        logits, actions, logp_old, adv, legal, weight, ref_logits, ref_logp, *coefs,
-        grad_scale=1.0 if on_device else float(grad_scale),
-        grad_scale_dev=grad_scale if on_device else None, dlogits=dlogits)
+    scale, scale_dev = (1.0, grad_scale) if torch.is_tensor(grad_scale) else (float(grad_scale), None)
+    loss, stats, logp, dlogits = _ext().policy_loss(
+        logits, actions, logp_old, adv, legal, weight, ref_logits, ref_logp, *coefs, None, scale, scale_dev,
+        dlogits, grad_dtype)
     return PolicyLoss(loss, stats[:7], logp), dlogits
 
 
@@ -184,14 +192,14 @@ class _PreferenceLoss(torch.autograd.Function):
         if d_loss is None:
             return (None,) * 7
         logits, actions, legal, lse, d_logp = ctx.saved_tensors
-        d = load_extension().action_logp_backward(logits, actions, legal, lse, None, d_logp, None,
+        d = _ext().action_logp_backward(logits, actions, legal, lse, None, d_logp, None,
                                                   scale=d_loss)
         return (d,) + (None,) * 6
 
 
 def _preference(logits, actions, offsets, ref_logp, legal, weight, options, grad):
     """((loss, margin, sequences' log p, accuracy), and what the backward needs)."""
-    ext = load_extension()
+    ext = _ext()
     logp, _, lse, d_logp = ext.action_logp(logits, actions, legal, weight, entropy=False,
                                            backward=True, zeros=grad)
     return ext.preference_pairs(logp, ref_logp, weight, lse, offsets, *options,

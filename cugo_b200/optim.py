@@ -23,7 +23,6 @@ from .ext import load_extension
 _STATES = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
 
 
-@torch.no_grad()
 def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor],
                exp_avgs: list[torch.Tensor], exp_avg_sqs: list[torch.Tensor], step: torch.Tensor, *,
                lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
@@ -42,11 +41,10 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor],
     ceil(size / 256) each), e4m3 codes (uint8 or float8_e4m3fn).  States start as zeros.  lr:
     a number, or one fp32 value on the device.  A norm that is infinite or NaN makes the
     step NaN, as clip_grad_norm_ does."""
-    for name, value, ok in (("betas", betas, 0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0),
-                            ("eps", eps, eps >= 0.0), ("weight_decay", weight_decay, weight_decay >= 0.0),
-                            ("lr", lr, torch.is_tensor(lr) or lr >= 0.0),
-                            ("max_grad_norm", max_grad_norm, max_grad_norm is None or max_grad_norm >= 0.0)):
-        if not ok:
+    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+        raise RuntimeError(f"adamw: betas = {betas} is out of range")
+    for name, value in (("lr", lr), ("eps", eps), ("weight_decay", weight_decay), ("max_grad_norm", max_grad_norm)):
+        if value is not None and not torch.is_tensor(value) and not value >= 0.0:
             raise RuntimeError(f"adamw: {name} = {value} is out of range")
     return load_extension().adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas[0], betas[1],
                                   eps, weight_decay, max_grad_norm, seed, exp_avg_scales,

@@ -83,8 +83,9 @@ def p_tolerance(old, new, h):
 def test_32_bit_states(sizes, g_type, clip, offset):
     t = tensors(sizes, torch.float32, g_type, 32, 1, offset)
     old, new, norm, c = expected(t, clip)
+    version = t["p"][0]._version
     got = step(t, clip)
-    assert int(t["step"]) == 5
+    assert int(t["step"]) == 5 and t["p"][0]._version > version
     assert (got is None) == (clip is None)
     if clip is not None:
         assert abs(float(got) - norm) <= 4 * U * norm

@@ -81,7 +81,6 @@ struct Options {
   const float* lr_dev;  // or null
   float b1, c1, b2, c2, eps, max_norm;
   uint32_t seed;
-  uint32_t one, sixteen;  // 1 and 16, not known when compiled: see mad
 };
 
 // A 32-bit mixer: xor-shifts and odd products (constants found by C. Wellons' search for
@@ -116,23 +115,23 @@ __device__ __forceinline__ int find(const Tensors<kMost>& a, int tile) {
   return low;
 }
 
-// 8 consecutive values from element i, whole and aligned where kWide is set, else those
-// before element n, and zeros.
+// A thread's 8 consecutive values, aligned and all there where kWide is set, else the first
+// n of them, and zeros.
 template <bool kWide>
-__device__ __forceinline__ void load8(const float* p, i64 i, i64 n, float (&f)[8]) {
+__device__ __forceinline__ void load8(const float* p, int n, float (&f)[8]) {
   if constexpr (kWide) {
-    const float4 a = *reinterpret_cast<const float4*>(p + i), b = *reinterpret_cast<const float4*>(p + i + 4);
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
     f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = i + e < n ? p[i + e] : 0.0f;
+    for (int e = 0; e < 8; ++e) f[e] = e < n ? p[e] : 0.0f;
   }
 }
 
 template <bool kWide>
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, i64 i, i64 n, float (&f)[8]) {
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, int n, float (&f)[8]) {
   if constexpr (kWide) {
-    const uint4 q = *reinterpret_cast<const uint4*>(p + i);
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -141,34 +140,34 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, i64 i, i64 n, floa
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = i + e < n ? __bfloat162float(p[i + e]) : 0.0f;
+    for (int e = 0; e < 8; ++e) f[e] = e < n ? __bfloat162float(p[e]) : 0.0f;
   }
 }
 
 template <bool kWide>
-__device__ __forceinline__ void store8(float* p, i64 i, i64 n, const float (&f)[8]) {
+__device__ __forceinline__ void store8(float* p, int n, const float (&f)[8]) {
   if constexpr (kWide) {
-    *reinterpret_cast<float4*>(p + i) = make_float4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<float4*>(p + i + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (i + e < n) p[i + e] = f[e];
+      if (e < n) p[e] = f[e];
   }
 }
 
 // The upper halves of f (rounded there already) as bf16.
 template <bool kWide>
-__device__ __forceinline__ void store8(__nv_bfloat16* p, i64 i, i64 n, const float (&f)[8]) {
+__device__ __forceinline__ void store8(__nv_bfloat16* p, int n, const float (&f)[8]) {
   if constexpr (kWide) {
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = __byte_perm(__float_as_uint(f[2 * e]), __float_as_uint(f[2 * e + 1]), 0x7632);
-    *reinterpret_cast<uint4*>(p + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (i + e < n) reinterpret_cast<uint16_t*>(p)[i + e] = static_cast<uint16_t>(__float_as_uint(f[e]) >> 16);
+      if (e < n) reinterpret_cast<uint16_t*>(p)[e] = static_cast<uint16_t>(__float_as_uint(f[e]) >> 16);
   }
 }
 
@@ -185,21 +184,21 @@ __device__ __forceinline__ void decode(uint32_t a, uint32_t b, float (&f)[8]) {
 }
 
 template <bool kWide>
-__device__ __forceinline__ void load_codes(const uint8_t* p, i64 i, i64 n, float (&f)[8]) {
+__device__ __forceinline__ void load_codes(const uint8_t* p, int n, float (&f)[8]) {
   uint32_t w[2] = {0, 0};
   if constexpr (kWide) {
-    const uint2 q = *reinterpret_cast<const uint2*>(p + i);
+    const uint2 q = *reinterpret_cast<const uint2*>(p);
     w[0] = q.x, w[1] = q.y;
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (i + e < n) w[e / 4] |= static_cast<uint32_t>(p[i + e]) << (8 * (e % 4));
+      if (e < n) w[e / 4] |= static_cast<uint32_t>(p[e]) << (8 * (e % 4));
   }
   decode(w[0], w[1], f);
 }
 
 template <bool kWide>
-__device__ __forceinline__ void store_codes(uint8_t* p, i64 i, i64 n, const float (&f)[8]) {
+__device__ __forceinline__ void store_codes(uint8_t* p, int n, const float (&f)[8]) {
   uint32_t w[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -208,11 +207,11 @@ __device__ __forceinline__ void store_codes(uint8_t* p, i64 i, i64 n, const floa
     w[e] = __byte_perm(a, b, 0x5410);
   }
   if constexpr (kWide) {
-    *reinterpret_cast<uint2*>(p + i) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (i + e < n) p[i + e] = static_cast<uint8_t>(w[e / 4] >> (8 * (e % 4)));
+      if (e < n) p[e] = static_cast<uint8_t>(w[e / 4] >> (8 * (e % 4)));
   }
 }
 
@@ -228,22 +227,14 @@ __device__ __forceinline__ int scale_byte(float largest) {
   return e < 27 ? 27 : e > 247 ? 247 : e;
 }
 
-// a b + c on the multipliers: of the 8-bit step's instructions most are logic and shifts,
-// which bound it, so its additions and comparisons go to the pipe that has room.
-__device__ __forceinline__ uint32_t mad(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("mad.lo.u32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
-
 // The magnitude a (at most 448) rounded to e4m3's grid, up where the random number r says
-// so: 16 bits, as a share of a step, r times `unit` having them from bit 4 on (what stands
-// below counts for less than 2^-16 of a step).  Below 2^-6 the steps are 2^-9, which 2^-6
-// more brings to the same place; above they are 1/8 of the power of two.
-__device__ __forceinline__ float round_e4m3(float a, uint32_t r, uint32_t unit) {
-  // 1 below 2^-6, else 0: a clamped line that is steeper than any float is near 2^-6.
-  const float small = __saturatef(fmaf(a, -0x1p100f, 0x1p94f));
-  const uint32_t bits = mad(r, unit, __float_as_uint(fmaf(small, 0.015625f, a))) & 0xfff00000u;
+// so: 16 bits, as a share of a step, from bit 4 on (what stands below counts for less than
+// 2^-16 of a step).  Below 2^-6 the steps are 2^-9, which 2^-6 more brings to the same
+// place; above they are 1/8 of the power of two.
+__device__ __forceinline__ float round_e4m3(float a, uint32_t r) {
+  float small;  // 1 below 2^-6, else 0
+  asm("set.lt.f32.f32 %0, %1, %2;" : "=f"(small) : "f"(a), "f"(0.015625f));
+  const uint32_t bits = (__float_as_uint(fmaf(small, 0.015625f, a)) + r) & 0xfff00000u;
   return fmaf(small, -0.015625f, __uint_as_float(bits));
 }
 
@@ -312,11 +303,29 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
   return r;
 }
 
-// The step of a warp's block `in` of tensor t, this thread's 8 elements from i on: their
-// values, with the states' codes not scaled yet (scales ms, vs).
+// Where a thread's 8 elements and its warp's scales are, and the first element's number.
+template <typename P>
+struct Place {
+  P* p;
+  void *m, *v;
+  uint8_t *ms, *vs;
+  i64 number;
+  int n;  // of the 8, how many are the tensor's
+};
+
+template <typename P, bool kEight>
+__device__ __forceinline__ Place<P> place_of(const Tensor& t, i64 block, int lane) {
+  const i64 i = block * kBlock + lane * kPer, left = t.n - i;
+  constexpr int kSize = kEight ? 1 : 4;
+  return {static_cast<P*>(t.p) + i, static_cast<char*>(t.m) + i * kSize, static_cast<char*>(t.v) + i * kSize,
+          t.ms + block, t.vs + block, t.first_block * kBlock + i, left < 0 ? 0 : left < 8 ? static_cast<int>(left) : 8};
+}
+
+// The step of a thread's 8 elements: their values, with the states' codes not scaled yet
+// (scales ms, vs).
 template <typename P, bool kEight, bool kWide>
-__device__ __forceinline__ void step8(const Tensor& t, const Options& o, const Scalars& s, i64 in, i64 i, int ms,
-                                      int vs, float (&p)[8], const float (&g)[8], float (&m)[8], float (&v)[8]) {
+__device__ __forceinline__ void step8(const Place<P>& at, const Options& o, const Scalars& s, int ms, int vs,
+                                      float (&p)[8], const float (&g)[8], float (&m)[8], float (&v)[8]) {
   constexpr bool kRandom = kEight || sizeof(P) == 2;
   float b1 = o.b1, b2 = o.b2;
   if constexpr (kEight) {  // the scale is a power of two: exact in the factor
@@ -325,7 +334,7 @@ __device__ __forceinline__ void step8(const Tensor& t, const Options& o, const S
   }
   const Two c1 = two(s.c1, s.c1), clip = two(s.clip, s.clip), c2 = two(o.c2, o.c2), d1 = two(b1, b1), d2 = two(b2, b2),
             keep = two(s.keep, s.keep);
-  float finite = 0.0f;  // NaN where a parameter is not finite after the step
+  float nan = 0.0f;  // NaN where a parameter is after the step
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
     const Two gg = two(g[e], g[e + 1]), q = mul(gg, clip);
@@ -336,30 +345,29 @@ __device__ __forceinline__ void step8(const Tensor& t, const Options& o, const S
     for (int h = 0; h < 2; ++h) {
       const float u = __fdividef(m[e + h], fmaf(sqrt_fast(v[e + h]), s.root, o.eps));
       p[e + h] = fmaf(-s.step_size, u, p[e + h]);
-      if constexpr (sizeof(P) == 2) finite = fmaf(p[e + h], 0.0f, finite);
     }
+    if constexpr (sizeof(P) == 2) nan = max_nan(nan, p[e], p[e + 1]);
   }
   uint32_t x[8];  // the mix before its last shift, x ^= x >> 16
   if constexpr (kRandom) {
-    // i is a multiple of 8, so element e's number differs in the last three bits only: the
+    // The number is a multiple of 8, so element e's differs in the last three bits only: the
     // mix's first shift is the same for all eight.
-    const i64 number = t.first_block * kBlock + i;
-    uint32_t n = static_cast<uint32_t>(number) ^ (s.key + static_cast<uint32_t>(number >> 32) * 0x9e3779b9u);
+    uint32_t n = static_cast<uint32_t>(at.number) ^ (s.key + static_cast<uint32_t>(at.number >> 32) * 0x9e3779b9u);
     n ^= n >> 16;
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = mix_middle(n ^ e);
   }
   if constexpr (sizeof(P) == 2) {
-    if (__any_sync(kFull, !(finite == 0.0f))) {  // infinities and NaN stay what they are
+    if (__any_sync(kFull, isnan(nan))) {  // NaN stays what it is, as infinities do below
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (fabsf(p[e]) < INFINITY) p[e] = __uint_as_float(__float_as_uint(p[e]) + random_p(x[e]));
+        if (!isnan(p[e])) p[e] = __uint_as_float(__float_as_uint(p[e]) + random_p(x[e]));
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] = __uint_as_float(mad(random_p(x[e]), o.one, __float_as_uint(p[e])));
+      for (int e = 0; e < 8; ++e) p[e] = __uint_as_float(__float_as_uint(p[e]) + random_p(x[e]));
     }
   }
-  store8<kWide>(static_cast<P*>(t.p), i, t.n, p);
+  store8<kWide>(at.p, at.n, p);
   if constexpr (kEight) {
     float top_m = warp_largest<true>(m), top_v = warp_largest<false>(v);
     const bool rare = !(top_m < INFINITY && top_v < INFINITY);
@@ -380,9 +388,9 @@ __device__ __forceinline__ void step8(const Tensor& t, const Options& o, const S
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t high = x[e] >> 16;
-      const float q = round_e4m3(fabsf(cm[e]), (x[e] ^ high) & 0xffffu, o.sixteen);
+      const float q = round_e4m3(fabsf(cm[e]), ((x[e] ^ high) & 0xffffu) * 16u);
       cm[e] = __uint_as_float(__float_as_uint(q) | (__float_as_uint(cm[e]) & 0x80000000u));
-      cv[e] = round_e4m3(cv[e], x[e] >> 12, o.one);
+      cv[e] = round_e4m3(cv[e], x[e] >> 12);
     }
     if (low < 0.001953125f) {  // 2^-9: a second moment above 0 does not become 0
 #pragma unroll
@@ -395,15 +403,15 @@ __device__ __forceinline__ void step8(const Tensor& t, const Options& o, const S
         if (!(v[e] < INFINITY)) cv[e] = __uint_as_float(0x7fc00000u);
       }
     }
-    store_codes<kWide>(static_cast<uint8_t*>(t.m), i, t.n, cm);
-    store_codes<kWide>(static_cast<uint8_t*>(t.v), i, t.n, cv);
+    store_codes<kWide>(static_cast<uint8_t*>(at.m), at.n, cm);
+    store_codes<kWide>(static_cast<uint8_t*>(at.v), at.n, cv);
     if ((threadIdx.x & 31) == 0) {
-      t.ms[in] = static_cast<uint8_t>(mb);
-      t.vs[in] = static_cast<uint8_t>(vb);
+      *at.ms = static_cast<uint8_t>(mb);
+      *at.vs = static_cast<uint8_t>(vb);
     }
   } else {
-    store8<kWide>(static_cast<float*>(t.m), i, t.n, m);
-    store8<kWide>(static_cast<float*>(t.v), i, t.n, v);
+    store8<kWide>(static_cast<float*>(at.m), at.n, m);
+    store8<kWide>(static_cast<float*>(at.v), at.n, v);
   }
 }
 
@@ -416,21 +424,23 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     const Tensor& t = a.t[find(a, tile)];
     const i64 first = (static_cast<i64>(tile - t.first_tile) * kWarps + (threadIdx.x >> 5)) * a.per_warp;
     for (int u = 0; u < a.per_warp; ++u) {
-      const i64 in = first + u, i = in * kBlock + (threadIdx.x & 31) * kPer;
-      if (in * kBlock >= t.n) break;  // the whole warp
+      const i64 block = first + u;
+      if (block * kBlock >= t.n) break;  // the whole warp
+      const Place<P> at = place_of<P, false>(t, block, threadIdx.x & 31);
+      const G* const grad = static_cast<const G*>(t.g) + (at.p - static_cast<const P*>(t.p));
       float p[8], g[8], m[8], v[8];
-      if (t.wide && (in + 1) * kBlock <= t.n) {
-        load8<true>(static_cast<const P*>(t.p), i, t.n, p);
-        load8<true>(static_cast<const G*>(t.g), i, t.n, g);
-        load8<true>(static_cast<const float*>(t.m), i, t.n, m);
-        load8<true>(static_cast<const float*>(t.v), i, t.n, v);
-        step8<P, false, true>(t, o, s, in, i, 0, 0, p, g, m, v);
+      if (t.wide && (block + 1) * kBlock <= t.n) {
+        load8<true>(at.p, 8, p);
+        load8<true>(grad, 8, g);
+        load8<true>(static_cast<const float*>(at.m), 8, m);
+        load8<true>(static_cast<const float*>(at.v), 8, v);
+        step8<P, false, true>(at, o, s, 0, 0, p, g, m, v);
       } else {
-        load8<false>(static_cast<const P*>(t.p), i, t.n, p);
-        load8<false>(static_cast<const G*>(t.g), i, t.n, g);
-        load8<false>(static_cast<const float*>(t.m), i, t.n, m);
-        load8<false>(static_cast<const float*>(t.v), i, t.n, v);
-        step8<P, false, false>(t, o, s, in, i, 0, 0, p, g, m, v);
+        load8<false>(at.p, at.n, p);
+        load8<false>(grad, at.n, g);
+        load8<false>(static_cast<const float*>(at.m), at.n, m);
+        load8<false>(static_cast<const float*>(at.v), at.n, v);
+        step8<P, false, false>(at, o, s, 0, 0, p, g, m, v);
       }
     }
   }
@@ -439,15 +449,16 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
 // A block that is not whole, or of a tensor that is not aligned; a call of its own, so that
 // its registers are no one else's.
 template <typename P, typename G>
-__device__ __noinline__ void step8_direct(const Tensor& t, const Options& o, const Scalars* scalars, i64 in, i64 i,
-                                          int ms, int vs) {
+__device__ __noinline__ void step8_direct(const Tensor& t, const Options& o, const Scalars* scalars, i64 block, int ms,
+                                          int vs) {
   const Scalars s = *scalars;
+  const Place<P> at = place_of<P, true>(t, block, threadIdx.x & 31);
   float p[8], g[8], m[8], v[8];
-  load8<false>(static_cast<const P*>(t.p), i, t.n, p);
-  load8<false>(static_cast<const G*>(t.g), i, t.n, g);
-  load_codes<false>(static_cast<const uint8_t*>(t.m), i, t.n, m);
-  load_codes<false>(static_cast<const uint8_t*>(t.v), i, t.n, v);
-  step8<P, true, false>(t, o, s, in, i, ms, vs, p, g, m, v);
+  load8<false>(at.p, at.n, p);
+  load8<false>(static_cast<const G*>(t.g) + (at.p - static_cast<const P*>(t.p)), at.n, g);
+  load_codes<false>(static_cast<const uint8_t*>(at.m), at.n, m);
+  load_codes<false>(static_cast<const uint8_t*>(at.v), at.n, v);
+  step8<P, true, false>(at, o, s, ms, vs, p, g, m, v);
 }
 
 // States in 8 bits: 60 instructions an element leave few registers for loads in flight, so
@@ -500,28 +511,34 @@ __global__ void __launch_bounds__(kThreads, 3) adamw8_kernel(const __grid_consta
     };
 #pragma unroll
     for (int u = 0; u < S::kDepth; ++u) fetch(u, own[u]);
+    Place<P> at = place_of<P, true>(t, first, lane);
     int slot = 0;
     for (int u = 0; u < count; ++u) {
-      const i64 in = first + u, i = in * kBlock + lane * kPer;
       const int bm = __shfl_sync(kFull, ms, u), bv = __shfl_sync(kFull, vs, u);
       asm volatile("cp.async.wait_group %0;" ::"n"(S::kDepth - 1) : "memory");
       __syncwarp();
       if (u < staged) {
         float p[8], g[8], m[8], v[8];
-        const char* const at = own[slot];
-        load8<true>(reinterpret_cast<const P*>(at), lane * kPer, kBlock, p);
-        load8<true>(reinterpret_cast<const G*>(at + S::kP), lane * kPer, kBlock, g);
-        const uint2 cm = *reinterpret_cast<const uint2*>(at + S::kP + S::kG + 8 * lane);
-        const uint2 cv = *reinterpret_cast<const uint2*>(at + S::kP + S::kG + kBlock + 8 * lane);
+        const char* const from = own[slot];
+        load8<true>(reinterpret_cast<const P*>(from) + lane * kPer, 8, p);
+        load8<true>(reinterpret_cast<const G*>(from + S::kP) + lane * kPer, 8, g);
+        const uint2 cm = *reinterpret_cast<const uint2*>(from + S::kP + S::kG + 8 * lane);
+        const uint2 cv = *reinterpret_cast<const uint2*>(from + S::kP + S::kG + kBlock + 8 * lane);
         decode(cm.x, cm.y, m);
         decode(cv.x, cv.y, v);
         __syncwarp();  // the slot is read
         fetch(u + S::kDepth, own[slot]);
-        step8<P, true, true>(t, o, s, in, i, bm, bv, p, g, m, v);
+        step8<P, true, true>(at, o, s, bm, bv, p, g, m, v);
       } else {
         fetch(u + S::kDepth, own[slot]);
-        step8_direct<P, G>(t, o, scalars, in, i, bm, bv);
+        step8_direct<P, G>(t, o, scalars, first + u, bm, bv);
       }
+      at.p += kBlock;
+      at.m = static_cast<char*>(at.m) + kBlock;
+      at.v = static_cast<char*>(at.v) + kBlock;
+      ++at.ms;
+      ++at.vs;
+      at.number += kBlock;
       slot = slot + 1 == S::kDepth ? 0 : slot + 1;
     }
   }
@@ -540,8 +557,8 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ 
     for (int u = 0; u < a.per_warp; ++u) {
       const i64 i = (first + u) * kBlock + (threadIdx.x & 31) * kPer;
       float g[8], q = 0.0f;
-      if (t.wide && i + kPer <= t.n) load8<true>(at, i, t.n, g);
-      else load8<false>(at, i, t.n, g);
+      if (t.wide && i + kPer <= t.n) load8<true>(at + i, 8, g);
+      else load8<false>(at + i, t.n - i < 8 ? static_cast<int>(t.n - i) : 8, g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) q = fmaf(g[e], g[e], q);
       sum += q;
@@ -724,8 +741,6 @@ int cugo_b200_adamw(int64_t count, void* const* params, const void* const* grads
   o.eps = static_cast<float>(eps);
   o.max_norm = static_cast<float>(max_norm);
   o.seed = seed;
-  o.one = 1;
-  o.sixteen = 16;
   const Lists l{params, grads, exp_avgs, exp_avg_sqs, eight ? exp_avg_scales : nullptr,
                 eight ? exp_avg_sq_scales : nullptr, sizes, count};
   Scalars* scalars = static_cast<Scalars*>(scratch);

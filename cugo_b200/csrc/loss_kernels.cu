@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
 // in four chunks of the slots.  Vectors that no slot holds (rows longer than eight blocks'
 // slots) are read from memory both times.
 
-constexpr int kLongThreads = 512;
+constexpr int kLongThreads = 256;
 constexpr int kGroup = 4;   // vectors of a thread looked at together
 constexpr int kChunks = 2;  // of a row's slots, waited for one after another
 
@@ -766,6 +766,8 @@ struct Part {
 
   // `entries` entries of a row from entry c0 on; of their vectors, the share of block
   // `rank` of `parts`.
+  __device__ __forceinline__ Part() : x(nullptr), z(nullptr), lm(nullptr), head(0), vectors(0), first(0), last(0),
+                                      vocab(0), z_wide(false) {}
   __device__ __forceinline__ Part(const Rows& r, i64 row, int c0, int entries, int parts, int rank) {
     x = static_cast<const T*>(r.logits) + row * r.ld + c0;
     z = r.ref ? static_cast<const T*>(r.ref) + row * r.ldr + c0 : nullptr;
@@ -999,7 +1001,7 @@ __device__ __forceinline__ void wait_copies() {
 
 // slots: vectors of a thread that shared memory holds.
 template <typename T, bool kRef, bool kPolicy>
-__global__ void __launch_bounds__(kLongThreads, 2)
+__global__ void __launch_bounds__(kLongThreads, 3)
     long_rows_kernel(const Rows r, const Score o, const Policy a, const int slots) {
   constexpr int kN = kVec<T>;
   extern __shared__ __align__(16) uint4 slot[];  // [slots][threads], then the reference's
@@ -1033,24 +1035,21 @@ __global__ void __launch_bounds__(kLongThreads, 2)
     const int n = (p.last - p.first - tid + step - 1) / step;
     return p.last - p.first <= tid ? 0 : n < slots ? n : slots;
   };
-  // Starts the copies of a chunk of a row's slots; always a group of its own.
-  const auto fetch = [&](bool wanted, i64 row, int c) {
-    if (wanted) {
-      const Part<T> p(r, row, 0, r.vocab, parts, rank);
-      const int n = slotted(p), end = (c + 1) * chunk < n ? (c + 1) * chunk : n;
-      const uint4* from = p.vector(p.first + tid + c * chunk * step);
-      const uint4* from_r = kRef ? reinterpret_cast<const uint4*>(p.z + p.head) + p.first + tid + c * chunk * step : nullptr;
-      uint4 *to = mine + c * chunk * step, *to_r = mine_r + c * chunk * step;
-      for (int k = c * chunk; k < end; ++k, from += step, to += step) {
-        copy16(to, from);
-        if constexpr (kRef) {
-          copy16(to_r, from_r);
-          from_r += step;
-          to_r += step;
-        }
-      }
+  // Starts the copies of a chunk of a part's slots, n of which are this thread's; always a
+  // group of its own.
+  const auto fetch = [&](const uint4* x, const uint4* z, int n, int c) {
+    const int end = (c + 1) * chunk < n ? (c + 1) * chunk : n;
+    int at = c * chunk * step;
+    for (int k = c * chunk; k < end; ++k, at += step) {
+      copy16(mine + at, x + at);
+      if constexpr (kRef) copy16(mine_r + at, z + at);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // This thread's first vector of a part in memory, and the reference's.
+  const auto first_x = [&](const Part<T>& p) { return p.vector(p.first + tid); };
+  const auto first_z = [&](const Part<T>& p) {
+    return kRef ? reinterpret_cast<const uint4*>(p.z + p.head) + p.first + tid : nullptr;
   };
 
   // The next row from `row` on that may count; those before it get their zeros here, so
@@ -1080,18 +1079,28 @@ __global__ void __launch_bounds__(kLongThreads, 2)
   int buffer = 0;
   i64 row = skip(blockIdx.x / parts), next_row;
   const bool write = kPolicy && a.dlogits;  // a second look
+  Part<T> p;
+  int n_slotted = 0;
+  if (row < r.rows) {
+    p = Part<T>(r, row, 0, r.vocab, parts, rank);
+    n_slotted = slotted(p);
+  }
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) fetch(row < r.rows, row, c);
+  for (int c = 0; c < kChunks; ++c) fetch(first_x(p), first_z(p), n_slotted, c);
   for (; row < r.rows; row = next_row) {
     next_row = skip(row + rows_step);
-    const bool next = next_row < r.rows;
-    const i64 action = r.actions[row];
-    const Part<T> p(r, row, 0, r.vocab, parts, rank);
-    const int i0 = p.first + tid, n_slotted = slotted(p);
+    Part<T> p_next = p;
+    int n_next = 0;
+    if (next_row < r.rows) {
+      p_next = Part<T>(r, next_row, 0, r.vocab, parts, rank);
+      n_next = slotted(p_next);
+    }
+    const uint4 *const x_next = first_x(p_next), *const z_next = first_z(p_next);
+    const int action = static_cast<int>(r.actions[row]), i0 = p.first + tid;
     const int n_loose = rank == 0 ? r.vocab - p.vectors * kN : 0;
     if (tid == 32) {
       row_in = row_inputs<kPolicy>(r, a, row);
-      row_x = p.one(p.x, static_cast<int>(action));
+      row_x = p.one(p.x, action);
     }
     bool careful = p.lm != nullptr;
     Running run;
@@ -1124,7 +1133,7 @@ __global__ void __launch_bounds__(kLongThreads, 2)
           add_vectors<T, kRef>(run, x, z);
         }
       }
-      if (!write) fetch(next, next_row, c);
+      if (!write) fetch(x_next, z_next, n_next, c);
     }
     if (!careful) {
 #pragma unroll 1
@@ -1218,7 +1227,6 @@ __global__ void __launch_bounds__(kLongThreads, 2)
         const Coefs c = result.c;  // of a row that counts; not used for another
         const float m = result.m, mr = result.mr;
         const bool used = result.used;
-        const int hot = static_cast<int>(action);
         with_type(a.dtype, [&](auto type) {
           constexpr int kType = decltype(type)::value;
           using S = Stored<kType>;
@@ -1258,7 +1266,7 @@ __global__ void __launch_bounds__(kLongThreads, 2)
                 place += step * kN;
               }
             }
-            fetch(next, next_row, q);
+            fetch(x_next, z_next, n_next, q);
           }
           if (plain)
 #pragma unroll 1
@@ -1268,16 +1276,18 @@ __global__ void __launch_bounds__(kLongThreads, 2)
               if constexpr (kRef) z[0] = p.ref_vector(i);
               write_vectors<T, kRef, kType>(c, m, mr, to + p.head + i * kN, 0, wide, x, z);
             }
-          if (used) write_hot<T, kRef, kType>(p, c, m, mr, hot, to, tid, step);
+          if (used) write_hot<T, kRef, kType>(p, c, m, mr, action, to, tid, step);
           if (tid < n_loose) {
             const int j = p.loose(tid);
-            store_one<kType>(to, j, used ? gradient_of<T, kRef>(p, c, m, mr, j, j == hot) : 0.0f);
+            store_one<kType>(to, j, used ? gradient_of<T, kRef>(p, c, m, mr, j, j == action) : 0.0f);
           }
           if (rank == 0)
             for (int j = r.vocab + tid; j < a.width; j += step) store_one<kType>(to, j, 0.0f);
         });
       }
     }
+    p = p_next;
+    n_slotted = n_next;
   }
   if (parts > 1) cluster.sync();  // no block leaves while another may read its sums
   if constexpr (kPolicy)
@@ -1549,29 +1559,28 @@ struct Plan {
   int threads, blocks, parts, slots, shared;
 };
 
-// A block per row, of as many threads as leave each about ten vectors; a cluster of blocks
-// where the row is longer than the slots of one (two blocks of 512 threads share an SM),
-// and where rows are few: up to 8, each with at least 4,096 entries.
+// A block per row, of as few threads as leave each about 16 vectors (a row costs a thread
+// some 300 instructions beside its vectors); a cluster of blocks where the row is longer
+// than the slots of one (three blocks share an SM, or as many as the slots allow), and
+// where rows are few: up to 8, each with at least 4,096 entries.
 Plan long_plan(i64 rows, int vocab, int size, bool ref, bool stage) {
   constexpr int kBudget = 224 << 10, kStatic = 3 << 10;  // an SM's shared memory, a block's other part
   Plan p{};
   const int copies = ref ? 2 : 1;
-  const i64 vectors = static_cast<i64>(vocab) * size / 16;
-  const auto most_slots = [&](int threads) { return (kBudget * threads / 1024 - kStatic) / (threads * 16 * copies); };
+  const i64 bytes = static_cast<i64>(vocab) * size * copies;
   p.parts = 1;
-  while (p.parts < 8 && vectors > static_cast<i64>(p.parts) * kLongThreads * most_slots(kLongThreads)) p.parts *= 2;
+  while (p.parts < 8 && bytes > static_cast<i64>(p.parts) * (kBudget / 3 - kStatic)) p.parts *= 2;
   while (p.parts < 8 && rows * p.parts < kSms && vocab / (2 * p.parts) >= 4096) p.parts *= 2;
-  const i64 each = (vectors + p.parts - 1) / p.parts;
-  p.threads = 128;
-  while (p.threads < kLongThreads && each > static_cast<i64>(p.threads) * most_slots(p.threads)) p.threads *= 2;
+  const i64 each = (static_cast<i64>(vocab) * size / 16 + p.parts - 1) / p.parts;  // vectors
+  p.threads = each <= 16 * 128 ? 128 : kLongThreads;
   if (stage) {
-    const i64 want = (each + p.threads - 1) / p.threads;
-    const i64 room = most_slots(p.threads);
+    const i64 want = (each + p.threads - 1) / p.threads, room = (kBudget - kStatic) / (p.threads * 16 * copies);
     p.slots = static_cast<int>(((want < room ? want : room) + kGroup - 1) / kGroup * kGroup);
     if (p.slots > room) p.slots -= kGroup;
   }
   p.shared = p.slots * p.threads * 16 * copies;
-  const int per_sm = 1024 / p.threads;
+  int per_sm = kBudget / (p.shared + kStatic);
+  if (per_sm > 768 / p.threads) per_sm = 768 / p.threads;  // by registers
   const i64 most = static_cast<i64>(kSms) * per_sm / p.parts;
   p.blocks = static_cast<int>(rows < most ? rows : most) * p.parts;
   return p;

@@ -765,10 +765,10 @@ struct Part {
   bool z_wide;        // the reference's vectors are aligned as the row's are
 
   // `entries` entries of a row from entry c0 on; of their vectors, the share of block
-  // `rank` of `parts`.
+  // `rank` of 2^log_parts.
   __device__ __forceinline__ Part() : x(nullptr), z(nullptr), lm(nullptr), head(0), vectors(0), first(0), last(0),
                                       vocab(0), z_wide(false) {}
-  __device__ __forceinline__ Part(const Rows& r, i64 row, int c0, int entries, int parts, int rank) {
+  __device__ __forceinline__ Part(const Rows& r, i64 row, int c0, int entries, int log_parts, int rank) {
     x = static_cast<const T*>(r.logits) + row * r.ld + c0;
     z = r.ref ? static_cast<const T*>(r.ref) + row * r.ldr + c0 : nullptr;
     lm = r.legal ? r.legal + row * r.ldm + c0 : nullptr;
@@ -777,7 +777,7 @@ struct Part {
     if (head > entries) head = entries;
     vectors = (entries - head) / kVec<T>;
     z_wide = (reinterpret_cast<uintptr_t>(z + head) & 15) == 0;
-    const int each = (vectors + parts - 1) / parts;
+    const int each = (vectors + (1 << log_parts) - 1) >> log_parts;
     first = each * rank < vectors ? each * rank : vectors;
     last = first + each < vectors ? first + each : vectors;
   }
@@ -938,9 +938,9 @@ __device__ __forceinline__ float gradient_of(const Part<T>& p, const Coefs& c, f
 // compared with it.
 template <typename T, bool kRef, int kType>
 __device__ __forceinline__ void write_hot(const Part<T>& p, const Coefs& c, float m, float mr, int action, void* row,
-                                          int tid, int step) {
+                                          int tid, int step) {  // step: a power of two
   const int v = (action - p.head) / kVec<T>;
-  if (action >= p.head && v >= p.first && v < p.last && (v - p.first) % step == tid)
+  if (action >= p.head && v >= p.first && v < p.last && ((v - p.first) & (step - 1)) == tid)
     store_one<kType>(row, action, gradient_of<T, kRef>(p, c, m, mr, action, true));
 }
 
@@ -1014,6 +1014,7 @@ __global__ void __launch_bounds__(kLongThreads, 3)
   const cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), rank = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x / 32, step = blockDim.x;
+  const int log_parts = __ffs(parts) - 1, log_step = __ffs(step) - 1;  // both are powers of two
   const int chunk = (slots + kChunks * kGroup - 1) / (kChunks * kGroup) * kGroup;
   uint4* const mine = slot + tid;
   uint4* const mine_r = mine + slots * step;
@@ -1024,23 +1025,38 @@ __global__ void __launch_bounds__(kLongThreads, 3)
   if constexpr (kPolicy) scale = grad_scale_of(a, block_denominator(a, r.weight, r.rows));
   const i64 rows_step = gridDim.x / parts;
 
-  // Whether a row may count (the action's own entry is still to be seen); the same in the
-  // whole cluster.
-  const auto maybe_used = [&](i64 row) {
-    const i64 action = r.actions[row];
-    return action >= 0 && action < r.vocab && !(r.weight && r.weight[row] == 0.0f);
+  // A row that may count (its action's own entry is still to be seen), or none; the same in
+  // the whole cluster.
+  struct Candidate {
+    i64 row;
+    int action;  // -1: it does not count
+  };
+  const auto candidate = [&](i64 row) {
+    Candidate c{row, -1};
+    if (row < r.rows) {
+      const i64 action = r.actions[row];
+      const float w = r.weight ? r.weight[row] : 1.0f;
+      if (action >= 0 && action < r.vocab && w != 0.0f) c.action = static_cast<int>(action);
+    }
+    return c;
   };
   // Of a part's vectors, how many are this thread's and in slots.
   const auto slotted = [&](const Part<T>& p) {
-    const int n = (p.last - p.first - tid + step - 1) / step;
+    const int n = (p.last - p.first - tid + step - 1) >> log_step;
     return p.last - p.first <= tid ? 0 : n < slots ? n : slots;
   };
   // Starts the copies of a chunk of a part's slots, n of which are this thread's; always a
   // group of its own.
   const auto fetch = [&](const uint4* x, const uint4* z, int n, int c) {
     const int end = (c + 1) * chunk < n ? (c + 1) * chunk : n;
-    int at = c * chunk * step;
-    for (int k = c * chunk; k < end; ++k, at += step) {
+    int k = c * chunk, at = k * step;
+    for (; k + kGroup <= end; k += kGroup, at += kGroup * step)
+#pragma unroll
+      for (int h = 0; h < kGroup; ++h) {
+        copy16(mine + at + h * step, x + at + h * step);
+        if constexpr (kRef) copy16(mine_r + at + h * step, z + at + h * step);
+      }
+    for (; k < end; ++k, at += step) {
       copy16(mine + at, x + at);
       if constexpr (kRef) copy16(mine_r + at, z + at);
     }
@@ -1052,10 +1068,11 @@ __global__ void __launch_bounds__(kLongThreads, 3)
     return kRef ? reinterpret_cast<const uint4*>(p.z + p.head) + p.first + tid : nullptr;
   };
 
-  // The next row from `row` on that may count; those before it get their zeros here, so
-  // that copies are always under way for the row that comes next.
-  const auto skip = [&](i64 row) {
-    for (; row < r.rows && !maybe_used(row); row += rows_step) {
+  // The next row from `c` on that may count; those before it get their zeros here, so that
+  // copies are always under way for the row that comes next.
+  const auto skip = [&](Candidate c) {
+    for (; c.row < r.rows && c.action < 0; c = candidate(c.row + rows_step)) {
+      const i64 row = c.row;
       if (tid == 0 && rank == 0) {
         if constexpr (!kPolicy) store_score(o, row, false, no_sums(), 0.0f);
         else if (a.logp) a.logp[row] = 0.0f;
@@ -1064,7 +1081,7 @@ __global__ void __launch_bounds__(kLongThreads, 3)
         if (a.dlogits)
           with_type(a.dtype, [&](auto type) {
             constexpr int kType = decltype(type)::value;
-            const Part<T> p(r, row, 0, r.vocab, parts, rank);
+            const Part<T> p(r, row, 0, r.vocab, log_parts, rank);
             Stored<kType>* const to = static_cast<Stored<kType>*>(a.dlogits) + row * a.ldd;
             write_zeros<T, kType>(p, to, grad_wide<T, kType>(to, p.head), tid, step);
             if (rank == 0) {
@@ -1073,30 +1090,32 @@ __global__ void __launch_bounds__(kLongThreads, 3)
             }
           });
     }
-    return row;
+    return c;
   };
 
   int buffer = 0;
-  i64 row = skip(blockIdx.x / parts), next_row;
+  Candidate now = skip(candidate(blockIdx.x >> log_parts)), next = now, after = now;
   const bool write = kPolicy && a.dlogits;  // a second look
   Part<T> p;
   int n_slotted = 0;
-  if (row < r.rows) {
-    p = Part<T>(r, row, 0, r.vocab, parts, rank);
+  if (now.row < r.rows) {
+    p = Part<T>(r, now.row, 0, r.vocab, log_parts, rank);
     n_slotted = slotted(p);
+    next = skip(candidate(now.row + rows_step));
   }
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) fetch(first_x(p), first_z(p), n_slotted, c);
-  for (; row < r.rows; row = next_row) {
-    next_row = skip(row + rows_step);
+  for (; now.row < r.rows; now = next, next = after) {
     Part<T> p_next = p;
     int n_next = 0;
-    if (next_row < r.rows) {
-      p_next = Part<T>(r, next_row, 0, r.vocab, parts, rank);
+    if (next.row < r.rows) {
+      p_next = Part<T>(r, next.row, 0, r.vocab, log_parts, rank);
       n_next = slotted(p_next);
     }
+    after = candidate(next.row + rows_step);  // looked at when this row is done
     const uint4 *const x_next = first_x(p_next), *const z_next = first_z(p_next);
-    const int action = static_cast<int>(r.actions[row]), i0 = p.first + tid;
+    const i64 row = now.row;
+    const int action = now.action, i0 = p.first + tid;
     const int n_loose = rank == 0 ? r.vocab - p.vectors * kN : 0;
     if (tid == 32) {
       row_in = row_inputs<kPolicy>(r, a, row);
@@ -1286,6 +1305,7 @@ __global__ void __launch_bounds__(kLongThreads, 3)
         });
       }
     }
+    after = skip(after);
     p = p_next;
     n_slotted = n_next;
   }
@@ -1374,7 +1394,7 @@ __global__ void __launch_bounds__(32 * kBackWarps, 4) logp_backward_kernel(const
   k.c0 = inv_s * (-g1 - g2 * ((b.d_entropy ? b.entropy[row] : 0.0f) - kLn2 * lse.y));
   k.c1 = inv_s * (-g2 * kLn2);
   k.c2 = 0.0f;
-  const Part<T> p(r, row, c0, r.vocab - c0 < kSpan ? r.vocab - c0 : kSpan, 1, 0);
+  const Part<T> p(r, row, c0, r.vocab - c0 < kSpan ? r.vocab - c0 : kSpan, 0, 0);
   const int hot = used ? static_cast<int>(r.actions[row]) - c0 : -1;
   with_type(b.dtype, [&](auto type) {
     constexpr int kType = decltype(type)::value;

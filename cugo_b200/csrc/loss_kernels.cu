@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
 // in four chunks of the slots.  Vectors that no slot holds (rows longer than eight blocks'
 // slots) are read from memory both times.
 
-constexpr int kLongThreads = 256;
+constexpr int kLongThreads = 256, kWideThreads = 512;
 constexpr int kGroup = 4;   // vectors of a thread looked at together
 constexpr int kChunks = 2;  // of a row's slots, waited for one after another
 
@@ -1000,12 +1000,12 @@ __device__ __forceinline__ void wait_copies() {
 }
 
 // slots: vectors of a thread that shared memory holds.
-template <typename T, bool kRef, bool kPolicy>
-__global__ void __launch_bounds__(kLongThreads, 3)
+template <typename T, bool kRef, bool kPolicy, int kThreads>
+__global__ void __launch_bounds__(kThreads, kThreads == kWideThreads ? 2 : 3)
     long_rows_kernel(const Rows r, const Score o, const Policy a, const int slots) {
   constexpr int kN = kVec<T>;
   extern __shared__ __align__(16) uint4 slot[];  // [slots][threads], then the reference's
-  __shared__ Sums warp_sums[kLongThreads / 32];
+  __shared__ Sums warp_sums[kThreads / 32];
   __shared__ Sums block_sums[2];
   __shared__ RowInputs row_in;   // thread 32's, for thread 0
   __shared__ float row_x;        // the action's entry
@@ -1580,27 +1580,43 @@ struct Plan {
 };
 
 // A block per row, of as few threads as leave each about 16 vectors (a row costs a thread
-// some 300 instructions beside its vectors); a cluster of blocks where the row is longer
-// than the slots of one (three blocks share an SM, or as many as the slots allow), and
-// where rows are few: up to 8, each with at least 4,096 entries.
-Plan long_plan(i64 rows, int vocab, int size, bool ref, bool stage) {
+// some 400 instructions beside its vectors; 8,192 rows of 16,384 bf16: 128 threads 58 us,
+// 256 threads 86 us); a cluster of blocks where the row is longer than the slots of one
+// (three blocks share an SM, or as many as the slots allow), and where rows are few: up
+// to 8, each with at least 4,096 entries.  A policy loss that has to cut its rows takes
+// fewer and larger blocks, two of 512 threads an SM, and reads what their slots do not
+// hold once more (2,048 rows of 131,072 bf16: 2 blocks a row and 13 of 16 vectors in
+// slots 242 us, 4 blocks of 256 threads and all 16 298 us).
+Plan long_plan(i64 rows, int vocab, int size, bool ref, bool stage, bool policy) {
   constexpr int kBudget = 224 << 10, kStatic = 3 << 10;  // an SM's shared memory, a block's other part
   Plan p{};
   const int copies = ref ? 2 : 1;
   const i64 bytes = static_cast<i64>(vocab) * size * copies;
+  const bool cut = bytes > kBudget / 3 - kStatic;
   p.parts = 1;
-  while (p.parts < 8 && bytes > static_cast<i64>(p.parts) * (kBudget / 3 - kStatic)) p.parts *= 2;
+  p.threads = kLongThreads;
+  int most_per_sm = 3;
+  if (cut && policy) {
+    p.threads = kWideThreads;
+    most_per_sm = 2;
+    while (p.parts < 8 && bytes > static_cast<i64>(p.parts) * (kBudget / 2 - kStatic) * 5 / 4) p.parts *= 2;
+  } else {
+    while (p.parts < 8 && bytes > static_cast<i64>(p.parts) * (kBudget / 3 - kStatic)) p.parts *= 2;
+  }
   while (p.parts < 8 && rows * p.parts < kSms && vocab / (2 * p.parts) >= 4096) p.parts *= 2;
   const i64 each = (static_cast<i64>(vocab) * size / 16 + p.parts - 1) / p.parts;  // vectors
-  p.threads = each <= 16 * 128 ? 128 : kLongThreads;
+  if (each <= 16 * 128) {
+    p.threads = 128;
+    most_per_sm = 6;
+  }
   if (stage) {
-    const i64 want = (each + p.threads - 1) / p.threads, room = (kBudget - kStatic) / (p.threads * 16 * copies);
-    p.slots = static_cast<int>(((want < room ? want : room) + kGroup - 1) / kGroup * kGroup);
-    if (p.slots > room) p.slots -= kGroup;
+    const i64 want = (each + p.threads - 1) / p.threads;
+    const i64 room = ((cut ? kBudget / most_per_sm : kBudget) - kStatic) / (p.threads * 16 * copies);
+    p.slots = static_cast<int>(want < room ? want : room);
   }
   p.shared = p.slots * p.threads * 16 * copies;
   int per_sm = kBudget / (p.shared + kStatic);
-  if (per_sm > 768 / p.threads) per_sm = 768 / p.threads;  // by registers
+  if (per_sm > most_per_sm) per_sm = most_per_sm;
   const i64 most = static_cast<i64>(kSms) * per_sm / p.parts;
   p.blocks = static_cast<int>(rows < most ? rows : most) * p.parts;
   return p;
@@ -1615,22 +1631,16 @@ inline bool is_run(i64 ld, i64 vocab, int size) { return ld >= vocab && (ld - vo
 // granule for its alignment.
 inline int run_bytes(i64 n, i64 ld, i64 width, int size) { return round16(((n - 1) * ld + width) * size + 15); }
 
-template <typename T, bool kRef, bool kPolicy>
-int launch_long(const Rows& r, const Score& o, const Policy& a, cudaStream_t stream, int& blocks) {
-  const auto kernel = long_rows_kernel<T, kRef, kPolicy>;
-  // The reference's vectors are copied beside the logits' where both are aligned alike.
-  constexpr int kSize = sizeof(T);
-  const bool stage = !r.legal && (!kRef || ((reinterpret_cast<uintptr_t>(r.ref) - reinterpret_cast<uintptr_t>(r.logits)) % 16 == 0 &&
-                               (r.rows <= 1 || (r.ldr - r.ld) * kSize % 16 == 0)));
-  const Plan p = long_plan(r.rows, r.vocab, kSize, kRef, stage);
-  blocks = p.blocks;
+template <typename T, bool kRef, bool kPolicy, int kThreads>
+int launch_planned(const Plan& p, const Rows& r, const Score& o, const Policy& a, cudaStream_t stream) {
+  const auto kernel = long_rows_kernel<T, kRef, kPolicy, kThreads>;
   if (p.shared > (40 << 10) &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.shared) != cudaSuccess)
     return CUGO_B200_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
-  cfg.dynamicSmemBytes = p.shared;
   cfg.gridDim = dim3(p.blocks);
   cfg.blockDim = dim3(p.threads);
+  cfg.dynamicSmemBytes = p.shared;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1639,6 +1649,19 @@ int launch_long(const Rows& r, const Score& o, const Policy& a, cudaStream_t str
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, r, o, a, p.slots) == cudaSuccess ? CUGO_B200_OK : CUGO_B200_ERR_LAUNCH;
+}
+
+template <typename T, bool kRef, bool kPolicy>
+int launch_long(const Rows& r, const Score& o, const Policy& a, cudaStream_t stream, int& blocks) {
+  // The reference's vectors are copied beside the logits' where both are aligned alike.
+  constexpr int kSize = sizeof(T);
+  const bool stage = !r.legal && (!kRef || ((reinterpret_cast<uintptr_t>(r.ref) - reinterpret_cast<uintptr_t>(r.logits)) % 16 == 0 &&
+                               (r.rows <= 1 || (r.ldr - r.ld) * kSize % 16 == 0)));
+  const Plan p = long_plan(r.rows, r.vocab, kSize, kRef, stage, kPolicy);
+  blocks = p.blocks;
+  if constexpr (kPolicy)
+    if (p.threads == kWideThreads) return launch_planned<T, kRef, kPolicy, kWideThreads>(p, r, o, a, stream);
+  return launch_planned<T, kRef, kPolicy, kLongThreads>(p, r, o, a, stream);
 }
 
 template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy, bool kStaged>

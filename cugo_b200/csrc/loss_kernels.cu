@@ -271,6 +271,7 @@ struct Policy {
   const float* adv;
   const float* ref_logp;  // or null
   float low, high, kl_coef, entropy_coef;
+  const float *kl_coef_dev, *entropy_coef_dev;  // or null; multiply the two
   float denominator;            // not 0: given; 0: *denominator_dev, the sum of the weights, or the rows
   const float* denominator_dev;
   const double* weight_sums;    // partial sums of the weights, or null (sum them here)
@@ -362,6 +363,14 @@ __device__ __forceinline__ Coefs policy_row(const Policy& a, const RowInputs& in
   c.c2 = ks * c2;
   terms = {{-gain, entropy, kl, expm1f(log_ratio) - log_ratio, ratio < a.low || ratio > a.high ? 1.0f : 0.0f, 1.0f}};
   return c;
+}
+
+// The same with its device-resident coefficients read (a captured graph keeps their
+// addresses).
+__device__ __forceinline__ Policy resolved(Policy a) {
+  if (a.kl_coef_dev) a.kl_coef *= *a.kl_coef_dev;
+  if (a.entropy_coef_dev) a.entropy_coef *= *a.entropy_coef_dev;
+  return a;
 }
 
 // The denominator of the means: given, the sum of the weights, or the rows.  Every block
@@ -456,7 +465,8 @@ struct Layout {
 
 template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy, bool kStaged>
 __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
-    short_rows_kernel(const Rows r, const Score o, const Policy a, const Layout lay) {
+    short_rows_kernel(const Rows r, const Score o, const Policy given, const Layout lay) {
+  const Policy a = kPolicy ? resolved(given) : given;
   constexpr int kRows = 32 / kLanes;
   extern __shared__ __align__(16) char shared[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % kLanes, sub = lane / kLanes;
@@ -1002,7 +1012,8 @@ __device__ __forceinline__ void wait_copies() {
 // slots: vectors of a thread that shared memory holds.
 template <typename T, bool kRef, bool kPolicy, int kThreads>
 __global__ void __launch_bounds__(kThreads, kThreads == kWideThreads ? 2 : 3)
-    long_rows_kernel(const Rows r, const Score o, const Policy a, const int slots) {
+    long_rows_kernel(const Rows r, const Score o, const Policy given, const int slots) {
+  const Policy a = kPolicy ? resolved(given) : given;
   constexpr int kN = kVec<T>;
   extern __shared__ __align__(16) uint4 slot[];  // [slots][threads], then the reference's
   __shared__ Sums warp_sums[kThreads / 32];
@@ -1337,8 +1348,9 @@ __global__ void __launch_bounds__(512) weight_sums_kernel(const float* weight, i
   }
 }
 
-__global__ void __launch_bounds__(32 * kSums) policy_means_kernel(const Policy a, const float* weight, i64 rows,
+__global__ void __launch_bounds__(32 * kSums) policy_means_kernel(const Policy given, const float* weight, i64 rows,
                                                                   int blocks, float* stats, float* loss) {
+  const Policy a = resolved(given);
   __shared__ double means[kSums];
   const double d = block_denominator(a, weight, rows);
   const int k = threadIdx.x >> 5;
@@ -1785,7 +1797,7 @@ int cugo_b200_policy_loss(const void* logits, int64_t ld, int32_t dtype, const v
                           const bool* legal, int64_t ldm, const int64_t* actions, const float* logp_old,
                           const float* adv, const float* weight, const float* ref_logp, int64_t rows,
                           int64_t vocab, float clip_low, float clip_high, float kl_coef, float entropy_coef,
-                          float denominator, const float* denominator_dev, float grad_scale,
+                          const float* kl_coef_dev, const float* entropy_coef_dev, float denominator, const float* denominator_dev, float grad_scale,
                           const float* grad_scale_dev, void* dlogits, int64_t ldd, int32_t grad_dtype,
                           int64_t width, float* logp, float* stats, float* loss, void* scratch,
                           int64_t scratch_bytes, cudaStream_t stream) {
@@ -1816,6 +1828,8 @@ int cugo_b200_policy_loss(const void* logits, int64_t ld, int32_t dtype, const v
   a.high = 1.0f + clip_high;
   a.kl_coef = kl_coef;
   a.entropy_coef = entropy_coef;
+  a.kl_coef_dev = kl_coef_dev;
+  a.entropy_coef_dev = entropy_coef_dev;
   a.denominator = denominator;
   a.denominator_dev = denominator_dev;
   a.grad_scale = grad_scale;

@@ -91,8 +91,8 @@ _SIGNATURES: dict[str, list] = {
     "cugo_b200_action_logp_backward": [_VP, _I64, _I32, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _VP,
                                        _I64, _I64, _VP, _I64, _I32, _VP],
     "cugo_b200_policy_loss": [_VP, _I64, _I32, _VP, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _VP,
-                              _I64, _I64, _F32, _F32, _F32, _F32, _F32, _VP, _F32, _VP, _VP, _I64,
-                              _I32, _I64, _VP, _VP, _VP, _VP, _I64, _VP],
+                              _I64, _I64, _F32, _F32, _F32, _F32, _VP, _VP, _F32, _VP, _F32, _VP, _VP,
+                              _I64, _I32, _I64, _VP, _VP, _VP, _VP, _I64, _VP],
     "cugo_b200_preference_pairs": [_VP, _VP, _VP, _VP, _VP, _I64, _I64, _F32, _F32, _I32, _VP,
                                    _VP, _VP, _VP, _VP, _VP, _I64, _VP],
     "cugo_b200_adamw": [_I64, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I32, _I32, _I32, _F64, _VP, _F64,
@@ -691,7 +691,8 @@ class CugoB200Extension:
         """The clipped policy loss (see the C declaration): (loss fp32 scalar, stats fp32 [8],
         logp fp32 [rows], d loss / d logits); the gradient goes to dlogits [rows, >= vocab]
         where given, or to a new tensor of grad_dtype where given, or is None; with
-        stats=False the gradient only."""
+        stats=False the gradient only.  kl_coef and entropy_coef may be one fp32 value on the
+        device."""
         op = "policy_loss"
         rows, vocab, device, x, m, w = self._rows(op, logits, actions, legal, weight)
         _check_vector(logp_old, op, "logp_old", rows, torch.float32, device)
@@ -707,6 +708,13 @@ class CugoB200Extension:
                 raise RuntimeError(f"{op}: give ref_logits or ref_logp, not both")
             _check_vector(ref_logp, op, "ref_logp", rows, torch.float32, device)
             ref_logp_ptr = ref_logp.data_ptr()
+        kl_dev = entropy_dev = None
+        if torch.is_tensor(kl_coef):
+            _check_scalar(kl_coef, op, "kl_coef", torch.float32, device)
+            kl_dev, kl_coef = kl_coef.data_ptr(), 1.0
+        if torch.is_tensor(entropy_coef):
+            _check_scalar(entropy_coef, op, "entropy_coef", torch.float32, device)
+            entropy_dev, entropy_coef = entropy_coef.data_ptr(), 1.0
         if denominator_dev is not None:
             _check_scalar(denominator_dev, op, "denominator", torch.float32, device)
         if grad_scale_dev is not None:
@@ -730,7 +738,8 @@ class CugoB200Extension:
                 grad = (dlogits.data_ptr(), ldd, _LOGIT_TYPES[dlogits.dtype], dlogits.size(1))
             _check(lib.cugo_b200_policy_loss(
                 *x, ref_ptr, ldr, *m, logp_old.data_ptr(), adv.data_ptr(), w, ref_logp_ptr, rows, vocab,
-                clip_low, clip_high, kl_coef, entropy_coef, denominator, _ptr(denominator_dev), grad_scale,
+                clip_low, clip_high, kl_coef, entropy_coef, kl_dev, entropy_dev, denominator,
+                _ptr(denominator_dev), grad_scale,
                 _ptr(grad_scale_dev), *grad, _ptr(logp), _ptr(out), _ptr(loss), scratch.data_ptr(), need,
                 _raw_stream(device)), op)
         return loss, out, logp, dlogits

@@ -121,7 +121,8 @@ def _coefs(clip_low, clip_high, kl_coef, entropy_coef, denominator):
         raise RuntimeError("policy_loss: the clip's bounds must not be negative")
     if denominator is not None and not denominator > 0.0:
         raise RuntimeError("policy_loss: the denominator must be positive")
-    return (float(clip_low), float(clip_high), float(kl_coef), float(entropy_coef),
+    kl_coef, entropy_coef = (c if torch.is_tensor(c) else float(c) for c in (kl_coef, entropy_coef))
+    return (float(clip_low), float(clip_high), kl_coef, entropy_coef,
             0.0 if denominator is None else float(denominator))
 
 
@@ -129,7 +130,8 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, logp_old: torch.Ten
                 adv: torch.Tensor, *, legal: torch.Tensor | None = None,
                 weight: torch.Tensor | None = None, ref_logits: torch.Tensor | None = None,
                 ref_logp: torch.Tensor | None = None, clip_low: float = 0.2,
-                clip_high: float | None = None, kl_coef: float = 0.0, entropy_coef: float = 0.0,
+                clip_high: float | None = None, kl_coef: float | torch.Tensor = 0.0,
+                entropy_coef: float | torch.Tensor = 0.0,
                 denominator: float | None = None) -> PolicyLoss:
     """The clipped policy loss, differentiable in the logits:
 
@@ -142,7 +144,8 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, logp_old: torch.Ten
     which is never negative and right in the mean; or 0.  D: the sum of the weights (the
     rows without weights; 0 gives a loss of 0), or `denominator` (a data-parallel job's
     total, say).  logp_old, adv, weight, ref_logp: fp32 [rows]; clip_high defaults to
-    clip_low."""
+    clip_low; kl_coef and entropy_coef may be one fp32 value on the device (a schedule that a
+    captured graph follows)."""
     coefs = _coefs(clip_low, clip_high, kl_coef, entropy_coef, denominator)
     if torch.is_grad_enabled() and logits.requires_grad:
         return PolicyLoss(*_PolicyLoss.apply(logits, actions, logp_old, adv, legal, weight, ref_logits,
@@ -156,8 +159,8 @@ def policy_loss_grad(logits: torch.Tensor, actions: torch.Tensor, logp_old: torc
                      adv: torch.Tensor, *, legal: torch.Tensor | None = None,
                      weight: torch.Tensor | None = None, ref_logits: torch.Tensor | None = None,
                      ref_logp: torch.Tensor | None = None, clip_low: float = 0.2,
-                     clip_high: float | None = None, kl_coef: float = 0.0,
-                     entropy_coef: float = 0.0, denominator: float | None = None,
+                     clip_high: float | None = None, kl_coef: float | torch.Tensor = 0.0,
+                     entropy_coef: float | torch.Tensor = 0.0, denominator: float | None = None,
                      grad_scale: float | torch.Tensor = 1.0, grad_dtype: torch.dtype | None = None,
                      dlogits: torch.Tensor | None = None) -> tuple[PolicyLoss, torch.Tensor]:
     """policy_loss and grad_scale (a number, or one fp32 value on the device) times its

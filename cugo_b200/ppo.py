@@ -29,6 +29,8 @@ import torch.nn.functional as F
 from torch import nn
 
 from .ext import load_extension
+from .losses import policy_loss, policy_loss_grad
+from .optim import AdamW
 
 FEATURES, ACTIONS, ORACLE_FEATURES = 720, 179, 50
 _ACT = {"relu": 1, "silu": 2}
@@ -653,12 +655,19 @@ class PpoStep:
     cross-entropy against the two-hot return for a critic with value bins),
     optionally the belief head's binary cross-entropy on the opponent's hand,
     gradient clipping per network, the optimizer step and the running statistics
-    (policy, value, entropy, KL, clip fraction, count, belief loss)."""
+    (policy, value, entropy, KL, clip fraction, count, belief loss, KL to the reference).
+
+    reference, kl_coef: a frozen actor (the league's, say) that the policy is held to by
+    kl_coef times KL(policy | reference) over the legal actions, in the policy loss of
+    losses.py.  An optim.AdamW whose groups are the networks clips their gradients itself
+    (max_grad_norm); grad_clip is for the other optimizers."""
 
     def __init__(self, actor: nn.Module, critic: nn.Module, optimizer: torch.optim.Optimizer,
                  clip: float = 0.2, value_coef: float = 0.5, grad_clip: float = 1.0,
-                 world: int = 1, belief: nn.Module | None = None, belief_coef: float = 0.0) -> None:
+                 world: int = 1, belief: nn.Module | None = None, belief_coef: float = 0.0,
+                 reference: nn.Module | None = None, kl_coef: float = 0.0) -> None:
         self.actor, self.critic, self.optimizer = actor, critic, optimizer
+        self.reference = reference
         self.clip, self.value_coef, self.grad_clip, self.world = clip, value_coef, grad_clip, world
         self.belief, self.belief_coef = belief, belief_coef
         self.groups = [list(actor.parameters()), list(critic.parameters())]
@@ -666,10 +675,23 @@ class PpoStep:
             self.groups.append(list(belief.parameters()))
         dev = next(actor.parameters()).device
         self.entropy_coef = torch.zeros((), device=dev)
-        self.sums = torch.zeros(7, device=dev)
+        self.kl_coef = torch.full((), kl_coef, device=dev)
+        self.sums = torch.zeros(8, device=dev)
         self.last_kl = torch.zeros((), device=dev)  # the latest minibatch's KL estimate
 
+    def clip_gradients(self) -> None:
+        if isinstance(self.optimizer, AdamW) and self.optimizer.clips:
+            return
+        for group in self.groups:
+            nn.utils.clip_grad_norm_(group, self.grad_clip, foreach=True)
+
+    @torch.no_grad()
+    def reference_logits(self, mb: Minibatch) -> torch.Tensor:
+        return self.reference(mb.features).float()
+
     def losses(self, mb: Minibatch):
+        """(policy loss, value loss, entropy, ratio, log ratio, belief loss), or with a
+        reference (policy_loss's result, value loss, None, None, None, belief loss)."""
         belief_loss = None
         if self.belief is not None:
             out, hidden = self.actor.forward_hidden(mb.features)
@@ -680,39 +702,50 @@ class PpoStep:
             logits = self.actor(mb.features).float()
         stock = mb.stock if getattr(self.critic, "stock", False) else None
         value = self.critic(critic_input(mb.features, mb.opp_hand, stock)).float()
-        log_probs = torch.log_softmax(logits.masked_fill(~mb.legal, -1.0e30), dim=1)
-        new_logp = log_probs.gather(1, mb.actions.unsqueeze(1)).squeeze(1)
-        log_ratio = new_logp - mb.logp_old
-        ratio = log_ratio.exp()
-        surrogate = torch.minimum(ratio * mb.adv, ratio.clamp(1 - self.clip, 1 + self.clip) * mb.adv)
-        policy_loss = -surrogate.mean()
-        entropy = -(log_probs.exp() * log_probs).sum(1).mean()
         if getattr(self.critic, "value_bins", 0):
             target = two_hot(mb.ret, self.critic.support)
             value_loss = -(target * torch.log_softmax(value, -1)).sum(-1).mean()
         else:
             value_loss = F.smooth_l1_loss(value, mb.ret)
-        return policy_loss, value_loss, entropy, ratio, log_ratio, belief_loss
+        if self.reference is not None:
+            out = policy_loss(logits, mb.actions, mb.logp_old, mb.adv, legal=mb.legal,
+                              ref_logits=self.reference_logits(mb), clip_low=self.clip,
+                              kl_coef=self.kl_coef, entropy_coef=self.entropy_coef)
+            return out, value_loss, None, None, None, belief_loss
+        log_probs = torch.log_softmax(logits.masked_fill(~mb.legal, -1.0e30), dim=1)
+        new_logp = log_probs.gather(1, mb.actions.unsqueeze(1)).squeeze(1)
+        log_ratio = new_logp - mb.logp_old
+        ratio = log_ratio.exp()
+        surrogate = torch.minimum(ratio * mb.adv, ratio.clamp(1 - self.clip, 1 + self.clip) * mb.adv)
+        surrogate_loss = -surrogate.mean()
+        entropy = -(log_probs.exp() * log_probs).sum(1).mean()
+        return surrogate_loss, value_loss, entropy, ratio, log_ratio, belief_loss
 
     def step(self, mb: Minibatch) -> None:
         """One update, eager (every kernel launched from Python)."""
         self.optimizer.zero_grad(set_to_none=False)
-        policy_loss, value_loss, entropy, ratio, log_ratio, belief_loss = self.losses(mb)
-        loss = policy_loss - self.entropy_coef * entropy + self.value_coef * value_loss
+        policy, value_loss, entropy, ratio, log_ratio, belief_loss = self.losses(mb)
+        if self.reference is not None:
+            loss = policy.loss + self.value_coef * value_loss
+        else:
+            loss = policy - self.entropy_coef * entropy + self.value_coef * value_loss
         if belief_loss is not None:
             loss = loss + self.belief_coef * belief_loss
         loss.backward()
         allreduce_gradients([p for g in self.groups for p in g], self.world)
-        for group in self.groups:
-            nn.utils.clip_grad_norm_(group, self.grad_clip, foreach=True)
+        self.clip_gradients()
         self.optimizer.step()
         with torch.no_grad():
-            kl = ((ratio - 1) - log_ratio).mean()
+            zero = torch.zeros_like(value_loss)
+            bl = belief_loss.detach() if belief_loss is not None else zero
+            if self.reference is not None:
+                _, policy, entropy, ref_kl, kl, clipped, _ = policy.stats.unbind()
+            else:
+                policy, ref_kl, kl = policy.detach(), zero, ((ratio - 1) - log_ratio).mean()
+                clipped = ((ratio - 1).abs() > self.clip).float().mean()
             self.last_kl.copy_(kl)
-            bl = belief_loss.detach() if belief_loss is not None else torch.zeros_like(kl)
-            self.sums += torch.stack((policy_loss.detach(), value_loss.detach(), entropy.detach(), kl,
-                                      ((ratio - 1).abs() > self.clip).float().mean(),
-                                      torch.ones_like(kl), bl))
+            self.sums += torch.stack((policy, value_loss.detach(), entropy.detach(), kl, clipped,
+                                      torch.ones_like(zero), bl, ref_kl))
 
 
 class NativePpoStep(PpoStep):
@@ -724,8 +757,10 @@ class NativePpoStep(PpoStep):
 
     def __init__(self, actor: FusedResidualMlp, critic: FusedResidualMlp,
                  optimizer: torch.optim.Optimizer, clip: float = 0.2, value_coef: float = 0.5,
-                 grad_clip: float = 1.0, world: int = 1) -> None:
-        super().__init__(actor, critic, optimizer, clip, value_coef, grad_clip, world)
+                 grad_clip: float = 1.0, world: int = 1, reference: nn.Module | None = None,
+                 kl_coef: float = 0.0) -> None:
+        super().__init__(actor, critic, optimizer, clip, value_coef, grad_clip, world,
+                         reference=reference, kl_coef=kl_coef)
         self.stats = torch.zeros(5, device=self.sums.device)
         self.ones = torch.ones(1, device=self.sums.device)
         # Each network's gradients live in one flat buffer, the bucket of its all-reduce.
@@ -761,8 +796,20 @@ class NativePpoStep(PpoStep):
         b = logits.shape[0]
         dy = torch.empty((b, _pad8(ACTIONS)), dtype=torch.bfloat16, device=logits.device)
         dv = torch.empty(b, dtype=torch.float32, device=logits.device)
-        ext.ppo_loss(logits, mb.legal, mb.actions, mb.logp_old, mb.adv, value, mb.ret, self.clip,
-                     self.entropy_coef, self.value_coef, dy, dv, self.stats)
+        if self.reference is None:
+            ext.ppo_loss(logits, mb.legal, mb.actions, mb.logp_old, mb.adv, value, mb.ret, self.clip,
+                         self.entropy_coef, self.value_coef, dy, dv, self.stats)
+        else:
+            out, _ = policy_loss_grad(logits, mb.actions, mb.logp_old, mb.adv, legal=mb.legal,
+                                      ref_logits=self.reference_logits(mb), clip_low=self.clip,
+                                      kl_coef=self.kl_coef, entropy_coef=self.entropy_coef, dlogits=dy)
+            d = value[:, 0] - mb.ret  # the smooth-L1 value loss and its slope
+            torch.mul(d.clamp(-1.0, 1.0), self.value_coef / b, out=dv)
+            self.stats[1:2] = torch.where(d.abs() < 1.0, 0.5 * d * d, d.abs() - 0.5).mean()
+            self.stats[0:1] = out.stats[1]
+            self.stats[2:3] = out.stats[2]
+            self.stats[3:5] = out.stats[4:6]
+            self.sums[7:8] += out.stats[3]
         if side is not None:  # the two backwards side by side
             side.wait_stream(main)
             dv.record_stream(side)
@@ -781,8 +828,7 @@ class NativePpoStep(PpoStep):
                                            self.flat.get("actor"))
             finish_allreduce(critic_bucket)
             finish_allreduce(actor_bucket)
-        for group in self.groups:
-            nn.utils.clip_grad_norm_(group, self.grad_clip, foreach=True)
+        self.clip_gradients()
         self.optimizer.step()
         self.last_kl.copy_(self.stats[3])
         self.sums[:5] += self.stats
@@ -792,12 +838,14 @@ class NativePpoStep(PpoStep):
 def make_ppo_step(actor: nn.Module, critic: nn.Module, optimizer: torch.optim.Optimizer,
                   clip: float = 0.2, value_coef: float = 0.5, grad_clip: float = 1.0,
                   world: int = 1, belief: nn.Module | None = None,
-                  belief_coef: float = 0.0) -> PpoStep:
+                  belief_coef: float = 0.0, reference: nn.Module | None = None,
+                  kl_coef: float = 0.0) -> PpoStep:
     """The native step where both networks are FusedResidualMlp (norm "none", scalar
     critic, no belief head), else the autograd one."""
     if belief is None and NativePpoStep.supports(actor, critic):
-        return NativePpoStep(actor, critic, optimizer, clip, value_coef, grad_clip, world)
-    return PpoStep(actor, critic, optimizer, clip, value_coef, grad_clip, world, belief, belief_coef)
+        return NativePpoStep(actor, critic, optimizer, clip, value_coef, grad_clip, world, reference, kl_coef)
+    return PpoStep(actor, critic, optimizer, clip, value_coef, grad_clip, world, belief, belief_coef,
+                   reference, kl_coef)
 
 
 class GraphedPpoStep:

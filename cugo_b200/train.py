@@ -40,6 +40,7 @@ from torch import nn
 
 from .evaluate import make_seeds
 from .ext import load_extension
+from .optim import AdamW
 from .ppo import GraphedPpoStep, Minibatch, critic_input, make_ppo_step
 from .rounds import DONE_BYTE, RunningSet, choose_actions, fused_sampler_params
 
@@ -270,6 +271,7 @@ class TrainStats:
     updates: int
     epochs: float
     belief_loss: float = float("nan")
+    ref_kl: float = float("nan")  # KL to the reference policy, where there is one
 
 
 class PpoTrainer:
@@ -280,20 +282,35 @@ class PpoTrainer:
     rank updates on its own rollout and PpoStep averages the gradients.  The ranks
     must take the same collective steps, so every epoch runs the smallest number of
     whole minibatches any rank has, and the early stop compares the KL averaged over
-    the ranks."""
+    the ranks.
+
+    optimizer: "adam" (the reference trainer's), or optim.AdamW with states in 32 bits
+    ("adamw") or 8 ("adamw8"), which clips each network's gradients in its own step and
+    decays the weights by weight_decay.  reference, kl_coef: as PpoStep's."""
 
     def __init__(self, actor: nn.Module, critic: nn.Module, lr: float = 3e-4,
                  minibatch: int = 32768, clip: float = 0.2, value_coef: float = 0.5,
                  grad_clip: float = 1.0, use_graph: bool = True, world: int = 1,
-                 belief: nn.Module | None = None, belief_coef: float = 0.0) -> None:
+                 belief: nn.Module | None = None, belief_coef: float = 0.0,
+                 optimizer: str = "adam", weight_decay: float = 0.0,
+                 reference: nn.Module | None = None, kl_coef: float = 0.0) -> None:
+        if optimizer not in ("adam", "adamw", "adamw8"):
+            raise ValueError("optimizer must be adam, adamw or adamw8")
+        if optimizer == "adam" and weight_decay:
+            raise ValueError("weight_decay needs the optimizer adamw or adamw8")
         self.actor, self.critic, self.minibatch = actor, critic, minibatch
         self.belief = belief
-        params = list(actor.parameters()) + list(critic.parameters())
-        params += list(belief.parameters()) if belief is not None else []
-        # The reference trainer's optimizer (python/train_ppo50.py:153-156).
-        self.optimizer = torch.optim.Adam(params, lr=lr, eps=1e-5, fused=True, capturable=use_graph)
+        networks = [list(n.parameters()) for n in (actor, critic, belief) if n is not None]
+        if optimizer == "adam":
+            # The reference trainer's optimizer (python/train_ppo50.py:153-156).
+            self.optimizer = torch.optim.Adam([p for n in networks for p in n], lr=lr, eps=1e-5,
+                                              fused=True, capturable=use_graph)
+        else:
+            self.optimizer = AdamW([{"params": n} for n in networks], lr=lr, eps=1e-5,
+                                   weight_decay=weight_decay, max_grad_norm=grad_clip,
+                                   state_bits=8 if optimizer == "adamw8" else 32)
         self.step = make_ppo_step(actor, critic, self.optimizer, clip, value_coef, grad_clip, world,
-                                  belief, belief_coef)
+                                  belief, belief_coef, reference, kl_coef)
         self.use_graph = use_graph
         self.world = world
         self.graphed: GraphedPpoStep | None = None
@@ -378,7 +395,8 @@ class PpoTrainer:
         return TrainStats(policy_loss=s[0] / count, value_loss=s[1] / count, entropy=s[2] / count,
                           kl=s[3] / count, clipfrac=s[4] / count, explained_var=explained_var,
                           updates=updates, epochs=updates / max(1, steps),
-                          belief_loss=s[6] / count if self.belief is not None else float("nan"))
+                          belief_loss=s[6] / count if self.belief is not None else float("nan"),
+                          ref_kl=s[7] / count if st.reference is not None else float("nan"))
 
 
 def iteration(ext: Any, trainer: PpoTrainer, storage: RolloutStorage, games: int,

@@ -414,8 +414,9 @@ CUGO_B200_API int cugo_b200_action_logp_backward(
  *                     - entropy_coef H + kl_coef K) / D
  * K is KL(p | q) over the legal entries with q from ref_logits (same dtype, rows ldr
  * apart), or with ref_logp (fp32 [rows], the reference's log p of the action) the
- * estimate exp(d) - 1 - d, d = ref_logp - log p; at most one of the two.  weight fp32
- * [rows] or null (1).  D = denominator where that is not 0, else *denominator_dev (device
+ * estimate exp(d) - 1 - d, d = ref_logp - log p; at most one of the two. *kl_coef_dev and
+ * *entropy_coef_dev (device fp32, may be null: 1) multiply the two coefficients.  weight
+ * fp32 [rows] or null (1).  D = denominator where that is not 0, else *denominator_dev (device
  * fp32) if given, else the sum of the weights, or the rows; D = 0 gives a loss and
  * gradients of 0.
  * dlogits (grad_dtype, rows ldd apart, may be null) gets d loss / d logits times
@@ -429,10 +430,11 @@ CUGO_B200_API int cugo_b200_policy_loss(
     const void* logits, int64_t ld, int32_t dtype, const void* ref_logits, int64_t ldr,
     const bool* legal, int64_t ldm, const int64_t* actions, const float* logp_old,
     const float* adv, const float* weight, const float* ref_logp, int64_t rows, int64_t vocab,
-    float clip_low, float clip_high, float kl_coef, float entropy_coef, float denominator,
-    const float* denominator_dev, float grad_scale, const float* grad_scale_dev, void* dlogits,
-    int64_t ldd, int32_t grad_dtype, int64_t width, float* logp, float* stats, float* loss,
-    void* scratch, int64_t scratch_bytes, cudaStream_t stream);
+    float clip_low, float clip_high, float kl_coef, float entropy_coef, const float* kl_coef_dev,
+    const float* entropy_coef_dev, float denominator, const float* denominator_dev, float grad_scale,
+    const float* grad_scale_dev, void* dlogits, int64_t ldd, int32_t grad_dtype, int64_t width,
+    float* logp, float* stats, float* loss, void* scratch, int64_t scratch_bytes,
+    cudaStream_t stream);
 
 CUGO_B200_API int64_t cugo_b200_policy_loss_scratch_bytes(int64_t rows);
 

@@ -66,7 +66,7 @@ def _policy(lib, rows=8, ref=None, ref_logp=None, low=0.2, high=0.2, dlogits=P, 
             stats=P, loss=None, scratch=P, nbytes=None, logp_old=P, adv=P, vocab=179):
     need = lib.cugo_b200_policy_loss_scratch_bytes(rows) if nbytes is None else nbytes
     return lib.cugo_b200_policy_loss(P, 180, 0, ref, 180, None, 0, P, logp_old, adv, None, ref_logp, rows, vocab,
-                                     low, high, 0.0, 0.0, 0.0, None, 1.0, None, dlogits, ldd, gdt, width, P,
+                                     low, high, 0.0, 0.0, None, None, 0.0, None, 1.0, None, dlogits, ldd, gdt, width, P,
                                      stats, loss, scratch, need, None)
 
 

@@ -3,7 +3,9 @@
     python -m cugo_b200.build [--force]
 
 The library is torch-free: CUDA sources under cugo_b200/csrc/ compiled by nvcc with
-the CUDA runtime linked statically, exporting the C ABI of include/cugo_b200.h.
+the CUDA runtime linked statically, exporting the C ABI of include/cugo_b200.h.  Beside
+it cugo_b200/lib/_cugo_b200_update.so, the policy update's calls on that ABI for Python
+(csrc/update_binding.cpp), compiled by the host compiler against torch.
 """
 from __future__ import annotations
 
@@ -12,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -19,6 +22,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB_DIR = PKG / "lib"
 LIB = LIB_DIR / "libcugo_b200.so"
+BINDING = LIB_DIR / "_cugo_b200_update.so"
+BINDING_SOURCE = CSRC / "update_binding.cpp"
 
 SOURCES = ["env_kernels.cu", "drivers.cu", "policy_kernels.cu", "mlp_kernels.cu", "seq_kernels.cu",
            "rollout_kernels.cu", "update_kernels.cu", "loss_kernels.cu", "optim_kernels.cu"]
@@ -40,32 +45,58 @@ def _inputs() -> list[Path]:
     return [f for f in files if f.exists()]
 
 
+def _newer(target: Path, inputs: list[Path]) -> bool:
+    return target.exists() and target.stat().st_mtime >= max(f.stat().st_mtime for f in inputs)
+
+
 def up_to_date() -> bool:
-    if not LIB.exists():
-        return False
-    newest = max(f.stat().st_mtime for f in _inputs())
-    return LIB.stat().st_mtime >= newest
+    return _newer(LIB, _inputs())
+
+
+def build_binding(force: bool = False) -> Path:
+    """The Python binding of the policy update's calls; links the library beside it."""
+    if not force and _newer(BINDING, [BINDING_SOURCE, ROOT / "include" / "cugo_b200.h", Path(__file__)]):
+        return BINDING
+    import sysconfig
+
+    import torch
+    home = Path(torch.__file__).resolve().parent
+    includes = [home / "include", home / "include" / "torch" / "csrc" / "api" / "include",
+                Path(nvcc()).resolve().parents[1] / "include", Path(sysconfig.get_paths()["include"])]
+    out = BINDING.with_suffix(".so.tmp")
+    subprocess.run([shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+                    *(f"-I{p}" for p in includes), str(BINDING_SOURCE), "-o", str(out),
+                    f"-L{home / 'lib'}", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10",
+                    "-lc10_cuda", f"-L{LIB_DIR}", "-lcugo_b200", "-Wl,-rpath,$ORIGIN"], check=True)
+    out.replace(BINDING)
+    return BINDING
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and up_to_date():
+        build_binding()
         return LIB
     LIB_DIR.mkdir(parents=True, exist_ok=True)
-    objs = []
     tmp = LIB_DIR / "obj"
     tmp.mkdir(exist_ok=True)
-    for src in SOURCES:
+
+    def compile_one(src: str) -> str:
         obj = tmp / (Path(src).stem + ".o")
         cmd = [nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, "-c", str(CSRC / src), "-o", str(obj)]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
             print(" ".join(cmd), file=sys.stderr)
         subprocess.run(cmd, check=True)
-        objs.append(str(obj))
+        return str(obj)
+
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        objs = list(pool.map(compile_one, SOURCES))
     out = LIB.with_suffix(".so.tmp")
     cmd = [nvcc(), *ARCH_FLAGS, "--cudart", "static", "-shared", *objs, "-o", str(out)]
     subprocess.run(cmd, check=True)
     out.replace(LIB)
+    build_binding(force)
     return LIB
 
 

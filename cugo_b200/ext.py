@@ -12,7 +12,7 @@ There is no CPU path: without CUDA or without the native library the loader rais
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
+import importlib.util
 from pathlib import Path
 from typing import Any
 
@@ -125,8 +125,6 @@ _INT64_FUNCTIONS = {"cugo_b200_colsum_scratch_floats": [_I64, _I32],
                     "cugo_b200_policy_loss_scratch_bytes": [_I64],
                     "cugo_b200_preference_pairs_scratch_bytes": [_I64],
                     "cugo_b200_adamw_scratch_bytes": [_I64]}
-_LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_PARAM_TYPES = {torch.float32: 0, torch.bfloat16: 1}
 _ERRORS = {-1: "invalid argument", -2: "misaligned pointer", -3: "kernel launch failed"}
 
 _LIB: ctypes.CDLL | None = None
@@ -162,6 +160,26 @@ def load_library(build_if_missing: bool = True) -> ctypes.CDLL:
     return lib
 
 
+_UPDATE: Any = None
+
+
+def load_update(build_if_missing: bool = True) -> Any:
+    """The binding of the policy update's calls (csrc/update_binding.cpp; losses.py and
+    optim.py are its callers), built first when it is missing."""
+    global _UPDATE
+    if _UPDATE is None:
+        load_library(build_if_missing)
+        if not _build.BINDING.exists():
+            if not build_if_missing:
+                raise RuntimeError(f"cugo_b200 native binding missing: {_build.BINDING}")
+            _build.build_binding()
+        spec = importlib.util.spec_from_file_location("_cugo_b200_update", _build.BINDING)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _UPDATE = module
+    return _UPDATE
+
+
 def _check(rc: int, op: str) -> None:
     if rc != 0:
         raise RuntimeError(f"cugo_b200 {op}: {_ERRORS.get(rc, f'error {rc}')}")
@@ -193,43 +211,6 @@ def _check_states(states: torch.Tensor, state_bytes: int) -> None:
         raise RuntimeError("states must have shape [N, STATE_BYTES]")
     if states.size(1) != state_bytes:
         raise RuntimeError("states second dimension must equal STATE_BYTES")
-
-
-def _check_matrix(t: torch.Tensor, op: str, name: str, rows: int, cols: int, device: int) -> int:
-    """t [rows, >= cols] with unit column stride and rows that do not overlap, on the CUDA
-    device of that number; returns its row stride."""
-    if t.get_device() != device:
-        raise RuntimeError(f"{op}: {name} must be on the logits' device")
-    shape = t.shape
-    if len(shape) != 2 or shape[0] != rows or shape[1] < cols:
-        raise RuntimeError(f"{op}: {name} has the wrong shape")
-    ld, unit = t.stride()
-    if (unit != 1 and shape[1] > 1) or (ld < shape[1] and rows > 1):
-        raise RuntimeError(f"{op}: {name} must be row-major (unit column stride)")
-    return ld
-
-
-def _check_vector(t: torch.Tensor, op: str, name: str, n: int, dtype: torch.dtype, device: int) -> None:
-    if t.dtype != dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
-        raise RuntimeError(f"{op}: {name} must be a contiguous {dtype} tensor of {n} entries")
-    if t.get_device() != device:
-        raise RuntimeError(f"{op}: {name} must be on cuda:{device}")
-
-
-def _check_scalar(t: torch.Tensor, op: str, name: str, dtype: torch.dtype, device: int) -> None:
-    if t.dtype != dtype or t.numel() != 1 or t.get_device() != device:
-        raise RuntimeError(f"{op}: {name} must be one {dtype} value on cuda:{device}")
-
-
-def _on_device(device: int):
-    """Makes it the current device for a call's launches and allocations; most calls find
-    it so, and the update's calls are short enough for the difference to count."""
-    return nullcontext() if torch.cuda.current_device() == device else torch.cuda.device(device)
-
-
-# The number of a device's current stream, without the object around it.
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
-    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _same_device(a: torch.Tensor, b: torch.Tensor, an: str, bn: str) -> None:
@@ -601,244 +582,6 @@ class CugoB200Extension:
                 _ptr(adv), _ptr(value), value.stride(0), _ptr(ret), b, float(clip),
                 _ptr(entropy_coef), float(value_coef), _ptr(dlogits), dlogits.stride(0),
                 _ptr(dvalue), _ptr(stats), self._stream(logits.device)), "ppo_loss")
-
-    # -- losses over rows of logits ----------------------------------------------
-    @staticmethod
-    def _rows(op: str, logits, actions, legal, weight):
-        """The checks of a loss's rows: (rows, entries, the device's number, the C call's
-        leading arguments up to legal's stride, its rest up to the entries)."""
-        device = logits.get_device()
-        if device < 0:
-            raise RuntimeError(f"{op}: logits must be a CUDA tensor")
-        code = _LOGIT_TYPES.get(logits.dtype)
-        if code is None:
-            raise RuntimeError(f"{op}: logits must be fp32, bf16 or fp16")
-        shape = logits.shape
-        if len(shape) != 2 or shape[1] < 1:
-            raise RuntimeError(f"{op}: logits must be [rows, entries >= 1]")
-        rows, vocab = shape
-        ld = _check_matrix(logits, op, "logits", rows, vocab, device)
-        _check_vector(actions, op, "actions", rows, torch.int64, device)
-        legal_ptr, ldm = None, 0
-        if legal is not None:
-            if legal.dtype != torch.bool or legal.shape != shape:
-                raise RuntimeError(f"{op}: legal must be bool of the logits' shape")
-            ldm, unit = legal.stride()
-            if ldm or rows < 2:  # one mask expanded over the rows is fine
-                ldm = _check_matrix(legal, op, "legal", rows, vocab, device)
-            elif legal.get_device() != device or (unit != 1 and vocab > 1):
-                raise RuntimeError(f"{op}: legal must be row-major on the logits' device")
-            legal_ptr = legal.data_ptr()
-        weight_ptr = None
-        if weight is not None:
-            _check_vector(weight, op, "weight", rows, torch.float32, device)
-            weight_ptr = weight.data_ptr()
-        return rows, vocab, device, (logits.data_ptr(), ld, code), (legal_ptr, ldm, actions.data_ptr()), weight_ptr
-
-    def action_logp(self, logits: torch.Tensor, actions: torch.Tensor,
-                    legal: torch.Tensor | None = None, weight: torch.Tensor | None = None,
-                    entropy: bool = True, backward: bool = False, zeros: bool = False):
-        """(logp, entropy, lse, zeros) of the rows' actions (see the C declaration), fp32;
-        entropy, lse (`backward`) and zeros only where asked for, else None."""
-        rows, vocab, device, x, m, w = self._rows("action_logp", logits, actions, legal, weight)
-        with _on_device(device):
-            dev = logits.device
-            logp = torch.empty(rows, dtype=torch.float32, device=dev)
-            ent = torch.empty_like(logp) if entropy else None
-            lse = torch.empty((rows, 2), dtype=torch.float32, device=dev) if backward else None
-            zero = torch.empty_like(logp) if zeros else None
-            _check(self._lib.cugo_b200_action_logp(
-                *x, *m, w, rows, vocab, logp.data_ptr(), _ptr(ent), _ptr(lse), _ptr(zero),
-                _raw_stream(device)), "action_logp")
-        return logp, ent, lse, zero
-
-    def action_logp_backward(self, logits, actions, legal, lse, entropy, d_logp, d_entropy,
-                             scale: torch.Tensor | None = None,
-                             out: torch.Tensor | None = None) -> torch.Tensor:
-        """d loss / d logits from the gradients of action_logp's outputs (see the C
-        declaration); out: [rows, vocab] of any of the three types, else the logits' type."""
-        op = "action_logp_backward"
-        rows, vocab, device, x, m, _ = self._rows(op, logits, actions, legal, None)
-        if lse.shape != (rows, 2) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.get_device() != device:
-            raise RuntimeError(f"{op}: lse must be the forward's fp32 [rows, 2]")
-        for t, name in ((entropy, "entropy"), (d_logp, "d_logp"), (d_entropy, "d_entropy")):
-            if t is not None:
-                _check_vector(t, op, name, rows, torch.float32, device)
-        if d_entropy is not None and entropy is None:
-            raise RuntimeError(f"{op}: d_entropy needs the forward's entropy")
-        if scale is not None:
-            _check_scalar(scale, op, "scale", torch.float32, device)
-        with _on_device(device):
-            if out is None:
-                out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
-            if out.dtype not in _LOGIT_TYPES:
-                raise RuntimeError(f"{op}: out must be fp32, bf16 or fp16")
-            ldd = _check_matrix(out, op, "out", rows, vocab, device)
-            _check(self._lib.cugo_b200_action_logp_backward(
-                *x, *m, lse.data_ptr(), _ptr(entropy), _ptr(d_logp), _ptr(d_entropy), _ptr(scale), rows,
-                vocab, out.data_ptr(), ldd, _LOGIT_TYPES[out.dtype], _raw_stream(device)), op)
-        return out
-
-    def policy_loss(self, logits: torch.Tensor, actions: torch.Tensor, logp_old: torch.Tensor,
-                    adv: torch.Tensor, legal: torch.Tensor | None = None,
-                    weight: torch.Tensor | None = None, ref_logits: torch.Tensor | None = None,
-                    ref_logp: torch.Tensor | None = None, clip_low: float = 0.2,
-                    clip_high: float = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0,
-                    denominator: float = 0.0, denominator_dev: torch.Tensor | None = None,
-                    grad_scale: float = 1.0, grad_scale_dev: torch.Tensor | None = None,
-                    dlogits: torch.Tensor | None = None, grad_dtype: torch.dtype | None = None,
-                    stats: bool = True):
-        """The clipped policy loss (see the C declaration): (loss fp32 scalar, stats fp32 [8],
-        logp fp32 [rows], d loss / d logits); the gradient goes to dlogits [rows, >= vocab]
-        where given, or to a new tensor of grad_dtype where given, or is None; with
-        stats=False the gradient only.  kl_coef and entropy_coef may be one fp32 value on the
-        device."""
-        op = "policy_loss"
-        rows, vocab, device, x, m, w = self._rows(op, logits, actions, legal, weight)
-        _check_vector(logp_old, op, "logp_old", rows, torch.float32, device)
-        _check_vector(adv, op, "adv", rows, torch.float32, device)
-        ref_ptr, ldr, ref_logp_ptr = None, 0, None
-        if ref_logits is not None:
-            if ref_logits.dtype != logits.dtype or ref_logits.shape != logits.shape:
-                raise RuntimeError(f"{op}: ref_logits must have the logits' type and shape")
-            ldr = _check_matrix(ref_logits, op, "ref_logits", rows, vocab, device)
-            ref_ptr = ref_logits.data_ptr()
-        if ref_logp is not None:
-            if ref_logits is not None:
-                raise RuntimeError(f"{op}: give ref_logits or ref_logp, not both")
-            _check_vector(ref_logp, op, "ref_logp", rows, torch.float32, device)
-            ref_logp_ptr = ref_logp.data_ptr()
-        kl_dev = entropy_dev = None
-        if torch.is_tensor(kl_coef):
-            _check_scalar(kl_coef, op, "kl_coef", torch.float32, device)
-            kl_dev, kl_coef = kl_coef.data_ptr(), 1.0
-        if torch.is_tensor(entropy_coef):
-            _check_scalar(entropy_coef, op, "entropy_coef", torch.float32, device)
-            entropy_dev, entropy_coef = entropy_coef.data_ptr(), 1.0
-        if denominator_dev is not None:
-            _check_scalar(denominator_dev, op, "denominator", torch.float32, device)
-        if grad_scale_dev is not None:
-            _check_scalar(grad_scale_dev, op, "grad_scale", torch.float32, device)
-        with _on_device(device):
-            lib, dev = self._lib, logits.device
-            need = lib.cugo_b200_policy_loss_scratch_bytes(rows)
-            scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-            loss = out = logp = None
-            if stats:
-                loss = torch.empty((), dtype=torch.float32, device=dev)
-                out = torch.empty(8, dtype=torch.float32, device=dev)
-                logp = torch.empty(rows, dtype=torch.float32, device=dev)
-            grad = (None, 0, 0, vocab)
-            if dlogits is None and grad_dtype is not None:
-                dlogits = torch.empty((rows, vocab), dtype=grad_dtype, device=dev)
-            if dlogits is not None:
-                if dlogits.dtype not in _LOGIT_TYPES:
-                    raise RuntimeError(f"{op}: dlogits must be fp32, bf16 or fp16")
-                ldd = _check_matrix(dlogits, op, "dlogits", rows, vocab, device)
-                grad = (dlogits.data_ptr(), ldd, _LOGIT_TYPES[dlogits.dtype], dlogits.size(1))
-            _check(lib.cugo_b200_policy_loss(
-                *x, ref_ptr, ldr, *m, logp_old.data_ptr(), adv.data_ptr(), w, ref_logp_ptr, rows, vocab,
-                clip_low, clip_high, kl_coef, entropy_coef, kl_dev, entropy_dev, denominator,
-                _ptr(denominator_dev), grad_scale,
-                _ptr(grad_scale_dev), *grad, _ptr(logp), _ptr(out), _ptr(loss), scratch.data_ptr(), need,
-                _raw_stream(device)), op)
-        return loss, out, logp, dlogits
-
-    def preference_pairs(self, logp: torch.Tensor, ref_logp: torch.Tensor,
-                         weight: torch.Tensor | None, lse: torch.Tensor, offsets: torch.Tensor,
-                         beta: float, smoothing: float = 0.0, average: bool = False,
-                         d_logp: torch.Tensor | None = None):
-        """The preference loss from action_logp's rows (see the C declaration): (loss, margin
-        fp32 [pairs], seq_logp fp32 [2 pairs], accuracy); d_logp fp32 [rows] is written."""
-        op = "preference_loss"
-        rows, device = logp.numel(), logp.get_device()
-        if offsets.dtype != torch.int64 or offsets.dim() != 1 or offsets.numel() % 2 != 1 \
-                or not offsets.is_contiguous() or offsets.get_device() != device:
-            raise RuntimeError(f"{op}: offsets must be contiguous int64 [2 pairs + 1] on the logits' device")
-        for t, name in ((logp, "logp"), (ref_logp, "ref_logp"), (weight, "weight"), (d_logp, "d_logp")):
-            if t is not None:
-                _check_vector(t, op, name, rows, torch.float32, device)
-        if not 0.0 <= smoothing <= 1.0:
-            raise RuntimeError(f"{op}: smoothing must lie in [0, 1]")
-        pairs = offsets.numel() // 2
-        with _on_device(device):
-            dev = logp.device
-            need = self._lib.cugo_b200_preference_pairs_scratch_bytes(pairs)
-            scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-            margin = torch.empty(pairs, dtype=torch.float32, device=dev)
-            seq = torch.empty(2 * pairs, dtype=torch.float32, device=dev)
-            loss = torch.empty((), dtype=torch.float32, device=dev)
-            accuracy = torch.empty_like(loss)
-            _check(self._lib.cugo_b200_preference_pairs(
-                logp.data_ptr(), ref_logp.data_ptr(), _ptr(weight), lse.data_ptr(), offsets.data_ptr(), pairs,
-                rows, beta, smoothing, average, margin.data_ptr(), seq.data_ptr(), _ptr(d_logp),
-                loss.data_ptr(), accuracy.data_ptr(), scratch.data_ptr(), need, _raw_stream(device)), op)
-        return loss, margin, seq, accuracy
-
-    # -- the AdamW step -------------------------------------------------------------
-    def adamw(self, params: list, grads: list, exp_avgs: list, exp_avg_sqs: list,
-              step: torch.Tensor, lr, beta1: float, beta2: float, eps: float, weight_decay: float,
-              max_grad_norm: float | None, seed: int, exp_avg_scales: list | None = None,
-              exp_avg_sq_scales: list | None = None) -> torch.Tensor | None:
-        """One AdamW step over the tensors, in place (see the C declaration); returns the
-        gradients' norm (fp32 scalar) where max_grad_norm clips it, else None."""
-        op, n = "adamw", len(params)
-        eight = exp_avg_scales is not None
-        if eight and exp_avg_sq_scales is None:
-            raise RuntimeError(f"{op}: 8-bit states need both lists of scales")
-        device = step.get_device()
-        if device < 0 or step.dtype != torch.int64 or step.numel() != 1:
-            raise RuntimeError(f"{op}: step must be one int64 value on a CUDA device")
-        p_code = g_code = 0
-        p_type = g_type = torch.float32
-        if n:
-            p_type, g_type = params[0].dtype, grads[0].dtype if grads else None
-            p_code, g_code = _PARAM_TYPES.get(p_type), _PARAM_TYPES.get(g_type)
-            if p_code is None or g_code is None:
-                raise RuntimeError(f"{op}: parameters and gradients must be fp32 or bf16")
-        sizes = [t.numel() for t in params]
-        states = (torch.uint8, torch.float8_e4m3fn) if eight else (torch.float32,)
-        lists = [("params", params, (p_type,), sizes), ("grads", grads, (g_type,), sizes),
-                 ("exp_avgs", exp_avgs, states, sizes), ("exp_avg_sqs", exp_avg_sqs, states, sizes)]
-        if eight:
-            scales, counts = (torch.uint8, torch.float8_e8m0fnu), [(k + 255) // 256 for k in sizes]
-            lists += [("exp_avg_scales", exp_avg_scales, scales, counts),
-                      ("exp_avg_sq_scales", exp_avg_sq_scales, scales, counts)]
-        array, pointers = _VP * n, []
-        for name, tensors, types, counts in lists:
-            if len(tensors) != n:
-                raise RuntimeError(f"{op}: the lists must have one tensor each per parameter")
-            if [t.numel() for t in tensors] != counts:
-                raise RuntimeError(f"{op}: {name} have the wrong sizes")
-            for t in tensors:
-                if t.dtype not in types or t.get_device() != device or not t.is_contiguous():
-                    raise RuntimeError(f"{op}: {name} must be contiguous, of one type ({types}) and on cuda:{device}")
-            at = [t.data_ptr() for t in tensors]
-            if len(set(at)) != n and tensors is not grads:
-                full = [p for p, k in zip(at, counts) if k]
-                if len(set(full)) != len(full):
-                    raise RuntimeError(f"{op}: a tensor is in {name} twice")
-            pointers.append(array(*at))
-        lr_dev = None
-        if torch.is_tensor(lr):
-            _check_scalar(lr, op, "lr", torch.float32, device)
-            lr_dev, lr = lr.data_ptr(), 0.0
-        with _on_device(device):
-            dev = step.device
-            need = self._lib.cugo_b200_adamw_scratch_bytes(n)
-            scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-            norm = None
-            if max_grad_norm is not None:
-                norm = torch.empty((), dtype=torch.float32, device=dev)
-            _check(self._lib.cugo_b200_adamw(
-                n, *pointers[:4], *(pointers[4:] if eight else (None, None)), (_I64 * n)(*sizes),
-                p_code, g_code, 8 if eight else 32, lr, lr_dev, beta1, beta2, eps, weight_decay,
-                0.0 if max_grad_norm is None else max_grad_norm, seed & 0xFFFFFFFF, step.data_ptr(),
-                _ptr(norm), scratch.data_ptr(), need, _raw_stream(device)), op)
-        # The kernel writes behind torch's back: what is kept by the tensors' versions (the
-        # networks' bf16 weights, autograd's checks of saved tensors) has to see it.
-        torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
-        return norm
 
     def _colsum_scratch(self, rows: int, n: int, device: torch.device) -> torch.Tensor:
         """The per-block partial sums' buffer, one per device, grown as needed (keep

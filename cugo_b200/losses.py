@@ -23,20 +23,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
-
-from .ext import load_extension
-
-_EXT = None
-
-
-def _ext():
-    """The extension, looked up once: these calls are short enough for the look to count."""
-    global _EXT
-    if _EXT is None:
-        _EXT = load_extension()
-    return _EXT
-
+from .ext import load_update
 
 STATS = ("loss", "policy", "entropy", "kl", "kl_old", "clip_fraction", "used")
 
@@ -61,69 +48,20 @@ class PreferenceLoss(NamedTuple):
     accuracy: torch.Tensor
 
 
-class _ActionLogp(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, actions, legal):
-        logp, entropy, lse, _ = _ext().action_logp(logits, actions, legal, backward=True)
-        ctx.save_for_backward(logits, actions, legal, lse, entropy)
-        ctx.set_materialize_grads(False)
-        return logp, entropy
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_logp, d_entropy):
-        if d_logp is None and d_entropy is None:
-            return None, None, None
-        logits, actions, legal, lse, entropy = ctx.saved_tensors
-        d_logp = d_logp if d_logp is None else d_logp.contiguous()
-        d_entropy = d_entropy if d_entropy is None else d_entropy.contiguous()
-        return _ext().action_logp_backward(logits, actions, legal, lse, entropy, d_logp,
-                                                     d_entropy), None, None
-
-
 def action_logp(logits: torch.Tensor, actions: torch.Tensor,
                 legal: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(log p of each row's action, entropy of each row's distribution), fp32 [rows] each,
     differentiable in the logits."""
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _ActionLogp.apply(logits, actions, legal)
-    logp, entropy, _, _ = _ext().action_logp(logits, actions, legal)
-    return logp, entropy
+    return load_update().action_logp(logits, actions, legal)
 
 
-class _PolicyLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, actions, logp_old, adv, legal, weight, ref_logits, ref_logp, coefs):
-        loss, stats, logp, _ = _ext().policy_loss(
-            logits, actions, logp_old, adv, legal, weight, ref_logits, ref_logp, *coefs)
-        ctx.save_for_backward(logits, actions, logp_old, adv, legal, weight, ref_logits, ref_logp)
-        ctx.coefs, ctx.denominator = coefs, stats[7:]
-        stats = stats[:7]
-        ctx.mark_non_differentiable(stats, logp)
-        ctx.set_materialize_grads(False)
-        return loss, stats, logp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_loss, *_):
-        if d_loss is None:
-            return (None,) * 9
-        logits = ctx.saved_tensors[0]
-        # With the denominator that the forward found; the logits are read once more.
-        d = _ext().policy_loss(*ctx.saved_tensors, *ctx.coefs[:4], 0.0, ctx.denominator,
-                               grad_scale_dev=d_loss, grad_dtype=logits.dtype, stats=False)[3]
-        return (d,) + (None,) * 8
-
-
-def _coefs(clip_low, clip_high, kl_coef, entropy_coef, denominator):
-    clip_high = clip_low if clip_high is None else clip_high
-    if clip_low < 0.0 or clip_high < 0.0:
-        raise RuntimeError("policy_loss: the clip's bounds must not be negative")
+def _options(clip_low, clip_high, kl_coef, entropy_coef, denominator) -> tuple:
+    """The binding's arguments from the clip to the denominator (0: found from the rows)."""
     if denominator is not None and not denominator > 0.0:
         raise RuntimeError("policy_loss: the denominator must be positive")
-    kl_coef, entropy_coef = (c if torch.is_tensor(c) else float(c) for c in (kl_coef, entropy_coef))
-    return (float(clip_low), float(clip_high), kl_coef, entropy_coef,
-            0.0 if denominator is None else float(denominator))
+    kl = (1.0, kl_coef) if torch.is_tensor(kl_coef) else (kl_coef, None)
+    entropy = (1.0, entropy_coef) if torch.is_tensor(entropy_coef) else (entropy_coef, None)
+    return (clip_low, clip_low if clip_high is None else clip_high, *kl, *entropy, denominator or 0.0)
 
 
 def policy_loss(logits: torch.Tensor, actions: torch.Tensor, logp_old: torch.Tensor,
@@ -146,13 +84,9 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, logp_old: torch.Ten
     total, say).  logp_old, adv, weight, ref_logp: fp32 [rows]; clip_high defaults to
     clip_low; kl_coef and entropy_coef may be one fp32 value on the device (a schedule that a
     captured graph follows)."""
-    coefs = _coefs(clip_low, clip_high, kl_coef, entropy_coef, denominator)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return PolicyLoss(*_PolicyLoss.apply(logits, actions, logp_old, adv, legal, weight, ref_logits,
-                                             ref_logp, coefs))
-    loss, stats, logp, _ = _ext().policy_loss(logits, actions, logp_old, adv, legal, weight, ref_logits,
-                                              ref_logp, *coefs)
-    return PolicyLoss(loss, stats[:7], logp)
+    return PolicyLoss(*load_update().policy_loss(
+        logits, actions, logp_old, adv, legal, weight, ref_logits, ref_logp,
+        *_options(clip_low, clip_high, kl_coef, entropy_coef, denominator)))
 
 
 def policy_loss_grad(logits: torch.Tensor, actions: torch.Tensor, logp_old: torch.Tensor,
@@ -168,45 +102,11 @@ def policy_loss_grad(logits: torch.Tensor, actions: torch.Tensor, logp_old: torc
     autograd.  The gradient goes to dlogits [rows, >= entries] (columns past the entries
     are set to 0: the padded operand of a head's GEMM), or to a new tensor of grad_dtype
     (the logits' type)."""
-    coefs = _coefs(clip_low, clip_high, kl_coef, entropy_coef, denominator)
-    if dlogits is None:
-        grad_dtype = grad_dtype or logits.dtype
-    elif grad_dtype is not None and grad_dtype != dlogits.dtype:
-        raise RuntimeError("policy_loss: dlogits is not of grad_dtype")
-    scale, scale_dev = (1.0, grad_scale) if torch.is_tensor(grad_scale) else (float(grad_scale), None)
-    loss, stats, logp, dlogits = _ext().policy_loss(
-        logits, actions, logp_old, adv, legal, weight, ref_logits, ref_logp, *coefs, None, scale, scale_dev,
-        dlogits, grad_dtype)
-    return PolicyLoss(loss, stats[:7], logp), dlogits
-
-
-class _PreferenceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, actions, offsets, ref_logp, legal, weight, options):
-        out, lse, d_logp = _preference(logits, actions, offsets, ref_logp, legal, weight, options, True)
-        ctx.save_for_backward(logits, actions, legal, lse, d_logp)
-        ctx.mark_non_differentiable(*out[1:])
-        ctx.set_materialize_grads(False)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_loss, *_):
-        if d_loss is None:
-            return (None,) * 7
-        logits, actions, legal, lse, d_logp = ctx.saved_tensors
-        d = _ext().action_logp_backward(logits, actions, legal, lse, None, d_logp, None,
-                                                  scale=d_loss)
-        return (d,) + (None,) * 6
-
-
-def _preference(logits, actions, offsets, ref_logp, legal, weight, options, grad):
-    """((loss, margin, sequences' log p, accuracy), and what the backward needs)."""
-    ext = _ext()
-    logp, _, lse, d_logp = ext.action_logp(logits, actions, legal, weight, entropy=False,
-                                           backward=True, zeros=grad)
-    return ext.preference_pairs(logp, ref_logp, weight, lse, offsets, *options,
-                                d_logp=d_logp), lse, d_logp
+    scale, scale_dev = (1.0, grad_scale) if torch.is_tensor(grad_scale) else (grad_scale, None)
+    loss, stats, logp, grad = load_update().policy_loss_grad(
+        logits, actions, logp_old, adv, legal, weight, ref_logits, ref_logp,
+        *_options(clip_low, clip_high, kl_coef, entropy_coef, denominator), scale, scale_dev, grad_dtype, dlogits)
+    return PolicyLoss(loss, stats, logp), grad
 
 
 def preference_loss(logits: torch.Tensor, actions: torch.Tensor, offsets: torch.Tensor,
@@ -227,9 +127,5 @@ def preference_loss(logits: torch.Tensor, actions: torch.Tensor, offsets: torch.
       loss = mean of -(1 - label_smoothing) log sigmoid(m) - label_smoothing log sigmoid(-m)
 
     A margin needs all its rows first, so the backward reads the logits a second time."""
-    options = (float(beta), float(label_smoothing), bool(average))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return PreferenceLoss(*_PreferenceLoss.apply(logits, actions, offsets, ref_logp, legal, weight,
-                                                     options))
-    out, _, _ = _preference(logits, actions, offsets, ref_logp, legal, weight, options, False)
-    return PreferenceLoss(*out)
+    return PreferenceLoss(*load_update().preference_loss(logits, actions, offsets, ref_logp, legal, weight,
+                                                         beta, label_smoothing, average))

@@ -18,7 +18,7 @@ from typing import Any, Iterable
 
 import torch
 
-from .ext import load_extension
+from .ext import load_update
 
 _STATES = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
 
@@ -41,14 +41,9 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor],
     ceil(size / 256) each), e4m3 codes (uint8 or float8_e4m3fn).  States start as zeros.  lr:
     a number, or one fp32 value on the device.  A norm that is infinite or NaN makes the
     step NaN, as clip_grad_norm_ does."""
-    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
-        raise RuntimeError(f"adamw: betas = {betas} is out of range")
-    for name, value in (("lr", lr), ("eps", eps), ("weight_decay", weight_decay), ("max_grad_norm", max_grad_norm)):
-        if value is not None and not torch.is_tensor(value) and not value >= 0.0:
-            raise RuntimeError(f"adamw: {name} = {value} is out of range")
-    return load_extension().adamw(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas[0], betas[1],
-                                  eps, weight_decay, max_grad_norm, seed, exp_avg_scales,
-                                  exp_avg_sq_scales)
+    rate = (0.0, lr) if torch.is_tensor(lr) else (lr, None)
+    return load_update().adamw(params, grads, exp_avgs, exp_avg_sqs, step, *rate, *betas, eps, weight_decay,
+                               max_grad_norm, seed, exp_avg_scales, exp_avg_sq_scales)
 
 
 class AdamW(torch.optim.Optimizer):

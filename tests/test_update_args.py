@@ -7,7 +7,6 @@ import ctypes
 import pytest
 import torch
 
-from cugo_b200 import ext as ext_mod
 from cugo_b200 import load_library
 
 OK, ARG, ALIGN, CAPACITY = 0, -1, -2, -4
@@ -17,11 +16,6 @@ P = 0x10000
 @pytest.fixture(scope="module")
 def lib():
     return load_library()
-
-
-@pytest.fixture()
-def cpu_ext(lib):
-    return ext_mod.CugoB200Extension(lib)
 
 
 def _logp(lib, logits=P, ld=180, dtype=0, legal=None, ldm=0, actions=P, weight=None, rows=8, vocab=179,
@@ -153,14 +147,16 @@ def test_adamw_arguments(lib):
     assert _adamw(lib, nbytes=q(3) - 1) == CAPACITY
 
 
-def test_tensors_off_the_gpu_are_refused(cpu_ext):
+def test_tensors_off_the_gpu_are_refused():
+    from cugo_b200 import losses, optim
     x, i, f = torch.zeros((4, 9)), torch.zeros(4, dtype=torch.int64), torch.zeros(4)
-    with pytest.raises(RuntimeError, match="logits must be a CUDA tensor"):
-        cpu_ext.action_logp(x, i)
-    with pytest.raises(RuntimeError, match="logits must be a CUDA tensor"):
-        cpu_ext.policy_loss(x, i, f, f)
+    for call in (lambda: losses.action_logp(x, i), lambda: losses.policy_loss(x, i, f, f),
+                 lambda: losses.policy_loss_grad(x, i, f, f), lambda: losses.preference_loss(x, i, i[:1], f),
+                 lambda: losses.action_logp(x.clone().requires_grad_(), i)):
+        with pytest.raises(RuntimeError, match="logits must be a CUDA tensor"):
+            call()
     with pytest.raises(RuntimeError, match="step must be one int64 value on a CUDA device"):
-        cpu_ext.adamw([f], [f], [f], [f], i[:1], 1e-3, 0.9, 0.99, 1e-8, 0.0, None, 0)
+        optim.adamw_step([f], [f], [f], [f], i[:1])
 
 
 def test_optimizer_groups_are_checked():

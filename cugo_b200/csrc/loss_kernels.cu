@@ -4,11 +4,13 @@
 // KL term (policy_loss), and the preference loss over pairs of sequences
 // (preference_pairs, on action_logp's rows).
 //
-// Mathematics of one row.  With x the logits, all sums run in base 2 and relative to the
-// row's maximum M:
-//   y_j = x_j log2(e) - M log2(e)   (one FMA; its rounding is the only one, so p_j keeps
-//                                    fp32's relative accuracy however large x is)
+// Mathematics of one row.  With x the logits, all sums run in base 2 and relative to
+// M = ceil(max x log2(e)), a whole number:
+//   y_j = x_j log2(e) - M   (one FMA; its rounding is the only one, so p_j keeps fp32's
+//                            relative accuracy however large x is)
 //   s = sum 2^y_j,  t = sum 2^y_j y_j,  log2 p_j = y_j - log2 s,  H = ln 2 (log2 s - t/s)
+// Parts of a row that have other maxima are brought together by powers of two, without a
+// rounding.
 // A reference row z_j (M', s') adds u = sum 2^y_j (y_j - z_j):
 //   KL(p|q) = ln 2 (u/s - log2 s + log2 s').
 // Every gradient wanted here is, with 1 at the taken action a,
@@ -17,9 +19,9 @@
 //
 // An illegal entry counts as -2^30, and so does every entry below that (-inf, -1e30, a mask
 // of the type's lowest value): its 2^y is 0 beside any other entry and every product
-// stays finite, so no entry needs a branch.  (M log2(e) is off by at most 2^-24 of itself,
-// the same for the whole row: below 2^31 that shifts y by less than 128, which the sums
-// bear.  The bound is a power of two, so that it has no such rounding itself.)  What
+// stays finite, so no entry needs a branch.  (M, as a float, is off by at most 2^-24 of
+// itself, the same for the whole row: below 2^31 that shifts y by less than 128, which the
+// sums bear.  The bound is a power of two, so that its own product is exact.)  What
 // stands in an illegal place (NaN, infinities) is never used; NaN in a legal place stays
 // NaN.  Sums over rows are taken in 64 bits, per warp or block, and
 // added over the blocks in order: the same result on every run.
@@ -52,6 +54,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+
+// A maximum in base-2 units, up to a whole number.
+__device__ __forceinline__ float base2(float x) { return ceilf(x * kLog2e); }
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -165,33 +170,13 @@ struct Coefs {
   float hot, c0, c1, c2;
 };
 
-// The sums of a row, or of a part of one (maxima in base-2 units).
+// The sums of a row, or of a part of one.
 struct Sums {
-  float m, s, t;    // maximum, sum 2^y, sum 2^y y
-  float mr, sr, u;  // the reference's maximum and sum, sum 2^y (y - z)
+  float m, s, t;    // M, sum 2^y, sum 2^y y
+  float mr, sr, u;  // the reference's, and sum 2^y (y - z)
 };
 
 __device__ __forceinline__ Sums no_sums() { return {kMasked2, 0.0f, 0.0f, kMasked2, 0.0f, 0.0f}; }
-
-// Two parts' sums brought to their common maxima and added.
-template <bool kRef>
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-  Sums r;
-  r.m = max_nan(a.m, b.m);
-  const float da = a.m - r.m, db = b.m - r.m;
-  const float fa = exp2_fast(da), fb = exp2_fast(db);
-  r.s = a.s * fa + b.s * fb;
-  r.t = fa * (a.t + da * a.s) + fb * (b.t + db * b.s);
-  r.mr = kMasked2;
-  r.sr = r.u = 0.0f;
-  if constexpr (kRef) {
-    r.mr = max_nan(a.mr, b.mr);
-    const float ra = a.mr - r.mr, rb = b.mr - r.mr;
-    r.sr = a.sr * exp2_fast(ra) + b.sr * exp2_fast(rb);
-    r.u = fa * (a.u + (da - ra) * a.s) + fb * (b.u + (db - rb) * b.s);
-  }
-  return r;
-}
 
 __device__ __forceinline__ float warp_max_nan(float v) {
   float r;
@@ -305,19 +290,36 @@ __device__ __forceinline__ RowInputs row_inputs(const Rows& r, const Policy& a, 
   return in;
 }
 
-// log p of an entry.  kLog2e is log2(e) (1 - 1.335e-8): the sums are those of the logits
-// times that, and d log p / d (a factor of the logits) = x_a - mean x, so to first order
-// the factor comes out by one more FMA.
-__device__ __forceinline__ float log_prob(float y_a, float log_s, float mean_y) {
-  return kLn2 * fmaf(1.335e-8f, y_a - mean_y, y_a - log_s);
+// log2(s) of a positive s as a whole number and the logarithm of what lies in [3/4, 3/2):
+// each is exact to its own size, which their sum is not.
+struct Log2 {
+  float whole, part;
+};
+
+__device__ __forceinline__ Log2 split_log2(float s) {
+  const int bits = __float_as_int(s), k = (bits - 0x3f400000) >> 23;
+  return {static_cast<float>(k), log2f(__int_as_float(bits - (k << 23)))};
+}
+
+// log p of an entry x_a: x_a - ln 2 (M + log2 s), the large terms in 64 bits and one rounding
+// at the end (log p of long sequences are added up, so what is alike in every row counts).
+// For the same reason two small things that are known come out again: kLog2e is log2(e)
+// (1 - kLow), which makes log Z less by that share of the mean logit, and 2^y as the
+// hardware has it is 3.0e-8 of itself too small in the mean (over [-24, 0), by value).
+__device__ __forceinline__ float log_prob(float x_a, const Sums& v, const Log2& log_s, float mean_y) {
+  constexpr double kLn2d = 0.693147180559945309, kLow = 1.0 - kLn2d * kLog2e, kHardware = 3.0e-8;
+  const double m = v.m;
+  const double log_z = kLn2d * (m + log_s.whole + log_s.part + kLow * (m + mean_y)) + kHardware;
+  return static_cast<float>(x_a - log_z);
 }
 
 // A row's outputs in action_logp.
-__device__ __forceinline__ void store_score(const Score& o, i64 row, bool used, const Sums& v, float y_a) {
-  const float log_s = used ? log2f(v.s) : INFINITY, mean_y = __fdividef(v.t, v.s);
-  if (o.logp) o.logp[row] = used ? log_prob(y_a, log_s, mean_y) : 0.0f;
-  if (o.entropy) o.entropy[row] = used ? kLn2 * (log_s - mean_y) : 0.0f;
-  if (o.lse) o.lse[row] = make_float2(used ? v.m : 0.0f, log_s);
+__device__ __forceinline__ void store_score(const Score& o, i64 row, bool used, const Sums& v, float x_a) {
+  const Log2 log_s = split_log2(v.s);
+  const float mean_y = __fdividef(v.t, v.s);
+  if (o.logp) o.logp[row] = used ? log_prob(x_a, v, log_s, mean_y) : 0.0f;
+  if (o.entropy) o.entropy[row] = used ? kLn2 * (log_s.whole + (log_s.part - mean_y)) : 0.0f;
+  if (o.lse) o.lse[row] = used ? make_float2(v.m, log_s.whole + log_s.part) : make_float2(0.0f, INFINITY);
   if (o.zeros) o.zeros[row] = 0.0f;
 }
 
@@ -330,13 +332,14 @@ struct Terms {
   }
 };
 
-// A row's loss terms and its gradient's coefficients, from its sums and its action's y.
+// A row's loss terms and its gradient's coefficients, from its sums and its action's entry.
 template <bool kRef>
-__device__ __forceinline__ Coefs policy_row(const Policy& a, const RowInputs& in, const Sums& v, float y_a,
+__device__ __forceinline__ Coefs policy_row(const Policy& a, const RowInputs& in, const Sums& v, float x_a,
                                             float scale, Terms& terms, float& logp) {
-  const float log_s = log2f(v.s), inv_s = 1.0f / v.s, mean_y = v.t * inv_s;
-  logp = log_prob(y_a, log_s, mean_y);
-  const float entropy = kLn2 * (log_s - mean_y), w = in.weight;
+  const Log2 log_s = split_log2(v.s);
+  const float inv_s = 1.0f / v.s, mean_y = v.t * inv_s, w = in.weight;
+  logp = log_prob(x_a, v, log_s, mean_y);
+  const float entropy = kLn2 * (log_s.whole + (log_s.part - mean_y));
   const float log_ratio = logp - in.logp_old;
   const float ratio = expf(log_ratio), adv = in.adv;
   const float bounded = ratio < a.low ? a.low : ratio > a.high ? a.high : ratio;
@@ -347,7 +350,7 @@ __device__ __forceinline__ Coefs policy_row(const Policy& a, const RowInputs& in
   float kl = 0.0f, mean_d = 0.0f, c2 = 0.0f;
   if constexpr (kRef) {
     mean_d = v.u * inv_s;
-    kl = kLn2 * (mean_d - log_s + log2f(v.sr));
+    kl = kLn2 * (mean_d - (log_s.whole + log_s.part) + log2f(v.sr));
     c2 = a.kl_coef * kLn2;
   } else if (a.ref_logp) {
     const float d = in.ref_logp - logp, e = expm1f(d);
@@ -566,8 +569,8 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
       if constexpr (kRef) top_r = max_nan(top_r, z[k], z[k + 1]);
     }
     Sums v;
-    v.m = max_lanes<kLanes>(top) * kLog2e;
-    v.mr = kRef ? max_lanes<kLanes>(top_r) * kLog2e : 0.0f;
+    v.m = base2(max_lanes<kLanes>(top));
+    v.mr = kRef ? base2(max_lanes<kLanes>(top_r)) : 0.0f;
     const Two unit = two(kLog2e, kLog2e), from = two(-v.m, -v.m), from_r = two(-v.mr, -v.mr);
     Two s2 = two(0.0f, 0.0f), t2 = s2, sr2 = s2, u2 = s2;
 #pragma unroll
@@ -595,15 +598,14 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
       v.sr = sum_lanes<kLanes>(both(sr2));
       v.u = sum_lanes<kLanes>(both(u2));
     }
-    const float y_a = fmaf(x_a, kLog2e, -v.m);
     if constexpr (!kPolicy) {
-      if (l == 0 && real) store_score(o, row, used, v, y_a);
+      if (l == 0 && real) store_score(o, row, used, v, x_a);
     } else {
       Coefs c{0.0f, 0.0f, 0.0f, 0.0f};
       float logp = 0.0f;
       if (used) {
         Terms terms;
-        c = policy_row<kRef>(a, in, v, y_a, scale, terms, logp);
+        c = policy_row<kRef>(a, in, v, x_a, scale, terms, logp);
         if (l == 0) terms.add_to(acc, in.weight);
       }
       if (a.logp && l == 0 && real) a.logp[row] = logp;
@@ -623,6 +625,7 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
         float hot = 0.0f;
         const bool mine = used && l == action % kLanes;
         if (mine) {
+          const float y_a = fmaf(x_a, kLog2e, -v.m);
           hot = fmaf(c.c1, y_a, c.c0);
           if constexpr (kRef) {
             const float z_a = fmaf(max_nan(to_float(z_row[action]), kMasked), kLog2e, -v.mr);
@@ -837,23 +840,28 @@ struct Running {
   Two s, t, sr, u;
 };
 
-// New maxima (base-2 units) where they are larger, also for NaN.
+__device__ __forceinline__ Running nothing_yet() {
+  const Two zero = two(0.0f, 0.0f);
+  return {kMasked2, kMasked2, zero, zero, zero, zero};
+}
+
+// New maxima (in base-2 units) where they are larger, also for NaN.
 template <bool kRef>
-__device__ __forceinline__ void raise(Running& v, float top, float top_r) {
-  if (!(top <= v.m)) {
-    const float d = v.m - top, f = exp2_fast(d);
+__device__ __forceinline__ void raise(Running& v, float m, float mr) {
+  if (!(m <= v.m)) {
+    const float d = v.m - m, f = exp2_fast(d);
     const Two dd = two(d, d), ff = two(f, f);
     v.t = mul(ff, fma(dd, v.s, v.t));
     if constexpr (kRef) v.u = mul(ff, fma(dd, v.s, v.u));
     v.s = mul(v.s, ff);
-    v.m = top;
+    v.m = m;
   }
   if constexpr (kRef) {
-    if (!(top_r <= v.mr)) {
-      const float d = v.mr - top_r, f = exp2_fast(d);
+    if (!(mr <= v.mr)) {
+      const float d = v.mr - mr, f = exp2_fast(d);
       v.u = fma(two(-d, -d), v.s, v.u);
       v.sr = mul(v.sr, two(f, f));
-      v.mr = top_r;
+      v.mr = mr;
     }
   }
 }
@@ -885,7 +893,7 @@ __device__ __forceinline__ void accumulate(Running& v, const float (&x)[kN], con
 template <typename T, bool kRef, int kCount>
 __device__ __forceinline__ void add_vectors(Running& v, const uint4 (&x)[kCount], const uint4 (&z)[kCount]) {
   constexpr int kN = kVec<T>;
-  raise<kRef>(v, extreme<T, true>(x) * kLog2e, kRef ? extreme<T, true>(z) * kLog2e : kMasked2);
+  raise<kRef>(v, base2(extreme<T, true>(x)), kRef ? base2(extreme<T, true>(z)) : kMasked2);
 #pragma unroll
   for (int k = 0; k < kCount; ++k) {
     float f[kN], q[kN];
@@ -910,7 +918,7 @@ __device__ __noinline__ void add_masked(Running& v, const Part<T>& p, int tid, i
     float f[kN], q[kN];
     p.masked(i, __ldg(p.vector(i)), f);
     if constexpr (kRef) p.masked(i, p.ref_vector(i), q);
-    raise<kRef>(v, largest(f) * kLog2e, kRef ? largest(q) * kLog2e : kMasked2);
+    raise<kRef>(v, base2(largest(f)), kRef ? base2(largest(q)) : kMasked2);
     accumulate<kRef>(v, f, q);
   }
 }
@@ -1133,9 +1141,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kWideThreads ? 2 : 3)
       row_x = p.one(p.x, action);
     }
     bool careful = p.lm != nullptr;
-    Running run;
-    run.m = run.mr = kMasked2;
-    run.s = run.t = run.sr = run.u = two(0.0f, 0.0f);
+    Running run = nothing_yet();
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       if (write && c > 0) wait_copies<0>();
@@ -1186,10 +1192,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == kWideThreads ? 2 : 3)
     }
     for (;;) {
       if (careful) {
-        run.m = run.mr = kMasked2;
-        run.s = run.t = run.sr = run.u = two(0.0f, 0.0f);
         // Copies for the call: what its arguments point to would leave the registers.
-        Running masked = run;
+        Running masked = nothing_yet();
         const Part<T> part = p;
         add_masked<T, kRef>(masked, part, tid, step);
         run = masked;
@@ -1201,7 +1205,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kWideThreads ? 2 : 3)
         const float f[2] = {p.one(p.x, c), kMasked};
         float q[2] = {kMasked, kMasked};
         if constexpr (kRef) q[0] = p.one(p.z, c);
-        raise<kRef>(run, f[0] * kLog2e, q[0] * kLog2e);
+        raise<kRef>(run, base2(f[0]), base2(q[0]));
         accumulate<kRef>(run, f, q);
       }
       Sums v = no_sums();
@@ -1230,15 +1234,14 @@ __global__ void __launch_bounds__(kThreads, kThreads == kWideThreads ? 2 : 3)
         result.again = !careful && !(fabsf(sum) < INFINITY);
         const RowInputs in = row_in;
         const bool used = !(row_x <= kMasked);
-        const float y_a = fmaf(row_x, kLog2e, -v.m);
         if (!result.again) {
           if constexpr (!kPolicy) {
-            if (rank == 0) store_score(o, row, used, v, y_a);
+            if (rank == 0) store_score(o, row, used, v, row_x);
           } else {
             float logp = 0.0f;
             if (used) {
               Terms terms;
-              result.c = policy_row<kRef>(a, in, v, y_a, scale, terms, logp);
+              result.c = policy_row<kRef>(a, in, v, row_x, scale, terms, logp);
               if (rank == 0) terms.add_to(block_acc, in.weight);
             }
             if (a.logp && rank == 0) a.logp[row] = logp;

@@ -69,7 +69,6 @@ struct Tensors {
 // What the step's scalars come to, written by prepare_kernel.
 struct Scalars {
   float clip;       // c
-  float c1;         // c (1 - b1)
   float step_size;  // lr / (1 - b1^t)
   float keep;       // 1 - lr wd
   float root;       // 1 / sqrt(1 - b2^t)
@@ -228,9 +227,9 @@ __device__ __forceinline__ int scale_byte(float largest) {
 }
 
 // The magnitude a (at most 448) rounded to e4m3's grid, up where the random number r says
-// so: 16 bits, as a share of a step, from bit 4 on (what stands below counts for less than
-// 2^-16 of a step).  Below 2^-6 the steps are 2^-9, which 2^-6 more brings to the same
-// place; above they are 1/8 of the power of two.
+// so: 16 bits, as a share of a step, from bit 4 on, and half of the last.  Below 2^-6 the
+// steps are 2^-9, which 2^-6 more brings to the same place; above they are 1/8 of the
+// power of two.
 __device__ __forceinline__ float round_e4m3(float a, uint32_t r) {
   float small;  // 1 below 2^-6, else 0
   asm("set.lt.f32.f32 %0, %1, %2;" : "=f"(small) : "f"(a), "f"(0.015625f));
@@ -303,6 +302,16 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
   return r;
 }
 
+// a + b, the products before them already rounded: the assembler merges a packed product
+// and a packed sum into one that is not, so the sum is taken apart.
+__device__ __forceinline__ void sum(Two a, Two b, float& x, float& y) {
+  float ax, ay, bx, by;
+  split(a, ax, ay);
+  split(b, bx, by);
+  x = __fadd_rn(ax, bx);
+  y = __fadd_rn(ay, by);
+}
+
 // Where a thread's 8 elements and its warp's scales are, and the first element's number.
 template <typename P>
 struct Place {
@@ -332,14 +341,21 @@ __device__ __forceinline__ void step8(const Place<P>& at, const Options& o, cons
     b1 *= scale_of(ms);
     b2 *= scale_of(vs);
   }
-  const Two c1 = two(s.c1, s.c1), clip = two(s.clip, s.clip), c2 = two(o.c2, o.c2), d1 = two(b1, b1), d2 = two(b2, b2),
+  const Two c1 = two(o.c1, o.c1), clip = two(s.clip, s.clip), c2 = two(o.c2, o.c2), d1 = two(b1, b1), d2 = two(b2, b2),
             keep = two(s.keep, s.keep);
   float nan = 0.0f;  // NaN where a parameter is after the step
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
-    const Two gg = two(g[e], g[e + 1]), q = mul(gg, clip);
-    split(fma2(two(m[e], m[e + 1]), d1, mul(gg, c1)), m[e], m[e + 1]);
-    split(fma2(two(v[e], v[e + 1]), d2, mul(mul(q, q), c2)), v[e], v[e + 1]);
+    const Two q = mul(two(g[e], g[e + 1]), clip), mm = two(m[e], m[e + 1]), vv = two(v[e], v[e + 1]);
+    if constexpr (kEight) {
+      // Every product rounded, as the formula is written: which way a state's code goes is
+      // then a matter of the formula, and not of how it was compiled.
+      sum(mul(mm, d1), mul(q, c1), m[e], m[e + 1]);
+      sum(mul(vv, d2), mul(mul(q, q), c2), v[e], v[e + 1]);
+    } else {
+      split(fma2(mm, d1, mul(q, c1)), m[e], m[e + 1]);
+      split(fma2(vv, d2, mul(mul(q, q), c2)), v[e], v[e + 1]);
+    }
     split(mul(two(p[e], p[e + 1]), keep), p[e], p[e + 1]);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -388,9 +404,9 @@ __device__ __forceinline__ void step8(const Place<P>& at, const Options& o, cons
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t high = x[e] >> 16;
-      const float q = round_e4m3(fabsf(cm[e]), ((x[e] ^ high) & 0xffffu) * 16u);
+      const float q = round_e4m3(fabsf(cm[e]), ((x[e] ^ high) & 0xffffu) * 16u + 8u);
       cm[e] = __uint_as_float(__float_as_uint(q) | (__float_as_uint(cm[e]) & 0x80000000u));
-      cv[e] = round_e4m3(cv[e], x[e] >> 12);
+      cv[e] = round_e4m3(cv[e], ((x[e] >> 12) & 0xffff0u) | 8u);
     }
     if (low < 0.001953125f) {  // 2^-9: a second moment above 0 does not become 0
 #pragma unroll
@@ -544,7 +560,8 @@ __global__ void __launch_bounds__(kThreads, 3) adamw8_kernel(const __grid_consta
   }
 }
 
-// Sums of the gradients' squares: 8 in fp32 per thread and block, from there in 64 bits.
+// Sums of the gradients' squares, in 64 bits from the squares on (exact there), so that the
+// norm, and with it every rounding of a clipped step, does not hang on the order.
 template <typename G, int kMost>
 __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Tensors<kMost> a, double* partial) {
   __shared__ double part[kThreads / 32];
@@ -556,12 +573,11 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ 
 #pragma unroll 2
     for (int u = 0; u < a.per_warp; ++u) {
       const i64 i = (first + u) * kBlock + (threadIdx.x & 31) * kPer;
-      float g[8], q = 0.0f;
+      float g[8];
       if (t.wide && i + kPer <= t.n) load8<true>(at + i, 8, g);
       else load8<false>(at + i, t.n - i < 8 ? static_cast<int>(t.n - i) : 8, g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) q = fmaf(g[e], g[e], q);
-      sum += q;
+      for (int e = 0; e < 8; ++e) sum = fma(static_cast<double>(g[e]), static_cast<double>(g[e]), sum);
     }
   }
   sum = sum_warp(sum);
@@ -600,7 +616,6 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const Options o, cons
   s.step_size = static_cast<float>(lr / (1.0 - pow(o.beta1, static_cast<double>(t))));
   s.keep = static_cast<float>(1.0 - lr * o.decay);
   s.root = static_cast<float>(1.0 / sqrt(1.0 - pow(o.beta2, static_cast<double>(t))));
-  s.c1 = s.clip * o.c1;
   s.key = mix(o.seed + static_cast<uint32_t>(t) * 0x9e3779b9u);
   *scalars = s;
 }

@@ -427,11 +427,12 @@ __device__ void store_partial(const Policy& a, const double (&acc)[kSums]) {
 //
 // Lane l of a row's kLanes holds entries l, l + kLanes, ..., kPer of them.  A warp takes
 // 32 / kLanes consecutive rows: few entries per lane would leave the row's reductions and
-// its one logarithm to most of the time.  Rows that lie one after another (a stride of
-// little more than the entries) are copied as one run of 16-byte vectors into the warp's
-// own shared memory, the next rows' while these are computed, so the loads are wide and in
-// flight however the rows are aligned (a row of 179 fp32 starts at any multiple of 4
-// bytes); the gradient leaves the same way.  Other rows (kStaged false) are read in place.
+// its one logarithm to most of the time.  Rows are copied by 16-byte vectors into the
+// warp's own shared memory, the next rows' while these are computed, so the loads are wide
+// and in flight however the rows are aligned (a row of 179 fp32 starts at any multiple of 4
+// bytes): as one run where they lie one after another (a stride of little more than the
+// entries), else each by itself.  A gradient whose rows lie one after another leaves the
+// same way.
 
 constexpr int kShortWarps = 4;
 
@@ -459,14 +460,21 @@ __device__ __forceinline__ void copy_run(char* to, const char* from, int bytes, 
   }
 }
 
-// The warp's shared memory, in bytes (multiples of 16): two stages, one gradient.
+// The warp's shared memory: two stages, one gradient.  Sizes in bytes, multiples of 16.
 struct Layout {
   int logits, ref, legal, grad;
+  // Row q of a stage stands q pitches behind the first: of a run, at the first row's address
+  // mod 16; of rows `apart`, at its own.
+  bool apart;
+  int pitch, pitch_ref, pitch_legal;
   __host__ __device__ int stage() const { return logits + ref + legal; }
   __host__ __device__ int warp() const { return 2 * stage() + grad; }
 };
 
-template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy, bool kStaged>
+template <typename V>
+__device__ __forceinline__ int skip16(const V* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p)) & 15; }
+
+template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy>
 __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
     short_rows_kernel(const Rows r, const Score o, const Policy given, const Layout lay) {
   const Policy a = kPolicy ? resolved(given) : given;
@@ -481,28 +489,37 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
   const i64 stride = (i64)gridDim.x * kShortWarps * kRows;
   i64 first = ((i64)blockIdx.x * kShortWarps + warp) * kRows;
 
-  // Where the rows of this warp's turn begin, and how far its next turn is; of staged rows
-  // the turn after, whose copies are started, too.
+  // One mask for all rows stays where the first two turns put it.
+  const bool own_masks = r.legal && r.ldm != 0, one_mask = r.legal && r.ldm == 0;
+
+  // Where the rows of this warp's turn begin, and how far its next turn is.
   const T* x_first = static_cast<const T*>(r.logits) + first * r.ld;
   const T* z_first = kRef ? static_cast<const T*>(r.ref) + first * r.ldr : nullptr;
   const bool* m_first = r.legal + first * r.ldm;
   const i64 x_step = stride * r.ld, z_step = kRef ? stride * r.ldr : 0, m_step = stride * r.ldm;
-  const int ld = static_cast<int>(r.ld), ldr = static_cast<int>(r.ldr), ldm = static_cast<int>(r.ldm);
-  const auto skip = [](const void* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p)) & 15; };
   const auto fetch = [&](i64 row, const T* x, const T* z, const bool* m, int at) {
-    if constexpr (kStaged) {
-      constexpr int kGap = kRows > 1 ? 64 : 0, kSize = sizeof(T);
-      const int n = r.rows - row < kRows ? static_cast<int>(r.rows - row) - 1 : kRows - 1;
-      char* to = shared + own + at * lay.stage();
-      constexpr int kMost = kRows * (kLanes * kPer * kSize + kGap);
-      copy_run<kMost>(to, reinterpret_cast<const char*>(x), (n * ld + vocab) * kSize, lane);
-      if constexpr (kRef)
-        copy_run<kMost>(to + lay.logits, reinterpret_cast<const char*>(z), (n * ldr + vocab) * kSize, lane);
-      if (r.legal)
-        copy_run<kRows * (kLanes * kPer + kGap)>(to + lay.logits + lay.ref, reinterpret_cast<const char*>(m),
-                                                 n * ldm + vocab, lane);
-      asm volatile("cp.async.commit_group;" ::: "memory");
+    constexpr int kGap = kRows > 1 ? 64 : 0, kRow = kLanes * kPer, kSize = sizeof(T);
+    constexpr int kRun = kRows * (kRow * kSize + kGap);
+    const int n = r.rows - row < kRows ? static_cast<int>(r.rows - row) - 1 : kRows - 1;
+    char* const to = shared + own + at * lay.stage();
+    const auto from = [](const auto* p) { return reinterpret_cast<const char*>(p); };
+    if (!lay.apart) {
+      copy_run<kRun>(to, from(x), n * lay.pitch + vocab * kSize, lane);
+      if constexpr (kRef) copy_run<kRun>(to + lay.logits, from(z), n * lay.pitch_ref + vocab * kSize, lane);
+      if (own_masks)
+        copy_run<kRows * (kRow + kGap)>(to + lay.logits + lay.ref, from(m), n * lay.pitch_legal + vocab, lane);
+    } else {
+#pragma unroll 1
+      for (int q = 0; q <= n; ++q) {
+        copy_run<kRow * kSize>(to + q * lay.pitch, from(x + q * r.ld), vocab * kSize, lane);
+        if constexpr (kRef)
+          copy_run<kRow * kSize>(to + lay.logits + q * lay.pitch_ref, from(z + q * r.ldr), vocab * kSize, lane);
+        if (own_masks)
+          copy_run<kRow>(to + lay.logits + lay.ref + q * lay.pitch_legal, from(m + q * r.ldm), vocab, lane);
+      }
     }
+    if (one_mask && row < 2 * stride) copy_run<kRow>(to + lay.logits + lay.ref, from(m), vocab, lane);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
   RowInputs next;
@@ -516,26 +533,23 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
     if (first + stride < r.rows) {
       fetch(first + stride, x_first + x_step, z_first + z_step, m_first + m_step, at ^ 1);
       next = row_inputs<kPolicy>(r, a, first + stride + sub < r.rows ? first + stride + sub : r.rows - 1);
-      if constexpr (kStaged) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    } else if constexpr (kStaged) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     __syncwarp();
     const bool real = first + sub < r.rows;
     const int back = real ? sub : static_cast<int>(r.rows - 1 - first);  // the row's place in the run
     const i64 row = first + back;
-    const int stage = own + at * lay.stage();
-    const T *x, *z_row = nullptr;
-    const bool* lm;
-    if constexpr (kStaged) {
-      x = reinterpret_cast<const T*>(shared + stage + skip(x_first)) + back * ld;
-      if constexpr (kRef) z_row = reinterpret_cast<const T*>(shared + stage + lay.logits + skip(z_first)) + back * ldr;
-      lm = reinterpret_cast<const bool*>(shared + stage + lay.logits + lay.ref + skip(m_first)) + back * ldm;
-    } else {
-      x = x_first + back * r.ld;
-      if constexpr (kRef) z_row = z_first + back * r.ldr;
-      lm = m_first + back * r.ldm;
-    }
+    const int stage = own + at * lay.stage(), place = lay.apart ? back : 0;
+    const T* const x =
+        reinterpret_cast<const T*>(shared + stage + back * lay.pitch + skip16(x_first + place * r.ld));
+    const T* z_row = nullptr;
+    if constexpr (kRef)
+      z_row = reinterpret_cast<const T*>(shared + stage + lay.logits + back * lay.pitch_ref +
+                                         skip16(z_first + place * r.ldr));
+    const bool* const lm = reinterpret_cast<const bool*>(shared + stage + lay.logits + lay.ref + back * lay.pitch_legal +
+                                                         skip16(m_first + place * r.ldm));
     bool used = real && in.weight != 0.0f && in.action >= 0 && in.action < vocab;
     const int action = used ? static_cast<int>(in.action) : 0;
     float x_a = max_nan(to_float(x[action]), kMasked);
@@ -543,21 +557,20 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
     used = used && !(x_a <= kMasked);
 
     float y[kPer], z[kPer], e[kPer];
-    // Entry l + kLanes k lies in the row where behind < -kLanes k.  A staged row may be
-    // read past its end (the stage is that long); what stands there is not used.
+    // Entry l + kLanes k lies in the row where behind < -kLanes k.  A row may be read past
+    // its end (the stage is that long); what stands there is not used.
     const int behind = l - vocab;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       const bool in_row = behind < -kLanes * k;
-      const int c = kStaged || in_row ? l + kLanes * k : vocab - 1;
+      const int c = l + kLanes * k;
       y[k] = in_row ? max_nan(to_float(x[c]), kMasked) : kMasked;
       if constexpr (kRef) z[k] = in_row ? max_nan(to_float(z_row[c]), kMasked) : kMasked;
     }
     if (r.legal) {
 #pragma unroll
       for (int k = 0; k < kPer; ++k) {
-        const int c = kStaged || behind < -kLanes * k ? l + kLanes * k : vocab - 1;
-        const bool open = lm[c];
+        const bool open = lm[l + kLanes * k];
         y[k] = open ? y[k] : kMasked;
         if constexpr (kRef) z[k] = open ? z[k] : kMasked;
       }
@@ -686,7 +699,7 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
 // times, so that the logits cross the memory bus once; a slot that has been looked at for
 // the last time is filled with the next row's vector at once, so the copies run on under
 // the second look, its stores and the next row's reductions.  The copies are waited for
-// in four chunks of the slots.  Vectors that no slot holds (rows longer than eight blocks'
+// in two chunks of the slots.  Vectors that no slot holds (rows longer than eight blocks'
 // slots) are read from memory both times.
 
 constexpr int kLongThreads = 256, kWideThreads = 512;
@@ -745,26 +758,53 @@ __device__ __forceinline__ float extreme(const uint4 (&x)[kCount]) {
   }
 }
 
-// Up to kN flags of `legal`, as bits.
+// The flags of a vector's entries, a byte each; read by words, which lie in the flags' own
+// 16-byte granules wherever the flags begin.
 template <int kN>
-__device__ __forceinline__ unsigned legal_bits(const bool* lm) {
-  unsigned bits = 0;
-  if ((reinterpret_cast<uintptr_t>(lm) & (kN - 1)) == 0) {
-    if constexpr (kN == 8) {
-      const uint2 q = *reinterpret_cast<const uint2*>(lm);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) bits |= ((q.x >> (8 * e)) & 1u) << e | ((q.y >> (8 * e)) & 1u) << (e + 4);
+struct Flags {
+  uint32_t w[kN / 4];
+
+  __device__ __forceinline__ static Flags load(const bool* lm) {
+    const auto at = reinterpret_cast<uintptr_t>(lm);
+    const int off = static_cast<int>(at & 3);
+    Flags f;
+    if ((at & (kN - 1)) == 0) {
+      if constexpr (kN == 8) {
+        const uint2 q = __ldg(reinterpret_cast<const uint2*>(lm));
+        f.w[0] = q.x;
+        f.w[1] = q.y;
+      } else {
+        f.w[0] = __ldg(reinterpret_cast<const uint32_t*>(lm));
+      }
     } else {
-      const uint32_t q = *reinterpret_cast<const uint32_t*>(lm);
+      const uint32_t* const q = reinterpret_cast<const uint32_t*>(at - off);
+      uint32_t low = __ldg(q);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bits |= ((q >> (8 * e)) & 1u) << e;
+      for (int k = 0; k < kN / 4; ++k) {
+        const uint32_t high = off || k + 1 < kN / 4 ? __ldg(q + k + 1) : 0u;
+        f.w[k] = __funnelshift_r(low, high, 8 * off);
+        low = high;
+      }
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < kN; ++e) bits |= static_cast<unsigned>(lm[e]) << e;
+    return f;
   }
-  return bits;
-}
+
+  // The entries whose flag is 0 as -inf.
+  template <typename T>
+  __device__ __forceinline__ uint4 apply(const uint4 raw) const {
+    uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // Each flag's byte over its entry's bytes, as all ones or zeros.
+      constexpr bool kSmall = sizeof(T) == 2;
+      const uint32_t open = kSmall ? __byte_perm(w[e / 2 % (kN / 4)], 0, e % 2 ? 0x3322 : 0x1100) * 0xffu
+                                   : __byte_perm(w[0], 0, 0x1111 * e) * 0xffu;
+      constexpr uint32_t kLow = !kSmall ? 0xff800000u : std::is_same_v<T, __nv_bfloat16> ? 0xff80ff80u : 0xfc00fc00u;
+      x[e] = (x[e] & open) | (kLow & ~open);
+    }
+    return make_uint4(x[0], x[1], x[2], x[3]);
+  }
+};
 
 // The row's part that a block takes, and its vectors.
 template <typename T>
@@ -811,18 +851,7 @@ struct Part {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  // A vector's entries with all masks applied.
-  __device__ __forceinline__ void masked(int v, const uint4 raw, float (&f)[kVec<T>]) const {
-    unpack<T>(raw, f);
-#pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) f[e] = max_nan(f[e], kMasked);
-    if (lm) {
-      const unsigned bits = legal_bits<kVec<T>>(lm + head + v * kVec<T>);
-#pragma unroll
-      for (int e = 0; e < kVec<T>; ++e)
-        if (!(bits >> e & 1u)) f[e] = kMasked;
-    }
-  }
+  __device__ __forceinline__ Flags<kVec<T>> flags(int v) const { return Flags<kVec<T>>::load(lm + head + v * kVec<T>); }
   // Entry number i of those outside the vectors, or -1: rank 0 takes them all.
   __device__ __forceinline__ int loose(int i) const {
     const int tail = head + vectors * kVec<T>;
@@ -903,6 +932,14 @@ __device__ __forceinline__ void add_vectors(Running& v, const uint4 (&x)[kCount]
   }
 }
 
+// A vector's entries, none below kMasked.
+template <typename T>
+__device__ __forceinline__ void bounded(const uint4 raw, float (&f)[kVec<T>]) {
+  unpack<T>(raw, f);
+#pragma unroll
+  for (int e = 0; e < kVec<T>; ++e) f[e] = max_nan(f[e], kMasked);
+}
+
 template <int kN>
 __device__ __forceinline__ float largest(const float (&x)[kN]) {
   const float top = max_nan(max_nan(x[0], x[1], x[2]), x[3]);
@@ -910,14 +947,15 @@ __device__ __forceinline__ float largest(const float (&x)[kN]) {
   else return top;
 }
 
-// A part's sums by `step` threads of which this is number tid, from memory, with masks.
-template <typename T, bool kRef>
-__device__ __noinline__ void add_masked(Running& v, const Part<T>& p, int tid, int step) {
+// Adds vectors of which entries may be masked.
+template <typename T, bool kRef, int kCount>
+__device__ __forceinline__ void add_bounded(Running& v, const uint4 (&x)[kCount], const uint4 (&z)[kCount]) {
   constexpr int kN = kVec<T>;
-  for (int i = p.first + tid; i < p.last; i += step) {
+#pragma unroll
+  for (int h = 0; h < kCount; ++h) {
     float f[kN], q[kN];
-    p.masked(i, __ldg(p.vector(i)), f);
-    if constexpr (kRef) p.masked(i, p.ref_vector(i), q);
+    bounded<T>(x[h], f);
+    if constexpr (kRef) bounded<T>(z[h], q);
     raise<kRef>(v, base2(largest(f)), kRef ? base2(largest(q)) : kMasked2);
     accumulate<kRef>(v, f, q);
   }
@@ -962,36 +1000,25 @@ __device__ __forceinline__ void write_hot(const Part<T>& p, const Coefs& c, floa
     store_one<kType>(row, action, gradient_of<T, kRef>(p, c, m, mr, action, true));
 }
 
-// A part's gradient by `step` threads of which this is number tid, from memory, with masks.
-template <typename T, bool kRef, int kType>
-__device__ __noinline__ void write_masked(const Part<T>& p, const Coefs& c, float m, float mr, void* row, bool wide,
-                                          int tid, int step) {
-  constexpr int kN = kVec<T>;
-  for (int i = p.first + tid; i < p.last; i += step) {
-    float f[kN], q[kN], g[kN];
-    p.masked(i, __ldg(p.vector(i)), f);
-    if constexpr (kRef) p.masked(i, p.ref_vector(i), q);
-    gradient<kRef>(c, m, mr, f, q, g);
-    store_grad<kType>(row, p.head + i * kN, g, wide);
-  }
-}
-
 template <typename T, int kType>
 __device__ __forceinline__ void write_zeros(const Part<T>& p, void* row, bool wide, int tid, int step) {
   float g[kVec<T>] = {};
   for (int i = p.first + tid; i < p.last; i += step) store_grad<kType>(row, p.head + i * kVec<T>, g, wide);
 }
 
-// The gradient of whole vectors as they are, `apart` entries from one to the next.
-template <typename T, bool kRef, int kType, int kCount>
+// The gradient of whole vectors, `apart` entries from one to the next.  kMasks: entries may
+// be masked.
+template <typename T, bool kRef, int kType, bool kMasks, int kCount>
 __device__ __forceinline__ void write_vectors(const Coefs& c, float m, float mr, Stored<kType>* to, int apart, bool wide,
                                               const uint4 (&x)[kCount], const uint4 (&z)[kCount]) {
   constexpr int kN = kVec<T>;
 #pragma unroll
   for (int k = 0; k < kCount; ++k) {
     float f[kN], q[kN], g[kN];
-    unpack<T>(x[k], f);
-    if constexpr (kRef) unpack<T>(z[k], q);
+    if constexpr (kMasks) bounded<T>(x[k], f);
+    else unpack<T>(x[k], f);
+    if constexpr (kRef && kMasks) bounded<T>(z[k], q);
+    else if constexpr (kRef) unpack<T>(z[k], q);
     gradient<kRef>(c, m, mr, f, q, g);
     store_grad<kType>(to, k * apart, g, wide);
   }
@@ -1017,19 +1044,25 @@ __device__ __forceinline__ void wait_copies() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
-// slots: vectors of a thread that shared memory holds.
-template <typename T, bool kRef, bool kPolicy, int kThreads>
-__global__ void __launch_bounds__(kThreads, kThreads == kWideThreads ? 2 : 3)
-    long_rows_kernel(const Rows r, const Score o, const Policy given, const int slots) {
-  const Policy a = kPolicy ? resolved(given) : given;
-  constexpr int kN = kVec<T>;
+// What the threads of a block of long rows share beside their slots.
+struct LongShared {
+  Sums warp_sums[kWideThreads / 32];
+  Sums block_sums[2];
+  RowInputs row_in;  // thread 32's, for thread 0
+  float row_x;       // the action's entry
+  RowResult result;  // thread 0's, for all
+  double acc[kSums];
+};
+
+// A block's rows from `row` on.  kMasks false: entries are taken as they are, until a row's
+// sums are not numbers; that row is returned (the number of rows, if there is none).
+// true: with legal, and entries of -inf and the like.  slots: vectors of a thread that shared
+// memory holds; buffer: whose turn it is of block_sums.
+template <typename T, bool kRef, bool kPolicy, bool kMasks>
+__device__ __forceinline__ i64 long_rows(const Rows& r, const Score& o, const Policy& a, const float scale,
+                                         const int slots, LongShared& sh, i64 row0, int& buffer) {
+  constexpr int kN = kVec<T>, kLook = kRef || kMasks ? 2 : kGroup;  // vectors looked at together
   extern __shared__ __align__(16) uint4 slot[];  // [slots][threads], then the reference's
-  __shared__ Sums warp_sums[kThreads / 32];
-  __shared__ Sums block_sums[2];
-  __shared__ RowInputs row_in;   // thread 32's, for thread 0
-  __shared__ float row_x;        // the action's entry
-  __shared__ RowResult result;   // thread 0's, for all
-  __shared__ double block_acc[kSums];
   const cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), rank = cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x / 32, step = blockDim.x;
@@ -1037,11 +1070,6 @@ __global__ void __launch_bounds__(kThreads, kThreads == kWideThreads ? 2 : 3)
   const int chunk = (slots + kChunks * kGroup - 1) / (kChunks * kGroup) * kGroup;
   uint4* const mine = slot + tid;
   uint4* const mine_r = mine + slots * step;
-  float scale = 0.0f;
-  if (tid == 0)
-#pragma unroll
-    for (int k = 0; k < kSums; ++k) block_acc[k] = 0.0;
-  if constexpr (kPolicy) scale = grad_scale_of(a, block_denominator(a, r.weight, r.rows));
   const i64 rows_step = gridDim.x / parts;
 
   // A row that may count (its action's own entry is still to be seen), or none; the same in
@@ -1112,8 +1140,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kWideThreads ? 2 : 3)
     return c;
   };
 
-  int buffer = 0;
-  Candidate now = skip(candidate(blockIdx.x >> log_parts)), next = now, after = now;
+  Candidate now = skip(candidate(row0)), next = now, after = now;
   const bool write = kPolicy && a.dlogits;  // a second look
   Part<T> p;
   int n_slotted = 0;
@@ -1137,177 +1164,187 @@ __global__ void __launch_bounds__(kThreads, kThreads == kWideThreads ? 2 : 3)
     const int action = now.action, i0 = p.first + tid;
     const int n_loose = rank == 0 ? r.vocab - p.vectors * kN : 0;
     if (tid == 32) {
-      row_in = row_inputs<kPolicy>(r, a, row);
-      row_x = p.one(p.x, action);
+      sh.row_in = row_inputs<kPolicy>(r, a, row);
+      sh.row_x = p.one(p.x, action);
     }
-    bool careful = p.lm != nullptr;
+    // Some vectors of the row, `step` apart, from slot k on or from vector i on in memory.
+    const auto masked = [&](int i, auto& x, auto& z) {
+      if constexpr (kMasks) {
+        constexpr int kCount = std::extent_v<std::remove_reference_t<decltype(x)>>;
+        if (p.lm) {
+          Flags<kN> f[kCount];
+#pragma unroll
+          for (int h = 0; h < kCount; ++h) f[h] = p.flags(i + h * step);
+#pragma unroll
+          for (int h = 0; h < kCount; ++h) {
+            x[h] = f[h].template apply<T>(x[h]);
+            if constexpr (kRef) z[h] = f[h].template apply<T>(z[h]);
+          }
+        }
+      }
+    };
+    const auto from_slots = [&](const uint4* at, const uint4* at_r, int k, auto& x, auto& z) {
+      constexpr int kCount = std::extent_v<std::remove_reference_t<decltype(x)>>;
+#pragma unroll
+      for (int h = 0; h < kCount; ++h) {
+        x[h] = at[h * step];
+        if constexpr (kRef) z[h] = at_r[h * step];
+      }
+      masked(i0 + k * step, x, z);
+    };
+    const auto from_memory = [&](int i, auto& x, auto& z) {
+      constexpr int kCount = std::extent_v<std::remove_reference_t<decltype(x)>>;
+#pragma unroll
+      for (int h = 0; h < kCount; ++h) {
+        x[h] = __ldg(p.vector(i + h * step));
+        if constexpr (kRef) z[h] = p.ref_vector(i + h * step);
+      }
+      masked(i, x, z);
+    };
     Running run = nothing_yet();
+    const auto add = [&](const auto& x, const auto& z) {
+      if constexpr (kMasks) add_bounded<T, kRef>(run, x, z);
+      else add_vectors<T, kRef>(run, x, z);
+    };
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       if (write && c > 0) wait_copies<0>();
       else wait_copies<kChunks - 1>();
       static_assert(kChunks == 2, "the waits are for two");
-      if (!careful) {
-        const int end = (c + 1) * chunk < n_slotted ? (c + 1) * chunk : n_slotted;
-        const uint4 *at = mine + c * chunk * step, *at_r = mine_r + c * chunk * step;
-        int k = c * chunk;
+      const int end = (c + 1) * chunk < n_slotted ? (c + 1) * chunk : n_slotted;
+      const uint4 *at = mine + c * chunk * step, *at_r = mine_r + c * chunk * step;
+      int k = c * chunk;
 #pragma unroll 1
-        for (; k + kGroup <= end; k += kGroup, at += kGroup * step, at_r += kGroup * step) {
-          uint4 x[kGroup], z[kGroup];
-#pragma unroll
-          for (int h = 0; h < kGroup; ++h) {
-            x[h] = at[h * step];
-            if constexpr (kRef) z[h] = at_r[h * step];
-          }
-          add_vectors<T, kRef>(run, x, z);
-        }
+      for (; k + kLook <= end; k += kLook, at += kLook * step, at_r += kLook * step) {
+        uint4 x[kLook], z[kLook];
+        from_slots(at, at_r, k, x, z);
+        add(x, z);
+      }
 #pragma unroll 1
-        for (; k < end; ++k, at += step, at_r += step) {
-          const uint4 x[1] = {*at};
-          uint4 z[1];
-          if constexpr (kRef) z[0] = *at_r;
-          add_vectors<T, kRef>(run, x, z);
-        }
+      for (; k < end; ++k, at += step, at_r += step) {
+        uint4 x[1], z[1];
+        from_slots(at, at_r, k, x, z);
+        add(x, z);
       }
       if (!write) fetch(x_next, z_next, n_next, c);
     }
-    if (!careful) {
+    {  // what no slot holds
+      int i = i0 + slots * step;
 #pragma unroll 1
-      for (int i = i0 + slots * step; i < p.last; i += 2 * step) {  // what no slot holds
+      for (; i + step < p.last; i += 2 * step) {
         uint4 x[2], z[2];
-        const bool both_there = i + step < p.last;
-        x[0] = __ldg(p.vector(i));
-        x[1] = both_there ? __ldg(p.vector(i + step)) : x[0];
-        if constexpr (kRef) {
-          z[0] = p.ref_vector(i);
-          z[1] = both_there ? p.ref_vector(i + step) : z[0];
-        }
-        if (both_there) {
-          add_vectors<T, kRef>(run, x, z);
+        from_memory(i, x, z);
+        add(x, z);
+      }
+      if (i < p.last) {
+        uint4 x[1], z[1];
+        from_memory(i, x, z);
+        add(x, z);
+      }
+    }
+    if (tid < n_loose) {
+      // One entry, and one that adds nothing beside it: were there nothing else, it would
+      // weigh as much as a masked entry, and a row of such does not count.
+      const int c = p.loose(tid);
+      const float f[2] = {p.one(p.x, c), kMasked};
+      float q[2] = {kMasked, kMasked};
+      if constexpr (kRef) q[0] = p.one(p.z, c);
+      raise<kRef>(run, base2(f[0]), base2(q[0]));
+      accumulate<kRef>(run, f, q);
+    }
+    Sums v = no_sums();
+    v.m = run.m;
+    v.s = both(run.s);
+    v.t = both(run.t);
+    if constexpr (kRef) {
+      v.mr = run.mr;
+      v.sr = both(run.sr);
+      v.u = both(run.u);
+    }
+    v = join_warp<kRef>(v);
+    if (lane == 0) sh.warp_sums[tid >> 5] = v;
+    __syncthreads();
+    if (tid < 32) v = join_warp<kRef>(lane < warps ? sh.warp_sums[lane] : no_sums());
+    if (parts > 1) {
+      if (tid == 0) sh.block_sums[buffer] = v;
+      cluster.sync();
+      // Every block adds the blocks' sums in the same order.
+      if (tid < 32)
+        v = join_warp<kRef>(lane < parts ? *cluster.map_shared_rank(&sh.block_sums[buffer], lane) : no_sums());
+      buffer ^= 1;
+    }
+    if (tid == 0) {
+      // Not a number: for an entry that is one, or for one of -inf.
+      const float sum = v.s + v.t + (kRef ? v.sr + v.u : 0.0f);
+      sh.result.again = !kMasks && !(fabsf(sum) < INFINITY);
+      const float row_x = sh.row_x;
+      const bool used = !(row_x <= kMasked);
+      if (!sh.result.again) {
+        if constexpr (!kPolicy) {
+          if (rank == 0) store_score(o, row, used, v, row_x);
         } else {
-          const uint4 x1[1] = {x[0]}, z1[1] = {z[0]};
-          add_vectors<T, kRef>(run, x1, z1);
+          const RowInputs in = sh.row_in;
+          float logp = 0.0f;
+          if (used) {
+            Terms terms;
+            sh.result.c = policy_row<kRef>(a, in, v, row_x, scale, terms, logp);
+            if (rank == 0) terms.add_to(sh.acc, in.weight);
+          }
+          if (a.logp && rank == 0) a.logp[row] = logp;
+          sh.result.m = v.m;
+          sh.result.mr = v.mr;
+          sh.result.used = used;
         }
       }
     }
-    for (;;) {
-      if (careful) {
-        // Copies for the call: what its arguments point to would leave the registers.
-        Running masked = nothing_yet();
-        const Part<T> part = p;
-        add_masked<T, kRef>(masked, part, tid, step);
-        run = masked;
-      }
-      if (tid < n_loose) {
-        // One entry, and one that adds nothing beside it: were there nothing else, it would
-        // weigh as much as a masked entry, and a row of such does not count.
-        const int c = p.loose(tid);
-        const float f[2] = {p.one(p.x, c), kMasked};
-        float q[2] = {kMasked, kMasked};
-        if constexpr (kRef) q[0] = p.one(p.z, c);
-        raise<kRef>(run, base2(f[0]), base2(q[0]));
-        accumulate<kRef>(run, f, q);
-      }
-      Sums v = no_sums();
-      v.m = run.m;
-      v.s = both(run.s);
-      v.t = both(run.t);
-      if constexpr (kRef) {
-        v.mr = run.mr;
-        v.sr = both(run.sr);
-        v.u = both(run.u);
-      }
-      v = join_warp<kRef>(v);
-      if (lane == 0) warp_sums[tid >> 5] = v;
-      __syncthreads();
-      if (tid < 32) v = join_warp<kRef>(lane < warps ? warp_sums[lane] : no_sums());
-      if (parts > 1) {
-        if (tid == 0) block_sums[buffer] = v;
-        cluster.sync();
-        // Every block adds the blocks' sums in the same order.
-        if (tid < 32) v = join_warp<kRef>(lane < parts ? *cluster.map_shared_rank(&block_sums[buffer], lane) : no_sums());
-        buffer ^= 1;
-      }
-      if (tid == 0) {
-        // Not a number: for an entry that is one, or for one of -inf.
-        const float sum = v.s + v.t + (kRef ? v.sr + v.u : 0.0f);
-        result.again = !careful && !(fabsf(sum) < INFINITY);
-        const RowInputs in = row_in;
-        const bool used = !(row_x <= kMasked);
-        if (!result.again) {
-          if constexpr (!kPolicy) {
-            if (rank == 0) store_score(o, row, used, v, row_x);
-          } else {
-            float logp = 0.0f;
-            if (used) {
-              Terms terms;
-              result.c = policy_row<kRef>(a, in, v, row_x, scale, terms, logp);
-              if (rank == 0) terms.add_to(block_acc, in.weight);
-            }
-            if (a.logp && rank == 0) a.logp[row] = logp;
-            result.m = v.m;
-            result.mr = v.mr;
-            result.used = used;
-          }
-        }
-      }
-      __syncthreads();  // the result is there; row_in and warp_sums are free again
-      if (careful || !result.again) break;
-      careful = true;
+    __syncthreads();  // the result is there; row_in and warp_sums are free again
+    if (!kMasks && sh.result.again) {
+      wait_copies<0>();
+      return row;
     }
     if constexpr (kPolicy) {
       if (write) {
-        const Coefs c = result.c;  // of a row that counts; not used for another
-        const float m = result.m, mr = result.mr;
-        const bool used = result.used;
+        const Coefs c = sh.result.c;  // of a row that counts; not used for another
+        const float m = sh.result.m, mr = sh.result.mr;
+        const bool used = sh.result.used;
         with_type(a.dtype, [&](auto type) {
           constexpr int kType = decltype(type)::value;
           using S = Stored<kType>;
           S* const to = static_cast<S*>(a.dlogits) + row * a.ldd;
           const bool wide = grad_wide<T, kType>(to, p.head);
-          if (!used) {
-            write_zeros<T, kType>(p, to, wide, tid, step);
-          } else if (careful) {
-            const Coefs coefs = c;
-            const Part<T> part = p;
-            write_masked<T, kRef, kType>(part, coefs, m, mr, to, wide, tid, step);
-          }
-          const bool plain = used && !careful;
+          const auto put = [&](S* place, const auto& x, const auto& z) {
+            write_vectors<T, kRef, kType, kMasks>(c, m, mr, place, step * kN, wide, x, z);
+          };
+          if (!used) write_zeros<T, kType>(p, to, wide, tid, step);
           for (int q = 0; q < kChunks; ++q) {
-            if (plain) {
+            if (used) {
               const int end = (q + 1) * chunk < n_slotted ? (q + 1) * chunk : n_slotted;
               const uint4 *at = mine + q * chunk * step, *at_r = mine_r + q * chunk * step;
               int k = q * chunk;
               S* place = to + p.head + (i0 + k * step) * kN;
 #pragma unroll 1
-              for (; k + kGroup <= end; k += kGroup, at += kGroup * step, at_r += kGroup * step) {
-                uint4 x[kGroup], z[kGroup];
-#pragma unroll
-                for (int h = 0; h < kGroup; ++h) {
-                  x[h] = at[h * step];
-                  if constexpr (kRef) z[h] = at_r[h * step];
-                }
-                write_vectors<T, kRef, kType>(c, m, mr, place, step * kN, wide, x, z);
-                place += kGroup * step * kN;
+              for (; k + kLook <= end; k += kLook, at += kLook * step, at_r += kLook * step) {
+                uint4 x[kLook], z[kLook];
+                from_slots(at, at_r, k, x, z);
+                put(place, x, z);
+                place += kLook * step * kN;
               }
 #pragma unroll 1
               for (; k < end; ++k, at += step, at_r += step) {
-                const uint4 x[1] = {*at};
-                uint4 z[1];
-                if constexpr (kRef) z[0] = *at_r;
-                write_vectors<T, kRef, kType>(c, m, mr, place, 0, wide, x, z);
+                uint4 x[1], z[1];
+                from_slots(at, at_r, k, x, z);
+                put(place, x, z);
                 place += step * kN;
               }
             }
             fetch(x_next, z_next, n_next, q);
           }
-          if (plain)
+          if (used)
 #pragma unroll 1
             for (int i = i0 + slots * step; i < p.last; i += step) {
-              const uint4 x[1] = {__ldcs(p.vector(i))};
-              uint4 z[1];
-              if constexpr (kRef) z[0] = p.ref_vector(i);
-              write_vectors<T, kRef, kType>(c, m, mr, to + p.head + i * kN, 0, wide, x, z);
+              uint4 x[1], z[1];
+              from_memory(i, x, z);
+              put(to + p.head + i * kN, x, z);
             }
           if (used) write_hot<T, kRef, kType>(p, c, m, mr, action, to, tid, step);
           if (tid < n_loose) {
@@ -1323,11 +1360,31 @@ __global__ void __launch_bounds__(kThreads, kThreads == kWideThreads ? 2 : 3)
     p = p_next;
     n_slotted = n_next;
   }
-  if (parts > 1) cluster.sync();  // no block leaves while another may read its sums
-  if constexpr (kPolicy)
-    if (tid == 0 && a.partial)
+  return r.rows;
+}
+
+template <typename T, bool kRef, bool kPolicy, int kThreads>
+__global__ void __launch_bounds__(kThreads, kThreads == kWideThreads ? 2 : 3)
+    long_rows_kernel(const Rows r, const Score o, const Policy given, const int slots) {
+  const Policy a = kPolicy ? resolved(given) : given;
+  __shared__ LongShared sh;
+  const cg::cluster_group cluster = cg::this_cluster();
+  float scale = 0.0f;
+  if (threadIdx.x == 0)
 #pragma unroll
-      for (int k = 0; k < kSums; ++k) a.partial[(i64)blockIdx.x * kSums + k] = block_acc[k];
+    for (int k = 0; k < kSums; ++k) sh.acc[k] = 0.0;
+  if constexpr (kPolicy) scale = grad_scale_of(a, block_denominator(a, r.weight, r.rows));
+  int buffer = 0;
+  i64 row = blockIdx.x / cluster.num_blocks();
+  // Rows as they are cost less than rows whose entries may be masked; the first one that
+  // turns out to have such, and all behind it, go the second way.
+  if (!r.legal) row = long_rows<T, kRef, kPolicy, false>(r, o, a, scale, slots, sh, row, buffer);
+  if (row < r.rows) long_rows<T, kRef, kPolicy, true>(r, o, a, scale, slots, sh, row, buffer);
+  if (cluster.num_blocks() > 1) cluster.sync();  // no block leaves while another may read its sums
+  if constexpr (kPolicy)
+    if (threadIdx.x == 0 && a.partial)
+#pragma unroll
+      for (int k = 0; k < kSums; ++k) a.partial[(i64)blockIdx.x * kSums + k] = sh.acc[k];
 }
 
 // ---- the means of policy_loss ---------------------------------------------------------------
@@ -1413,27 +1470,32 @@ __global__ void __launch_bounds__(32 * kBackWarps, 4) logp_backward_kernel(const
   const int hot = used ? static_cast<int>(r.actions[row]) - c0 : -1;
   with_type(b.dtype, [&](auto type) {
     constexpr int kType = decltype(type)::value;
-    Stored<kType>* const to = static_cast<Stored<kType>*>(b.dlogits) + row * b.ldd + c0;
+    using S = Stored<kType>;
+    S* const to = static_cast<S*>(b.dlogits) + row * b.ldd + c0;
     const bool wide = grad_wide<T, kType>(to, p.head);
     if (!used) {
       write_zeros<T, kType>(p, to, wide, lane, 32);
     } else {
-      bool careful = p.lm != nullptr;
-      int i = lane;
-      for (; !careful && i + (kGroup - 1) * 32 < p.last; i += kGroup * 32) {
-        uint4 x[kGroup];
+      const auto write = [&](int i, auto count) {
+        constexpr int kCount = decltype(count)::value;
+        uint4 x[kCount];
 #pragma unroll
-        for (int h = 0; h < kGroup; ++h) x[h] = __ldcs(p.vector(i + 32 * h));
-        careful = !(extreme<T, false>(x) > kMasked);
-        if (careful) break;
-        write_vectors<T, false, kType>(k, lse.x, 0.0f, to + p.head + i * kVec<T>, 32 * kVec<T>, wide, x, x);
-      }
-      for (; i < p.last; i += 32) {  // what is left of a group, or may be masked
-        float f[kVec<T>], g[kVec<T>];
-        p.masked(i, __ldcs(p.vector(i)), f);
-        gradient<false>(k, lse.x, 0.0f, f, f, g);
-        store_grad<kType>(to, p.head + i * kVec<T>, g, wide);
-      }
+        for (int h = 0; h < kCount; ++h) x[h] = __ldcs(p.vector(i + 32 * h));
+        if (p.lm) {
+          Flags<kVec<T>> f[kCount];
+#pragma unroll
+          for (int h = 0; h < kCount; ++h) f[h] = p.flags(i + 32 * h);
+#pragma unroll
+          for (int h = 0; h < kCount; ++h) x[h] = f[h].template apply<T>(x[h]);
+        }
+        S* const at = to + p.head + i * kVec<T>;
+        const int apart = 32 * kVec<T>;
+        if (!p.lm && extreme<T, false>(x) > kMasked) write_vectors<T, false, kType, false>(k, lse.x, 0.0f, at, apart, wide, x, x);
+        else write_vectors<T, false, kType, true>(k, lse.x, 0.0f, at, apart, wide, x, x);
+      };
+      int i = lane;
+      for (; i + (kGroup - 1) * 32 < p.last; i += kGroup * 32) write(i, std::integral_constant<int, kGroup>{});
+      for (; i < p.last; i += 32) write(i, std::integral_constant<int, 1>{});
       write_hot<T, false, kType>(p, k, lse.x, 0.0f, hot, to, lane, 32);
     }
     for (int i = lane; i < p.vocab - p.vectors * kVec<T>; i += 32) {
@@ -1637,14 +1699,11 @@ Plan long_plan(i64 rows, int vocab, int size, bool ref, bool stage, bool policy)
   return p;
 }
 
-inline int round16(i64 n) { return static_cast<int>((n + 15) / 16 * 16); }
-
-// Whether rows lie one after another: up to 64 bytes between them are copied along.
-inline bool is_run(i64 ld, i64 vocab, int size) { return ld >= vocab && (ld - vocab) * size <= 64; }
+inline i64 round16(i64 n) { return (n + 15) / 16 * 16; }
 
 // Bytes of a run of n rows in shared memory, its last row `width` entries long, with a
 // granule for its alignment.
-inline int run_bytes(i64 n, i64 ld, i64 width, int size) { return round16(((n - 1) * ld + width) * size + 15); }
+inline i64 run_bytes(i64 n, i64 ld, i64 width, int size) { return round16(((n - 1) * ld + width) * size + 15); }
 
 template <typename T, bool kRef, bool kPolicy, int kThreads>
 int launch_planned(const Plan& p, const Rows& r, const Score& o, const Policy& a, cudaStream_t stream) {
@@ -1670,8 +1729,9 @@ template <typename T, bool kRef, bool kPolicy>
 int launch_long(const Rows& r, const Score& o, const Policy& a, cudaStream_t stream, int& blocks) {
   // The reference's vectors are copied beside the logits' where both are aligned alike.
   constexpr int kSize = sizeof(T);
-  const bool stage = !r.legal && (!kRef || ((reinterpret_cast<uintptr_t>(r.ref) - reinterpret_cast<uintptr_t>(r.logits)) % 16 == 0 &&
-                               (r.rows <= 1 || (r.ldr - r.ld) * kSize % 16 == 0)));
+  const auto apart = reinterpret_cast<uintptr_t>(r.ref) - reinterpret_cast<uintptr_t>(r.logits);
+  const bool alike = apart % 16 == 0 && (r.rows <= 1 || (r.ldr - r.ld) * kSize % 16 == 0);
+  const bool stage = !kRef || alike;
   const Plan p = long_plan(r.rows, r.vocab, kSize, kRef, stage, kPolicy);
   blocks = p.blocks;
   if constexpr (kPolicy)
@@ -1679,9 +1739,9 @@ int launch_long(const Rows& r, const Score& o, const Policy& a, cudaStream_t str
   return launch_planned<T, kRef, kPolicy, kLongThreads>(p, r, o, a, stream);
 }
 
-template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy, bool kStaged>
+template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy>
 int launch_short(const Rows& r, const Score& o, const Policy& a, const Layout& lay, cudaStream_t stream, int& blocks) {
-  const auto kernel = short_rows_kernel<T, kLanes, kPer, kRef, kPolicy, kStaged>;
+  const auto kernel = short_rows_kernel<T, kLanes, kPer, kRef, kPolicy>;
   const int shared = lay.warp() * kShortWarps;
   if (shared > (44 << 10) &&  // with the static part, past what needs no opt-in
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShortShared) != cudaSuccess)
@@ -1695,36 +1755,34 @@ int launch_short(const Rows& r, const Score& o, const Policy& a, const Layout& l
   return launch_status();
 }
 
-// The staged form where everything of a row lies in runs and two stages fit.
 template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy>
-bool stage_layout(const Rows& r, const Policy& a, Layout& lay) {
+Layout short_layout(const Rows& r, const Policy& a) {
   constexpr int kRows = 32 / kLanes, kLong = kLanes * kPer;  // entries that a row is read to
-  const int size = sizeof(T);
-  lay = {};
-  if (kRows > 1 && (!is_run(r.ld, r.vocab, size) || (kRef && !is_run(r.ldr, r.vocab, size)) ||
-                    (r.legal && !is_run(r.ldm, r.vocab, 1))))
-    return false;
-  lay.logits = run_bytes(kRows, kRows > 1 ? r.ld : 0, kLong, size);
-  if (kRef) lay.ref = run_bytes(kRows, kRows > 1 ? r.ldr : 0, kLong, size);
-  if (r.legal) lay.legal = run_bytes(kRows, kRows > 1 ? r.ldm : 0, kLong, 1);
-  if (lay.warp() * kShortWarps > kShortShared) return false;
+  Layout lay = {};
+  // Rows lie one after another: up to 64 bytes between them are copied along.
+  const auto run = [&](i64 ld, int size) { return ld >= r.vocab && (ld - r.vocab) * size <= 64; };
+  lay.apart = kRows > 1 && !(run(r.ld, sizeof(T)) && (!kRef || run(r.ldr, sizeof(T))) && (!r.legal || r.ldm == 0 || run(r.ldm, 1)));
+  const auto place = [&](i64 ld, int size, int& pitch) {
+    pitch = static_cast<int>(lay.apart ? run_bytes(1, 0, kLong, size) : kRows > 1 ? ld * size : 0);
+    return lay.apart ? kRows * pitch : static_cast<int>(run_bytes(kRows, kRows > 1 ? ld : 0, kLong, size));
+  };
+  lay.logits = place(r.ld, sizeof(T), lay.pitch);
+  if (kRef) lay.ref = place(r.ldr, sizeof(T), lay.pitch_ref);
+  if (r.legal) lay.legal = place(r.ldm, 1, lay.pitch_legal);
+  if (r.ldm == 0) lay.pitch_legal = 0;
   // Between the rows of a wider gradient stands what is not this call's to write.
   if (a.dlogits && (kRows == 1 || a.ldd == a.width)) {
     const i64 grad = run_bytes(kRows, kRows > 1 ? a.ldd : 0, a.width, type_bytes(a.dtype));
     if ((lay.warp() + grad) * kShortWarps <= kShortShared) lay.grad = static_cast<int>(grad);
   }
-  return true;
+  return lay;
 }
 
 template <typename T, bool kRef, bool kPolicy>
 int launch_rows(const Rows& r, const Score& o, const Policy& a, cudaStream_t stream, int& blocks) {
-  Layout lay;
-#define CUGO_SHORT(lanes, per)                                                  \
-  if (r.vocab <= (lanes) * (per)) {                                             \
-    if (stage_layout<T, lanes, per, kRef, kPolicy>(r, a, lay))                  \
-      return launch_short<T, lanes, per, kRef, kPolicy, true>(r, o, a, lay, stream, blocks); \
-    return launch_short<T, 32, 32, kRef, kPolicy, false>(r, o, a, Layout{}, stream, blocks); \
-  }
+#define CUGO_SHORT(lanes, per) \
+  if (r.vocab <= (lanes) * (per)) \
+    return launch_short<T, lanes, per, kRef, kPolicy>(r, o, a, short_layout<T, lanes, per, kRef, kPolicy>(r, a), stream, blocks);
   CUGO_SHORT(8, 4)
   CUGO_SHORT(8, 8)
   CUGO_SHORT(8, 24)
@@ -1748,6 +1806,7 @@ inline i64 weight_blocks(i64 rows) {
 }
 
 constexpr int kMostBlocks = 8 * kSms;  // of any launch over rows
+constexpr i64 kMostEntries = 1 << 30;  // of a row, its zeros behind included: loops over them count in 32 bits
 
 }  // namespace
 
@@ -1756,7 +1815,7 @@ extern "C" {
 int cugo_b200_action_logp(const void* logits, int64_t ld, int32_t dtype, const bool* legal, int64_t ldm,
                           const int64_t* actions, const float* weight, int64_t rows, int64_t vocab,
                           float* logp, float* entropy, float* lse, float* zeros, cudaStream_t stream) {
-  if (vocab < 1 || vocab > INT32_MAX) return CUGO_B200_ERR_ARG;
+  if (vocab < 1 || vocab > kMostEntries) return CUGO_B200_ERR_ARG;
   const Rows r{logits, ld, nullptr, 0, legal, ldm, actions, weight, rows, static_cast<int>(vocab)};
   if (int rc = check_rows(r, dtype)) return rc;
   if (rows > 0 && !logp && !entropy && !lse) return CUGO_B200_ERR_ARG;
@@ -1772,7 +1831,7 @@ int cugo_b200_action_logp_backward(const void* logits, int64_t ld, int32_t dtype
                                    const float* entropy, const float* d_logp, const float* d_entropy,
                                    const float* scale, int64_t rows, int64_t vocab, void* dlogits,
                                    int64_t ldd, int32_t grad_dtype, cudaStream_t stream) {
-  if (vocab < 1 || vocab > INT32_MAX) return CUGO_B200_ERR_ARG;
+  if (vocab < 1 || vocab > kMostEntries) return CUGO_B200_ERR_ARG;
   const Rows r{logits, ld, nullptr, 0, legal, ldm, actions, nullptr, rows, static_cast<int>(vocab)};
   if (int rc = check_rows(r, dtype)) return rc;
   if (!type_ok(grad_dtype) || (rows > 0 && (!lse || (d_entropy && !entropy)))) return CUGO_B200_ERR_ARG;
@@ -1800,11 +1859,11 @@ int cugo_b200_policy_loss(const void* logits, int64_t ld, int32_t dtype, const v
                           const bool* legal, int64_t ldm, const int64_t* actions, const float* logp_old,
                           const float* adv, const float* weight, const float* ref_logp, int64_t rows,
                           int64_t vocab, float clip_low, float clip_high, float kl_coef, float entropy_coef,
-                          const float* kl_coef_dev, const float* entropy_coef_dev, float denominator, const float* denominator_dev, float grad_scale,
-                          const float* grad_scale_dev, void* dlogits, int64_t ldd, int32_t grad_dtype,
-                          int64_t width, float* logp, float* stats, float* loss, void* scratch,
-                          int64_t scratch_bytes, cudaStream_t stream) {
-  if (vocab < 1 || vocab > INT32_MAX || width > INT32_MAX) return CUGO_B200_ERR_ARG;
+                          const float* kl_coef_dev, const float* entropy_coef_dev, float denominator,
+                          const float* denominator_dev, float grad_scale, const float* grad_scale_dev, void* dlogits,
+                          int64_t ldd, int32_t grad_dtype, int64_t width, float* logp, float* stats, float* loss,
+                          void* scratch, int64_t scratch_bytes, cudaStream_t stream) {
+  if (vocab < 1 || vocab > kMostEntries || width > kMostEntries) return CUGO_B200_ERR_ARG;
   const Rows r{logits, ld, ref_logits, ldr, legal, ldm, actions, weight, rows, static_cast<int>(vocab)};
   if (int rc = check_rows(r, dtype)) return rc;
   if ((!stats && !dlogits) || (loss && !stats) || (rows > 0 && (!logp_old || !adv)) || (ref_logits && ref_logp))

@@ -111,6 +111,19 @@ struct Rows {
   }
 };
 
+// Whether the memory from the first to the last entry of two matrices overlaps.
+bool overlap(const Tensor& a, const Tensor& b) {
+  const auto end = [](const Tensor& t) {
+    int64_t n = 1;
+    for (int64_t d = 0; d < t.dim(); ++d) {
+      if (t.size(d) == 0) return static_cast<const char*>(nullptr);
+      n += (t.size(d) - 1) * t.stride(d);
+    }
+    return static_cast<const char*>(t.const_data_ptr()) + n * t.element_size();
+  };
+  return static_cast<const char*>(a.const_data_ptr()) < end(b) && static_cast<const char*>(b.const_data_ptr()) < end(a);
+}
+
 cudaStream_t stream_of(int device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
 
 Tensor bytes(int64_t n, const at::TensorOptions& options) { return at::empty({n}, options.dtype(at::kByte)); }
@@ -224,6 +237,7 @@ PolicyOut policy(const Tensor& logits, const PolicyArgs& p, bool stats, const Ma
     if (ref) fail(op, "give ref_logits or ref_logp, not both");
     vector(op, "ref_logp", *p.ref_logp, r.rows, at::kFloat, r.device);
   }
+  if (p.denominator != 0.0 && static_cast<float>(p.denominator) == 0.0f) fail(op, "the denominator must be positive");
   // The same in double and in the kernel's float: a bound that rounds to less than 0 is not one.
   if (!(p.clip_low >= 0.0) || !(p.clip_high >= 0.0)) fail(op, "the clip's bounds must not be negative");
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(r.device));
@@ -242,6 +256,9 @@ PolicyOut policy(const Tensor& logits, const PolicyArgs& p, bool stats, const Ma
     if (code < 0) fail(op, "dlogits must be fp32, bf16 or fp16");
     ldd = matrix(op, "dlogits", o.grad, r.rows, r.vocab, r.device);
     width = o.grad.size(1);
+    // A long row's action is looked at once more after its gradient has been written.
+    if (there(dlogits) && (overlap(o.grad, logits) || (ref && overlap(o.grad, *p.ref_logits))))
+      fail(op, "dlogits must not share memory with the logits");
   }
   const int64_t need = cugo_b200_policy_loss_scratch_bytes(r.rows);
   Tensor scratch = bytes(need, r.fp32);
@@ -256,6 +273,7 @@ PolicyOut policy(const Tensor& logits, const PolicyArgs& p, bool stats, const Ma
             ldd, code, width, out_floats(o.logp), out_floats(o.stats), out_floats(o.loss), scratch.mutable_data_ptr(),
             need, stream_of(r.device)),
         op);
+  if (there(dlogits) && !dlogits->is_inference()) dlogits->unsafeGetTensorImpl()->bump_version();
   return o;
 }
 

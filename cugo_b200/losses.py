@@ -10,14 +10,17 @@ one does not: any number of entries, fp32, bf16 or fp16 logits, rows of any stri
 Rows.  logits [rows, entries] with unit column stride; legal bool of the same shape (or
 one mask expanded over the rows), or None; actions int64 [rows].  An entry that is not
 legal has probability 0, and so has one at or below -2^30 (-inf, -1e30, the type's lowest
-value).  What stands in such a place is not used, NaN included.  A row does not count --
+value); legal entries are taken to lie below 2^30.  What stands in a masked place is not
+used, NaN included.  A row does not count --
 log p, entropy and gradients are 0 -- where its action is outside the entries or masked,
 or its weight is 0; so a row that its mask leaves empty never counts.
 
 Everything is computed in 32 bits from the logits' own type; sums over rows in 64 bits and
 in a fixed order, so every run gives the same bits.  The calls enqueue on the current
 stream of the logits' device, do not wait for it, and can be captured in CUDA graphs.
-Backwards of backwards are not built."""
+A backward that is captured needs a graph of its own leaves' making: torch ties a leaf's
+accumulation to the stream of the graph that still holds it, so eager graphs of the same
+leaves have to be gone by then.  Backwards of backwards are not built."""
 from __future__ import annotations
 
 from typing import NamedTuple
@@ -100,7 +103,7 @@ def policy_loss_grad(logits: torch.Tensor, actions: torch.Tensor, logp_old: torc
     """policy_loss and grad_scale (a number, or one fp32 value on the device) times its
     gradient, in one pass over the logits, for a step that runs its backward without
     autograd.  The gradient goes to dlogits [rows, >= entries] (columns past the entries
-    are set to 0: the padded operand of a head's GEMM), or to a new tensor of grad_dtype
+    are set to 0: the padded operand of a head's GEMM; memory of its own), or to a new tensor of grad_dtype
     (the logits' type)."""
     scale, scale_dev = (1.0, grad_scale) if torch.is_tensor(grad_scale) else (grad_scale, None)
     loss, stats, logp, grad = load_update().policy_loss_grad(

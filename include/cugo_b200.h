@@ -377,7 +377,7 @@ CUGO_B200_API int cugo_b200_ppo_loss(const float* logits, int64_t ldl, const boo
 
 /* ---- losses over rows of logits ----------------------------------------------------
  *
- * Rows of `vocab` logits (any number from 1 to 2^31 - 1; dtype 0 fp32, 1 bf16, 2 fp16),
+ * Rows of `vocab` logits (any number from 1 to 2^30; dtype 0 fp32, 1 bf16, 2 fp16),
  * ld elements apart.  legal (bool, rows ldm bytes apart, 0: one mask for all rows; null:
  * every entry) masks entries; an entry at or below -2^30 counts as masked too (-inf,
  * -1e30, the type's lowest value), whatever stands in a masked place is not used, and
@@ -421,7 +421,8 @@ CUGO_B200_API int cugo_b200_action_logp_backward(
  * gradients of 0.
  * dlogits (grad_dtype, rows ldd apart, may be null) gets d loss / d logits times
  * grad_scale and *grad_scale_dev (device fp32, may be null); columns vocab .. width - 1
- * are set to 0.  logp fp32 [rows] (may be null).  stats fp32 [8] (may be null where
+ * are set to 0 (width at most 2^30); memory of its own, not the logits'.  logp fp32 [rows]
+ * (may be null).  stats fp32 [8] (may be null where
  * dlogits is not): the loss, the weighted means of policy loss, H, K, the KL estimate
  * (r - 1) - log r, the share of clipped ratios and the share of rows that count, and D;
  * loss (fp32, may be null): the loss once more.  scratch: at least

@@ -436,6 +436,30 @@ def test_few_long_rows(vocab):
         near(d, want, grad_tol(vocab, p, actions, size, torch.bfloat16, want), "gradient")
 
 
+def test_a_given_gradient_is_a_new_version():
+    """What autograd has kept of the tensor that the gradient goes to is out of date."""
+    from cugo_b200.losses import policy_loss_grad
+    x, actions, _, _ = make(6, 20, torch.float32, 0)
+    f, d = torch.zeros(6, device=DEV), torch.ones((6, 24), device=DEV)
+    w = torch.ones((6, 24), device=DEV, requires_grad=True)
+    y = (w * d).sum()
+    policy_loss_grad(x, actions, f, f, dlogits=d)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+@pytest.mark.parametrize("rows", [1, 5, 600])
+def test_one_mask_gives_the_bits_of_many(rows):
+    from cugo_b200.losses import policy_loss_grad
+    for vocab in (30, 179, 700, 1500):
+        x, actions, old, adv, _ = policy_case(rows, vocab, torch.float32, False, 0, "none", False)
+        one = torch.rand(vocab, device=DEV) < 0.4
+        one[actions[::2]] = True
+        a, da = policy_loss_grad(x, actions, old, adv, legal=one.expand(rows, vocab), entropy_coef=0.1)
+        b, db = policy_loss_grad(x, actions, old, adv, legal=one.repeat(rows, 1), entropy_coef=0.1)
+        assert torch.equal(a.stats, b.stats) and torch.equal(a.logp, b.logp) and torch.equal(da, db)
+
+
 def test_refusals():
     from cugo_b200.losses import action_logp, policy_loss, policy_loss_grad, preference_loss
     x, actions, mask, _ = make(6, 20, torch.float32, 0, True)
@@ -460,6 +484,10 @@ def test_refusals():
         (lambda: policy_loss_grad(x, actions, f, f, dlogits=x[:, :19].clone()), "dlogits"),
         (lambda: policy_loss_grad(x, actions, f, f, dlogits=x.double()), "dlogits"),
         (lambda: policy_loss_grad(x, actions, f, f, dlogits=x.clone(), grad_dtype=torch.half), "grad_dtype"),
+        (lambda: policy_loss(x, actions, f, f, denominator=1e-60), "denominator"),
+        (lambda: policy_loss_grad(x, actions, f, f, dlogits=x), "share memory"),
+        (lambda: policy_loss_grad(x[:5], actions[:5], f[:5], f[:5], dlogits=x[1:]), "share memory"),
+        (lambda: policy_loss_grad(x, actions, f, f, ref_logits=x.clone(), dlogits=x[:, :]), "share memory"),
         (lambda: preference_loss(x, actions, torch.zeros(2, dtype=torch.int64, device=DEV), f), "offsets"),
         (lambda: preference_loss(x, actions, torch.zeros(3, dtype=torch.int32, device=DEV), f), "offsets"),
         (lambda: preference_loss(x, actions, torch.zeros(3, dtype=torch.int64, device=DEV), f,

@@ -29,6 +29,7 @@ def test_action_logp_arguments(lib):
     assert _logp(lib, rows=-1) == ARG
     assert _logp(lib, vocab=0) == ARG
     assert _logp(lib, vocab=1 << 31) == ARG
+    assert _logp(lib, vocab=(1 << 30) + 1, ld=1 << 31) == ARG
     assert _logp(lib, dtype=3) == ARG
     assert _logp(lib, logits=None) == ARG
     assert _logp(lib, actions=None) == ARG
@@ -77,6 +78,7 @@ def test_policy_loss_arguments(lib):
     assert _policy(lib, logp_old=None) == ARG
     assert _policy(lib, adv=None) == ARG
     assert _policy(lib, width=178) == ARG
+    assert _policy(lib, width=(1 << 30) + 1, ldd=1 << 31) == ARG
     assert _policy(lib, ldd=180, width=184) == ARG
     assert _policy(lib, gdt=5) == ARG
     assert _policy(lib, dlogits=P + 1) == ALIGN

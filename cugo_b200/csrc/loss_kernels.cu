@@ -689,18 +689,23 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
 // ---- long rows: a block, or a cluster of blocks, per row -----------------------------------
 //
 // A row is cut into 16-byte vectors (a head of up to one vector to its first 16-byte
-// boundary, and a tail, entry by entry), and over the blocks of a cluster where it is
+// boundary, and a tail, entry by entry), and over the blocks of a cluster where it is much
 // longer than a block's shared memory, or where there are few rows.  A thread looks at
-// its vectors twice: once for its sums, with a maximum of its own that rescales them when
-// it grows, once for the gradient.  Between the two the warps' sums are joined through
+// its vectors once for its sums, with a maximum of its own that rescales them when it
+// grows, and where a gradient is wanted once more for that.  Between the two the warps' sums are joined through
 // shared memory, and the blocks' of a cluster through distributed shared memory.
 //
-// A thread's vectors stand in its own slots of shared memory, from which it takes them both
-// times, so that the logits cross the memory bus once; a slot that has been looked at for
-// the last time is filled with the next row's vector at once, so the copies run on under
-// the second look, its stores and the next row's reductions.  The copies are waited for
-// in two chunks of the slots.  Vectors that no slot holds (rows longer than eight blocks'
-// slots) are read from memory both times.
+// A thread's vectors come through its own slots of shared memory; a slot that has been
+// looked at for the last time is filled at once, with the same row's vector further on or
+// with the next row's, so the copies run on under the second look, its stores and the
+// next row's reductions.  They are waited for in two chunks of the slots.  For a gradient
+// the slots keep the row, so that it crosses the memory bus once; vectors of it that no
+// slot holds are read from memory both times.
+//
+// Bound by instructions once rows are long (about 6 an entry for the sums, 11 with the
+// gradient) and by each row's joins and barriers (some 400 and 700 instructions a warp)
+// where they are short.  Sums: 2,048 rows of 131,072 bf16 in 96 us, 5.6 TB/s; 8,192 of
+// 16,384 in 60 us, 4.5 TB/s.  With the gradient: 2,048 of 131,072 in 230 us, 4.7 TB/s.
 
 constexpr int kLongThreads = 256, kWideThreads = 512;
 constexpr int kGroup = 4;   // vectors of a thread looked at together
@@ -1206,29 +1211,43 @@ __device__ __forceinline__ i64 long_rows(const Rows& r, const Score& o, const Po
       if constexpr (kMasks) add_bounded<T, kRef>(run, x, z);
       else add_vectors<T, kRef>(run, x, z);
     };
+    // The row by as many vectors as the slots hold; slots that need not be kept for a second
+    // look are filled again at once, with the row's vectors further on or the next row's.
+    const int in_part = p.last - p.first, n_all = in_part <= tid ? 0 : (in_part - tid + step - 1) >> log_step;
+    int base = 0;  // vectors before those in the slots
+    for (;; base += slots) {
+      const int n = n_all - base < slots ? n_all - base : slots;
+      const bool more = !write && slots > 0 && (base + slots) * step < in_part;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      if (write && c > 0) wait_copies<0>();
-      else wait_copies<kChunks - 1>();
-      static_assert(kChunks == 2, "the waits are for two");
-      const int end = (c + 1) * chunk < n_slotted ? (c + 1) * chunk : n_slotted;
-      const uint4 *at = mine + c * chunk * step, *at_r = mine_r + c * chunk * step;
-      int k = c * chunk;
+      for (int c = 0; c < kChunks; ++c) {
+        if (write && c > 0) wait_copies<0>();
+        else wait_copies<kChunks - 1>();
+        static_assert(kChunks == 2, "the waits are for two");
+        const int end = (c + 1) * chunk < n ? (c + 1) * chunk : n;
+        const uint4 *at = mine + c * chunk * step, *at_r = mine_r + c * chunk * step;
+        int k = c * chunk;
 #pragma unroll 1
-      for (; k + kLook <= end; k += kLook, at += kLook * step, at_r += kLook * step) {
-        uint4 x[kLook], z[kLook];
-        from_slots(at, at_r, k, x, z);
-        add(x, z);
-      }
+        for (; k + kLook <= end; k += kLook, at += kLook * step, at_r += kLook * step) {
+          uint4 x[kLook], z[kLook];
+          from_slots(at, at_r, base + k, x, z);
+          add(x, z);
+        }
 #pragma unroll 1
-      for (; k < end; ++k, at += step, at_r += step) {
-        uint4 x[1], z[1];
-        from_slots(at, at_r, k, x, z);
-        add(x, z);
+        for (; k < end; ++k, at += step, at_r += step) {
+          uint4 x[1], z[1];
+          from_slots(at, at_r, base + k, x, z);
+          add(x, z);
+        }
+        if (more) {
+          const int behind = base + slots, left = n_all - behind;
+          fetch(first_x(p) + behind * step, kRef ? first_z(p) + behind * step : nullptr, left < slots ? left : slots, c);
+        } else if (!write) {
+          fetch(x_next, z_next, n_next, c);
+        }
       }
-      if (!write) fetch(x_next, z_next, n_next, c);
+      if (!more) break;
     }
-    {  // what no slot holds
+    if (write || slots == 0) {  // what no slot holds
       int i = i0 + slots * step;
 #pragma unroll 1
       for (; i + step < p.last; i += 2 * step) {
@@ -1656,44 +1675,43 @@ struct Plan {
   int threads, blocks, parts, slots, shared;
 };
 
-// A block per row, of as few threads as leave each about 16 vectors (a row costs a thread
-// some 400 instructions beside its vectors; 8,192 rows of 16,384 bf16: 128 threads 58 us,
-// 256 threads 86 us); a cluster of blocks where the row is longer than the slots of one
-// (three blocks share an SM, or as many as the slots allow), and where rows are few: up
-// to 8, each with at least 4,096 entries.  A policy loss that has to cut its rows takes
-// fewer and larger blocks, two of 512 threads an SM, and reads what their slots do not
-// hold once more (2,048 rows of 131,072 bf16: 2 blocks a row and 13 of 16 vectors in
-// slots 242 us, 4 blocks of 256 threads and all 16 298 us).
-Plan long_plan(i64 rows, int vocab, int size, bool ref, bool stage, bool policy) {
+// A block per row; few rows get up to 8, each with at least 4,096 entries.
+//
+// Sums only: the slots pass the row through, so its length does not matter, and small blocks
+// spread the rows' reductions best (six of 128 threads an SM against three of 256: 8,192
+// rows of 16,384 bf16 60 and 74 us, 2,048 of 131,072 96 and 97 us).
+//
+// With a gradient the slots keep the row for the second look, and what they do not hold is
+// read twice.  Short ones as above; from 16 vectors a thread on 256 threads, three blocks an
+// SM; rows above a third of an SM's shared memory take 512 threads, two blocks, which hold
+// half as much again each (4,096 rows of 49,152 bf16: 176 against 188 us); above three
+// quarters of it, two such blocks a row (2,048 rows of 131,072: 256 us, one block 268 us, four
+// of 256 threads that hold it all 335 us; of 65,536: 270, one block 243 us).  A cluster's
+// barriers cost more than what is read again, so no row takes more.
+Plan long_plan(i64 rows, int vocab, int size, bool ref, bool stage, bool write) {
   constexpr int kBudget = 224 << 10, kStatic = 3 << 10;  // an SM's shared memory, a block's other part
   Plan p{};
   const int copies = ref ? 2 : 1;
-  const i64 bytes = static_cast<i64>(vocab) * size * copies;
-  const bool cut = bytes > kBudget / 3 - kStatic;
+  const i64 bytes = static_cast<i64>(vocab) * size;
   p.parts = 1;
   p.threads = kLongThreads;
-  int most_per_sm = 3;
-  if (cut && policy) {
+  int per_sm = 3;
+  if (write && bytes > kBudget / 3) {
     p.threads = kWideThreads;
-    most_per_sm = 2;
-    while (p.parts < 8 && bytes > static_cast<i64>(p.parts) * (kBudget / 2 - kStatic) * 5 / 4) p.parts *= 2;
-  } else {
-    while (p.parts < 8 && bytes > static_cast<i64>(p.parts) * (kBudget / 3 - kStatic)) p.parts *= 2;
+    per_sm = 2;
+    if (bytes > kBudget * 3 / 4) p.parts = 2;
   }
   while (p.parts < 8 && rows * p.parts < kSms && vocab / (2 * p.parts) >= 4096) p.parts *= 2;
-  const i64 each = (static_cast<i64>(vocab) * size / 16 + p.parts - 1) / p.parts;  // vectors
-  if (each <= 16 * 128) {
+  const i64 each = (bytes / 16 + p.parts - 1) / p.parts;  // vectors
+  if (!write || each <= 16 * 128) {
     p.threads = 128;
-    most_per_sm = 6;
+    per_sm = 6;
   }
   if (stage) {
-    const i64 want = (each + p.threads - 1) / p.threads;
-    const i64 room = ((cut ? kBudget / most_per_sm : kBudget) - kStatic) / (p.threads * 16 * copies);
+    const i64 want = (each + p.threads - 1) / p.threads, room = (kBudget / per_sm - kStatic) / (p.threads * 16 * copies);
     p.slots = static_cast<int>(want < room ? want : room);
   }
   p.shared = p.slots * p.threads * 16 * copies;
-  int per_sm = kBudget / (p.shared + kStatic);
-  if (per_sm > most_per_sm) per_sm = most_per_sm;
   const i64 most = static_cast<i64>(kSms) * per_sm / p.parts;
   p.blocks = static_cast<int>(rows < most ? rows : most) * p.parts;
   return p;
@@ -1732,7 +1750,7 @@ int launch_long(const Rows& r, const Score& o, const Policy& a, cudaStream_t str
   const auto apart = reinterpret_cast<uintptr_t>(r.ref) - reinterpret_cast<uintptr_t>(r.logits);
   const bool alike = apart % 16 == 0 && (r.rows <= 1 || (r.ldr - r.ld) * kSize % 16 == 0);
   const bool stage = !kRef || alike;
-  const Plan p = long_plan(r.rows, r.vocab, kSize, kRef, stage, kPolicy);
+  const Plan p = long_plan(r.rows, r.vocab, kSize, kRef, stage, a.dlogits != nullptr);
   blocks = p.blocks;
   if constexpr (kPolicy)
     if (p.threads == kWideThreads) return launch_planned<T, kRef, kPolicy, kWideThreads>(p, r, o, a, stream);

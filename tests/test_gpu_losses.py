@@ -130,7 +130,14 @@ def test_policy_loss(vocab, dtype, rows, legal, pad, kl, weights):
     near(d, want, grad_tol(vocab, p, actions, size, dtype, want), "one pass")
     y = x.detach().requires_grad_()
     again = policy_loss(y, actions, old, adv, **k)
-    assert torch.equal(again.stats, out.stats) and torch.equal(again.logp, out.logp)
+    if vocab <= 1024:
+        assert torch.equal(again.stats, out.stats) and torch.equal(again.logp, out.logp)
+    else:
+        # Without its gradient a long row goes over other threads, which add in another order:
+        # each of the two is within its bound of the definition (above), so they are within
+        # twice that of one another.
+        near(again.stats, out.stats.double(), 2 * worst * (1 + stats.abs()), "stats of the loss alone")
+        near(again.logp, out.logp.double(), 2 * chain(vocab) * U * (1 + logp.abs()), "logp of the loss alone")
     g, = torch.autograd.grad(again.loss * 3.0, y)
     near(g, 3 * want, 3 * grad_tol(vocab, p, actions, size, dtype, want), "autograd")
     # Into a wider buffer of another type, scaled by a device value.

@@ -45,6 +45,7 @@ constexpr int kBlock = 256;              // elements of a scale
 constexpr int kThreads = 256, kPer = 8;  // 8 warps, a scale's block at a time each
 constexpr int kWarps = kThreads / 32;
 constexpr int kSms = 148;
+constexpr int kBlocks = 4;  // of a scale, that a warp takes of many
 constexpr int kNormBlocks = 8 * kSms;
 constexpr int kFewTensors = 40, kMostTensors = 400;
 
@@ -477,8 +478,12 @@ __device__ __noinline__ void step8_direct(const Tensor& t, const Options& o, con
   step8<P, true, false>(at, o, s, ms, vs, p, g, m, v);
 }
 
-// States in 8 bits: 60 instructions an element leave few registers for loads in flight, so
-// a warp's blocks are copied to shared memory ahead of the arithmetic, kDepth of them.
+// States in 8 bits: some 70 instructions an element leave few registers for loads in flight,
+// so a warp's blocks are copied to shared memory ahead of the arithmetic, kDepth of them.
+// bf16 parameters and gradients are bound by the instructions (a step of 276 million of
+// them 659 us, 4.2 TB/s); fp32 ones by memory (57 million, with the norm's reading 234 us,
+// 4.8 TB/s).  Two, three and four blocks an SM: 661, 625 and 707 us (bf16, before the
+// products were rounded each).
 template <typename P, typename G>
 struct Stage {
   static constexpr int kP = kBlock * sizeof(P), kG = kBlock * sizeof(G), kBytes = kP + kG + 2 * kBlock;
@@ -561,7 +566,9 @@ __global__ void __launch_bounds__(kThreads, 3) adamw8_kernel(const __grid_consta
 }
 
 // Sums of the gradients' squares, in 64 bits from the squares on (exact there), so that the
-// norm, and with it every rounding of a clipped step, does not hang on the order.
+// norm, and with it every rounding of a clipped step, does not hang on the order.  57 million
+// fp32 gradients 57 us, 4.0 TB/s (35 us is the floor; the conversions to 64 bits, and tiles
+// that do not fill the last round).
 template <typename G, int kMost>
 __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Tensors<kMost> a, double* partial) {
   __shared__ double part[kThreads / 32];
@@ -570,14 +577,25 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ 
     const Tensor& t = a.t[find(a, tile)];
     const i64 first = (static_cast<i64>(tile - t.first_tile) * kWarps + (threadIdx.x >> 5)) * a.per_warp;
     const G* const at = static_cast<const G*>(t.g);
-#pragma unroll 2
-    for (int u = 0; u < a.per_warp; ++u) {
-      const i64 i = (first + u) * kBlock + (threadIdx.x & 31) * kPer;
-      float g[8];
-      if (t.wide && i + kPer <= t.n) load8<true>(at + i, 8, g);
-      else load8<false>(at + i, t.n - i < 8 ? static_cast<int>(t.n - i) : 8, g);
+    const auto add = [&](const float (&g)[8]) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = fma(static_cast<double>(g[e]), static_cast<double>(g[e]), sum);
+    };
+    const int lane = threadIdx.x & 31;
+    if (t.wide && a.per_warp == kBlocks && (first + kBlocks) * kBlock <= t.n) {  // all loads at once
+      float g[kBlocks][8];
+#pragma unroll
+      for (int u = 0; u < kBlocks; ++u) load8<true>(at + (first + u) * kBlock + lane * kPer, 8, g[u]);
+#pragma unroll
+      for (int u = 0; u < kBlocks; ++u) add(g[u]);
+    } else {
+      for (int u = 0; u < a.per_warp; ++u) {
+        const i64 i = (first + u) * kBlock + lane * kPer;
+        float g[8];
+        if (t.wide && i + kPer <= t.n) load8<true>(at + i, 8, g);
+        else load8<false>(at + i, t.n - i < 8 ? static_cast<int>(t.n - i) : 8, g);
+        add(g);
+      }
     }
   }
   sum = sum_warp(sum);
@@ -664,7 +682,7 @@ int launch_sized(const Lists& l, bool eight, const Options& o, double* partial, 
   // that leaves an SM less than two rounds of tiles, one, for balance.
   i64 total = 0;
   for (i64 k = 0; k < l.count; ++k) total += l.n[k] / kBlock;
-  const int per_warp = total >= static_cast<i64>(kSms) * 4 * kWarps * 4 * 2 ? 4 : 1;
+  const int per_warp = total >= static_cast<i64>(kSms) * 4 * kWarps * kBlocks * 2 ? kBlocks : 1;
   Tensors<kMost> a;
   int partials = 0;
   if (norm) {

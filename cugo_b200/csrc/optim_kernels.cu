@@ -481,8 +481,8 @@ __device__ __noinline__ void step8_direct(const Tensor& t, const Options& o, con
 // States in 8 bits: some 70 instructions an element leave few registers for loads in flight,
 // so a warp's blocks are copied to shared memory ahead of the arithmetic, kDepth of them.
 // bf16 parameters and gradients are bound by the instructions (a step of 276 million of
-// them 659 us, 4.2 TB/s); fp32 ones by memory (57 million, with the norm's reading 234 us,
-// 4.8 TB/s).  Two, three and four blocks an SM: 661, 625 and 707 us (bf16, before the
+// them 659 us, 4.2 TB/s); fp32 ones by memory (71 million, with the norm's reading 233 us,
+// 6.0 TB/s).  Two, three and four blocks an SM: 661, 625 and 707 us (bf16, before the
 // products were rounded each).
 template <typename P, typename G>
 struct Stage {
@@ -566,9 +566,8 @@ __global__ void __launch_bounds__(kThreads, 3) adamw8_kernel(const __grid_consta
 }
 
 // Sums of the gradients' squares, in 64 bits from the squares on (exact there), so that the
-// norm, and with it every rounding of a clipped step, does not hang on the order.  57 million
-// fp32 gradients 57 us, 4.0 TB/s (35 us is the floor; the conversions to 64 bits, and tiles
-// that do not fill the last round).
+// norm, and with it every rounding of a clipped step, does not hang on the order.  71 million
+// fp32 gradients 57 us, 5.0 TB/s (44 us in 32 bits).
 template <typename G, int kMost>
 __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Tensors<kMost> a, double* partial) {
   __shared__ double part[kThreads / 32];

@@ -9,8 +9,8 @@ one does not: any number of entries, fp32, bf16 or fp16 logits, rows of any stri
 
 Rows.  logits [rows, entries] with unit column stride; legal bool of the same shape (or
 one mask expanded over the rows), or None; actions int64 [rows].  An entry that is not
-legal has probability 0, and so has one at or below -2^30 (-inf, -1e30, the type's lowest
-value); legal entries are taken to lie below 2^30.  What stands in a masked place is not
+legal has probability 0, and so has one at or below -2^30 (-inf, -1e30, the lowest value of
+fp32 and bf16); legal entries are taken to lie below 2^30.  What stands in a masked place is not
 used, NaN included.  A row does not count --
 log p, entropy and gradients are 0 -- where its action is outside the entries or masked,
 or its weight is 0; so a row that its mask leaves empty never counts.

@@ -380,7 +380,7 @@ CUGO_B200_API int cugo_b200_ppo_loss(const float* logits, int64_t ldl, const boo
  * Rows of `vocab` logits (any number from 1 to 2^30; dtype 0 fp32, 1 bf16, 2 fp16),
  * ld elements apart.  legal (bool, rows ldm bytes apart, 0: one mask for all rows; null:
  * every entry) masks entries; an entry at or below -2^30 counts as masked too (-inf,
- * -1e30, the type's lowest value), whatever stands in a masked place is not used, and
+ * -1e30, the lowest value of fp32 and bf16), whatever stands in a masked place is not used, and
  * logits are taken to lie below 2^30.  A row does not count -- its outputs and
  * gradients are 0 -- where its action is outside [0, vocab) or masked, or its weight is
  * 0.  Arithmetic and sums over a row in 32 bits, sums over rows in 64 bits, in a fixed

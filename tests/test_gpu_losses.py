@@ -443,6 +443,83 @@ def test_few_long_rows(vocab):
         near(d, want, grad_tol(vocab, p, actions, size, torch.bfloat16, want), "gradient")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(3, 131072), (700, 2501), (500, 33000), (400, 50000), (300, 100001)])
+def test_masked_entries_turn_up_late(rows, vocab, dtype):
+    """Long rows of which some, not the first ones, have entries of -inf, and one a NaN: each
+    plan for such rows, with and without a reference, forward and backward."""
+    from cugo_b200.losses import action_logp, policy_loss_grad
+    for kl in ("none", "full"):
+        x, actions, old, adv, k = policy_case(rows, vocab, dtype, False, 0, kl, False)
+        g = torch.Generator(device=DEV).manual_seed(rows)
+        shut = torch.rand((rows, vocab), device=DEV, generator=g) < 0.3
+        shut &= torch.rand((rows, 1), device=DEV, generator=g) < 0.3
+        shut.scatter_(1, actions[:, None], False)
+        shut[0] = False
+        shut[rows - 1] = True                                   # a row that does not count
+        x = x.masked_fill(shut, -float("inf"))
+        if kl == "full":
+            k["ref_logits"] = k["ref_logits"].masked_fill(shut, -float("inf"))
+        out, d = policy_loss_grad(x, actions, old, adv, **k)
+        want, stats, logp, p, used = policy64(x, actions, old, adv, **k)
+        assert not bool(used[rows - 1])
+        worst, size = policy_tols(vocab, x, actions, k, adv, p, stats, rows)
+        near(out.stats, stats, worst * (1 + stats.abs()), "stats")
+        near(out.logp, logp, chain(vocab) * U * (1 + logp.abs()), "logp")
+        near(d, want, grad_tol(vocab, p, actions, size, dtype, want), "gradient")
+        # The same as a mask, whatever stands in the masked places.
+        k["legal"] = ~shut
+        noisy = torch.where(shut, torch.full_like(x, float("nan")), x)
+        if kl == "full":
+            k["ref_logits"] = torch.where(shut, torch.full_like(x, float("inf")), k["ref_logits"])
+        out, d = policy_loss_grad(noisy, actions, old, adv, **k)
+        near(out.stats, stats, worst * (1 + stats.abs()), "stats, masked")
+        near(d, want, grad_tol(vocab, p, actions, size, dtype, want), "gradient, masked")
+    y = x.requires_grad_()
+    got, entropy = action_logp(y, actions)
+    leaf, want, want_h, p, _ = action_logp64(x, actions)
+    near(got.detach(), want.detach(), chain(vocab) * U * (1 + want.detach().abs()), "log p")
+    near(entropy.detach(), want_h.detach(), chain(vocab) * U * (1 + 2 * want_h.detach() + math.log(vocab)), "entropy")
+    d, = torch.autograd.grad(got.sum() + 0.5 * entropy.sum(), y)
+    want_d, = torch.autograd.grad(want.sum() + 0.5 * want_h.sum(), leaf)
+    size = torch.full((rows,), 2.0 + 2 * (24 + 2 * math.log(vocab)), device=DEV, dtype=torch.float64)
+    near(d, want_d, grad_tol(vocab, p, actions, size, dtype, want_d), "backward")
+    bad = x.detach().clone()
+    bad[1, 5] = float("nan")
+    worse, _ = action_logp(bad, actions)
+    assert bool(torch.isnan(worse[1])) and int(torch.isnan(worse).sum()) == 1
+    near(worse[2:], got[2:].detach().double(), 2 * chain(vocab) * U * (1 + want.detach()[2:].abs()), "beside a NaN")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [3, 30, 64, 179, 384, 1000, 1500, 4100])
+def test_rows_far_apart_and_masks_anywhere(vocab, dtype):
+    """Rows, reference rows, masks and gradients with strides of their own, flags that begin at
+    any byte; what lies between the gradient's rows stays as it was."""
+    from cugo_b200.losses import policy_loss_grad
+    rows = 37
+    for shift, gap in ((0, 77), (1, 100), (3, 33), (6, 0)):
+        x, actions, old, adv, k = policy_case(rows, vocab, dtype, True, 0, "full", True)
+        g = torch.Generator(device=DEV).manual_seed(shift)
+
+        def apart(t, more):
+            wide = torch.zeros((rows, vocab + more + shift), dtype=t.dtype, device=DEV)
+            if t.dtype != torch.bool:
+                wide.fill_(float("nan"))
+            wide[:, shift:shift + vocab] = t
+            return wide[:, shift:shift + vocab]
+
+        want, stats, _, p, _ = policy64(x, actions, old, adv, **k)
+        worst, size = policy_tols(vocab, x, actions, k, adv, p, stats, rows)
+        k["legal"], k["ref_logits"] = apart(k["legal"], gap), apart(k["ref_logits"], 2 * gap + 1)
+        room = torch.full((rows, vocab + 9 + shift), 7.0, dtype=dtype, device=DEV)
+        out, d = policy_loss_grad(apart(x, gap), actions, old, adv, **k, dlogits=room[:, shift:shift + vocab + 2])
+        near(out.stats, stats, worst * (1 + stats.abs()), "stats")
+        near(d[:, :vocab], want, grad_tol(vocab, p, actions, size, dtype, want), "gradient")
+        assert not bool(d[:, vocab:].any())
+        assert bool((room[:, :shift] == 7).all()) and bool((room[:, shift + vocab + 2:] == 7).all())
+
+
 def test_a_given_gradient_is_a_new_version():
     """What autograd has kept of the tensor that the gradient goes to is out of date."""
     from cugo_b200.losses import policy_loss_grad

@@ -1180,7 +1180,7 @@ __device__ __forceinline__ i64 long_rows(const Rows& r, const Score& o, const Po
     const i64 row = now.row;
     const int action = now.action, i0 = p.first + tid;
     const int n_loose = rank == 0 ? r.vocab - p.vectors * kN : 0;
-    if (tid == 32) {
+    if (tid == (step > 32 ? 32 : 0)) {
       sh.row_in = row_inputs<kPolicy>(r, a, row);
       sh.row_x = p.one(p.x, action);
     }
@@ -1439,27 +1439,37 @@ __global__ void __launch_bounds__(512) weight_sums_kernel(const float* weight, i
   }
 }
 
-__global__ void __launch_bounds__(32 * kSums) policy_means_kernel(const Policy given, const float* weight, i64 rows,
-                                                                  int blocks, float* stats, float* loss) {
+constexpr int kMeansGroups = 4;  // warps, at most, that add a kind of partial sums
+
+__global__ void __launch_bounds__(32 * kSums * kMeansGroups)
+    policy_means_kernel(const Policy given, const float* weight, i64 rows, int blocks, float* stats, float* loss) {
   const Policy a = resolved(given);
-  __shared__ double means[kSums];
+  __shared__ double part[kSums][kMeansGroups], means[kSums];
   const double d = block_denominator(a, weight, rows);
-  const int k = threadIdx.x >> 5;
+  const int groups = blockDim.x / (32 * kSums), step = 32 * groups;
+  const int warp = threadIdx.x >> 5, k = warp / groups, group = warp % groups;
   double t = 0.0;
-  for (int b = threadIdx.x & 31; b < blocks; b += 32 * 8) {  // eight loads in flight
+  for (int b = 32 * group + (threadIdx.x & 31); b < blocks; b += 8 * step) {  // eight loads in flight
     double x[8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) x[q] = b + 32 * q < blocks ? a.partial[(b + 32 * q) * kSums + k] : 0.0;
+    for (int q = 0; q < 8; ++q) x[q] = b + q * step < blocks ? a.partial[(b + q * step) * kSums + k] : 0.0;
 #pragma unroll
     for (int q = 0; q < 8; ++q) t += x[q];
   }
   t = sum_warp(t);
-  if ((threadIdx.x & 31) == 0) means[k] = d == 0.0 ? 0.0 : t / d;
+  if ((threadIdx.x & 31) == 0) part[k][group] = t;
+  __syncthreads();
+  if (threadIdx.x < kSums) {
+    t = part[threadIdx.x][0];
+    for (int g = 1; g < groups; ++g) t += part[threadIdx.x][g];
+    t = d == 0.0 ? 0.0 : t / d;
+    means[threadIdx.x] = t;
+    stats[threadIdx.x + 1] = static_cast<float>(t);
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
     stats[0] = static_cast<float>(means[0] - a.entropy_coef * means[1] + a.kl_coef * means[2]);
     if (loss) *loss = stats[0];
-    for (int q = 0; q < kSums; ++q) stats[q + 1] = static_cast<float>(means[q]);
     stats[kStats] = static_cast<float>(d);
   }
 }
@@ -1699,19 +1709,21 @@ struct Plan {
 
 // A block per row; few rows get up to 8, each with at least 4,096 entries.
 //
-// Sums only: the slots pass the row through, so its length does not matter, and small blocks
-// spread the rows' reductions best (six of 128 threads an SM against three of 256: 8,192
-// rows of 16,384 bf16 60 and 74 us, 2,048 of 131,072 96 and 97 us).
+// Sums only: the slots pass the row through, and small blocks spread the rows' reductions
+// best: 24 of one warp an SM up to 1,024 vectors (65,536 rows of 2,000 bf16: 97 us, six of
+// 128 threads 185 us; 20,000 of 8,192: 68 and 86 us), six of 128 threads above (8,192 rows of
+// 16,384 with the loss's terms 68 us, of one warp 72 us; 2,048 of 131,072 96 and 111 us).
 //
 // With a gradient the slots keep the row for the second look, and what they do not hold is
-// read twice.  Short ones as above; from 16 vectors a thread on 256 threads, three blocks an
-// SM; rows above a third of an SM's shared memory take 512 threads, two blocks, which hold
+// read twice.  One warp up to 512 vectors (65,536 rows of 2,000 bf16: 198 us, 128 threads
+// 317 us), two up to 1,024 (20,000 rows of 5,000: 116, one warp 122, 128 threads 137 us),
+// four up to 2,048; then 256 threads, three blocks an SM; rows above a third of an SM's shared memory take 512 threads, two blocks, which hold
 // half as much again each (4,096 rows of 49,152 bf16: 176 against 188 us); above three
 // quarters of it, two such blocks a row (2,048 rows of 131,072: 256 us, one block 268 us, four
 // of 256 threads that hold it all 335 us; of 65,536: 270, one block 243 us).  A cluster's
 // barriers cost more than what is read again, so no row takes more.
 Plan long_plan(i64 rows, int vocab, int size, bool ref, bool stage, bool write) {
-  constexpr int kBudget = 224 << 10, kStatic = 3 << 10;  // an SM's shared memory, a block's other part
+  constexpr int kBudget = 224 << 10, kStatic = 2 << 10;  // an SM's shared memory, a block's other part
   Plan p{};
   const int copies = ref ? 2 : 1;
   const i64 bytes = static_cast<i64>(vocab) * size;
@@ -1727,7 +1739,11 @@ Plan long_plan(i64 rows, int vocab, int size, bool ref, bool stage, bool write) 
   const i64 each = (bytes / 16 + p.parts - 1) / p.parts;  // vectors
   if (!write || each <= 16 * 128) {
     p.threads = 128;
-    per_sm = 6;
+    if (rows > 6 * kSms) {
+      if (each <= (write ? 512 : 1024)) p.threads = 32;
+      else if (write && each * copies <= 1536) p.threads = 64;
+    }
+    per_sm = 768 / p.threads;
   }
   if (stage) {
     const i64 want = (each + p.threads - 1) / p.threads, room = (kBudget / per_sm - kStatic) / (p.threads * 16 * copies);
@@ -1761,7 +1777,7 @@ int launch_planned(const Plan& p, const Rows& r, const Score& o, const Policy& a
   attr[0].val.clusterDim.x = p.parts;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = p.parts > 1;  // of clusters, even of one block, at most eight blocks share an SM
   return cudaLaunchKernelEx(&cfg, kernel, r, o, a, p.slots) == cudaSuccess ? CUGO_B200_OK : CUGO_B200_ERR_LAUNCH;
 }
 
@@ -1845,7 +1861,7 @@ inline i64 weight_blocks(i64 rows) {
   return b < kSms ? b : kSms;
 }
 
-constexpr int kMostBlocks = 8 * kSms;  // of any launch over rows
+constexpr int kMostBlocks = 24 * kSms;  // of any launch over rows
 constexpr i64 kMostEntries = 1 << 30;  // of a row, its zeros behind included: loops over them count in 32 bits
 
 }  // namespace
@@ -1954,7 +1970,7 @@ int cugo_b200_policy_loss(const void* logits, int64_t ld, int32_t dtype, const v
   const int rc = ref_logits ? launch_typed<true, true>(dtype, r, Score{}, a, stream, blocks)
                             : launch_typed<false, true>(dtype, r, Score{}, a, stream, blocks);
   if (rc || !stats) return rc;
-  policy_means_kernel<<<1, 32 * kSums, 0, stream>>>(a, weight, rows, blocks, stats, loss);
+  policy_means_kernel<<<1, 32 * kSums * (blocks > 4 * kSms ? kMeansGroups : 1), 0, stream>>>(a, weight, rows, blocks, stats, loss);
   return launch_status();
 }
 

@@ -444,7 +444,8 @@ def test_few_long_rows(vocab):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,vocab", [(3, 131072), (700, 2501), (500, 33000), (400, 50000), (300, 100001)])
+@pytest.mark.parametrize("rows,vocab", [(3, 131072), (700, 2501), (1000, 1501), (4000, 2501), (950, 9001), (500, 33000),
+                                        (400, 50000), (300, 100001)])
 def test_masked_entries_turn_up_late(rows, vocab, dtype):
     """Long rows of which some, not the first ones, have entries of -inf, and one a NaN: each
     plan for such rows, with and without a reference, forward and backward."""

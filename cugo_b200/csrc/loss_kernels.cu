@@ -1707,7 +1707,9 @@ struct Plan {
   int threads, blocks, parts, slots, shared;
 };
 
-// A block per row; few rows get up to 8, each with at least 4,096 entries.
+// A block per row; few rows get up to 8, each with at least 4,096 entries, and none less
+// than 128 threads (300 rows of 4,000 bf16, sums only: four warps 4.3 us, one 5.4 us; 900
+// rows 6.6 and 5.8 us).
 //
 // Sums only: the slots pass the row through, and small blocks spread the rows' reductions
 // best: 24 of one warp an SM up to 1,024 vectors (65,536 rows of 2,000 bf16: 97 us, six of

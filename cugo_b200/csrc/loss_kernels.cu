@@ -1719,8 +1719,8 @@ struct Plan {
 // With a gradient the slots keep the row for the second look, and what they do not hold is
 // read twice.  One warp up to 512 vectors (65,536 rows of 2,000 bf16: 198 us, 128 threads
 // 317 us), two up to 1,024 (20,000 rows of 5,000: 116, one warp 122, 128 threads 137 us),
-// four up to 2,048; then 256 threads, three blocks an SM; rows above a third of an SM's shared memory take 512 threads, two blocks, which hold
-// half as much again each (4,096 rows of 49,152 bf16: 176 against 188 us); above three
+// four up to 2,048; then 256 threads, three blocks an SM; rows above a third of an SM's
+// shared memory take 512 threads, two blocks, which hold half as much again each (4,096 rows of 49,152 bf16: 176 against 188 us); above three
 // quarters of it, two such blocks a row (2,048 rows of 131,072: 256 us, one block 268 us, four
 // of 256 threads that hold it all 335 us; of 65,536: 270, one block 243 us).  A cluster's
 // barriers cost more than what is read again, so no row takes more.

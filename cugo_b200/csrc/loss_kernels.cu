@@ -1540,8 +1540,10 @@ __global__ void __launch_bounds__(32 * kBackWarps, 4) logp_backward_kernel(const
         }
         S* const at = to + p.head + i * kVec<T>;
         const int apart = 32 * kVec<T>;
-        if (!p.lm && extreme<T, false>(x) > kMasked) write_vectors<T, false, kType, false>(k, lse.x, 0.0f, at, apart, wide, x, x);
-        else write_vectors<T, false, kType, true>(k, lse.x, 0.0f, at, apart, wide, x, x);
+        if (!p.lm && extreme<T, false>(x) > kMasked)
+          write_vectors<T, false, kType, false>(k, lse.x, 0.0f, at, apart, wide, x, x);
+        else
+          write_vectors<T, false, kType, true>(k, lse.x, 0.0f, at, apart, wide, x, x);
       };
       int i = lane;
       for (; i + (kGroup - 1) * 32 < p.last; i += kGroup * 32) write(i, std::integral_constant<int, kGroup>{});
@@ -1720,10 +1722,11 @@ struct Plan {
 // read twice.  One warp up to 512 vectors (65,536 rows of 2,000 bf16: 198 us, 128 threads
 // 317 us), two up to 1,024 (20,000 rows of 5,000: 116, one warp 122, 128 threads 137 us),
 // four up to 2,048; then 256 threads, three blocks an SM; rows above a third of an SM's
-// shared memory take 512 threads, two blocks, which hold half as much again each (4,096 rows of 49,152 bf16: 176 against 188 us); above three
-// quarters of it, two such blocks a row (2,048 rows of 131,072: 256 us, one block 268 us, four
-// of 256 threads that hold it all 335 us; of 65,536: 270, one block 243 us).  A cluster's
-// barriers cost more than what is read again, so no row takes more.
+// shared memory take 512 threads, two blocks, which hold half as much again each (4,096
+// rows of 49,152 bf16: 176 against 188 us); above three quarters of it, two such blocks a
+// row (2,048 rows of 131,072: 256 us, one block 268 us, four of 256 threads that hold it all
+// 335 us; of 65,536: 270, one block 243 us).  A cluster's barriers cost more than what is
+// read again, so no row takes more.
 Plan long_plan(i64 rows, int vocab, int size, bool ref, bool stage, bool write) {
   constexpr int kBudget = 224 << 10, kStatic = 2 << 10;  // an SM's shared memory, a block's other part
   Plan p{};
@@ -1819,7 +1822,8 @@ Layout short_layout(const Rows& r, const Policy& a) {
   Layout lay = {};
   // Rows lie one after another: up to 64 bytes between them are copied along.
   const auto run = [&](i64 ld, int size) { return ld >= r.vocab && (ld - r.vocab) * size <= 64; };
-  lay.apart = kRows > 1 && !(run(r.ld, sizeof(T)) && (!kRef || run(r.ldr, sizeof(T))) && (!r.legal || r.ldm == 0 || run(r.ldm, 1)));
+  const bool masks_run = !r.legal || r.ldm == 0 || run(r.ldm, 1);
+  lay.apart = kRows > 1 && !(run(r.ld, sizeof(T)) && (!kRef || run(r.ldr, sizeof(T))) && masks_run);
   const auto place = [&](i64 ld, int size, int& pitch) {
     pitch = static_cast<int>(lay.apart ? run_bytes(1, 0, kLong, size) : kRows > 1 ? ld * size : 0);
     return lay.apart ? kRows * pitch : static_cast<int>(run_bytes(kRows, kRows > 1 ? ld : 0, kLong, size));
@@ -1838,9 +1842,11 @@ Layout short_layout(const Rows& r, const Policy& a) {
 
 template <typename T, bool kRef, bool kPolicy>
 int launch_rows(const Rows& r, const Score& o, const Policy& a, cudaStream_t stream, int& blocks) {
-#define CUGO_SHORT(lanes, per) \
-  if (r.vocab <= (lanes) * (per)) \
-    return launch_short<T, lanes, per, kRef, kPolicy>(r, o, a, short_layout<T, lanes, per, kRef, kPolicy>(r, a), stream, blocks);
+#define CUGO_SHORT(lanes, per)                                                              \
+  if (r.vocab <= (lanes) * (per)) {                                                         \
+    const Layout lay = short_layout<T, lanes, per, kRef, kPolicy>(r, a);                    \
+    return launch_short<T, lanes, per, kRef, kPolicy>(r, o, a, lay, stream, blocks);        \
+  }
   CUGO_SHORT(8, 4)
   CUGO_SHORT(8, 8)
   CUGO_SHORT(8, 24)
@@ -1972,7 +1978,8 @@ int cugo_b200_policy_loss(const void* logits, int64_t ld, int32_t dtype, const v
   const int rc = ref_logits ? launch_typed<true, true>(dtype, r, Score{}, a, stream, blocks)
                             : launch_typed<false, true>(dtype, r, Score{}, a, stream, blocks);
   if (rc || !stats) return rc;
-  policy_means_kernel<<<1, 32 * kSums * (blocks > 4 * kSms ? kMeansGroups : 1), 0, stream>>>(a, weight, rows, blocks, stats, loss);
+  const int groups = blocks > 4 * kSms ? kMeansGroups : 1;
+  policy_means_kernel<<<1, 32 * kSums * groups, 0, stream>>>(a, weight, rows, blocks, stats, loss);
   return launch_status();
 }
 

@@ -434,8 +434,8 @@ __device__ __forceinline__ void step8(const Place<P>& at, const Options& o, cons
 
 // States in 32 bits: 8 elements of everything straight into registers.
 template <typename P, typename G, int kMost>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Tensors<kMost> a, const __grid_constant__ Options o,
-                                                         const Scalars* scalars) {
+__global__ void __launch_bounds__(kThreads)
+    adamw_kernel(const __grid_constant__ Tensors<kMost> a, const __grid_constant__ Options o, const Scalars* scalars) {
   const Scalars s = *scalars;
   for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const Tensor& t = a.t[find(a, tile)];
@@ -496,8 +496,8 @@ __device__ __forceinline__ void copy16(char* to, const void* from) {
 }
 
 template <typename P, typename G, int kMost>
-__global__ void __launch_bounds__(kThreads, 3) adamw8_kernel(const __grid_constant__ Tensors<kMost> a, const __grid_constant__ Options o,
-                                                             const Scalars* scalars) {
+__global__ void __launch_bounds__(kThreads, 3)
+    adamw8_kernel(const __grid_constant__ Tensors<kMost> a, const __grid_constant__ Options o, const Scalars* scalars) {
   using S = Stage<P, G>;
   __shared__ __align__(16) char shared[kWarps][S::kDepth][S::kBytes];
   const Scalars s = *scalars;

@@ -896,3 +896,6 @@ class GraphedPpoStep:
         if self.graph is None:
             self._capture()
         self.graph.replay()
+        # A replay writes the parameters without telling torch: what goes by their versions
+        # (the networks' bf16 weights, autograd's checks of saved tensors) has to see it.
+        torch.autograd.graph.increment_version([p for g in self.step.groups for p in g])

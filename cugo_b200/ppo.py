@@ -338,6 +338,10 @@ class FusedResidualMlp(nn.Module):
             self._wkey = key
         return self._wcache
 
+    def forget_weights(self) -> None:
+        """Drops the converted weights: the next call makes its own."""
+        self._wkey = self._wcache = self._tkey = self._tcache = None
+
     def _infer(self, x: torch.Tensor, params: list[torch.Tensor]) -> torch.Tensor:
         """Forward without autograd: one GEMM launch per layer with the activations in
         the epilogues and a scalar head as a row reduction, or, where
@@ -854,15 +858,43 @@ class GraphedPpoStep:
     (python/cugo_ppo50.py:625-657): three warm-up steps on a side stream, the
     weights and optimizer moments restored, one captured step.  The optimizer must
     be capturable (torch.optim.Adam(..., capturable=True)); data-parallel runs
-    (world > 1) step eagerly."""
+    (world > 1) step eagerly.
+
+    A replay reads the parameters of all networks, the reference's too, as they are then: the
+    conversions to bf16 are part of the capture.  Where the reference, a parameter's memory or
+    an optimizer state's is another one than the captured step's, the step is captured anew."""
 
     def __init__(self, step: PpoStep, template: Minibatch) -> None:
         self.step = step
         self.static = Minibatch(*(t.clone() for t in template.tensors()))
         self.graph: torch.cuda.CUDAGraph | None = None
+        self._held: list[torch.Tensor] = []  # what the captured step works on beside the minibatch
+        self._held_at: tuple = ()
+        self._reference: nn.Module | None = None
+
+    def _works_on(self) -> list[torch.Tensor]:
+        st = self.step
+        params = [p for g in st.groups for p in g]
+        states = [v for p in params if p in st.optimizer.state
+                  for v in st.optimizer.state[p].values() if torch.is_tensor(v)]
+        reference = [] if st.reference is None else [*st.reference.parameters(), *st.reference.buffers()]
+        return params + states + reference
+
+    def _key(self) -> tuple:
+        return tuple(t.data_ptr() for t in self._works_on())
+
+    def _forget_weights(self) -> None:
+        """No network of the step keeps converted weights: a capture records their making, and
+        an eager call does not take the graph's."""
+        st = self.step
+        for net in (st.actor, st.critic, st.belief, st.reference):
+            for m in net.modules() if net is not None else ():
+                if isinstance(m, FusedResidualMlp):
+                    m.forget_weights()
 
     def _capture(self) -> None:
         st = self.step
+        self.graph = None
         params = [p for g in st.groups for p in g]
         saved_sums = st.sums.clone()
         weights = [p.detach().clone() for p in params]
@@ -882,10 +914,16 @@ class GraphedPpoStep:
                 for k, v in st.optimizer.state[p].items():
                     if torch.is_tensor(v):
                         v.copy_(before[k]) if before is not None else v.zero_()
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        self._forget_weights()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
             st.step(self.static)
+        self._forget_weights()
         st.sums.copy_(saved_sums)
+        # Held, so that none of their memory is another tensor's while a replay may use it.
+        self._held = [t.detach() for t in self._works_on()] + [p.grad for p in params if p.grad is not None]
+        self._held_at, self._reference = self._key(), st.reference
+        self.graph = graph
 
     def __call__(self, mb: Minibatch) -> None:
         if self.step.world > 1:
@@ -893,7 +931,7 @@ class GraphedPpoStep:
             return
         for dst, src in zip(self.static.tensors(), mb.tensors(), strict=True):
             dst.copy_(src)
-        if self.graph is None:
+        if self.graph is None or self._reference is not self.step.reference or self._held_at != self._key():
             self._capture()
         self.graph.replay()
         # A replay writes the parameters without telling torch: what goes by their versions

@@ -2,8 +2,13 @@
 beside them see of what a replay has written."""
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
+
+from tests.test_gpu_ppo import _minibatch, _twins
+from tests.test_gpu_update_step import _adamw, _networks
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -28,3 +33,88 @@ def test_networks_read_the_weights_of_the_latest_replay(ext, optimizer):
             with torch.no_grad():
                 assert torch.equal(net(x[:, :width]), fresh(x[:, :width])), (k, width)
             assert torch.equal(train_forward(net, x[:, :width])[0], train_forward(fresh, x[:, :width])[0]), (k, width)
+
+
+def _pair_of_steps(seed=5, native=True):
+    """An eager step and a graphed one of equal networks, each with a reference of its own."""
+    from cugo_b200.ppo import NativePpoStep, PpoStep
+    steps = []
+    for _ in range(2):
+        actor, critic, reference = _networks(seed)
+        make = NativePpoStep if native else PpoStep
+        steps.append(make(actor, critic, _adamw(actor, critic), reference=reference, kl_coef=0.3))
+    return steps
+
+
+def _assert_equal_steps(eager, graphed):
+    torch.cuda.synchronize()
+    for a, b in zip(eager.groups, graphed.groups):
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+    assert torch.allclose(eager.sums, graphed.sums, rtol=1e-4, atol=1e-6)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_reference_that_changes_between_replays(native):
+    """The reference takes other weights in place, is called eagerly, other memory is written:
+    the graphed step goes on as the eager one does."""
+    from cugo_b200.ppo import GraphedPpoStep
+    eager, step = _pair_of_steps(native=native)
+    batches = [_minibatch(2048, 10 + i) for i in range(4)]
+    graphed = GraphedPpoStep(step, batches[0])
+    for i, mb in enumerate(batches):
+        if i in (1, 3):
+            state = _twins(720, 179, seed=60 + i)[0].state_dict()
+            for s in (eager, step):
+                s.reference.load_state_dict(state)
+            with torch.no_grad():
+                step.reference(mb.features)
+            junk = [torch.full((k, 720), float("nan"), dtype=torch.bfloat16, device=DEV) for k in (179, 512, 720, 512)]
+        eager.step(mb)
+        graphed(mb)
+        _assert_equal_steps(eager, step)
+    del junk
+
+
+def test_another_reference_between_replays():
+    """Another network in the reference's place, and other tensors in its parameters'."""
+    from cugo_b200.ppo import GraphedPpoStep
+    eager, step = _pair_of_steps(6)
+    batches = [_minibatch(2048, 30 + i) for i in range(3)]
+    graphed = GraphedPpoStep(step, batches[0])
+    for i, mb in enumerate(batches):
+        if i == 1:
+            for s in (eager, step):
+                s.reference = _twins(720, 179, seed=70)[0]
+        if i == 2:
+            state = _twins(720, 179, seed=71)[0].state_dict()
+            for s in (eager, step):
+                s.reference.load_state_dict({k: v.clone() for k, v in state.items()}, assign=True)
+        eager.step(mb)
+        graphed(mb)
+        _assert_equal_steps(eager, step)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_loaded_optimizer_between_replays(bits):
+    """States that are loaded between two replays are the ones that the next one goes on with."""
+    from cugo_b200.ppo import GraphedPpoStep, NativePpoStep
+    steps = []
+    for _ in range(2):
+        actor, critic, _ = _networks(9)
+        steps.append(NativePpoStep(actor, critic, _adamw(actor, critic, state_bits=bits)))
+    eager, step = steps
+    batches = [_minibatch(2048, 40 + i) for i in range(3)]
+    graphed = GraphedPpoStep(step, batches[0])
+    saved = None
+    for i, mb in enumerate(batches):
+        if i == 2:
+            for s in steps:
+                s.optimizer.load_state_dict(saved)
+        eager.step(mb)
+        graphed(mb)
+        if i == 0:
+            torch.cuda.synchronize()
+            saved = copy.deepcopy(eager.optimizer.state_dict())
+        _assert_equal_steps(eager, step)
+    assert all(int(s["step"]) == 2 for s in step.optimizer.state.values())

@@ -909,7 +909,8 @@ class GraphedPpoStep:
         with torch.no_grad():  # undo the warm-up updates in place (the graph keeps these tensors)
             for p, w in zip(params, weights):
                 p.copy_(w)
-            for p in params:
+            # New states first: a step count that they share with older ones is put back after.
+            for p in sorted(params, key=lambda p: p in moments):
                 before = moments.get(p)
                 for k, v in st.optimizer.state[p].items():
                     if torch.is_tensor(v):

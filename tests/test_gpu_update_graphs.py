@@ -118,3 +118,21 @@ def test_a_loaded_optimizer_between_replays(bits):
             saved = copy.deepcopy(eager.optimizer.state_dict())
         _assert_equal_steps(eager, step)
     assert all(int(s["step"]) == 2 for s in step.optimizer.state.values())
+
+
+def test_a_capture_leaves_the_step_count_of_parameters_with_states():
+    """The warm-up before a capture is undone also where only some of a group's parameters
+    had states: the count that they share stays."""
+    from cugo_b200.ppo import GraphedPpoStep, NativePpoStep
+    actor, critic, _ = _networks(8)
+    opt = _adamw(actor, critic)
+    mb = _minibatch(2048, 50)
+    step = NativePpoStep(actor, critic, opt)
+    step.step(mb)
+    last = list(actor.parameters())[-1]
+    del opt.state[last]
+    before = [p.detach().clone() for p in actor.parameters()]
+    graphed = GraphedPpoStep(step, mb)
+    graphed(mb)
+    assert int(opt.state[next(actor.parameters())]["step"]) == 2 and int(opt.state[last]["step"]) == 2
+    assert any(not torch.equal(p, q) for p, q in zip(actor.parameters(), before))

@@ -104,9 +104,9 @@ class AdamW(torch.optim.Optimizer):
                 continue
             if any(p.grad.is_sparse for p in ps):
                 raise RuntimeError("adamw: sparse gradients are not supported")
-            shared = next((self.state[p]["step"] for p in group["params"] if p in self.state), None)
+            shared = next((self.state[p]["step"] for p in group["params"] if self.state.get(p)), None)
             for p in ps:
-                if p not in self.state:
+                if not self.state.get(p):  # none, or an entry that a look has left
                     if shared is None:
                         shared = torch.zeros(1, dtype=torch.int64, device=p.device)
                     self.state[p] = self._new_state(p, group["state_bits"], shared)
@@ -130,7 +130,7 @@ class AdamW(torch.optim.Optimizer):
             group["grad_norm"] = None
             shared = None
             for p, key in zip(group["params"], old["params"]):
-                if key not in saved:
+                if not saved.get(key):
                     continue
                 if shared is None:
                     shared = saved[key]["step"].detach().to(p.device, torch.int64).clone().reshape(1)

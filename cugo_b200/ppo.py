@@ -899,7 +899,7 @@ class GraphedPpoStep:
         saved_sums = st.sums.clone()
         weights = [p.detach().clone() for p in params]
         moments = {p: {k: v.clone() for k, v in st.optimizer.state[p].items() if torch.is_tensor(v)}
-                   for p in params if p in st.optimizer.state}
+                   for p in params if st.optimizer.state.get(p)}
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):

@@ -136,3 +136,14 @@ def test_a_capture_leaves_the_step_count_of_parameters_with_states():
     graphed(mb)
     assert int(opt.state[next(actor.parameters())]["step"]) == 2 and int(opt.state[last]["step"]) == 2
     assert any(not torch.equal(p, q) for p, q in zip(actor.parameters(), before))
+
+
+def test_a_capture_after_a_look_at_the_states():
+    """The empty entries that a look leaves in the optimizer's states are no states."""
+    from cugo_b200.ppo import GraphedPpoStep, NativePpoStep
+    actor, critic, _ = _networks(8)
+    opt = _adamw(actor, critic)
+    assert all(opt.state[p] == {} for p in actor.parameters())
+    mb = _minibatch(2048, 50)
+    GraphedPpoStep(NativePpoStep(actor, critic, opt), mb)(mb)
+    assert all(int(opt.state[p]["step"]) == 1 for n in (actor, critic) for p in n.parameters())

@@ -1,0 +1,47 @@
+"""CPU: what optim.AdamW does before it calls its kernels, whose call is replaced here by one
+that records its arguments."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from cugo_b200 import optim
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    made = []
+
+    def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, **k):
+        made.append((params, grads, exp_avgs, exp_avg_sqs, step, k))
+        step += 1
+
+    monkeypatch.setattr(optim, "adamw_step", adamw_step)
+    return made
+
+
+def _parameters(count=3):
+    ps = [torch.nn.Parameter(torch.zeros(300 + k)) for k in range(count)]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    return ps
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_that_was_looked_up_before_the_first_step(calls, bits):
+    """torch's state is a defaultdict: a look leaves an empty entry."""
+    ps = _parameters()
+    opt = optim.AdamW(ps, state_bits=bits)
+    assert opt.state[ps[0]] == {} and opt.state[ps[2]] == {}
+    opt.step()
+    opt.step()
+    (params, _, avgs, _, step, k), _ = calls
+    assert params == ps and [a.shape for a in avgs] == [p.shape for p in ps] and int(step) == 2
+    assert all(opt.state[p]["step"] is step for p in ps)
+    assert (k["exp_avg_scales"] is None) == (bits == 32)
+    # Saved and loaded with an empty entry among the others.
+    opt.state[ps[1]].clear()
+    other = optim.AdamW(_parameters(), state_bits=bits)
+    other.load_state_dict(opt.state_dict())
+    other.step()
+    assert int(calls[-1][4]) == 3 and len(calls[-1][2]) == 3

@@ -11,7 +11,10 @@ random bits drawn from (seed, step, the element's number): steps that are smalle
 type's own are kept in the mean, and every run gives the same bits.
 
 Everything that changes from step to step -- the step count, the norm, a learning rate
-given as a tensor -- lives on the device, so a step can be captured in a CUDA graph."""
+given as a tensor -- lives on the device, so a step can be captured in a CUDA graph, once
+the parameters have their states.  A replay does not raise the parameters' versions, by which
+the networks know that their bf16 weights are old: `torch.autograd.graph.increment_version`
+does (ppo.GraphedPpoStep calls it)."""
 from __future__ import annotations
 
 from typing import Any, Iterable
@@ -21,6 +24,14 @@ import torch
 from .ext import load_update
 
 _STATES = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
+
+
+def _capturing(device: torch.device) -> bool:
+    """Whether the device's current stream records a CUDA graph."""
+    if device.type != "cuda":
+        return False
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
 
 
 def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor],
@@ -107,6 +118,9 @@ class AdamW(torch.optim.Optimizer):
             shared = next((self.state[p]["step"] for p in group["params"] if self.state.get(p)), None)
             for p in ps:
                 if not self.state.get(p):  # none, or an entry that a look has left
+                    if _capturing(p.device):
+                        raise RuntimeError("adamw: a replay would set new states to 0 again: take a step "
+                                           "with every parameter before it is captured")
                     if shared is None:
                         shared = torch.zeros(1, dtype=torch.int64, device=p.device)
                     self.state[p] = self._new_state(p, group["state_bits"], shared)

@@ -147,3 +147,25 @@ def test_a_capture_after_a_look_at_the_states():
     mb = _minibatch(2048, 50)
     GraphedPpoStep(NativePpoStep(actor, critic, opt), mb)(mb)
     assert all(int(opt.state[p]["step"]) == 1 for n in (actor, critic) for p in n.parameters())
+
+
+def test_a_first_step_is_not_captured():
+    """Refused, and nothing is left behind: a step, then the capture, go on from there."""
+    from cugo_b200.optim import AdamW
+    p, q = (torch.nn.Parameter(torch.ones(500, device=DEV)) for _ in range(2))
+    opts = [AdamW([x], lr=0.1) for x in (p, q)]
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before it is captured"):
+        with torch.cuda.graph(graph):
+            opts[0].step()
+    for opt in opts:
+        opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opts[0].step()
+    for _ in range(2):
+        graph.replay()
+        opts[1].step()
+    torch.cuda.synchronize()
+    assert torch.equal(p, q) and int(opts[0].state[p]["step"]) == 3

@@ -45,3 +45,19 @@ def test_a_state_that_was_looked_up_before_the_first_step(calls, bits):
     other.load_state_dict(opt.state_dict())
     other.step()
     assert int(calls[-1][4]) == 3 and len(calls[-1][2]) == 3
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_are_not_made_inside_a_capture(calls, monkeypatch, bits):
+    """A replay would set them to 0 again: the first step of a parameter is refused there."""
+    ps = _parameters(2)
+    opt = optim.AdamW(ps, state_bits=bits)
+    ps[1].grad, grad = None, ps[1].grad
+    opt.step()  # ps[0] has a state
+    ps[1].grad = grad
+    monkeypatch.setattr(optim, "_capturing", lambda device: True)
+    with pytest.raises(RuntimeError, match="before it is captured"):
+        opt.step()
+    ps[1].grad = None
+    opt.step()
+    assert len(calls) == 2 and ps[1] not in opt.state

@@ -128,6 +128,13 @@ cudaStream_t stream_of(int device) { return c10::cuda::getCurrentCUDAStream(devi
 
 Tensor bytes(int64_t n, const at::TensorOptions& options) { return at::empty({n}, options.dtype(at::kByte)); }
 
+// The kernels see the primal of a dual tensor only: its tangent would be lost without a word.
+void primal_only(const char* op, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (t && t->defined() && t->_fw_grad(0).defined()) fail(op, "forward-mode derivatives are not built");
+}
+const Tensor* given(const Maybe& t) { return t ? &*t : nullptr; }
+
 // A backward that autograd would differentiate again.
 void once(const char* op) {
   if (at::GradMode::is_enabled()) fail(op, "the gradient's own gradient is not built");
@@ -182,6 +189,7 @@ struct ActionLogp : torch::autograd::Function<ActionLogp> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("action_logp");
+    primal_only("action_logp", {&grads[0], &grads[1]});
     Tensor d;
     if (grads[0].defined() || grads[1].defined()) {
       const auto s = ctx->get_saved_variables();
@@ -195,6 +203,7 @@ struct ActionLogp : torch::autograd::Function<ActionLogp> {
 bool differentiable(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
 std::tuple<Tensor, Tensor> action_logp(const Tensor& logits, const Tensor& actions, const Maybe& legal) {
+  primal_only("action_logp", {&logits});
   if (differentiable(logits)) {
     const auto out = ActionLogp::apply(logits, actions, legal);
     return {out[0], out[1]};
@@ -222,6 +231,8 @@ struct PolicyOut {
 PolicyOut policy(const Tensor& logits, const PolicyArgs& p, bool stats, const Maybe& denominator, double grad_scale,
                  const Maybe& grad_scale_dev, const Maybe& dlogits, std::optional<at::ScalarType> grad_type) {
   const char* op = "policy_loss";
+  primal_only(op, {&logits, &p.logp_old, &p.adv, given(p.weight), given(p.ref_logits), given(p.ref_logp),
+                   given(p.kl_coef_dev), given(p.entropy_coef_dev), given(grad_scale_dev), given(dlogits)});
   const Rows r(op, logits, p.actions, p.legal, p.weight);
   vector(op, "logp_old", p.logp_old, r.rows, at::kFloat, r.device);
   vector(op, "adv", p.adv, r.rows, at::kFloat, r.device);
@@ -353,6 +364,7 @@ PreferenceOut preference(const Tensor& logits, const Tensor& actions, const Tens
                          const Maybe& legal, const Maybe& weight, double beta, double smoothing, bool average,
                          bool grad) {
   const char* op = "preference_loss";
+  primal_only(op, {&logits, &ref_logp, given(weight)});
   Scored s = score(op, logits, actions, legal, weight, false, true, grad);
   const int device = cuda_index(logits);
   const int64_t rows = logits.size(0);
@@ -388,6 +400,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("preference_loss");
+    primal_only("preference_loss", {&grads[0]});
     variable_list d(9);
     if (grads[0].defined()) {
       const auto s = ctx->get_saved_variables();
@@ -437,6 +450,9 @@ Maybe adamw(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs
             std::optional<double> max_grad_norm, int64_t seed, const std::optional<Tensors>& exp_avg_scales,
             const std::optional<Tensors>& exp_avg_sq_scales) {
   const char* op = "adamw";
+  for (const Tensors* list : {&params, &grads, &exp_avgs, &exp_avg_sqs})
+    for (const Tensor& t : *list) primal_only(op, {&t});
+  primal_only(op, {given(lr_dev)});
   const auto range = [&](const char* name, double value, bool ok) {
     if (!ok) fail(op, std::string(name) + " = " + std::to_string(value) + " is out of range");
   };

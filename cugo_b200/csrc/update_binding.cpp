@@ -9,6 +9,7 @@
 // the tensors' device.  Errors are std::runtime_error: RuntimeError in Python.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -128,8 +129,10 @@ cudaStream_t stream_of(int device) { return c10::cuda::getCurrentCUDAStream(devi
 
 Tensor bytes(int64_t n, const at::TensorOptions& options) { return at::empty({n}, options.dtype(at::kByte)); }
 
-// The kernels see the primal of a dual tensor only: its tangent would be lost without a word.
+// The kernels see the primal of a dual tensor only, and a trace sees their outputs'
+// allocation only: a tangent, or the call itself, would be lost without a word.
 void primal_only(const char* op, std::initializer_list<const Tensor*> tensors) {
+  if (torch::jit::tracer::isTracing()) fail(op, "the call cannot be traced");
   for (const Tensor* t : tensors)
     if (t && t->defined() && t->_fw_grad(0).defined()) fail(op, "forward-mode derivatives are not built");
 }

@@ -42,3 +42,17 @@ def test_forward_mode_derivatives_are_refused():
                 pytest.fail(f"call {k}")
         with pytest.raises(RuntimeError, match="CUDA tensor"):  # beside duals, not of them
             losses.action_logp(X, I)
+
+
+def test_a_trace_is_refused():
+    """torch.jit.trace would record the outputs' allocation and not the call."""
+    calls = [
+        lambda x: losses.action_logp(x, I),
+        lambda x: losses.policy_loss(x, I, F, F).loss,
+        lambda x: losses.policy_loss_grad(x, I, F, F)[1],
+        lambda x: losses.preference_loss(x, I, O, F).loss,
+        lambda x: optim.adamw_step([x], [X], [X], [X], I[:1], max_grad_norm=1.0),
+    ]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, (X,))

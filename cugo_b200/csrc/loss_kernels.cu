@@ -12,7 +12,9 @@
 // Parts of a row that have other maxima are brought together by powers of two, without a
 // rounding.
 // A reference row z_j (M', s') adds u = sum 2^y_j (y_j - z_j):
-//   KL(p|q) = ln 2 (u/s - log2 s + log2 s').
+//   KL(p|q) = ln 2 (u/s - log2 s + log2 s'),
+// which is infinite where the reference masks an entry that the row does not: such an entry
+// is looked for, its p may be 0 in 32 bits.
 // Every gradient wanted here is, with 1 at the taken action a,
 //   d_j = hot [j = a] + 2^y_j (c_0 + c_1 y_j + c_2 (y_j - z_j)),
 // so a row needs its sums, four coefficients and one more look at its entries.
@@ -173,8 +175,13 @@ struct Coefs {
 // The sums of a row, or of a part of one.
 struct Sums {
   float m, s, t;    // M, sum 2^y, sum 2^y y
-  float mr, sr, u;  // the reference's, and sum 2^y (y - z)
+  // The reference's, and sum 2^y (y - z).  sr's sign is set where the reference masks an entry
+  // that the row does not.
+  float mr, sr, u;
 };
+
+__device__ __forceinline__ bool infinite(float sr) { return __float_as_int(sr) < 0; }
+__device__ __forceinline__ float marked(float sr, bool infinite) { return infinite ? -sr : sr; }
 
 __device__ __forceinline__ Sums no_sums() { return {kMasked2, 0.0f, 0.0f, kMasked2, 0.0f, 0.0f}; }
 
@@ -203,7 +210,7 @@ __device__ __forceinline__ Sums join_warp(Sums v) {
   if constexpr (kRef) {
     r.mr = warp_max_nan(v.mr);
     const float dr = v.mr - r.mr;
-    r.sr = sum_warp(v.sr * exp2_fast(dr));
+    r.sr = marked(sum_warp(fabsf(v.sr) * exp2_fast(dr)), __any_sync(kFull, infinite(v.sr)));
     r.u = sum_warp(f * (v.u + (d - dr) * v.s));
   }
   return r;
@@ -352,6 +359,7 @@ __device__ __forceinline__ Coefs policy_row(const Policy& a, const RowInputs& in
     mean_d = v.u * inv_s;
     kl = kLn2 * (mean_d - (log_s.whole + log_s.part) + log2f(v.sr));
     c2 = a.kl_coef * kLn2;
+    if (c2 == 0.0f) mean_d = 0.0f;  // which may be infinite
   } else if (a.ref_logp) {
     const float d = in.ref_logp - logp, e = expm1f(d);
     kl = e - d;
@@ -568,7 +576,7 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
     if (r.legal && !lm[action]) x_a = kMasked;
     used = used && !(x_a <= kMasked);
 
-    float y[kPer], z[kPer], e[kPer];
+    float y[kPer], z[kPer], e[kPer], low = 0.0f, one = 0.0f;  // low: the reference's, past the row's end too
     // Entry l + kLanes k lies in the row where behind < -kLanes k.  A row may be read past
     // its end (the stage is that long); what stands there is not used.
     const int behind = l - vocab;
@@ -577,7 +585,12 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
       const bool in_row = behind < -kLanes * k;
       const int c = l + kLanes * k;
       y[k] = in_row ? max_nan(to_float(x[c]), kMasked) : kMasked;
-      if constexpr (kRef) z[k] = in_row ? max_nan(to_float(z_row[c]), kMasked) : kMasked;
+      if constexpr (kRef) {
+        const float raw = to_float(z_row[c]);
+        if (k % 2) low = min3(low, one, raw);
+        else one = raw;
+        z[k] = in_row ? max_nan(raw, kMasked) : kMasked;
+      }
     }
     if (r.legal) {
 #pragma unroll
@@ -587,6 +600,10 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
         if constexpr (kRef) z[k] = open ? z[k] : kMasked;
       }
     }
+    bool infinite = false;  // the reference masks an entry that the row does not
+    if (kRef && low <= kMasked)
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) infinite = infinite || (z[k] <= kMasked && y[k] > kMasked);
     float top = kMasked, top_r = kMasked;
 #pragma unroll
     for (int k = 0; k < kPer; k += 2) {
@@ -621,7 +638,7 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
     v.sr = v.u = 0.0f;
     if constexpr (kRef) {
       v.sr = sum_lanes<kLanes>(both(sr2));
-      v.u = sum_lanes<kLanes>(both(u2));
+      v.u = sum_lanes<kLanes>(both(u2) + (infinite ? INFINITY : 0.0f));
     }
     if constexpr (!kPolicy) {
       if (l == 0 && real) store_score(o, row, used, v, x_a);
@@ -884,11 +901,12 @@ struct Part {
 struct Running {
   float m, mr;
   Two s, t, sr, u;
+  bool infinite;  // the reference masks an entry that the row does not
 };
 
 __device__ __forceinline__ Running nothing_yet() {
   const Two zero = two(0.0f, 0.0f);
-  return {kMasked2, kMasked2, zero, zero, zero, zero};
+  return {kMasked2, kMasked2, zero, zero, zero, zero, false};
 }
 
 // New maxima (in base-2 units) where they are larger, also for NaN.
@@ -935,11 +953,14 @@ __device__ __forceinline__ void accumulate(Running& v, const float (&x)[kN], con
 }
 
 // Adds whole vectors as they are: one look at their largest entry for all.  An entry of
-// -inf makes the sums NaN (0 times -inf); the row is then taken again with care.
+// -inf makes the sums NaN (0 times -inf), and so does a masked entry of the reference (whose
+// fp16 knows no other than -inf); the row is then taken again with care.
 template <typename T, bool kRef, int kCount>
 __device__ __forceinline__ void add_vectors(Running& v, const uint4 (&x)[kCount], const uint4 (&z)[kCount]) {
   constexpr int kN = kVec<T>;
   raise<kRef>(v, base2(extreme<T, true>(x)), kRef ? base2(extreme<T, true>(z)) : kMasked2);
+  if constexpr (kRef && !std::is_same_v<T, __half>)
+    if (extreme<T, false>(z) <= kMasked) v.u = two(NAN, NAN);
 #pragma unroll
   for (int k = 0; k < kCount; ++k) {
     float f[kN], q[kN];
@@ -972,7 +993,11 @@ __device__ __forceinline__ void add_bounded(Running& v, const uint4 (&x)[kCount]
   for (int h = 0; h < kCount; ++h) {
     float f[kN], q[kN];
     bounded<T>(x[h], f);
-    if constexpr (kRef) bounded<T>(z[h], q);
+    if constexpr (kRef) {
+      bounded<T>(z[h], q);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) v.infinite = v.infinite || (q[e] <= kMasked && f[e] > kMasked);
+    }
     raise<kRef>(v, base2(largest(f)), kRef ? base2(largest(q)) : kMasked2);
     accumulate<kRef>(v, f, q);
   }
@@ -1279,7 +1304,10 @@ __device__ __forceinline__ i64 long_rows(const Rows& r, const Score& o, const Po
       const int c = p.loose(tid);
       const float f[2] = {p.one(p.x, c), kMasked};
       float q[2] = {kMasked, kMasked};
-      if constexpr (kRef) q[0] = p.one(p.z, c);
+      if constexpr (kRef) {
+        q[0] = p.one(p.z, c);
+        run.infinite = run.infinite || (q[0] <= kMasked && f[0] > kMasked);
+      }
       raise<kRef>(run, base2(f[0]), base2(q[0]));
       accumulate<kRef>(run, f, q);
     }
@@ -1289,7 +1317,7 @@ __device__ __forceinline__ i64 long_rows(const Rows& r, const Score& o, const Po
     v.t = both(run.t);
     if constexpr (kRef) {
       v.mr = run.mr;
-      v.sr = both(run.sr);
+      v.sr = marked(both(run.sr), run.infinite);
       v.u = both(run.u);
     }
     v = join_warp<kRef>(v);
@@ -1308,6 +1336,10 @@ __device__ __forceinline__ i64 long_rows(const Rows& r, const Score& o, const Po
       // Not a number: for an entry that is one, or for one of -inf.
       const float sum = v.s + v.t + (kRef ? v.sr + v.u : 0.0f);
       sh.result.again = !kMasks && !(fabsf(sum) < INFINITY);
+      if (kRef && infinite(v.sr)) {
+        v.sr = -v.sr;
+        v.u += INFINITY;
+      }
       const float row_x = sh.row_x;
       const bool used = !(row_x <= kMasked);
       if (!sh.result.again) {
@@ -1468,7 +1500,9 @@ __global__ void __launch_bounds__(32 * kSums * kMeansGroups)
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    stats[0] = static_cast<float>(means[0] - a.entropy_coef * means[1] + a.kl_coef * means[2]);
+    // A KL that may be infinite takes no part in the loss where its coefficient is 0.
+    const double kl = a.kl_coef == 0.0f ? 0.0 : a.kl_coef * means[2];
+    stats[0] = static_cast<float>(means[0] - a.entropy_coef * means[1] + kl);
     if (loss) *loss = stats[0];
     stats[kStats] = static_cast<float>(d);
   }

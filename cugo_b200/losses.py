@@ -80,7 +80,9 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, logp_old: torch.Ten
       loss = sum w (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A)
                     - entropy_coef H + kl_coef K) / D
 
-    K: KL(p | q) over the legal entries, q from ref_logits; or, from ref_logp (the
+    K: KL(p | q) over the legal entries, q from ref_logits (infinite, and the row's gradient
+    with it, where q masks an entry that p does not; with a coefficient of 0 it takes no part
+    in loss and gradient); or, from ref_logp (the
     reference's log p of the actions), the estimate exp(d) - 1 - d with d = ref_logp - log p,
     which is never negative and right in the mean; or 0.  D: the sum of the weights (the
     rows without weights; 0 gives a loss of 0), or `denominator` (a data-parallel job's

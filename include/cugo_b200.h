@@ -413,7 +413,8 @@ CUGO_B200_API int cugo_b200_action_logp_backward(
  *   loss = sum_i w_i (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A)
  *                     - entropy_coef H + kl_coef K) / D
  * K is KL(p | q) over the legal entries with q from ref_logits (same dtype, rows ldr
- * apart), or with ref_logp (fp32 [rows], the reference's log p of the action) the
+ * apart; infinite where q masks an entry that p does not, which takes no part where the
+ * coefficient is 0), or with ref_logp (fp32 [rows], the reference's log p of the action) the
  * estimate exp(d) - 1 - d, d = ref_logp - log p; at most one of the two. *kl_coef_dev and
  * *entropy_coef_dev (device fp32, may be null: 1) multiply the two coefficients.  weight
  * fp32 [rows] or null (1).  D = denominator where that is not 0, else *denominator_dev (device

@@ -296,9 +296,12 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     PolicyOut o = policy(logits, p, true, std::nullopt, 1.0, std::nullopt, std::nullopt, std::nullopt);
     const auto or_none = [](const Maybe& t) { return t.value_or(Tensor()); };
     Tensor stats = o.stats.narrow(0, 0, 7);
+    // Beside the statistics in memory, but with a version of its own: a caller may change
+    // those in place before the backward.
+    const Tensor denominator = o.stats.narrow(0, 7, 1).variable_data();
     ctx->save_for_backward({logits, p.actions, p.logp_old, p.adv, or_none(p.legal), or_none(p.weight),
                             or_none(p.ref_logits), or_none(p.ref_logp), or_none(p.kl_coef_dev),
-                            or_none(p.entropy_coef_dev), o.stats.narrow(0, 7, 1)});
+                            or_none(p.entropy_coef_dev), denominator});
     ctx->saved_data["coefs"] = std::vector<double>{p.clip_low, p.clip_high, p.kl_coef, p.entropy_coef};
     ctx->mark_non_differentiable({stats, o.logp});
     ctx->set_materialize_grads(false);

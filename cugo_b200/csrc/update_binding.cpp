@@ -12,11 +12,11 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <optional>
 #include <stdexcept>
 #include <string>
 #include <tuple>
-#include <unordered_set>
 #include <vector>
 
 #include "../../include/cugo_b200.h"
@@ -433,11 +433,17 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> preference_loss(const Tensor& logits,
 
 using Tensors = std::vector<Tensor>;
 
+// The memory of a call's tensor.
+struct Span {
+  const char *begin, *end;
+  const char* name;
+  bool written;
+};
+
 void check_list(const char* name, const Tensors& list, const std::vector<int64_t>& sizes,
-                std::initializer_list<at::ScalarType> types, int device, bool distinct) {
+                std::initializer_list<at::ScalarType> types, int device, bool written, std::vector<Span>& spans) {
   const char* op = "adamw";
   if (list.size() != sizes.size()) fail(op, "the lists must have one tensor each per parameter");
-  std::unordered_set<const void*> seen;
   for (size_t k = 0; k < list.size(); ++k) {
     const Tensor& t = list[k];
     if (t.numel() != sizes[k]) fail(op, std::string(name) + " have the wrong sizes");
@@ -446,8 +452,24 @@ void check_list(const char* name, const Tensors& list, const std::vector<int64_t
     if (!of_type || cuda_index(t) != device || !t.is_contiguous())
       fail(op, std::string(name) + " must be contiguous, of one type (" + c10::toString(*types.begin()) +
                    ") and on cuda:" + std::to_string(device));
-    if (distinct && sizes[k] && !seen.insert(t.const_data_ptr()).second)
-      fail(op, std::string("a tensor is in ") + name + " twice");
+    if (sizes[k]) {
+      const char* const begin = static_cast<const char*>(t.const_data_ptr());
+      spans.push_back({begin, begin + t.nbytes(), name, written});
+    }
+  }
+}
+
+// What is written is no other tensor of the call, in whole or in part.
+void check_apart(std::vector<Span>& spans) {
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  const Span *last = nullptr, *last_written = nullptr;  // those so far that end last
+  for (const Span& s : spans) {
+    const Span* const other = s.written ? last : last_written;
+    if (other && s.begin < other->end)
+      fail("adamw", std::string("a tensor is in the call twice, or shares memory with another (in ") + other->name +
+                        " and " + s.name + ")");
+    if (!last || s.end > last->end) last = &s;
+    if (s.written && (!last_written || s.end > last_written->end)) last_written = &s;
   }
 }
 
@@ -486,18 +508,26 @@ Maybe adamw(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs
     sizes[k] = params[k].numel();
     blocks[k] = (sizes[k] + 255) / 256;
   }
-  check_list("params", params, sizes, {p_type}, device, true);
-  check_list("grads", grads, sizes, {g_type}, device, false);
+  std::vector<Span> spans;
+  spans.reserve(6 * n + 2);
+  check_list("params", params, sizes, {p_type}, device, true, spans);
+  check_list("grads", grads, sizes, {g_type}, device, false, spans);
   for (const auto& [name, list] : {std::pair<const char*, const Tensors&>{"exp_avgs", exp_avgs},
                                    std::pair<const char*, const Tensors&>{"exp_avg_sqs", exp_avg_sqs}}) {
-    if (eight) check_list(name, list, sizes, {at::kByte, at::kFloat8_e4m3fn}, device, true);
-    else check_list(name, list, sizes, {at::kFloat}, device, true);
+    if (eight) check_list(name, list, sizes, {at::kByte, at::kFloat8_e4m3fn}, device, true, spans);
+    else check_list(name, list, sizes, {at::kFloat}, device, true, spans);
   }
   if (eight) {
-    check_list("exp_avg_scales", *exp_avg_scales, blocks, {at::kByte, at::kFloat8_e8m0fnu}, device, true);
-    check_list("exp_avg_sq_scales", *exp_avg_sq_scales, blocks, {at::kByte, at::kFloat8_e8m0fnu}, device, true);
+    check_list("exp_avg_scales", *exp_avg_scales, blocks, {at::kByte, at::kFloat8_e8m0fnu}, device, true, spans);
+    check_list("exp_avg_sq_scales", *exp_avg_sq_scales, blocks, {at::kByte, at::kFloat8_e8m0fnu}, device, true, spans);
   }
   const float* lr_ptr = scalar(op, "lr", lr_dev, device);
+  const auto one = [&](const char* name, const void* at, size_t size, bool written) {
+    if (at) spans.push_back({static_cast<const char*>(at), static_cast<const char*>(at) + size, name, written});
+  };
+  one("step", step.const_data_ptr(), sizeof(int64_t), true);
+  one("lr", lr_ptr, sizeof(float), false);
+  check_apart(spans);
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
   std::vector<void*> at[6];
   for (auto& a : at) a.resize(n);

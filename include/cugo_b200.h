@@ -461,7 +461,8 @@ CUGO_B200_API int64_t cugo_b200_preference_pairs_scratch_bytes(int64_t pairs);
 /* ---- the AdamW step ---------------------------------------------------------------
  *
  * One step over `count` tensors, given as host arrays of device pointers and sizes
- * (elements; contiguous tensors, none twice):
+ * (elements; contiguous tensors; those that are written share no memory with any other,
+ * which is the caller's to see to):
  *   g = g min(1, max_norm / (|g| + 1e-6))   where norm is given (the norm of all tensors)
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
  *   p = (1 - lr weight_decay) p - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)

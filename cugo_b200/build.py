@@ -5,7 +5,9 @@
 The library is torch-free: CUDA sources under cugo_b200/csrc/ compiled by nvcc with
 the CUDA runtime linked statically, exporting the C ABI of include/cugo_b200.h.  Beside
 it cugo_b200/lib/_cugo_b200_update.so, the policy update's calls on that ABI for Python
-(csrc/update_binding.cpp), compiled by the host compiler against torch.
+(csrc/update_binding.cpp), compiled by the host compiler against torch; where that cannot
+be (no torch with CUDA, no g++, no Python headers) the library is built all the same, and
+losses.py and optim.py raise when they are called.
 """
 from __future__ import annotations
 
@@ -73,9 +75,18 @@ def build_binding(force: bool = False) -> Path:
     return BINDING
 
 
+def _try_binding(force: bool = False) -> None:
+    """The binding where it can be built; the library stands without it."""
+    try:
+        build_binding(force)
+    except (ImportError, OSError, subprocess.CalledProcessError) as e:
+        print(f"cugo_b200: {BINDING.name} (the Python calls of losses.py and optim.py) was not built: {e}",
+              file=sys.stderr)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and up_to_date():
-        build_binding()
+        _try_binding()
         return LIB
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     tmp = LIB_DIR / "obj"
@@ -96,7 +107,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     cmd = [nvcc(), *ARCH_FLAGS, "--cudart", "static", "-shared", *objs, "-o", str(out)]
     subprocess.run(cmd, check=True)
     out.replace(LIB)
-    build_binding(force)
+    _try_binding(force)
     return LIB
 
 

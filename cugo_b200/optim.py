@@ -48,10 +48,10 @@ def adamw_step(params: list[torch.Tensor], grads: list[torch.Tensor],
 
     with t = step + 1, which is stored back (int64, one value on the device).  params: fp32
     or bf16; grads: fp32 or bf16; all contiguous, one type per list; parameters, states and
-    step share no memory with any other tensor of the call.  exp_avgs, exp_avg_sqs: fp32; or, with the lists of scales (uint8 or float8_e8m0fnu,
-    ceil(size / 256) each), e4m3 codes (uint8 or float8_e4m3fn).  States start as zeros.  lr:
-    a number, or one fp32 value on the device.  A norm that is infinite or NaN makes the
-    step NaN, as clip_grad_norm_ does."""
+    step share no memory with any other tensor of the call.  exp_avgs, exp_avg_sqs: fp32; or,
+    with the lists of scales (uint8 or float8_e8m0fnu, ceil(size / 256) each), e4m3 codes
+    (uint8 or float8_e4m3fn).  States start as zeros.  lr: a number, or one fp32 value on the
+    device.  A norm that is infinite or NaN makes the step NaN, as clip_grad_norm_ does."""
     rate = (0.0, lr) if torch.is_tensor(lr) else (lr, None)
     return load_update().adamw(params, grads, exp_avgs, exp_avg_sqs, step, *rate, *betas, eps, weight_decay,
                                max_grad_norm, seed, exp_avg_scales, exp_avg_sq_scales)

@@ -55,9 +55,23 @@ def up_to_date() -> bool:
     return _newer(LIB, _inputs())
 
 
+def _built_for() -> str:
+    """What a binding of this process has to be built against; the binding holds it as text."""
+    import sysconfig
+
+    import torch
+    return f"cugo_b200 binding for torch {torch.__version__}, {sysconfig.get_config_var('SOABI')};"
+
+
+def binding_fits() -> bool:
+    """Whether there is a binding that was built against this process's torch and Python."""
+    return BINDING.exists() and _built_for().encode() in BINDING.read_bytes()
+
+
 def build_binding(force: bool = False) -> Path:
     """The Python binding of the policy update's calls; links the library beside it."""
-    if not force and _newer(BINDING, [BINDING_SOURCE, ROOT / "include" / "cugo_b200.h", Path(__file__)]):
+    if not force and binding_fits() and _newer(BINDING, [BINDING_SOURCE, ROOT / "include" / "cugo_b200.h",
+                                                         Path(__file__)]):
         return BINDING
     import sysconfig
 
@@ -67,6 +81,7 @@ def build_binding(force: bool = False) -> Path:
                 Path(nvcc()).resolve().parents[1] / "include", Path(sysconfig.get_paths()["include"])]
     out = BINDING.with_suffix(".so.tmp")
     subprocess.run([shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+                    f'-DCUGO_BUILT_FOR="{_built_for()}"',
                     f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
                     *(f"-I{p}" for p in includes), str(BINDING_SOURCE), "-o", str(out),
                     f"-L{home / 'lib'}", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10",

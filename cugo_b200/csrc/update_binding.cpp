@@ -563,6 +563,7 @@ Maybe adamw(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs
 }  // namespace
 
 PYBIND11_MODULE(_cugo_b200_update, m) {
+  m.attr("built_for") = CUGO_BUILT_FOR;  // the build reads it in the file, before it is loaded
   m.def("action_logp", &action_logp);
   m.def("policy_loss", &policy_loss);
   m.def("policy_loss_grad", &policy_loss_grad);

@@ -165,13 +165,14 @@ _UPDATE: Any = None
 
 def load_update(build_if_missing: bool = True) -> Any:
     """The binding of the policy update's calls (csrc/update_binding.cpp; losses.py and
-    optim.py are its callers), built first when it is missing."""
+    optim.py are its callers), built first when it is missing or was built against another
+    torch or Python than this process's."""
     global _UPDATE
     if _UPDATE is None:
         load_library(build_if_missing)
-        if not _build.BINDING.exists():
+        if not _build.binding_fits():
             if not build_if_missing:
-                raise RuntimeError(f"cugo_b200 native binding missing: {_build.BINDING}")
+                raise RuntimeError(f"cugo_b200 native binding missing, or not of this torch: {_build.BINDING}")
             _build.build_binding()
         spec = importlib.util.spec_from_file_location("_cugo_b200_update", _build.BINDING)
         module = importlib.util.module_from_spec(spec)

@@ -16,14 +16,12 @@ def tree(tmp_path, monkeypatch):
     monkeypatch.setattr(build, "LIB_DIR", tmp_path)
     monkeypatch.setattr(build, "LIB", tmp_path / build.LIB.name)
     monkeypatch.setattr(build, "BINDING", tmp_path / build.BINDING.name)
-    if hasattr(build, "BUILT_FOR"):
-        monkeypatch.setattr(build, "BUILT_FOR", tmp_path / build.BUILT_FOR.name)
     commands = []
 
     def run(command, check):
         assert check
         commands.append(command)
-        Path(command[command.index("-o") + 1]).write_text("built")
+        Path(command[command.index("-o") + 1]).write_text(" ".join(command))
 
     monkeypatch.setattr(build.subprocess, "run", run)
     return commands
@@ -51,3 +49,30 @@ def test_the_library_is_built_without_a_host_compiler(tree, monkeypatch, capsys,
     assert "was not built" in capsys.readouterr().err
     with pytest.raises(type(error)):
         build.build_binding()
+
+
+def test_a_binding_of_another_torch_is_built_again(tree, monkeypatch):
+    """The binding goes by the torch and Python it was built against, not by its date alone."""
+    from cugo_b200 import ext
+    build.build(force=True)
+    count = len(tree)
+    build.build_binding()
+    assert build.binding_fits() and len(tree) == count
+    import torch
+    version = torch.__version__
+    monkeypatch.setattr(torch, "__version__", version + ".other")
+    assert not build.binding_fits()
+    monkeypatch.setattr(ext, "_UPDATE", None)
+    monkeypatch.setattr(ext, "load_library", lambda build_if_missing=True: None)
+    with pytest.raises(RuntimeError, match="not of this torch"):
+        ext.load_update(build_if_missing=False)
+    with pytest.raises(ImportError):  # built, and then no module: a small text file
+        ext.load_update()
+    assert len(tree) == count + 1 and build.binding_fits()
+    monkeypatch.setattr(torch, "__version__", version)
+    build.build_binding()
+    assert len(tree) == count + 2
+    # One whose build is not known.
+    build.BINDING.write_text("built")
+    build.build_binding()
+    assert len(tree) == count + 3

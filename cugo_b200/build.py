@@ -12,11 +12,13 @@ losses.py and optim.py raise when they are called.
 from __future__ import annotations
 
 import argparse
+import fcntl
 import os
 import shutil
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
+from contextlib import contextmanager
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -47,6 +49,19 @@ def _inputs() -> list[Path]:
     return [f for f in files if f.exists()]
 
 
+@contextmanager
+def _alone():
+    """One build at a time: ranks that start together would write the same files.  Who waited
+    finds what the first one built."""
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    folder = os.open(LIB_DIR, os.O_RDONLY)  # the lock's holder: no file of its own
+    try:
+        fcntl.flock(folder, fcntl.LOCK_EX)
+        yield
+    finally:
+        os.close(folder)
+
+
 def _newer(target: Path, inputs: list[Path]) -> bool:
     return target.exists() and target.stat().st_mtime >= max(f.stat().st_mtime for f in inputs)
 
@@ -70,6 +85,11 @@ def binding_fits() -> bool:
 
 def build_binding(force: bool = False) -> Path:
     """The Python binding of the policy update's calls; links the library beside it."""
+    with _alone():
+        return _build_binding(force)
+
+
+def _build_binding(force: bool) -> Path:
     if not force and binding_fits() and _newer(BINDING, [BINDING_SOURCE, ROOT / "include" / "cugo_b200.h",
                                                          Path(__file__)]):
         return BINDING
@@ -93,17 +113,21 @@ def build_binding(force: bool = False) -> Path:
 def _try_binding(force: bool = False) -> None:
     """The binding where it can be built; the library stands without it."""
     try:
-        build_binding(force)
+        _build_binding(force)
     except (ImportError, OSError, subprocess.CalledProcessError) as e:
         print(f"cugo_b200: {BINDING.name} (the Python calls of losses.py and optim.py) was not built: {e}",
               file=sys.stderr)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
+    with _alone():
+        return _build(force, verbose)
+
+
+def _build(force: bool, verbose: bool) -> Path:
     if not force and up_to_date():
         _try_binding()
         return LIB
-    LIB_DIR.mkdir(parents=True, exist_ok=True)
     tmp = LIB_DIR / "obj"
     tmp.mkdir(exist_ok=True)
 

@@ -76,3 +76,31 @@ def test_a_binding_of_another_torch_is_built_again(tree, monkeypatch):
     build.BINDING.write_text("built")
     build.build_binding()
     assert len(tree) == count + 3
+
+
+def test_builds_that_start_together(tree, monkeypatch):
+    """Two ranks without a library: one builds, the other waits and finds it."""
+    import threading
+    import time
+    written, inside, most = build.subprocess.run, [], []
+
+    def run(command, check):
+        name = command[command.index("-o") + 1]
+        inside.append(name)
+        most.append(inside.count(name))
+        time.sleep(0.05)
+        written(command, check)
+        inside.remove(name)
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    for call, commands in ((build.build, len(build.SOURCES) + 2), (build.build_binding, 1)):
+        for f in (build.LIB, build.BINDING) if call is build.build else (build.BINDING,):
+            f.unlink(missing_ok=True)
+        before = len(tree)
+        threads = [threading.Thread(target=call) for _ in range(3)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert len(tree) - before == commands and max(most) == 1, call.__name__
+        assert build.LIB.exists() and build.binding_fits()

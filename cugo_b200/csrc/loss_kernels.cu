@@ -308,24 +308,43 @@ __device__ __forceinline__ Log2 split_log2(float s) {
   return {static_cast<float>(k), log2f(__int_as_float(bits - (k << 23)))};
 }
 
+// Whether a row's whole weight is at its entry x_a: in 32 bits (all), and of the only open
+// entry, whose products are then the row's sums (only).
+struct Certain {
+  bool all, only;
+};
+
+__device__ __forceinline__ Certain certain(float x_a, const Sums& v) {
+  const float y = fmaf(x_a, kLog2e, -v.m), e = exp2_fast(y);
+  return {e >= v.s, e >= v.s && v.t == e * y};
+}
+
 // log p of an entry x_a: x_a - ln 2 (M + log2 s), the large terms in 64 bits and one rounding
 // at the end (log p of long sequences are added up, so what is alike in every row counts).
 // For the same reason two small things that are known come out again: kLog2e is log2(e)
 // (1 - kLow), which makes log Z less by that share of the mean logit, and 2^y as the
-// hardware has it is 3.0e-8 of itself too small in the mean (over [-24, 0), by value).
-__device__ __forceinline__ float log_prob(float x_a, const Sums& v, const Log2& log_s, float mean_y) {
+// hardware has it is 3.0e-8 of itself too small in the mean (over [-24, 0), by value).  Never
+// above 0, and 0 where nothing else has weight, which no mean knows about.
+__device__ __forceinline__ float log_prob(float x_a, const Sums& v, const Log2& log_s, float mean_y, bool all) {
   constexpr double kLn2d = 0.693147180559945309, kLow = 1.0 - kLn2d * kLog2e, kHardware = 3.0e-8;
   const double m = v.m;
   const double log_z = kLn2d * (m + log_s.whole + log_s.part + kLow * (m + mean_y)) + kHardware;
-  return static_cast<float>(x_a - log_z);
+  const float log_p = static_cast<float>(x_a - log_z);
+  return all || log_p > 0.0f ? 0.0f : log_p;
+}
+
+__device__ __forceinline__ float entropy_of(const Log2& log_s, float mean_y, bool only) {
+  const float h = kLn2 * (log_s.whole + (log_s.part - mean_y));
+  return only || h < 0.0f ? 0.0f : h;
 }
 
 // A row's outputs in action_logp.
 __device__ __forceinline__ void store_score(const Score& o, i64 row, bool used, const Sums& v, float x_a) {
   const Log2 log_s = split_log2(v.s);
   const float mean_y = __fdividef(v.t, v.s);
-  if (o.logp) o.logp[row] = used ? log_prob(x_a, v, log_s, mean_y) : 0.0f;
-  if (o.entropy) o.entropy[row] = used ? kLn2 * (log_s.whole + (log_s.part - mean_y)) : 0.0f;
+  const Certain sure = certain(x_a, v);
+  if (o.logp) o.logp[row] = used ? log_prob(x_a, v, log_s, mean_y, sure.all) : 0.0f;
+  if (o.entropy) o.entropy[row] = used ? entropy_of(log_s, mean_y, sure.only) : 0.0f;
   if (o.lse) o.lse[row] = used ? make_float2(v.m, log_s.whole + log_s.part) : make_float2(0.0f, INFINITY);
   if (o.zeros) o.zeros[row] = 0.0f;
 }
@@ -345,8 +364,9 @@ __device__ __forceinline__ Coefs policy_row(const Policy& a, const RowInputs& in
                                             float scale, Terms& terms, float& logp) {
   const Log2 log_s = split_log2(v.s);
   const float inv_s = 1.0f / v.s, mean_y = v.t * inv_s, w = in.weight;
-  logp = log_prob(x_a, v, log_s, mean_y);
-  const float entropy = kLn2 * (log_s.whole + (log_s.part - mean_y));
+  const Certain sure = certain(x_a, v);
+  logp = log_prob(x_a, v, log_s, mean_y, sure.all);
+  const float entropy = entropy_of(log_s, mean_y, sure.only);
   const float log_ratio = logp - in.logp_old;
   const float ratio = expf(log_ratio), adv = in.adv;
   const float bounded = ratio < a.low ? a.low : ratio > a.high ? a.high : ratio;

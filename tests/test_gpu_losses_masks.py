@@ -58,3 +58,30 @@ def test_a_reference_that_masks_an_open_entry(vocab, dtype, value, masked):
             assert bool(torch.isfinite(out.loss)) and bool(torch.isfinite(d).all())
             assert abs(float(out.loss) - float(plain.loss)) < 1e-5 * (1 + abs(float(plain.loss)))
             assert float((d.float() - want.float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [1, 2, 33, 179, 700, 2500, 40000])
+def test_a_single_open_entry_is_certain(vocab, dtype):
+    """Forced moves: log p and entropy are 0, the ratio to a behaviour policy's log p of 0 is
+    1, whatever the logit is; by mask and by value.  And log p is never above 0, the entropy
+    never below."""
+    from cugo_b200.losses import action_logp, policy_loss, policy_loss_grad
+    rows = 900
+    g = torch.Generator(device=DEV).manual_seed(vocab)
+    x = (torch.randn((rows, vocab), device=DEV, generator=g) * 20).to(dtype)
+    x[:8] = 0
+    actions = torch.randint(vocab, (rows,), device=DEV, generator=g)
+    legal = torch.zeros((rows, vocab), dtype=torch.bool, device=DEV).scatter_(1, actions[:, None], True)
+    zero = torch.zeros(rows, device=DEV)
+    for y, mask in ((x, legal), (x.masked_fill(~legal, -INF), None), (x.masked_fill(~legal, -INF), legal)):
+        logp, entropy = action_logp(y, actions, mask)
+        assert not bool(logp.any()) and not bool(entropy.any())
+        for out in (policy_loss(y, actions, zero, zero + 1, legal=mask, ref_logits=y),
+                    policy_loss_grad(y, actions, zero, zero + 1, legal=mask)[0]):
+            assert not bool(out.logp.any())
+            assert out.stats[1:3].tolist() == [-1.0, 0.0] and float(out.stats[4]) == 0.0
+    # Nearly all of the weight at one entry.
+    sharp = x.clone().scatter_(1, actions[:, None], x.amax(1, keepdim=True) + 14)
+    logp, entropy = action_logp(sharp, actions)
+    assert float(logp.max()) <= 0.0 and float(entropy.min()) >= 0.0

@@ -1758,6 +1758,11 @@ int check_rows(const Rows& r, int dtype) {
 
 constexpr int kShortShared = 222 << 10;  // bytes of shared memory that a block of short rows may have
 
+// An SM's shared memory for long rows, a block's other part, and the bytes of slots that a
+// block of `per_sm` may have.
+constexpr int kLongShared = 224 << 10, kLongStatic = 2 << 10;
+constexpr int long_slots(int per_sm) { return kLongShared / per_sm - kLongStatic; }
+
 // How a launch goes over long rows.
 struct Plan {
   int threads, blocks, parts, slots, shared;
@@ -1782,17 +1787,16 @@ struct Plan {
 // 335 us; of 65,536: 270, one block 243 us).  A cluster's barriers cost more than what is
 // read again, so no row takes more.
 Plan long_plan(i64 rows, int vocab, int size, bool ref, bool stage, bool write) {
-  constexpr int kBudget = 224 << 10, kStatic = 2 << 10;  // an SM's shared memory, a block's other part
   Plan p{};
   const int copies = ref ? 2 : 1;
   const i64 bytes = static_cast<i64>(vocab) * size;
   p.parts = 1;
   p.threads = kLongThreads;
   int per_sm = 3;
-  if (write && bytes > kBudget / 3) {
+  if (write && bytes > kLongShared / 3) {
     p.threads = kWideThreads;
     per_sm = 2;
-    if (bytes > kBudget * 3 / 4) p.parts = 2;
+    if (bytes > kLongShared * 3 / 4) p.parts = 2;
   }
   while (p.parts < 8 && rows * p.parts < kSms && vocab / (2 * p.parts) >= 4096) p.parts *= 2;
   const i64 each = (bytes / 16 + p.parts - 1) / p.parts;  // vectors
@@ -1805,7 +1809,7 @@ Plan long_plan(i64 rows, int vocab, int size, bool ref, bool stage, bool write) 
     per_sm = 768 / p.threads;
   }
   if (stage) {
-    const i64 want = (each + p.threads - 1) / p.threads, room = (kBudget / per_sm - kStatic) / (p.threads * 16 * copies);
+    const i64 want = (each + p.threads - 1) / p.threads, room = long_slots(per_sm) / (p.threads * 16 * copies);
     p.slots = static_cast<int>(want < room ? want : room);
   }
   p.shared = p.slots * p.threads * 16 * copies;
@@ -1823,8 +1827,11 @@ inline i64 run_bytes(i64 n, i64 ld, i64 width, int size) { return round16(((n - 
 template <typename T, bool kRef, bool kPolicy, int kThreads>
 int launch_planned(const Plan& p, const Rows& r, const Score& o, const Policy& a, cudaStream_t stream) {
   const auto kernel = long_rows_kernel<T, kRef, kPolicy, kThreads>;
+  // The most that any plan asks of this kernel, whatever this one does: the attribute is the
+  // process's, and another thread may be between its setting and its launch.
+  constexpr int kMost = long_slots(kThreads == kWideThreads ? 2 : 3);
   if (p.shared > (40 << 10) &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.shared) != cudaSuccess)
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess)
     return CUGO_B200_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.blocks);

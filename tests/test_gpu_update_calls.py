@@ -1,6 +1,9 @@
 """GPU: how the policy update's calls get along with what goes on around them."""
 from __future__ import annotations
 
+import ctypes
+import subprocess
+
 import pytest
 import torch
 
@@ -79,3 +82,33 @@ def test_tensors_that_share_memory_are_refused():
     adamw_step([*p, flat[:0]], [*g, flat[:0]], [*eight[0], codes[0][:0]], [*eight[1], codes[1][:0]], step,
                exp_avg_scales=[*scales[0], codes[2][:0]], exp_avg_sq_scales=[*scales[1], codes[3][:0]])
     assert int(step) == 2
+
+
+def test_threads_with_rows_of_two_lengths(ext, tmp_path):
+    """C callers on four threads whose rows take two amounts of shared memory of the same
+    kernel: every call runs."""
+    from cugo_b200 import load_library
+    from cugo_b200.build import ROOT
+    helper = tmp_path / "loss_threads.so"
+    subprocess.run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-pthread",
+                    str(ROOT / "tests" / "native" / "loss_threads.cpp"), "-o", str(helper)], check=True)
+    lib, run = load_library(), ctypes.CDLL(str(helper)).loss_threads
+    run.restype = ctypes.c_int64
+    rows, vocabs = 160, (22000, 36000, 22000, 36000)
+    need = lib.cugo_b200_policy_loss_scratch_bytes(rows)
+    x, d = ([torch.zeros((rows, v), dtype=torch.bfloat16, device=DEV) for v in vocabs] for _ in range(2))
+    scratch = [torch.zeros(need, dtype=torch.uint8, device=DEV) for _ in vocabs]
+    actions, zeros = torch.zeros(rows, dtype=torch.int64, device=DEV), torch.zeros(rows, device=DEV)
+    streams = [torch.cuda.Stream() for _ in vocabs]
+
+    def pointers(values):
+        return (ctypes.c_void_p * len(vocabs))(*values)
+
+    torch.cuda.synchronize()
+    failed = run(ctypes.cast(lib.cugo_b200_policy_loss, ctypes.c_void_p), len(vocabs), 5000, ctypes.c_int64(rows),
+                 (ctypes.c_int64 * len(vocabs))(*vocabs), pointers(t.data_ptr() for t in x),
+                 pointers(t.data_ptr() for t in d), pointers(t.data_ptr() for t in scratch), ctypes.c_int64(need),
+                 pointers(s.cuda_stream for s in streams), ctypes.c_void_p(actions.data_ptr()),
+                 ctypes.c_void_p(zeros.data_ptr()))
+    torch.cuda.synchronize()
+    assert failed == 0

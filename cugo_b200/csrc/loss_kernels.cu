@@ -1734,6 +1734,14 @@ inline int launch_status() {
   return cudaGetLastError() == cudaSuccess ? CUGO_B200_OK : CUGO_B200_ERR_LAUNCH;
 }
 
+// The status of a call that returns its error.  The runtime keeps that until it is asked for
+// the last one: taken here, it is not the next call's.
+inline int status(cudaError_t rc) {
+  if (rc == cudaSuccess) return CUGO_B200_OK;
+  cudaGetLastError();
+  return CUGO_B200_ERR_LAUNCH;
+}
+
 inline bool type_ok(int t) { return t == kFp32 || t == kBf16 || t == kFp16; }
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
@@ -1830,9 +1838,9 @@ int launch_planned(const Plan& p, const Rows& r, const Score& o, const Policy& a
   // The most that any plan asks of this kernel, whatever this one does: the attribute is the
   // process's, and another thread may be between its setting and its launch.
   constexpr int kMost = long_slots(kThreads == kWideThreads ? 2 : 3);
-  if (p.shared > (40 << 10) &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess)
-    return CUGO_B200_ERR_LAUNCH;
+  if (p.shared > (40 << 10))
+    if (int rc = status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost)))
+      return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.blocks);
   cfg.blockDim = dim3(p.threads);
@@ -1844,7 +1852,7 @@ int launch_planned(const Plan& p, const Rows& r, const Score& o, const Policy& a
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.parts > 1;  // of clusters, even of one block, at most eight blocks share an SM
-  return cudaLaunchKernelEx(&cfg, kernel, r, o, a, p.slots) == cudaSuccess ? CUGO_B200_OK : CUGO_B200_ERR_LAUNCH;
+  return status(cudaLaunchKernelEx(&cfg, kernel, r, o, a, p.slots));
 }
 
 template <typename T, bool kRef, bool kPolicy>
@@ -1865,9 +1873,9 @@ template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy>
 int launch_short(const Rows& r, const Score& o, const Policy& a, const Layout& lay, cudaStream_t stream, int& blocks) {
   const auto kernel = short_rows_kernel<T, kLanes, kPer, kRef, kPolicy>;
   const int shared = lay.warp() * kShortWarps;
-  if (shared > (44 << 10) &&  // with the static part, past what needs no opt-in
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShortShared) != cudaSuccess)
-    return CUGO_B200_ERR_LAUNCH;
+  if (shared > (44 << 10))  // with the static part, past what needs no opt-in
+    if (int rc = status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShortShared)))
+      return rc;
   constexpr int kRows = kShortWarps * 32 / kLanes;
   const i64 want = (r.rows + kRows - 1) / kRows;
   int per_sm = (226 << 10) / (shared + (3 << 10));
@@ -2000,10 +2008,9 @@ int cugo_b200_policy_loss(const void* logits, int64_t ld, int32_t dtype, const v
   }
   if (!aligned(scratch, 8)) return CUGO_B200_ERR_ALIGN;
   if (rows == 0) {
-    if (stats && cudaMemsetAsync(stats, 0, (kStats + 1) * sizeof(float), stream) != cudaSuccess)
-      return CUGO_B200_ERR_LAUNCH;
-    if (loss && cudaMemsetAsync(loss, 0, sizeof(float), stream) != cudaSuccess) return CUGO_B200_ERR_LAUNCH;
-    return CUGO_B200_OK;
+    if (stats)
+      if (int rc = status(cudaMemsetAsync(stats, 0, (kStats + 1) * sizeof(float), stream))) return rc;
+    return loss ? status(cudaMemsetAsync(loss, 0, sizeof(float), stream)) : CUGO_B200_OK;
   }
   if (!scratch || scratch_bytes < cugo_b200_policy_loss_scratch_bytes(rows)) return CUGO_B200_ERR_CAPACITY;
   double* sums = static_cast<double*>(scratch);
@@ -2056,11 +2063,10 @@ int cugo_b200_preference_pairs(const float* logp, const float* ref_logp, const f
   if (pairs > 0 && (!offsets || !margin || !seq_logp)) return CUGO_B200_ERR_ARG;
   if (rows > 0 && (!logp || !ref_logp || !lse)) return CUGO_B200_ERR_ARG;
   if (!aligned(scratch, 8) || !aligned(lse, 8)) return CUGO_B200_ERR_ALIGN;
-  if (pairs == 0)
-    return cudaMemsetAsync(loss, 0, sizeof(float), stream) == cudaSuccess &&
-                   cudaMemsetAsync(accuracy, 0, sizeof(float), stream) == cudaSuccess
-               ? CUGO_B200_OK
-               : CUGO_B200_ERR_LAUNCH;
+  if (pairs == 0) {
+    if (int rc = status(cudaMemsetAsync(loss, 0, sizeof(float), stream))) return rc;
+    return status(cudaMemsetAsync(accuracy, 0, sizeof(float), stream));
+  }
   if (!scratch || scratch_bytes < cugo_b200_preference_pairs_scratch_bytes(pairs)) return CUGO_B200_ERR_CAPACITY;
   const Pairs a{logp, ref_logp, weight, reinterpret_cast<const float2*>(lse), offsets, pairs, rows, beta, smoothing,
                 average != 0, margin, seq_logp, d_logp, static_cast<double*>(scratch), {loss, accuracy}};

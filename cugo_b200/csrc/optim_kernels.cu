@@ -643,6 +643,14 @@ inline int launch_status() {
   return cudaGetLastError() == cudaSuccess ? CUGO_B200_OK : CUGO_B200_ERR_LAUNCH;
 }
 
+// The status of a call that returns its error.  The runtime keeps that until it is asked for
+// the last one: taken here, it is not the next call's.
+inline int status(cudaError_t rc) {
+  if (rc == cudaSuccess) return CUGO_B200_OK;
+  cudaGetLastError();
+  return CUGO_B200_ERR_LAUNCH;
+}
+
 // The call's tensors, host arrays of `count`.
 struct Lists {
   void* const* p;
@@ -695,7 +703,7 @@ int launch_sized(const Lists& l, bool eight, const Options& o, double* partial, 
       partials += blocks;
     }
     if (partials == 0) {  // no elements at all: a norm of 0
-      if (cudaMemsetAsync(partial, 0, sizeof(double), stream) != cudaSuccess) return CUGO_B200_ERR_LAUNCH;
+      if (int rc = status(cudaMemsetAsync(partial, 0, sizeof(double), stream))) return rc;
       partials = 1;
     }
   }

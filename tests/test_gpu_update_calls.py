@@ -112,3 +112,39 @@ def test_threads_with_rows_of_two_lengths(ext, tmp_path):
                  ctypes.c_void_p(zeros.data_ptr()))
     torch.cuda.synchronize()
     assert failed == 0
+
+
+@pytest.mark.parametrize("vocab", [179, 40000])
+def test_a_launch_that_failed_is_not_reported_twice(ext, vocab):
+    """A launch into a stream whose capture has been invalidated is refused on the host; the
+    next call, on a good stream, knows nothing of it."""
+    from cugo_b200 import load_library
+    lib = load_library()
+    cu = ctypes.CDLL("libcuda.so.1")
+    rows = 300
+    x = torch.zeros((rows, vocab), device=DEV)
+    actions = torch.zeros(rows, dtype=torch.int64, device=DEV)
+    out = torch.zeros(rows, device=DEV)
+    lse, d = torch.zeros((rows, 2), device=DEV), torch.zeros((rows, vocab), device=DEV)
+    torch.cuda.synchronize()
+
+    def forward(stream):
+        return lib.cugo_b200_action_logp(x.data_ptr(), vocab, 0, None, 0, actions.data_ptr(), None, rows, vocab,
+                                         out.data_ptr(), None, lse.data_ptr(), None, stream)
+
+    def backward(stream):
+        return lib.cugo_b200_action_logp_backward(x.data_ptr(), vocab, 0, None, 0, actions.data_ptr(), lse.data_ptr(),
+                                                  None, out.data_ptr(), None, None, rows, vocab, d.data_ptr(), vocab,
+                                                  0, stream)
+
+    stream = torch.cuda.Stream()
+    handle = ctypes.c_void_p(stream.cuda_stream)
+    good = torch.cuda.current_stream().cuda_stream
+    assert forward(good) == 0
+    assert cu.cuStreamBeginCapture_v2(handle, 2) == 0  # relaxed
+    assert cu.cuStreamSynchronize(handle) != 0         # not allowed here: the capture is void
+    assert forward(stream.cuda_stream) == -3
+    graph = ctypes.c_void_p()
+    assert cu.cuStreamEndCapture(handle, ctypes.byref(graph)) != 0
+    assert backward(good) == 0
+    torch.cuda.synchronize()

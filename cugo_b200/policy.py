@@ -103,6 +103,10 @@ class ResidualMlpPolicy:
             self._bkey = key
         return self._b32
 
+    def forget_weights(self) -> None:
+        """Drops the converted biases: the next call makes its own."""
+        self._bkey = self._b32 = None
+
     @torch.no_grad()
     def forward(self, features: torch.Tensor) -> torch.Tensor:
         """[M, inputs] features (bf16, or fp32 cast to bf16 as autocast does) ->

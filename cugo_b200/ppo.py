@@ -862,7 +862,8 @@ class GraphedPpoStep:
 
     A replay reads the parameters of all networks, the reference's too, as they are then: the
     conversions to bf16 are part of the capture.  Where the reference, a parameter's memory or
-    an optimizer state's is another one than the captured step's, the step is captured anew."""
+    an optimizer state's is another one than the captured step's, the step is captured anew (as
+    before any capture of a backward, no eager autograd graph of the networks may be alive)."""
 
     def __init__(self, step: PpoStep, template: Minibatch) -> None:
         self.step = step
@@ -877,8 +878,10 @@ class GraphedPpoStep:
         params = [p for g in st.groups for p in g]
         states = [v for p in params if p in st.optimizer.state
                   for v in st.optimizer.state[p].values() if torch.is_tensor(v)]
-        reference = [] if st.reference is None else [*st.reference.parameters(), *st.reference.buffers()]
-        return params + states + reference
+        net = st.reference
+        if isinstance(net, nn.Module):
+            return [*params, *states, *net.parameters(), *net.buffers()]
+        return [*params, *states, *getattr(net, "weights", ()), *getattr(net, "biases", ())]  # a ResidualMlpPolicy
 
     def _key(self) -> tuple:
         return tuple(t.data_ptr() for t in self._works_on())
@@ -888,13 +891,15 @@ class GraphedPpoStep:
         an eager call does not take the graph's."""
         st = self.step
         for net in (st.actor, st.critic, st.belief, st.reference):
-            for m in net.modules() if net is not None else ():
-                if isinstance(m, FusedResidualMlp):
+            for m in net.modules() if isinstance(net, nn.Module) else (net,):
+                if hasattr(m, "forget_weights"):
                     m.forget_weights()
 
     def _capture(self) -> None:
         st = self.step
-        self.graph = None
+        if self.graph is not None:  # its replays are over before its memory goes
+            torch.cuda.current_stream().synchronize()
+            self.graph = None
         params = [p for g in st.groups for p in g]
         saved_sums = st.sums.clone()
         weights = [p.detach().clone() for p in params]

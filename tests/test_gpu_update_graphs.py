@@ -169,3 +169,27 @@ def test_a_first_step_is_not_captured():
         opts[1].step()
     torch.cuda.synchronize()
     assert torch.equal(p, q) and int(opts[0].state[p]["step"]) == 3
+
+
+def test_a_reference_that_is_an_inference_policy():
+    """A ResidualMlpPolicy as the reference: its weights and biases may change in place between
+    replays too, and be replaced."""
+    from cugo_b200.policy import ResidualMlpPolicy
+    from cugo_b200.ppo import GraphedPpoStep
+    eager, step = _pair_of_steps(11)
+    for s in (eager, step):
+        s.reference = ResidualMlpPolicy.from_state_dict(_twins(720, 179, seed=80)[0].state_dict(), 3, device=DEV)
+    batches = [_minibatch(2048, 60 + i) for i in range(4)]
+    graphed = GraphedPpoStep(step, batches[0])
+    for i, mb in enumerate(batches):
+        for s in (eager, step) if i == 1 else ():
+            for t in (*s.reference.weights, *s.reference.biases):
+                t.mul_(1.5)
+        if i == 2:
+            with torch.no_grad():
+                step.reference(mb.features)
+            for s in (eager, step):
+                s.reference.biases = [b * 0.5 for b in s.reference.biases]
+        eager.step(mb)
+        graphed(mb)
+        _assert_equal_steps(eager, step)

@@ -470,9 +470,11 @@ __device__ void store_partial(const Policy& a, const double (&acc)[kSums]) {
 //
 // Bound by instructions, most of them per entry (the mask, two exponentials with a
 // reference, the sums, the gradient), the rest a row's reductions and its loss terms.
-// 262,144 rows of 179 fp32 with masks: 55 us, 4.4 TB/s (a warp per row that reads in place:
+// 262,144 rows of 179 fp32 with masks: 56 us, 4.3 TB/s (a warp per row that reads in place:
 // 267 us); policy loss of 32,768 such rows with the full KL and a bf16 gradient: 23 us,
-// 2.8 TB/s.
+// 2.9 TB/s, and 3 us for the means.  That one is held at 12 warps an SM by shared memory
+// (14.7 KB a warp).  Rows of 385 to 1,024 entries with a reference and a gradient spill 212
+// bytes a thread (16,384 rows of 1,000 bf16: 54 us, 1.8 TB/s).
 
 constexpr int kShortWarps = 4;
 
@@ -741,8 +743,9 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
 // boundary, and a tail, entry by entry), and over the blocks of a cluster where it is much
 // longer than a block's shared memory, or where there are few rows.  A thread looks at
 // its vectors once for its sums, with a maximum of its own that rescales them when it
-// grows, and where a gradient is wanted once more for that.  Between the two the warps' sums are joined through
-// shared memory, and the blocks' of a cluster through distributed shared memory.
+// grows, and where a gradient is wanted once more for that.  Between the two the warps' sums
+// are joined through shared memory, and the blocks' of a cluster through distributed shared
+// memory.
 //
 // A thread's vectors come through its own slots of shared memory; a slot that has been
 // looked at for the last time is filled at once, with the same row's vector further on or
@@ -751,10 +754,14 @@ __global__ void __launch_bounds__(32 * kShortWarps, kPolicy ? 4 : 6)
 // the slots keep the row, so that it crosses the memory bus once; vectors of it that no
 // slot holds are read from memory both times.
 //
-// Bound by instructions once rows are long (about 6 an entry for the sums, 11 with the
-// gradient) and by each row's joins and barriers (some 400 and 700 instructions a warp)
-// where they are short.  Sums: 2,048 rows of 131,072 bf16 in 96 us, 5.6 TB/s; 8,192 of
-// 16,384 in 60 us, 4.5 TB/s.  With the gradient: 2,048 of 131,072 in 230 us, 4.7 TB/s.
+// Sums alone are bound by the exponentials (their pipe 61% at 16,384 entries) and by each
+// row's joins and barriers (some 400 instructions a warp): 2,048 rows of 131,072 bf16 in
+// 96 us, 5.6 TB/s; 8,192 of 16,384 in 60 us, 4.5 TB/s.  With a gradient no pipe is full
+// (exponentials 50%, memory 43%, 2.0 instructions a cycle): a block's warps go through the
+// first look, the joins and the second look in step.  2,048 of 131,072 in 254 us, 4.2 TB/s
+// (233 us where a fifth of them has weight 0 and is not read), with the full KL 417 us; its
+// kernels spill 4 to 38 bytes a thread.  What may be masked costs a bound per entry: 8,192
+// of 16,384 with flags 106 us for the sums, 195 us with the gradient (120 us without).
 
 constexpr int kLongThreads = 256, kWideThreads = 512;
 constexpr int kGroup = 4;   // vectors of a thread looked at together
@@ -1616,7 +1623,7 @@ __global__ void __launch_bounds__(32 * kBackWarps, 4) logp_backward_kernel(const
 // Sequence j holds rows offsets[j] .. offsets[j + 1] - 1 (bounds outside the rows are
 // brought inside); pair i prefers sequence 2 i to 2 i + 1.  kLanes threads take a pair:
 // the two scores in 64 bits, the margin, then the rows' d loss / d logp.  A few hundred bytes
-// a sequence: latency only (128 pairs 6 us, 16 pairs of up to 1,024 rows 12 us).
+// a sequence: latency only (128 pairs 7 us, 16 pairs of up to 1,024 rows 12 us).
 
 struct Pairs {
   const float* logp;
@@ -1889,7 +1896,8 @@ template <typename T, int kLanes, int kPer, bool kRef, bool kPolicy>
 Layout short_layout(const Rows& r, const Policy& a) {
   constexpr int kRows = 32 / kLanes, kLong = kLanes * kPer;  // entries that a row is read to
   Layout lay = {};
-  // Rows lie one after another: up to 64 bytes between them are copied along.
+  // Rows lie one after another: up to 64 bytes between them are copied along (262,144 rows of
+  // 179 fp32, 64 bytes apart: 56 us, each by itself 78 us; 400,000 of 60: 54 and 90 us).
   const auto run = [&](i64 ld, int size) { return ld >= r.vocab && (ld - r.vocab) * size <= 64; };
   const bool masks_run = !r.legal || r.ldm == 0 || run(r.ldm, 1);
   lay.apart = kRows > 1 && !(run(r.ld, sizeof(T)) && (!kRef || run(r.ldr, sizeof(T))) && masks_run);
@@ -2070,7 +2078,10 @@ int cugo_b200_preference_pairs(const float* logp, const float* ref_logp, const f
   if (!scratch || scratch_bytes < cugo_b200_preference_pairs_scratch_bytes(pairs)) return CUGO_B200_ERR_CAPACITY;
   const Pairs a{logp, ref_logp, weight, reinterpret_cast<const float2*>(lse), offsets, pairs, rows, beta, smoothing,
                 average != 0, margin, seq_logp, d_logp, static_cast<double*>(scratch), {loss, accuracy}};
-  // Short sequences: a warp per pair; long ones: a block per pair.
+  // Short sequences: a warp per pair; long ones: a block per pair.  By the mean, which the
+  // host knows: 256 rows a pair, 16 pairs: warp 10.5 us, block 14.7; 148 pairs: 12.6 and 16.3;
+  // 1,000: 15 and 50.  2,048 rows a pair: 35 and 15, 45 and 17, 45 and 52.  One long pair among
+  // many short ones is one warp's.
   int blocks;
   if (rows / pairs <= 256) {
     const i64 want = (pairs + kPairThreads / 32 - 1) / (kPairThreads / 32);

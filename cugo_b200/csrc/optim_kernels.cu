@@ -303,8 +303,9 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
   return r;
 }
 
-// a + b, the products before them already rounded: the assembler merges a packed product
-// and a packed sum into one that is not, so the sum is taken apart.
+// a + b, the products before them already rounded.  Where both stay packed the results are
+// those of one operation without the rounding between (codes differed from the formula's), so
+// the sum is taken apart.
 __device__ __forceinline__ void sum(Two a, Two b, float& x, float& y) {
   float ax, ay, bx, by;
   split(a, ax, ay);
@@ -479,7 +480,8 @@ __device__ __noinline__ void step8_direct(const Tensor& t, const Options& o, con
 }
 
 // States in 8 bits: some 70 instructions an element leave few registers for loads in flight,
-// so a warp's blocks are copied to shared memory ahead of the arithmetic, kDepth of them.
+// so a warp's blocks are copied to shared memory ahead of the arithmetic, kDepth of them
+// (20 to 32 bytes a thread are spilled all the same).
 // bf16 parameters and gradients are bound by the instructions (a step of 276 million of
 // them 659 us, 4.2 TB/s); fp32 ones by memory (71 million, with the norm's reading 233 us,
 // 6.0 TB/s).  Two, three and four blocks an SM: 661, 625 and 707 us (bf16, before the

@@ -10,17 +10,19 @@ one does not: any number of entries, fp32, bf16 or fp16 logits, rows of any stri
 Rows.  logits [rows, entries] with unit column stride; legal bool of the same shape (or
 one mask expanded over the rows), or None; actions int64 [rows].  An entry that is not
 legal has probability 0, and so has one at or below -2^30 (-inf, -1e30, the lowest value of
-fp32 and bf16); legal entries are taken to lie below 2^30.  What stands in a masked place is not
-used, NaN included.  A row does not count --
-log p, entropy and gradients are 0 -- where its action is outside the entries or masked,
-or its weight is 0; so a row that its mask leaves empty never counts.
+fp32 and bf16; fp16's, -65,504, is an entry); legal entries are taken to lie below 2^30.
+What stands in a masked place is not used, NaN included.  A row does not count -- log p,
+entropy and gradients are 0 -- where its action is outside the entries or masked, or its
+weight is 0; so a row that its mask leaves empty never counts.  log p is never above 0 and
+the entropy never below; an action that is a row's only open entry has both 0.
 
 Everything is computed in 32 bits from the logits' own type; sums over rows in 64 bits and
 in a fixed order, so every run gives the same bits.  The calls enqueue on the current
 stream of the logits' device, do not wait for it, and can be captured in CUDA graphs.
 A backward that is captured needs a graph of its own leaves' making: torch ties a leaf's
 accumulation to the stream of the graph that still holds it, so eager graphs of the same
-leaves have to be gone by then.  Backwards of backwards are not built."""
+leaves have to be gone by then.  Backwards of backwards, forward-mode derivatives and
+traces are not built: such calls raise."""
 from __future__ import annotations
 
 from typing import NamedTuple

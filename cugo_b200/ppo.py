@@ -861,9 +861,10 @@ class GraphedPpoStep:
     (world > 1) step eagerly.
 
     A replay reads the parameters of all networks, the reference's too, as they are then: the
-    conversions to bf16 are part of the capture.  Where the reference, a parameter's memory or
-    an optimizer state's is another one than the captured step's, the step is captured anew (as
-    before any capture of a backward, no eager autograd graph of the networks may be alive)."""
+    conversions to bf16 are part of the capture.  Where the reference, a parameter's memory, an
+    optimizer state's or a number among the step's and the optimizer's options is another one
+    than the captured step's, the step is captured anew (as before any capture of a backward, no
+    eager autograd graph of the networks may be alive)."""
 
     def __init__(self, step: PpoStep, template: Minibatch) -> None:
         self.step = step
@@ -884,7 +885,10 @@ class GraphedPpoStep:
         return [*params, *states, *getattr(net, "weights", ()), *getattr(net, "biases", ())]  # a ResidualMlpPolicy
 
     def _key(self) -> tuple:
-        return tuple(t.data_ptr() for t in self._works_on())
+        st = self.step
+        numbers = [v for g in st.optimizer.param_groups for v in g.values() if isinstance(v, (int, float, tuple))]
+        return (st.clip, st.value_coef, st.grad_clip, st.belief_coef, *numbers,
+                *(t.data_ptr() for t in self._works_on()))
 
     def _forget_weights(self) -> None:
         """No network of the step keeps converted weights: a capture records their making, and

@@ -193,3 +193,21 @@ def test_a_reference_that_is_an_inference_policy():
         eager.step(mb)
         graphed(mb)
         _assert_equal_steps(eager, step)
+
+
+def test_options_that_change_between_replays():
+    """A learning rate given as a number, the clip of the ratios, a decay: the next replay goes
+    by the new ones."""
+    from cugo_b200.ppo import GraphedPpoStep
+    eager, step = _pair_of_steps(12)
+    batches = [_minibatch(2048, 70 + i) for i in range(4)]
+    graphed = GraphedPpoStep(step, batches[0])
+    for i, mb in enumerate(batches):
+        for s in (eager, step):
+            for g in s.optimizer.param_groups if i in (1, 3) else ():
+                g["lr"], g["weight_decay"] = 1e-3 / i, 0.1 * i
+            if i == 2:
+                s.clip, s.value_coef = 0.05, 2.0
+        eager.step(mb)
+        graphed(mb)
+        _assert_equal_steps(eager, step)
